@@ -7,6 +7,9 @@ Python call surface (lingbot/layers/attention.py).
 """
 from . import _lib  # noqa: F401
 from .layers.attention import attention, flash_attention, sage_attention  # noqa: F401
-from .layers import kv_quant, prologue  # noqa: F401
+from .layers import kv_quant, linear, norm, prologue, rotary  # noqa: F401
+from .layers.norm import gated_norm  # noqa: F401
+from .layers.rotary import Rotary, grid_positions, rotary_embed  # noqa: F401
 
-__all__ = ["attention", "flash_attention", "sage_attention", "kv_quant", "prologue"]
+__all__ = ["attention", "flash_attention", "sage_attention", "gated_norm", "Rotary", "grid_positions", "rotary_embed",
+           "kv_quant", "linear", "norm", "prologue", "rotary"]

@@ -1,4 +1,5 @@
-"""ctypes binding of liblbw_attn.so (the C-ABI declared in include/lbw_attn.h and include/lbw_gemm.h)."""
+"""ctypes binding of liblbw_attn.so (the C-ABI declared in include/lbw_attn.h, include/lbw_gemm.h and
+include/lbw_block.h)."""
 import ctypes
 import os
 
@@ -45,6 +46,19 @@ GEMM_SIGNATURES = {
     "lbw_quant_mx_fp8_tw": (_i32, [_p, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p]),
 }
 
+# the block operators' entry points; mirrors include/lbw_block.h
+BLOCK_SIGNATURES = {
+    "lbw_gated_norm": (_i32, [_p, _p, _i32, _i32] + [_i64] * 7 + [_p, _i64, _i64] * 3 +
+                       [_i64, _p, _p, _p, _i32, _i32, _f32, _f32, _f32, _p, _p, _p]),
+    "lbw_gated_norm_bwd": (_i32, [_p, _p, _p, _p, _i32, _i32] + [_i64] * 7 + [_p, _i64, _i64] * 2 + [_i32, _i64, _i64] +
+                           [_p, _p, _p, _i32, _i32, _f32, _f32, _f32] + [_p] * 10),
+    "lbw_gated_norm_bwd_workspace_bytes": (_i64, [_i64] * 5),
+    "lbw_rotary": (_i32, [_p, _p, _i32] + [_i64] * 12 + [_p, _i32] + [_i64] * 4 + [_p, _p, _i64, _i32, _i32, _f32,
+                                                                                   _p, _p] + [_i64] * 6 + [_p]),
+    "lbw_quant_w4": (_i32, [_p, _i32, _i64, _i64, _i64, _i32, _i64, _p, _p, _p, _p]),
+    "lbw_gemm_w4": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _i32, _i64, _i64, _p, _p, _p]),
+}
+
 
 def sources_sha16():
     """First 16 hex digits of a sha256 over what liblbw_attn.so is built from: the HIP sources and headers (csrc/,
@@ -55,7 +69,7 @@ def sources_sha16():
     here = os.path.dirname(os.path.abspath(__file__))
     files = [os.path.join(here, "csrc", f) for f in sorted(os.listdir(os.path.join(here, "csrc")))
              if f.endswith((".hip", ".h"))]
-    files += [os.path.join(os.path.dirname(here), "include", f) for f in ("lbw_attn.h", "lbw_gemm.h")]
+    files += [os.path.join(os.path.dirname(here), "include", f) for f in ("lbw_attn.h", "lbw_block.h", "lbw_gemm.h")]
     h = hashlib.sha256(" ".join(build.HIPCC_FLAGS).encode())
     for f in files:
         with open(f, "rb") as fh:
@@ -79,7 +93,7 @@ def load(path=LIB_PATH):
         raise ImportError(f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
                           "or `python lingbot_world_v2_realtime_amd/build.py`")
     lib = ctypes.CDLL(path)
-    for name, (res, args) in (*SIGNATURES.items(), *GEMM_SIGNATURES.items()):
+    for name, (res, args) in (*SIGNATURES.items(), *GEMM_SIGNATURES.items(), *BLOCK_SIGNATURES.items()):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -19,7 +19,7 @@ from torch.autograd import forward_ad
 
 from .. import kernels
 
-__all__ = ["FP8Linear", "MXFP8Linear", "convert_to_fp8", "fp8_eligible", "use_tuned_gemms", "tune_gemms",
+__all__ = ["FP8Linear", "MXFP8Linear", "W4Linear", "convert_to_fp8", "convert_to_w4", "fp8_eligible", "use_tuned_gemms", "tune_gemms",
            "GEMM_TABLE"]
 
 # hipBLASLt solutions for the DiT's rowwise FP8 GEMMs at the chunk shape (6032 tokens), as a TunableOp results file (what
@@ -179,6 +179,58 @@ class MXFP8Linear(torch.nn.Module):
         if bias is not None:
             y = y + bias
         return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)
+
+
+class W4Linear(torch.nn.Module):
+    """4-bit replacement of an nn.Linear for the calls that are bound by their weights' bytes: one row (the time
+    embedding and the modulation it gives), a few sequences, a context's tokens. Codes of 4 bits with a bf16 scale for each `group`
+    columns (32, 64 or 128): fmt 'int4', with `zeros` a zero point for each group too, or 'fp4' (e2m1). Weights are
+    quantised once (lbw_quant_w4), a call is one kernel (lbw_gemm_w4) on bf16 or fp16 activations, other types cast to
+    bf16; out in that type. Codes are exact in the products and every scale, sum and the bias fp32. No gradient reaches the
+    input: a call that would record one is refused. A bias that records one is added after the kernel."""
+
+    def __init__(self, lin, group=128, fmt="int4", zeros=False):
+        super().__init__()
+        w = lin.weight.detach()
+        if w.dtype not in (torch.bfloat16, torch.float32):
+            w = w.float()
+        w4, scale, zero = kernels.quant_w4(w.contiguous(), group, fmt, zeros)
+        self.register_buffer("w4", w4)
+        self.register_buffer("w4_scale", scale)
+        self.register_buffer("w4_zero", zero)
+        self.bias = lin.bias
+        self.in_features, self.out_features, self.fmt = lin.in_features, lin.out_features, fmt
+
+    def forward(self, x):
+        shape = x.shape
+        if not _plain(x):
+            raise RuntimeError("W4Linear has no gradient with respect to its input: call it under torch.no_grad(), or on "
+                               "a detached input")
+        x2 = x.reshape(-1, shape[-1])
+        if x2.dtype not in (torch.bfloat16, torch.float16):
+            x2 = x2.to(torch.bfloat16)
+        if x2.shape[1] > 1 and x2.stride(1) != 1:
+            x2 = x2.contiguous()
+        bias = self.bias
+        if bias is not None:
+            bias = bias.to(x2.dtype)
+        fused = bias is None or (_plain(bias) and bias.is_contiguous())
+        y = kernels.gemm_w4(x2, self.w4, self.w4_scale, self.w4_zero, bias if fused else None, self.out_features,
+                            self.fmt)
+        if not fused:
+            y = y + bias
+        return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)
+
+
+def convert_to_w4(blocks, group=128, fmt="int4", zeros=False, min_features=1024):
+    """Replace every nn.Linear below `blocks` with both dimensions at least min_features by W4Linear, in place. Returns
+    (replaced, linears seen)."""
+    found = [(path, m) for path, m in blocks.named_modules() if path and isinstance(m, torch.nn.Linear)]
+    chosen = [(path, m) for path, m in found if min(m.in_features, m.out_features) >= min_features]
+    for path, m in chosen:
+        owner, _, attr = path.rpartition(".")
+        setattr(blocks.get_submodule(owner), attr, W4Linear(m, group, fmt, zeros))
+    return len(chosen), len(found)
 
 
 def fp8_eligible(lin, mx=False):
