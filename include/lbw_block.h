@@ -101,7 +101,7 @@ int lbw_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t l
  *          i = 0 .. 7; its nibble s holds i = s for LBW_W4_FP4 and i = 2 s (s < 4), 2 s - 7 (s >= 4) for LBW_W4_INT4
  *   scale  bf16  [nt][kt][16][128 / group]
  *   zero   uint8 [nt][kt][16][128 / group], LBW_W4_INT4 only, or null
- * A weight is scale * value. Rows and columns past n and k hold scale 0 where a whole group lies there, and any code.
+ * (All 16-byte aligned.) A weight is scale * value. Rows and columns past n and k hold scale 0 where a whole group lies there, and any code.
  *
  * lbw_quant_w4 makes them from w [n][k] (bf16, or fp32 when w_is_fp32; row stride s_row): scale = amax / 6 (fp4),
  * amax / 7 (int4 without zeros) or (max(x, 0) - min(x, 0)) / 15 (with zeros), rounded to bf16, codes to the nearest

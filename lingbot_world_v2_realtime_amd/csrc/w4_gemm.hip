@@ -14,6 +14,7 @@ namespace {
 
 constexpr int TN = 16, TK = 128;      // a tile of the stored weights
 constexpr int TILE_BYTES = TN * TK / 2;
+enum Form { INT4, INT4_ZEROS, FP4 };   // of the stored codes (the zeros' form apart: a load less, and no branch around it)
 
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -90,10 +91,10 @@ template <int DT>
 constexpr uint32_t ONES = DT == LBW_DTYPE_FP16 ? 0x3C003C00u : 0x3F803F80u;
 
 // The 8 codes of a word as 16-bit operands: integer codes as 1 + c / 16, fp4 codes as their values.
-template <int DT, bool FP4>
+template <int DT, Form F>
 __device__ __forceinline__ v4i operand(uint32_t w) {
   v4i r;
-  if constexpr (FP4) {
+  if constexpr (F == FP4) {
     if constexpr (DT == LBW_DTYPE_FP16) {
       r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 0));
       r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 1));
@@ -126,108 +127,372 @@ struct GemmArgs {
   void* out;
 };
 
-// x[row][col .. col + 8), zero past K; rows past M read row M - 1 (their results are dropped)
+// x from row m0 on, read 8 columns at a time. VEC: by buffer loads, a base for the workgroup and 32 bits of offset a lane (64-bit
+// addresses of 16 rows took 32 registers, spills, and more clocks than the products); what lies past the last row or past K
+// reads as zero by the buffer's bounds. Else value by value. Zero past K is needed: the tiles hold anything there.
 template <bool VEC>
-__device__ __forceinline__ v4i load_x(const GemmArgs& a, int64_t row, int64_t col) {
-  const uint16_t* p = (const uint16_t*)a.x + row * a.x_s_row;
-  if constexpr (VEC) {
-    return col < a.k ? *(const v4i*)(p + col) : v4i{0, 0, 0, 0};
+struct RowsOfX {
+  __amdgpu_buffer_rsrc_t rsrc;
+  const uint16_t* p;
+  int64_t rows, k, stride;
+  __device__ __forceinline__ RowsOfX(const GemmArgs& a, int64_t m0) {
+    rows = a.m - m0;
+    k = a.k;
+    stride = a.x_s_row;
+    p = (const uint16_t*)a.x + m0 * stride;
+    // (a workgroup reads 64 rows at most: 2^30 bytes)
+    const int64_t bytes = 2 * ((min(rows, (int64_t)64) - 1) * stride + k);
+    if constexpr (VEC) rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(uint32_t)bytes, 0x00020000);
+  }
+  // the offset of a lane that reads from row `row`: what load takes, with its column
+  __device__ __forceinline__ uint32_t offset(int row) const { return (uint32_t)(row * stride) * 2u; }
+  __device__ __forceinline__ v4i load(int row, uint32_t off, int64_t col) const {
+    if constexpr (VEC) {
+      const uint32_t at = col < k ? off + 2u * (uint32_t)col : 0xFFFFFFF0u;
+      return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+    } else {
+      v4i r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = row < rows;
+        const uint32_t lo = in && col + 2 * e < k ? p[row * stride + col + 2 * e] : 0u;
+        const uint32_t hi = in && col + 2 * e + 1 < k ? p[row * stride + col + 2 * e + 1] : 0u;
+        r[e] = (int)(lo | hi << 16);
+      }
+      return r;
+    }
+  }
+};
+
+// Four columns of the output from n on (a multiple of 4), with the bias: 8 bytes at once where the output's rows allow it.
+template <int DT>
+__device__ __forceinline__ void store_out(const GemmArgs& a, int64_t m, int64_t n, v4f y) {
+  if (a.n % 4 == 0) {
+    if (a.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += load1<DT>(a.bias, n + e);
+    }
+    *(v2i*)((uint16_t*)a.out + m * a.n + n) = v2i{(int)pack2<DT>(y[0], y[1]), (int)pack2<DT>(y[2], y[3])};
   } else {
-    v4i r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.n) store1<DT>(a.out, m * a.n + n + e, y[e] + (a.bias ? load1<DT>(a.bias, n + e) : 0.f));
+  }
+}
+
+// The scales (bf16) and zeros of a tile's rows 4 q .. 4 q + 3, the ones whose products a lane holds: 4 PER of each.
+template <Form F, int PER>
+struct Scales {
+  uint32_t s[2 * PER], z[PER];
+  template <int N>
+  static __device__ __forceinline__ void words(uint32_t* to, const void* p) {
+    if constexpr (N == 1) {
+      to[0] = *(const uint32_t*)p;
+    } else if constexpr (N == 2) {
+      const uint2 v = *(const uint2*)p;
+      to[0] = v.x;
+      to[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const uint4 v = ((const uint4*)p)[i / 4];
+        to[i] = v.x;
+        to[i + 1] = v.y;
+        to[i + 2] = v.z;
+        to[i + 3] = v.w;
+      }
+    }
+  }
+  // row: 16 times the tile's number and 4 q
+  __device__ __forceinline__ void load(const uint16_t* scale, const uint8_t* zero, int64_t row) {
+    words<2 * PER>(s, scale + PER * row);
+    if constexpr (F == INT4_ZEROS) words<PER>(z, zero + PER * row);
+  }
+  // what the sums of group g are multiplied by
+  __device__ __forceinline__ v4f scale_of(int g) const {
+    v4f r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t lo = col + 2 * e < a.k ? p[col + 2 * e] : 0u, hi = col + 2 * e + 1 < a.k ? p[col + 2 * e + 1] : 0u;
-      r[e] = (int)(lo | hi << 16);
+      const int i = PER * e + g;
+      r[e] = __uint_as_float(i & 1 ? s[i >> 1] & 0xFFFF0000u : s[i >> 1] << 16) * (F == FP4 ? 1.f : 16.f);
     }
     return r;
   }
+  // where they start, from the sum of x: the codes' offset -(16 + z) / 16 comes off (for z = 8 it has already been multiplied
+  // in, once for all columns)
+  __device__ __forceinline__ v4f start(int g, float sum) const {
+    v4f r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = PER * e + g;
+      r[e] = F == INT4_ZEROS ? sum * (-1.f - 0.0625f * (float)(z[i >> 2] >> 8 * (i & 3) & 0xFFu)) : sum;
+    }
+    return r;
+  }
+};
+
+// The sum of each of 16 rows of x over a group, from its operands (ones times them: every row of the result is the sums), as
+// Scales::start takes it.
+template <int DT, Form F, int STEPS>
+__device__ __forceinline__ float group_sum(const v4i* x) {
+  if constexpr (F == FP4) return 0.f;
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+  const v4i ones = {(int)ONES<DT>, (int)ONES<DT>, (int)ONES<DT>, (int)ONES<DT>};
+#pragma unroll
+  for (int j = 0; j < STEPS; ++j) sum = mfma<DT>(ones, x[j], sum);
+  return F == INT4 ? -1.5f * sum[0] : sum[0];
 }
 
-// 16 columns of the output and 16 MT rows a workgroup; its waves take the K tiles in turn and add their sums through LDS.
-template <int DT, bool FP4, int GROUP, int MT, bool VEC>
-__global__ __launch_bounds__(512) void w4_rows_kernel(GemmArgs a) {
-  constexpr int PER = TK / GROUP, STEPS = GROUP / 32;
-  extern __shared__ float part[];   // [waves][MT][256]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// Both kernels multiply weights by x transposed: a lane then holds 4 neighbouring columns of a row of the output, which
+// it stores at once, and one sum of x for them.
+
+// Few rows: 16 MT rows and 16 NT columns a workgroup. Its waves share out the K tiles (so that the few workgroups of a
+// narrow output still have loads in flight on every SIMD) and add their sums through LDS at the end. x comes in rows of 256
+// bytes, four a load, and is turned into operands through LDS, each wave in a part of its own (no barrier): loads in the
+// operands' own order, 16 rows of 64 bytes each, took 120 clocks apiece, all rows in one bank of the cache's tags. A row's
+// 16-byte pieces are exchanged by its number, so that 16 rows' pieces lie in all banks. The next tile's x and codes are in
+// flight while a tile is multiplied.
+template <int DT, Form F, int GROUP, int MT, int NT, int MOST, bool VEC>
+__global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
+  constexpr int PER = TK / GROUP, STEPS = GROUP / 32, ROWS = 16 * MT, COLS = TN * NT;
+  extern __shared__ __align__(16) char lds[];   // x: [waves][ROWS][256]; afterwards the sums: [waves][ROWS][COLS] fp32
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int r = lane & 15, q = lane >> 4;
-  const int64_t nt = blockIdx.x, m0 = (int64_t)blockIdx.y * 16 * MT;
-  int64_t row[MT];
-  v4f out[MT];
+  const int64_t m0 = (int64_t)blockIdx.y * ROWS, nt0 = (int64_t)blockIdx.x * NT, nts = (a.n + TN - 1) / TN;
+  char* mine = lds + wave * (ROWS * 256);
+  const RowsOfX<VEC> rows(a, m0);
+  const uint32_t off0 = rows.offset(q), four = rows.offset(4);
+  int64_t tile[NT];
+  v4f out[NT][MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    row[i] = min(m0 + 16 * i + r, a.m - 1);
-    out[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < NT; ++n) {
+    tile[n] = min(nt0 + n, nts - 1) * a.kt;   // (a tile past the last: read the last again, its results are dropped)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) out[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-  const v4i ones = {(int)ONES<DT>, (int)ONES<DT>, (int)ONES<DT>, (int)ONES<DT>};
-  for (int64_t t = wave; t < a.kt; t += waves) {
-    const int64_t tile = nt * a.kt + t;
-    const v4i w = *(const v4i*)(a.w4 + tile * TILE_BYTES + 16 * lane);
-    float s[PER], z[PER];
+  v4i w[NT], x[4 * MT];
+  Scales<F, PER> sc[NT];
+  const auto load = [&](int64_t t) {
 #pragma unroll
-    for (int g = 0; g < PER; ++g) {
-      s[g] = bf16_to_f32(a.scale[(tile * TN + r) * PER + g]);
-      z[g] = !FP4 && a.zero ? (float)a.zero[(tile * TN + r) * PER + g] : 8.f;
+    for (int n = 0; n < NT; ++n) {
+      w[n] = *(const v4i*)(a.w4 + (tile[n] + t) * TILE_BYTES + 16 * lane);
+      sc[n].load(a.scale, a.zero, (tile[n] + t) * TN + 4 * q);
     }
 #pragma unroll
+    for (int i = 0; i < 4 * MT; ++i) x[i] = rows.load(4 * i + q, off0 + i * four, t * TK + 8 * r);   // row 4 i + q
+  };
+  load(wave);   // (there are no more waves than tiles)
+  for (int64_t t = wave; t < a.kt; t += waves) {
+#pragma unroll
+    for (int i = 0; i < 4 * MT; ++i)
+      *(v4i*)(mine + (4 * i + q) * 256 + ((r ^ (4 * i + q) & 15) << 4)) = x[i];
+    v4i wc[NT];
+    Scales<F, PER> cc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      wc[n] = w[n];
+      cc[n] = sc[n];
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (t + waves < a.kt) load(t + waves);
+#pragma unroll
     for (int g = 0; g < PER; ++g) {
-      v4f acc[MT], sum[MT];
+      v4i xo[MT][STEPS];
+      float sum[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = sum[i] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < MT; ++i) {
 #pragma unroll
-      for (int j = 0; j < STEPS; ++j) {
-        const int st = g * STEPS + j;
-        const v4i b = operand<DT, FP4>((uint32_t)w[st]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const v4i x = load_x<VEC>(a, row[i], t * TK + 32 * st + 8 * q);
-          acc[i] = mfma<DT>(x, b, acc[i]);
-          if constexpr (!FP4) sum[i] = mfma<DT>(x, ones, sum[i]);
-        }
+        for (int j = 0; j < STEPS; ++j)
+          xo[i][j] = *(const v4i*)(mine + (16 * i + r) * 256 + (((4 * (g * STEPS + j) + q) ^ r) << 4));
+        sum[i] = group_sum<DT, F, STEPS>(xo[i]);
       }
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int n = 0; n < NT; ++n) {
+        const v4f s = cc[n].scale_of(g);
+        v4f acc[MT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (FP4) out[i][e] = fmaf(s[g], acc[i][e], out[i][e]);
-          else out[i][e] = fmaf(16.f * s[g], acc[i][e], fmaf(-s[g] * (16.f + z[g]), sum[i][e], out[i][e]));
+        for (int i = 0; i < MT; ++i) acc[i] = cc[n].start(g, sum[i]);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+          const v4i b = operand<DT, F>((uint32_t)wc[n][g * STEPS + j]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i] = mfma<DT>(b, xo[i][j], acc[i]);
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[n][i][e] = fmaf(s[e], acc[i][e], out[n][i][e]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();   // every wave has read its x
+  float* part = (float*)lds;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *(v4f*)(part + (wave * ROWS + 16 * i + r) * COLS + TN * n + 4 * q) = out[n][i];
+  __syncthreads();
+  for (int i = 4 * threadIdx.x; i < ROWS * COLS; i += 4 * blockDim.x) {
+    const int64_t m = m0 + i / COLS, n = nt0 * TN + i % COLS;
+    if (m >= a.m || n >= a.n) continue;
+    v4f y = *(const v4f*)(part + i);
+    for (int w = 1; w < waves; ++w) y += *(const v4f*)(part + w * (ROWS * COLS) + i);
+    store_out<DT>(a, m, n, y);
+  }
+}
+
+// Many rows: 64 rows x 256 columns a workgroup, four waves of 64 x 64, two workgroups a CU (which drift apart, so that one's
+// matrix work runs under the other's conversions: 57.5 us for 1508 x 8960 x 1536 against 62.7 with eight waves in step on 128 rows).
+// x passes through LDS, a K tile at a time in two buffers (rows and pieces as above): wave w loads rows 16 w .. 16 w + 15 in the
+// operands' own order, forms their sums over each group while they are in registers, and leaves both there. Codes go from
+// memory to registers, a tile ahead.
+constexpr int GM = 64, GN = 256;
+constexpr int X_TILE = GM * TK * 2;   // bytes
+
+template <int DT, Form F, int GROUP>
+__global__ __launch_bounds__(256, 2) void w4_gemm_kernel(GemmArgs a, int m_tiles) {
+  constexpr int PER = TK / GROUP, STEPS = GROUP / 32;
+  __shared__ __align__(16) char xs[2][X_TILE];
+  __shared__ float sums[2][PER][GM];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int r = lane & 15, q = lane >> 4;
+  // an XCD takes workgroups that follow each other down the rows: they read the same weights
+  const int total = gridDim.x, per_xcd = (total + 7) / 8;
+  const int id = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (id >= m_tiles * (int)((a.n + GN - 1) / GN)) return;
+  const int64_t m0 = (int64_t)(id % m_tiles) * GM, nt0 = (int64_t)(id / m_tiles) * (GN / TN) + 4 * wave;
+  const int64_t nts = (a.n + TN - 1) / TN;
+  const RowsOfX<true> rows(a, m0);
+  const uint32_t off = rows.offset(16 * wave + r);
+  int64_t tile[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) tile[n] = min(nt0 + n, nts - 1) * a.kt;
+  v4f out[4][4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  v4i xr[4], w[4];
+  Scales<F, PER> sc[4];
+  const auto load = [&](int64_t t) {
+#pragma unroll
+    for (int st = 0; st < 4; ++st) xr[st] = rows.load(16 * wave + r, off, t * TK + 32 * st + 8 * q);
+  };
+  const auto load_w = [&](int n, int64_t t) {
+    w[n] = *(const v4i*)(a.w4 + (tile[n] + t) * TILE_BYTES + 16 * lane);
+    sc[n].load(a.scale, a.zero, (tile[n] + t) * TN + 4 * q);
+  };
+  // this wave's 16 rows of x and their sums into buffer `to` (the four quarters of a wave hold the same sums)
+  const auto leave = [&](int to) {
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+      *(v4i*)(xs[to] + (16 * wave + r) * 256 + (((4 * st + q) ^ r) << 4)) = xr[st];
+    if constexpr (F != FP4) {
+#pragma unroll
+      for (int g = 0; g < PER; ++g) sums[to][g][16 * wave + r] = group_sum<DT, F, STEPS>(&xr[g * STEPS]);
+    }
+  };
+  load(0);
+#pragma unroll
+  for (int n = 0; n < 4; ++n) load_w(n, 0);
+  leave(0);
+  __syncthreads();
+  for (int64_t t = 0; t < a.kt; ++t) {
+    const int buf = (int)(t & 1);
+    const int64_t next = min(t + 1, a.kt - 1);   // (the last tile again at the end: no branch in the loop)
+#pragma unroll
+    for (int g = 0; g < PER; ++g) {
+      v4i x[4][STEPS];
+      float sum[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j)
+          x[i][j] = *(const v4i*)(xs[buf] + (16 * i + r) * 256 + (((4 * (g * STEPS + j) + q) ^ r) << 4));
+        sum[i] = F == FP4 ? 0.f : sums[buf][g][16 * i + r];
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const v4f s = sc[n].scale_of(g);
+        v4f acc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = sc[n].start(g, sum[i]);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+          const v4i b = operand<DT, F>((uint32_t)w[n][g * STEPS + j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = mfma<DT>(b, x[i][j], acc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[n][i][e] = fmaf(s[e], acc[i][e], out[n][i][e]);
+        if (g == PER - 1) load_w(n, next);   // into the registers just read: no second set
+        if (g == 0 && n == 0) {
+          // (not earlier, for its registers; and held here: the scheduler moves the loads down to where they are waited for)
+          __builtin_amdgcn_sched_barrier(0);
+          load(next);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);     // (or the groups' operands are all loaded at once, and spilled)
+    }
+    // the other buffer was last read before the barrier that ended the previous tile
+    leave(buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + 16 * i + r;
+    if (m >= a.m) continue;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int64_t col = (nt0 + n) * TN + 4 * q;
+      if (col < a.n) store_out<DT>(a, m, col, out[n][i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[(wave * MT + i) * 256 + (4 * q + e) * 16 + r] = out[i][e];
-  __syncthreads();
-  for (int i = threadIdx.x; i < MT * 256; i += blockDim.x) {
-    const int64_t m = m0 + (i >> 4), n = nt * TN + (i & 15);
-    if (m >= a.m || n >= a.n) continue;
-    float y = 0.f;
-    for (int w = 0; w < waves; ++w) y += part[w * MT * 256 + i];
-    if (a.bias) y += load1<DT>(a.bias, n);
-    store1<DT>(a.out, m * a.n + n, y);
-  }
 }
 
-template <int DT, bool FP4, int GROUP, int MT, bool VEC>
-void launch_rows(const GemmArgs& a, hipStream_t stream) {
-  const int waves = a.kt < 8 ? (int)a.kt : 8;
-  const dim3 grid((unsigned)((a.n + TN - 1) / TN), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
-  w4_rows_kernel<DT, FP4, GROUP, MT, VEC><<<grid, 64 * waves, waves * MT * 256 * sizeof(float), stream>>>(a);
+// `most` (at most MOST) waves
+template <int DT, Form F, int GROUP, int MT, int NT, int MOST, bool VEC>
+void launch_rows(const GemmArgs& a, int most, hipStream_t stream) {
+  // the fewest rounds of K tiles that `most` waves allow, in as few waves
+  const int64_t rounds = (a.kt + most - 1) / most;
+  const int waves = (int)((a.kt + rounds - 1) / rounds);
+  const dim3 grid((unsigned)((a.n + TN * NT - 1) / (TN * NT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
+  const int each = MT * (NT > 4 ? NT : 4) * 1024;   // bytes of LDS a wave needs
+  w4_rows_kernel<DT, F, GROUP, MT, NT, MOST, VEC><<<grid, 64 * waves, waves * each, stream>>>(a);
 }
 
-template <int DT, bool FP4, int GROUP>
+// Which kernel. Few rows are a matter of latency: the smallest tile whose workgroups all run at once, one a CU, since a second
+// round costs more than a larger tile, and a larger tile more than a part of the first round left empty (bf16, int4, groups of
+// 128; rows x columns x K, us):
+//   24 x 1536 x 8960:   16 x 16 tiles 7.3,  32 x 16 9.8,  32 x 48 19.6     32 x 8960 x 1536: 32 x 16 7.6, 32 x 48 6.0
+//   128 x 1536 x 8960:  32 x 16 17.3, 16 x 48 12.3, 32 x 48 17.8          256 x 1536 x 8960: 16 x 48 20.6, 32 x 48 18.1
+// With 32 x 48 tiles past one round two workgroups of four waves share a CU better than one of six (512 x 1536 x 8960: 28.6
+// against 34.4). Whole tiles of 64 x 256 win from more than half a tile a CU on: 256 x 8960 x 1536 (140 tiles) 20.7 against 22.1,
+// 512 x 8960 x 1536 (280) 30.7 against 40.0, but 1508 x 1536 x 8960 (144) 96 against 79.
+template <int DT, Form F, int GROUP>
 void launch_group(const GemmArgs& a, bool vec, hipStream_t stream) {
-  if (!vec) launch_rows<DT, FP4, GROUP, 2, false>(a, stream);
-  else if (a.m <= 16) launch_rows<DT, FP4, GROUP, 1, true>(a, stream);
-  else if (a.m <= 32) launch_rows<DT, FP4, GROUP, 2, true>(a, stream);
-  else launch_rows<DT, FP4, GROUP, 4, true>(a, stream);
+  const auto grid = [&](int rows, int cols) { return ((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols); };
+  constexpr int CUS = 256;
+  if (!vec) launch_rows<DT, F, GROUP, 2, 1, 8, false>(a, 8, stream);
+  else if (a.m <= 16) launch_rows<DT, F, GROUP, 1, 1, 8, true>(a, 8, stream);
+  else if (grid(32, 16) <= CUS) launch_rows<DT, F, GROUP, 2, 1, 8, true>(a, 8, stream);
+  else if (grid(16, 48) <= CUS) launch_rows<DT, F, GROUP, 1, 3, 8, true>(a, 8, stream);
+  else if (grid(GM, GN) < 160) launch_rows<DT, F, GROUP, 2, 3, 6, true>(a, grid(32, 48) <= CUS ? 6 : 4, stream);
+  else w4_gemm_kernel<DT, F, GROUP><<<(unsigned)((grid(GM, GN) + 7) / 8 * 8), 4 * GM, 0, stream>>>(a, (int)grid(GM, 1 << 30));
 }
 
-template <int DT, bool FP4>
+template <int DT, Form F>
 void launch_format(const GemmArgs& a, int64_t group, bool vec, hipStream_t stream) {
-  if (group == 32) launch_group<DT, FP4, 32>(a, vec, stream);
-  else if (group == 64) launch_group<DT, FP4, 64>(a, vec, stream);
-  else launch_group<DT, FP4, 128>(a, vec, stream);
+  if (group == 32) launch_group<DT, F, 32>(a, vec, stream);
+  else if (group == 64) launch_group<DT, F, 64>(a, vec, stream);
+  else launch_group<DT, F, 128>(a, vec, stream);
 }
 
 bool sizes_ok(int64_t n, int64_t k, int fmt, int64_t group) {
@@ -245,7 +510,8 @@ extern "C" int lbw_quant_w4(const void* w, int w_is_fp32, int64_t n, int64_t k, 
                             uint8_t* w4, uint16_t* scale, uint8_t* zero, void* stream) {
   if (!w || !w4 || !scale) return LBW_E_NULL;
   if (!sizes_ok(n, k, fmt, group) || (zero && fmt == LBW_W4_FP4)) return LBW_E_SHAPE;
-  if ((uintptr_t)w % (w_is_fp32 ? 4 : 2) || (uintptr_t)w4 % 16 || (uintptr_t)scale % 2) return LBW_E_ALIGN;
+  if ((uintptr_t)w % (w_is_fp32 ? 4 : 2) || (uintptr_t)w4 % 16 || (uintptr_t)scale % 16 || (uintptr_t)zero % 16)
+    return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const dim3 grid((unsigned)((k + TK - 1) / TK), (unsigned)((n + TN - 1) / TN));
   if (grid.y > 65535) return LBW_E_SHAPE;
@@ -261,14 +527,19 @@ extern "C" int lbw_gemm_w4(const void* x, int dtype, int64_t m, int64_t k, int64
   if (!sizes_ok(n, k, fmt, group) || (zero && fmt == LBW_W4_FP4) || m < 1 || m > (1 << 20) ||
       (dtype != LBW_DTYPE_BF16 && dtype != LBW_DTYPE_FP16))
     return LBW_E_SHAPE;
-  if ((uintptr_t)x % 2 || (uintptr_t)w4 % 16 || (uintptr_t)scale % 2 || (uintptr_t)bias % 2 || (uintptr_t)out % 2)
+  if ((uintptr_t)x % 2 || (uintptr_t)w4 % 16 || (uintptr_t)scale % 16 || (uintptr_t)zero % 16 || (uintptr_t)bias % 2 || (uintptr_t)out % 8)
     return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const GemmArgs a = {x, m, k, x_s_row, w4, scale, zero, n, (k + TK - 1) / TK, bias, out};
-  const bool vec = k % 8 == 0 && x_s_row % 8 == 0 && (uintptr_t)x % 16 == 0;
-  const bool fp4 = fmt == LBW_W4_FP4, half = dtype == LBW_DTYPE_FP16;
+  // (a workgroup's rows have to lie within the 32 bits of a buffer's offsets)
+  const bool vec = k % 8 == 0 && x_s_row % 8 == 0 && x_s_row >= 0 && x_s_row < (1 << 23) && (uintptr_t)x % 16 == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (half) fp4 ? launch_format<LBW_DTYPE_FP16, true>(a, group, vec, s) : launch_format<LBW_DTYPE_FP16, false>(a, group, vec, s);
-  else fp4 ? launch_format<LBW_DTYPE_BF16, true>(a, group, vec, s) : launch_format<LBW_DTYPE_BF16, false>(a, group, vec, s);
+  const auto by_form = [&](auto dt) {
+    if (fmt == LBW_W4_FP4) launch_format<dt.value, FP4>(a, group, vec, s);
+    else if (zero) launch_format<dt.value, INT4_ZEROS>(a, group, vec, s);
+    else launch_format<dt.value, INT4>(a, group, vec, s);
+  };
+  if (dtype == LBW_DTYPE_FP16) by_form(std::integral_constant<int, LBW_DTYPE_FP16>{});
+  else by_form(std::integral_constant<int, LBW_DTYPE_BF16>{});
   return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
 }

@@ -790,7 +790,7 @@ def gemm_w4(x, w4, scale, zero=None, bias=None, out_features=None, fmt="int4"):
     n = 16 * w4.shape[0] if out_features is None else int(out_features)
     group = 128 // scale.shape[-1] if scale.dim() == 4 and scale.shape[-1] in (1, 2, 4) else 0
     codes, scales = _w4_shapes(n, k, group)
-    if w4.dtype != torch.uint8 or tuple(w4.shape) != codes or not w4.is_contiguous() or w4.data_ptr() % 16:
+    if w4.dtype != torch.uint8 or tuple(w4.shape) != codes or not w4.is_contiguous():
         raise ValueError(f"w4 must be contiguous uint8 {codes} for {n} x {k}, got {w4.dtype} {tuple(w4.shape)}")
     if scale.dtype != torch.bfloat16 or tuple(scale.shape) != scales or not scale.is_contiguous():
         raise ValueError(f"scale must be contiguous bfloat16 {scales}, got {scale.dtype} {tuple(scale.shape)}")
@@ -799,6 +799,8 @@ def gemm_w4(x, w4, scale, zero=None, bias=None, out_features=None, fmt="int4"):
     if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
         raise ValueError(f"bias must be contiguous {x.dtype} ({n},), got {bias.dtype} {tuple(bias.shape)}")
     _same_device("gemm_w4", x, w4, scale, zero, bias)
+    # weights at an address the kernel does not load from (views of a larger buffer) as copies
+    w4, scale, zero = (t.clone() if t is not None and t.data_ptr() % 16 else t for t in (w4, scale, zero))
     out = torch.empty(m, n, dtype=x.dtype, device=x.device)
     if m == 0:
         return out

@@ -474,8 +474,11 @@ def _check_w4(m, n, k, group, fmt, zeros, dtype, bias, x=None):
     _within(out, (want, mag + want.abs()), f"{m}x{n}x{k} group {group} {fmt} {zeros} {dtype}", k / 16 + 24)
 
 
+# every kernel and tile, with rows, columns and K that end inside a tile: 16 x 16 (to 16 rows), 32 x 16, 16 x 48 and 32 x 48
+# (by the workgroups they give), 64 x 256 (from 160 of those on)
 W4_SIZES = [(1, 16, 128), (1, 1, 1), (3, 37, 300), (16, 64, 1536), (17, 48, 256), (33, 100, 520), (65, 130, 384),
-            (130, 257, 640), (300, 144, 1000), (2, 1536, 8960), (129, 16, 128)]
+            (130, 257, 640), (300, 144, 1000), (2, 1536, 8960), (129, 16, 128), (100, 1203, 264), (70, 4004, 392),
+            (300, 1601, 136), (450, 5204, 520), (1030, 2310, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", W4_SIZES)
@@ -504,14 +507,17 @@ def test_gemm_w4_strides():
     _check_w4(9, 48, 250, 64, "fp4", False, "bf16", True, x=wide[:9, :250])
     packed, _, _ = _w4(3, 48, 256, 64, "int4", True)
     assert kernels.gemm_w4(wide[:0, :256], *packed).shape == (0, 48)
+    # weights inside a larger buffer, at any address
+    moved = [torch.cat((t.flatten()[:1], t.flatten()))[1:].view(t.shape) for t in packed]
+    assert torch.equal(kernels.gemm_w4(wide[:, :256], *moved), kernels.gemm_w4(wide[:, :256], *packed))
 
 
 def test_gemm_w4_rows_do_not_mix():
     """A row's result is the same bits alone as among others of its kernel, and a NaN stays in its row."""
     from lingbot_world_v2_realtime_amd import kernels
     packed, _, _ = _w4(52, 64, 512, 128, "int4", True)
-    x = torch.randn(300, 512, device=DEV, generator=_rand(53)).bfloat16()
-    for m in (16, 64, 300):
+    for m in (16, 64, 300, 10240):
+        x = torch.randn(m, 512, device=DEV, generator=_rand(53)).bfloat16()
         clean = kernels.gemm_w4(x[:m], *packed)
         bad = x[:m].clone()
         bad[m // 2, 77] = float("nan")
