@@ -4,6 +4,7 @@ import ctypes
 import os
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "liblbw_attn.so")
+BLOCK_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_block.so")   # kernels.block_binding
 
 _i64, _i32, _f32, _p = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
 
@@ -68,7 +69,7 @@ def sources_sha16():
     from . import build
     here = os.path.dirname(os.path.abspath(__file__))
     files = [os.path.join(here, "csrc", f) for f in sorted(os.listdir(os.path.join(here, "csrc")))
-             if f.endswith((".hip", ".h"))]
+             if f.endswith((".hip", ".h", ".cpp"))]
     files += [os.path.join(os.path.dirname(here), "include", f) for f in ("lbw_attn.h", "lbw_block.h", "lbw_gemm.h")]
     h = hashlib.sha256(" ".join(build.HIPCC_FLAGS).encode())
     for f in files:

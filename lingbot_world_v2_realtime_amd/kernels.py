@@ -1,7 +1,6 @@
 """Thin torch-side wrappers over the C-ABI: device memory and the current stream come from torch, the work is
 done by the HIP kernels in liblbw_attn.so. Nothing here computes on the CPU."""
 import ctypes
-import functools
 import operator
 
 import torch
@@ -464,174 +463,51 @@ def gemm_fp8_mx(x8, x_scale_t, w8, w_scale_t, bias=None):
 
 # ---------------------------------------------------------------- the block around the attention
 
-ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # LBW_DTYPE_* of include/lbw_block.h
-NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 NORM_MAX_WIDTH = 12288
 ROTARY_MAX_DIM = 512
 W4_FORMATS = {"int4": 0, "fp4": 1}
 W4_GROUPS = (32, 64, 128)
+_NORM_INPUTS = ("x", "y", "gate", "shift", "scale", "weight", "bias", "post_weight")
 
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
-
-
-def _on_own_device(fn):
-    """The call made with its first tensor's device as the current one: a stream belongs to its device, and the kernels are
-    launched on the current device's."""
-    name = fn.__code__.co_varnames[0]
-
-    @functools.wraps(fn)
-    def call(*args, **kw):
-        idx = (args[0] if args else kw[name]).get_device()
-        if idx < 0 or idx == _current_device():
-            return fn(*args, **kw)
-        with torch.cuda.device(idx):
-            return fn(*args, **kw)
-    return call
+_BLOCK = None
 
 
-def _row_code(name, x):
-    code = ROW_DTYPES.get(x.dtype)
-    if code is None:
-        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
-    if not x.is_cuda:
-        raise ValueError(f"{name} must be a device tensor (the block operators have no CPU implementation)")
-    return code
+def block_binding():
+    """The native binding of the block operators (csrc/block_binding.cpp): their checks of arguments, outputs and launch."""
+    global _BLOCK
+    if _BLOCK is None:
+        _lib.load()
+        try:
+            from . import _block
+        except ImportError as e:
+            raise ImportError(f"{_lib.BLOCK_PATH} is missing or was built for another torch ({e}): build it with "
+                              "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+        _block.on_status(_lib.check)
+        _BLOCK = _block
+    return _BLOCK
 
 
-def _unit_stride(x):
-    return x.shape[-1] <= 1 or x.stride(-1) == 1
-
-
-def _norm_vectors(x, vectors, group_len):
-    """The norm's vectors (name -> tensor or None), checked against x [B, L, C]: their format code, their (pointer, batch
-    stride, row stride) by name, the modulation rows of an entry, and the tokens of one."""
-    b, n, c = x.shape
-    code = groups = None
-    out = {}
-    for name, v in vectors.items():
-        if v is None:
-            out[name] = (None, 0, 0)
-            continue
-        if code is None:
-            code = v.dtype
-        if v.dtype != code or v.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"the vectors must all be {x.dtype} or all float32, got {name} of {v.dtype}")
-        rows = name in ("gate", "shift", "scale") and v.dim() == 3
-        if not _unit_stride(v) or (tuple(v.shape) != (c,) and not (rows and v.shape[0] == b and v.shape[2] == c)):
-            raise ValueError(f"{name} must be [{c}]" + (f" or [{b}, rows, {c}]" if rows or v.dim() == 3 else "") +
-                             f" with contiguous channels, got {tuple(v.shape)} / {v.stride()}")
-        if not rows:
-            out[name] = (v.data_ptr(), 0, 0)
-            continue
-        if groups is not None and groups != v.shape[1]:
-            raise ValueError(f"modulation vectors with {groups} and {v.shape[1]} rows")
-        groups = v.shape[1]
-        out[name] = (v.data_ptr(), v.stride(0), v.stride(1))
-    if groups is None:
-        if group_len is not None:
-            raise ValueError("group_len is for modulation vectors with rows ([B, rows, C])")
-        return code, out, 1, max(n, 1)
-    if groups < 1:
-        raise ValueError("modulation vectors need a row at least")
-    if group_len is None:
-        group_len = max(-(-n // groups), 1)
-    if group_len < 1 or group_len * groups < n:
-        raise ValueError(f"{groups} modulation rows of {group_len} tokens do not cover {n} tokens")
-    return code, out, groups, group_len
-
-
-def _norm_inputs(x, y, vectors, group_len, norm, post_norm):
-    dtype = _row_code("x", x)
-    if x.dim() != 3 or not _unit_stride(x) or not 1 <= x.shape[2] <= NORM_MAX_WIDTH:
-        raise ValueError(f"x must be [B, L, C] with contiguous channels, C up to {NORM_MAX_WIDTH}, got "
-                         f"{tuple(x.shape)} / {x.stride()}")
-    if norm not in NORM_KINDS or post_norm not in NORM_KINDS:
-        raise ValueError(f"norm and post_norm must be 'layer', 'rms' or None, got {norm!r} / {post_norm!r}")
-    if y is not None:
-        if y.dtype != x.dtype:
-            raise TypeError(f"x ({x.dtype}) and y ({y.dtype}) must have one dtype")
-        if y.shape != x.shape or not _unit_stride(y):
-            raise ValueError(f"y {tuple(y.shape)} / {y.stride()} must be {tuple(x.shape)} with contiguous channels")
-    elif post_norm is not None or vectors["gate"] is not None or vectors["post_weight"] is not None:
-        raise ValueError("gate, post_norm and post_weight act on the branch: give y")
-    if norm is None:
-        if any(vectors[name] is not None for name in ("weight", "bias", "shift", "scale")):
-            raise ValueError("weight, bias, shift and scale follow the norm: give one")
-        if y is None:
-            raise ValueError("nothing to do: give y or a norm")
-    _same_device("gated_norm", x, y, *vectors.values())
-    vec, ptrs, groups, group_len = _norm_vectors(x, vectors, group_len)
-    return dtype, dtype if vec is None else ROW_DTYPES[vec], ptrs, groups, group_len
-
-
-@_on_own_device
 def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=None, post_weight=None, norm="layer",
                post_norm=None, eps=1e-6, residual_scale=1.0, branch_scale=1.0, group_len=None, want_stream=True):
     """s = residual_scale * x + branch_scale * gate * (post_norm(y) * post_weight), h = (norm(s) * weight + bias) *
     (1 + scale) + shift in one pass (lbw_gated_norm): (s or None, h or None). x, y [B, L, C] bf16, fp16 or fp32 with any
     strides of B and L; vectors of x's dtype or fp32, [C], the modulations also [B, rows, C] with group_len tokens a row
     (default: the rows share the tokens evenly). s is made where want_stream, h where there is a norm."""
-    dtype, vec, v, _, group_len = _norm_inputs(
-        x, y, {"gate": gate, "shift": shift, "scale": scale, "weight": weight, "bias": bias,
-               "post_weight": post_weight}, group_len, norm, post_norm)
-    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_stream or norm is None else None
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if norm is not None else None
-    b, n, c = x.shape
-    if b * n == 0:
-        return s, h
-    ys = y.stride() if y is not None else (0, 0)
-    st = _lib.load().lbw_gated_norm(
-        x.data_ptr(), _ptr(y), dtype, vec, b, n, c, x.stride(0), x.stride(1), ys[0], ys[1], *v["gate"], *v["shift"],
-        *v["scale"], group_len, v["weight"][0], v["bias"][0], v["post_weight"][0], NORM_KINDS[norm],
-        NORM_KINDS[post_norm], eps, residual_scale, branch_scale, _ptr(s), _ptr(h), _stream(x))
-    _lib.check(st, "lbw_gated_norm")
-    return s, h
+    return block_binding().gated_norm(x, y, gate, shift, scale, weight, bias, post_weight, norm, post_norm, eps,
+                                      residual_scale, branch_scale, group_len, want_stream)
 
 
-@_on_own_device
 def gated_norm_bwd(x, ds, dh, y=None, gate=None, shift=None, scale=None, weight=None, bias=None, post_weight=None,
                    norm="layer", post_norm=None, eps=1e-6, residual_scale=1.0, branch_scale=1.0, group_len=None,
-                   wants=("x", "y", "gate", "shift", "scale", "weight", "bias", "post_weight")):
+                   wants=_NORM_INPUTS):
     """The gradients of gated_norm (lbw_gated_norm_bwd) from those of its outputs (ds, dh [B, L, C] of x's dtype, either
     None): a dict name -> gradient of each given input named in `wants`, in its shape and dtype."""
-    vectors = {"gate": gate, "shift": shift, "scale": scale, "weight": weight, "bias": bias,
-               "post_weight": post_weight}
-    dtype, vec, v, groups, group_len = _norm_inputs(x, y, vectors, group_len, norm, post_norm)
-    for name, d in (("ds", ds), ("dh", dh)):
-        if d is not None and (d.dtype != x.dtype or d.shape != x.shape or not d.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {x.dtype} {tuple(x.shape)}, got {d.dtype} {tuple(d.shape)}")
-    _same_device("gated_norm_bwd", x, ds, dh)
-    b, n, c = x.shape
-    given = {"x": x, "y": y, **vectors}
-    names = [name for name in given if given[name] is not None and name in wants]
-    if ds is None and dh is None or b * n == 0:
-        return {name: torch.zeros(given[name].shape, dtype=given[name].dtype, device=x.device) for name in names}
-    grads = {}
-    for name in names:
-        # what only the norm's output depends on has no gradient without dh
-        idle = dh is None and name in ("shift", "scale", "weight", "bias")
-        new = torch.zeros if idle else torch.empty
-        grads[name] = new(given[name].shape, dtype=given[name].dtype, device=x.device)
-    ptr = {name: grads[name].data_ptr() if name in grads and not (
-        dh is None and name in ("shift", "scale", "weight", "bias")) else None for name in given}
-    lib = _lib.load()
-    ws = None
-    if any(ptr[name] is not None for name in vectors):
-        nbytes = lib.lbw_gated_norm_bwd_workspace_bytes(b, n, c, groups, group_len)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    rowwise = sum(bit for bit, t in ((1, gate), (2, shift), (4, scale)) if t is not None and t.dim() == 3)
-    ys = y.stride() if y is not None else (0, 0)
-    st = lib.lbw_gated_norm_bwd(
-        _ptr(ds), _ptr(dh), x.data_ptr(), _ptr(y), dtype, vec, b, n, c, x.stride(0), x.stride(1), ys[0], ys[1],
-        *v["gate"], *v["scale"], rowwise, groups, group_len, v["weight"][0], v["bias"][0],
-        v["post_weight"][0], NORM_KINDS[norm], NORM_KINDS[post_norm], eps, residual_scale, branch_scale, ptr["x"],
-        ptr["y"], ptr["gate"], ptr["shift"], ptr["scale"], ptr["weight"], ptr["bias"], ptr["post_weight"], _ptr(ws),
-        _stream(x))
-    _lib.check(st, "lbw_gated_norm_bwd")
-    return grads
+    bits = sum(1 << i for i, name in enumerate(_NORM_INPUTS) if name in wants)
+    grads = block_binding().gated_norm_bwd(x, y, gate, shift, scale, weight, bias, post_weight, norm, post_norm, eps,
+                                           residual_scale, branch_scale, group_len, ds, dh, bits)
+    return {name: g for name, g in zip(_NORM_INPUTS, grads) if g is not None}
 
 
-@_on_own_device
 def rotary(q, k, positions, freq, axis=None, pairs="interleaved", factor=1.0, layout="NHD", inverse=False,
            q_out=None, k_out=None):
     """q [B, L, Hq, D] and k [B, L, Hk, D] or None (HND: [B, H, L, D]; bf16, fp16 or fp32, any strides with contiguous
@@ -639,75 +515,7 @@ def rotary(q, k, positions, freq, axis=None, pairs="interleaved", factor=1.0, la
     [B, L], with several axes [L, axes] or [B, L, axes], or an int, the first token's position. freq: float64 [pairs],
     radians a position; axis: int32 [pairs], or None with one axis. pairs: 'interleaved' (channels 2 i, 2 i + 1) or
     'half' (i, pairs + i). inverse: the opposite rotation. The outputs may be the inputs themselves."""
-    lib = _lib.load()
-    dtype = _row_code("q", q)
-    b, n, hq, *qs = _dims(q, layout)
-    d = q.shape[3]
-    ks, hk = (0, 0, 0), 0
-    if k is not None:
-        if k.dtype != q.dtype:
-            raise TypeError(f"q ({q.dtype}) and k ({k.dtype}) must have one dtype")
-        kb, kn, hk, *ks = _dims(k, layout)
-        if (kb, kn, k.shape[3]) != (b, n, d):
-            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
-    elif k_out is not None:
-        raise ValueError("k_out without k")
-    if not _unit_stride(q) or (k is not None and not _unit_stride(k)):
-        raise ValueError("q and k must have contiguous channels")
-    if pairs not in ("interleaved", "half"):
-        raise ValueError(f"pairs must be 'interleaved' or 'half', got {pairs!r}")
-    if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous() or freq.shape[0] < 1:
-        raise ValueError(f"freq must be contiguous float64 [pairs], got {freq.dtype} {tuple(freq.shape)}")
-    if not 2 * freq.shape[0] <= d <= ROTARY_MAX_DIM:
-        raise ValueError(f"{freq.shape[0]} pairs do not fit heads of {d} (of {ROTARY_MAX_DIM} at most)")
-    if axis is not None and (axis.dtype != torch.int32 or axis.shape != freq.shape or not axis.is_contiguous()):
-        raise ValueError(f"axis must be contiguous int32 {tuple(freq.shape)}, got {axis.dtype} {tuple(axis.shape)}")
-    pos, ps, start, axes = None, (0, 0, 0), 0, 1
-    if isinstance(positions, torch.Tensor):
-        pos = positions
-        if pos.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"positions must be int32 or int64, got {pos.dtype}")
-        shape = tuple(pos.shape)
-        tail = () if axis is None else shape[-1:]
-        if shape not in ((n,) + tail, (b, n) + tail):
-            raise ValueError(f"positions must be [{n}] or [{b}, {n}]" + (" x axes" if axis is not None else "") +
-                             f", got {shape}")
-        st = pos.stride()
-        ps = (0, *st) if len(shape) == 1 + len(tail) else st
-        if axis is None:
-            ps = (*ps, 0)
-        else:
-            axes = shape[-1]
-            if axes < 1:
-                raise ValueError("positions need an axis at least")
-    elif axis is not None:
-        raise ValueError("several axes need a positions tensor")
-    else:
-        start = operator.index(positions)
-    outs = []
-    for name, x, o in (("q_out", q, q_out), ("k_out", k, k_out)):
-        if x is not None and o is None:
-            o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif x is not None and (o.dtype != x.dtype or o.shape != x.shape or not _unit_stride(o)):
-            raise ValueError(f"{name} must be {x.dtype} {tuple(x.shape)} with contiguous channels")
-        if x is not None and o.data_ptr() == x.data_ptr() and o.stride() != x.stride() and o.numel():
-            raise ValueError(f"{name} overlaps its input in another order")
-        if x is not None and any(st == 0 and size > 1 for st, size in zip(o.stride(), o.shape)):
-            raise ValueError(f"{name} has elements that share their memory")
-        outs.append(o)
-    _same_device("rotary", q, k, pos, freq, axis, *outs)
-    if q.numel() + (k.numel() if k is not None else 0) == 0:
-        return tuple(outs)
-    if hq < 1 or (k is not None and hk < 1):
-        raise ValueError("q and k need a head at least")
-    os_ = _dims(outs[0], layout)[3:]
-    ks_ = _dims(outs[1], layout)[3:] if k is not None else (0, 0, 0)
-    st = lib.lbw_rotary(q.data_ptr(), _ptr(k), dtype, b, n, hq, hk, d, freq.shape[0], *qs, *ks, _ptr(pos),
-                        int(pos is not None and pos.dtype == torch.int64), *ps, start, freq.data_ptr(), _ptr(axis),
-                        axes, int(pairs == "interleaved"), int(inverse), factor, outs[0].data_ptr(), _ptr(outs[1]),
-                        *os_, *ks_, _stream(q))
-    _lib.check(st, "lbw_rotary")
-    return tuple(outs)
+    return block_binding().rotary(q, k, positions, freq, axis, pairs, factor, layout, inverse, q_out, k_out)
 
 
 def _w4_shapes(n, k, group):
@@ -717,7 +525,6 @@ def _w4_shapes(n, k, group):
     return (nt, kt, 1024), (nt, kt, 16, 128 // group)
 
 
-@_on_own_device
 def quant_w4(w, group=128, fmt="int4", zeros=False):
     """4-bit codes of a weight [N, K] (bf16 or fp32, unit column stride) with a bf16 scale for each `group` columns
     (32, 64 or 128), in the tiles gemm_w4 takes (lbw_quant_w4): (w4 uint8 [N/16, K/128, 1024], scale bf16
@@ -727,7 +534,7 @@ def quant_w4(w, group=128, fmt="int4", zeros=False):
         raise ValueError("w must be a device tensor (the 4-bit path has no CPU implementation)")
     if w.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"w must be bfloat16 or float32, got {w.dtype}")
-    if w.dim() != 2 or not _unit_stride(w) or w.numel() == 0:
+    if w.dim() != 2 or w.numel() == 0 or (w.shape[1] > 1 and w.stride(1) != 1):
         raise ValueError(f"w must be [N, K] with contiguous rows, got {tuple(w.shape)} / {w.stride()}")
     if fmt not in W4_FORMATS or (zeros and fmt != "int4"):
         raise ValueError(f"fmt must be 'int4' or 'fp4' (zeros: 'int4' only), got {fmt!r}")
@@ -736,8 +543,9 @@ def quant_w4(w, group=128, fmt="int4", zeros=False):
     w4 = torch.empty(codes, dtype=torch.uint8, device=w.device)
     scale = torch.empty(scales, dtype=torch.bfloat16, device=w.device)
     zero = torch.empty(scales, dtype=torch.uint8, device=w.device) if zeros else None
-    st = _lib.load().lbw_quant_w4(w.data_ptr(), int(w.dtype == torch.float32), n, k, w.stride(0), W4_FORMATS[fmt],
-                                  group, w4.data_ptr(), scale.data_ptr(), _ptr(zero), _stream(w))
+    with torch.cuda.device(w.device):   # a stream belongs to its device, and kernels are launched on the current one
+        st = _lib.load().lbw_quant_w4(w.data_ptr(), int(w.dtype == torch.float32), n, k, w.stride(0),
+                                      W4_FORMATS[fmt], group, w4.data_ptr(), scale.data_ptr(), _ptr(zero), _stream(w))
     _lib.check(st, "lbw_quant_w4")
     return w4, scale, zero
 
@@ -772,42 +580,11 @@ def pack_w4(codes, scale, zero=None, fmt="int4"):
     return w4, per_tile(scale, torch.bfloat16), per_tile(zero, torch.uint8) if zero is not None else None
 
 
-@_on_own_device
 def gemm_w4(x, w4, scale, zero=None, bias=None, out_features=None, fmt="int4"):
     """x [M, K] (bf16 or fp16, unit column stride) times 4-bit weights [N, K] in the tiles of quant_w4 / pack_w4
     (lbw_gemm_w4), bias of x's dtype [N] or None -> [M, N] of x's dtype: codes exact, sums, scales and bias in fp32, one
     rounding. out_features: N where it is not a multiple of 16 (default: every row the tiles hold)."""
-    dtype = DTYPE_CODE.get(x.dtype)
-    if dtype is None:
-        raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
-    if not x.is_cuda:
-        raise ValueError("x must be a device tensor (the 4-bit path has no CPU implementation)")
-    if x.dim() != 2 or not _unit_stride(x) or x.shape[1] < 1:
-        raise ValueError(f"x must be [M, K] with contiguous rows, got {tuple(x.shape)} / {x.stride()}")
-    if fmt not in W4_FORMATS or (zero is not None and fmt != "int4"):
-        raise ValueError(f"fmt must be 'int4' or 'fp4' (zeros: 'int4' only), got {fmt!r}")
-    m, k = x.shape
-    n = 16 * w4.shape[0] if out_features is None else int(out_features)
-    group = 128 // scale.shape[-1] if scale.dim() == 4 and scale.shape[-1] in (1, 2, 4) else 0
-    codes, scales = _w4_shapes(n, k, group)
-    if w4.dtype != torch.uint8 or tuple(w4.shape) != codes or not w4.is_contiguous():
-        raise ValueError(f"w4 must be contiguous uint8 {codes} for {n} x {k}, got {w4.dtype} {tuple(w4.shape)}")
-    if scale.dtype != torch.bfloat16 or tuple(scale.shape) != scales or not scale.is_contiguous():
-        raise ValueError(f"scale must be contiguous bfloat16 {scales}, got {scale.dtype} {tuple(scale.shape)}")
-    if zero is not None and (zero.dtype != torch.uint8 or tuple(zero.shape) != scales or not zero.is_contiguous()):
-        raise ValueError(f"zero must be contiguous uint8 {scales}, got {zero.dtype} {tuple(zero.shape)}")
-    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
-        raise ValueError(f"bias must be contiguous {x.dtype} ({n},), got {bias.dtype} {tuple(bias.shape)}")
-    _same_device("gemm_w4", x, w4, scale, zero, bias)
-    # weights at an address the kernel does not load from (views of a larger buffer) as copies
-    w4, scale, zero = (t.clone() if t is not None and t.data_ptr() % 16 else t for t in (w4, scale, zero))
-    out = torch.empty(m, n, dtype=x.dtype, device=x.device)
-    if m == 0:
-        return out
-    st = _lib.load().lbw_gemm_w4(x.data_ptr(), dtype, m, k, x.stride(0), w4.data_ptr(), scale.data_ptr(), _ptr(zero),
-                                 W4_FORMATS[fmt], group, n, _ptr(bias), out.data_ptr(), _stream(x))
-    _lib.check(st, "lbw_gemm_w4")
-    return out
+    return block_binding().gemm_w4(x, w4, scale, zero, bias, out_features, fmt)
 
 
 _ATTN_WS = {}

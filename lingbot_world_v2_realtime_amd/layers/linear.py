@@ -203,7 +203,8 @@ class W4Linear(torch.nn.Module):
 
     def forward(self, x):
         shape = x.shape
-        if not _plain(x):
+        block = kernels.block_binding()
+        if not block.plain(x):
             raise RuntimeError("W4Linear has no gradient with respect to its input: call it under torch.no_grad(), or on "
                                "a detached input")
         x2 = x.reshape(-1, shape[-1])
@@ -214,9 +215,9 @@ class W4Linear(torch.nn.Module):
         bias = self.bias
         if bias is not None:
             bias = bias.to(x2.dtype)
-        fused = bias is None or (_plain(bias) and bias.is_contiguous())
-        y = kernels.gemm_w4(x2, self.w4, self.w4_scale, self.w4_zero, bias if fused else None, self.out_features,
-                            self.fmt)
+        fused = bias is None or (block.plain(bias) and bias.is_contiguous())
+        y = block.gemm_w4(x2, self.w4, self.w4_scale, self.w4_zero, bias if fused else None, self.out_features,
+                          self.fmt)
         if not fused:
             y = y + bias
         return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)

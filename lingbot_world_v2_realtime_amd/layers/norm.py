@@ -9,31 +9,23 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import kernels
-from .linear import _plain
 
 __all__ = ["gated_norm"]
 
-_VECTORS = ("gate", "shift", "scale", "weight", "bias", "post_weight")
-
-
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, opts, x, y, *vectors):
-        named = dict(zip(_VECTORS, vectors))
-        ctx.opts = {key: v for key, v in opts.items() if key != "want_stream"}
+    def forward(ctx, opts, *args):
+        ctx.opts = opts
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, y, *vectors)
-        return kernels.gated_norm(x, y, **named, **opts)
+        ctx.save_for_backward(*args)
+        return kernels.block_binding().gated_norm(*args, *opts, args[1] is not None)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, ds, dh):
-        x, y, *vectors = ctx.saved_tensors
-        names = ("x", "y") + _VECTORS
-        wants = [name for name, needed in zip(names, ctx.needs_input_grad[1:]) if needed]
+        wants = sum(1 << i for i, needed in enumerate(ctx.needs_input_grad[1:]) if needed)
         ds, dh = (d if d is None else d.contiguous() for d in (ds, dh))
-        grads = kernels.gated_norm_bwd(x, ds, dh, y, **dict(zip(_VECTORS, vectors)), **ctx.opts, wants=wants)
-        return (None, *(grads.get(name) for name in names))
+        return None, *kernels.block_binding().gated_norm_bwd(*ctx.saved_tensors, *ctx.opts, ds, dh, wants)
 
 
 def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=None, post_weight=None, norm="layer",
@@ -53,14 +45,15 @@ def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=N
     Differentiable in x, y and every vector (once: there is no second derivative). The backward reads x and y again and
     keeps nothing else; the sums over rows are in fp32 and in a fixed order.
     """
-    vectors = (gate, shift, scale, weight, bias, post_weight)
-    dtypes = {v.dtype for v in vectors if v is not None}
-    if len(dtypes) > 1:
-        vectors = tuple(v if v is None or v.dtype == torch.float32 else v.float() for v in vectors)
-    opts = {"norm": norm, "post_norm": post_norm, "eps": eps, "residual_scale": residual_scale,
-            "branch_scale": branch_scale, "group_len": group_len, "want_stream": y is not None}
-    if _plain(x, y, *vectors):
-        s, h = kernels.gated_norm(x, y, **dict(zip(_VECTORS, vectors)), **opts)
+    block = kernels.block_binding()
+    if block.mixed(gate, shift, scale, weight, bias, post_weight):
+        gate, shift, scale, weight, bias, post_weight = (
+            v if v is None or v.dtype == torch.float32 else v.float()
+            for v in (gate, shift, scale, weight, bias, post_weight))
+    args = (x, y, gate, shift, scale, weight, bias, post_weight)
+    opts = (norm, post_norm, eps, residual_scale, branch_scale, group_len)
+    if block.plain(*args):
+        s, h = block.gated_norm(*args, *opts, y is not None)
     else:
-        s, h = _GatedNorm.apply(opts, x, y, *vectors)
+        s, h = _GatedNorm.apply(opts, *args)
     return h if s is None else s if h is None else (s, h)

@@ -13,7 +13,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import kernels
-from .linear import _plain
 
 __all__ = ["Rotary", "rotary_embed", "grid_positions"]
 
@@ -108,9 +107,10 @@ def rotary_embed(q, k, positions, rope, tensor_layout="NHD", inplace=False):
     Channels past the plan's are copied. Angles are formed in 64 bits, the rotation in fp32, with one rounding.
     inplace: q and k are overwritten and returned (not where a gradient is recorded; every element must have memory of
     its own). Returns (q, k); differentiable in both."""
-    if _plain(q, k):
-        return kernels.rotary(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor, tensor_layout,
-                              q_out=q if inplace else None, k_out=k if inplace else None)
+    block = kernels.block_binding()
+    if block.plain(q, k):
+        return block.rotary(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor, tensor_layout, False,
+                            q if inplace else None, k if inplace else None)
     if inplace:
         raise ValueError("q and k cannot be rotated in place where a gradient is recorded")
     return _RotaryEmbed.apply(q, k, positions, rope, tensor_layout)
