@@ -14,9 +14,13 @@
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
+#include <algorithm>
 #include <array>
+#include <optional>
 #include <sstream>
 #include <string>
 
@@ -26,6 +30,9 @@
 namespace {
 
 using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Maybe = std::optional<Tensor>;
 
 PyObject* status_handler = nullptr;
 
@@ -117,12 +124,23 @@ struct On {
   explicit On(const Tensor& t) : guard(t.device().index()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-void done(int status, const char* what) {
+// A bad status: raised by the Python side's function, or, in a backward pass (which runs without the interpreter), as torch's error.
+void done(int status, const char* what, bool python = true) {
   if (status == LBW_OK) return;
+  TORCH_CHECK(python, what, " failed: status ", status, " (", lbw_status_string(status), ")");
   PyObject* r = status_handler ? PyObject_CallFunction(status_handler, "is", status, what) : nullptr;
   Py_XDECREF(r);
   if (PyErr_Occurred()) throw python_error();
   value_error(what, " failed: status ", status);
+}
+
+Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+
+// Whether autograd has to see the call: a gradient is recorded, or an input carries a forward-mode tangent (which it refuses).
+bool records_gradient(std::initializer_list<Tensor> ts) {
+  for (const Tensor& t : ts)
+    if (t.defined() && ((c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())) return true;
+  return false;
 }
 
 Tensor new_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }   // (packed, whatever t's strides)
@@ -157,96 +175,202 @@ int norm_kind(const char* name, PyObject* o) {
   value_error(name, " must be 'layer', 'rms' or None");
 }
 
-// The arguments of a norm and of its gradient: x, y, the vectors, norm, post_norm, eps, residual_scale, branch_scale, group_len.
-struct Norm {
-  static constexpr int ARGS = 2 + VECTORS + 6;
-  const Tensor &x, &y;
-  const Tensor* v[VECTORS];
-  int norm, post, dtype, vec_dtype;
+// The options of a norm: what its gradient needs besides the tensors.
+struct NormOptions : torch::CustomClassHolder {
+  int norm, post, dtype, vec_dtype, rowwise = 0;
   float eps, a, b;
   int64_t batch, len, width, groups = 1, group_len;
-  int rowwise = 0;
+};
 
-  explicit Norm(PyObject* const* o) : x(tensor("x", o[0])), y(tensor("y", o[1], true)) {
-    for (int i = 0; i < VECTORS; ++i) v[i] = &tensor(VECTOR_NAMES[i], o[2 + i], true);
-    o += 2 + VECTORS;
-    dtype = vec_dtype = row_format("x", x);
+struct Norm {
+  static constexpr int ARGS = 2 + VECTORS + 6;
+  Tensor x, y, v[VECTORS];
+  c10::intrusive_ptr<NormOptions> o;
+
+  Norm() = default;
+  // x, y, the vectors, norm, post_norm, eps, residual_scale, branch_scale, group_len, checked
+  explicit Norm(PyObject* const* args) : x(tensor("x", args[0])), y(tensor("y", args[1], true)), o(c10::make_intrusive<NormOptions>()) {
+    for (int i = 0; i < VECTORS; ++i) v[i] = tensor(VECTOR_NAMES[i], args[2 + i], true);
+    args += 2 + VECTORS;
+    o->dtype = o->vec_dtype = row_format("x", x);
     if (x.dim() != 3 || !unit_stride(x) || x.size(2) < 1 || x.size(2) > LBW_NORM_MAX_WIDTH)
       value_error("x must be [B, L, C] with contiguous channels, C up to ", LBW_NORM_MAX_WIDTH, ", got ", dims(x.sizes()), " / ",
                   dims(x.strides()));
-    batch = x.size(0), len = x.size(1), width = x.size(2);
-    norm = norm_kind("norm", o[0]), post = norm_kind("post_norm", o[1]);
-    eps = (float)number("eps", o[2]), a = (float)number("residual_scale", o[3]), b = (float)number("branch_scale", o[4]);
+    o->batch = x.size(0), o->len = x.size(1), o->width = x.size(2);
+    o->norm = norm_kind("norm", args[0]), o->post = norm_kind("post_norm", args[1]);
+    o->eps = (float)number("eps", args[2]), o->a = (float)number("residual_scale", args[3]);
+    o->b = (float)number("branch_scale", args[4]);
     if (y.defined()) {
       if (y.scalar_type() != x.scalar_type()) type_error("x (", x.scalar_type(), ") and y (", y.scalar_type(), ") must have one dtype");
       if (y.sizes() != x.sizes() || !unit_stride(y))
         value_error("y ", dims(y.sizes()), " / ", dims(y.strides()), " must be ", dims(x.sizes()), " with contiguous channels");
-    } else if (post || v[GATE]->defined() || v[POST_WEIGHT]->defined()) {
+    } else if (o->post || v[GATE].defined() || v[POST_WEIGHT].defined()) {
       value_error("gate, post_norm and post_weight act on the branch: give y");
     }
-    if (!norm) {
+    if (!o->norm) {
       for (int i : {WEIGHT, BIAS, SHIFT, SCALE})
-        if (v[i]->defined()) value_error("weight, bias, shift and scale follow the norm: give one");
+        if (v[i].defined()) value_error("weight, bias, shift and scale follow the norm: give one");
       if (!y.defined()) value_error("nothing to do: give y or a norm");
     }
-    same_device("gated_norm", x, y, *v[0], *v[1], *v[2], *v[3], *v[4], *v[5]);
+    same_device("gated_norm", x, y, v[0], v[1], v[2], v[3], v[4], v[5]);
     const Tensor* first = nullptr;
     int64_t rows = -1;
     for (int i = 0; i < VECTORS; ++i) {
-      const Tensor& t = *v[i];
+      const Tensor& t = v[i];
       if (!t.defined()) continue;
       const auto d = t.scalar_type();
       if ((d != x.scalar_type() && d != at::kFloat) || (first && d != first->scalar_type()))
         type_error("the vectors must all be ", x.scalar_type(), " or all float32, got ", VECTOR_NAMES[i], " of ", d);
       first = &t;
       const bool many = i <= SCALE && t.dim() == 3;
-      if (!unit_stride(t) || !(many ? t.size(0) == batch && t.size(2) == width : t.dim() == 1 && t.size(0) == width))
-        value_error(VECTOR_NAMES[i], " must be [", width, "]", i <= SCALE ? text(" or [", batch, ", rows, ", width, "]") : "",
-                    " with contiguous channels, got ", dims(t.sizes()), " / ", dims(t.strides()));
+      if (!unit_stride(t) || !(many ? t.size(0) == o->batch && t.size(2) == o->width : t.dim() == 1 && t.size(0) == o->width))
+        value_error(VECTOR_NAMES[i], " must be [", o->width, "]",
+                    i <= SCALE ? text(" or [", o->batch, ", rows, ", o->width, "]") : "", " with contiguous channels, got ",
+                    dims(t.sizes()), " / ", dims(t.strides()));
       if (!many) continue;
-      rowwise |= 1 << i;
+      o->rowwise |= 1 << i;
       if (rows >= 0 && rows != t.size(1)) value_error("modulation vectors with ", rows, " and ", t.size(1), " rows");
       rows = t.size(1);
     }
-    if (first) vec_dtype = row_format("vectors", *first);
-    group_len = o[5] == Py_None ? 0 : integer("group_len", o[5]);
+    if (first) o->vec_dtype = row_format("vectors", *first);
+    const int64_t len = o->len;
     if (rows < 0) {
-      if (o[5] != Py_None) value_error("group_len is for modulation vectors with rows ([B, rows, C])");
-      group_len = len > 0 ? len : 1;
+      if (args[5] != Py_None) value_error("group_len is for modulation vectors with rows ([B, rows, C])");
+      o->group_len = len > 0 ? len : 1;
       return;
     }
     if (rows < 1) value_error("modulation vectors need a row at least");
-    groups = rows;
-    if (o[5] == Py_None) group_len = std::max<int64_t>((len + rows - 1) / rows, 1);
-    // (a row may hold more tokens than there are: no overflow in the product)
-    if (group_len < 1 || (len + group_len - 1) / group_len > rows || group_len > (1 << 30))
-      value_error(rows, " modulation rows of ", group_len, " tokens do not cover ", len, " tokens");
+    o->groups = rows;
+    o->group_len = args[5] == Py_None ? std::max<int64_t>((len + rows - 1) / rows, 1) : integer("group_len", args[5]);
+    if (o->group_len < 1 || o->group_len > (1 << 30) || (len + o->group_len - 1) / o->group_len > rows)
+      value_error(rows, " modulation rows of ", o->group_len, " tokens do not cover ", len, " tokens");
   }
-  int64_t stride(int i, int dim) const { return rowwise >> i & 1 ? v[i]->stride(dim) : 0; }
-  bool empty() const { return batch * len == 0; }
+  int64_t stride(int i, int dim) const { return o->rowwise >> i & 1 ? v[i].stride(dim) : 0; }
+  bool empty() const { return o->batch * o->len == 0; }
+  int64_t y_stride(int dim) const { return y.defined() ? y.stride(dim) : 0; }
+
+  // (s or none, h or none)
+  std::array<Tensor, 2> forward(bool want_stream) const {
+    Tensor s = want_stream || !o->norm ? new_like(x) : Tensor(), h = o->norm ? new_like(x) : Tensor();
+    if (!empty()) {
+      const On on(x);
+      done(lbw_gated_norm(x.data_ptr(), ptr(y), o->dtype, o->vec_dtype, o->batch, o->len, o->width, x.stride(0), x.stride(1),
+                          y_stride(0), y_stride(1), ptr(v[GATE]), stride(GATE, 0), stride(GATE, 1), ptr(v[SHIFT]),
+                          stride(SHIFT, 0), stride(SHIFT, 1), ptr(v[SCALE]), stride(SCALE, 0), stride(SCALE, 1), o->group_len,
+                          ptr(v[WEIGHT]), ptr(v[BIAS]), ptr(v[POST_WEIGHT]), o->norm, o->post, o->eps, o->a, o->b, ptr(s),
+                          ptr(h), on.stream),
+           "lbw_gated_norm");
+    }
+    return {s, h};
+  }
+
+  // The gradients of x, y and the vectors, those with their bit in `wants`. ds and dh are packed, of x's type and shape.
+  std::array<Tensor, 2 + VECTORS> backward(const Tensor& ds, const Tensor& dh, int64_t wants, bool python) const {
+    std::array<Tensor, 2 + VECTORS> g;
+    void* p[2 + VECTORS] = {};
+    bool sums = false;
+    const bool none = (!ds.defined() && !dh.defined()) || empty();
+    for (int i = 0; i < 2 + VECTORS; ++i) {
+      const Tensor& t = i == 0 ? x : i == 1 ? y : v[i - 2];
+      if (!(wants >> i & 1) || !t.defined()) continue;
+      // what only the norm's output depends on has a gradient of zero without dh
+      const bool idle = none || (!dh.defined() && i >= 2 + SHIFT && i <= 2 + BIAS);
+      g[i] = idle ? at::zeros(t.sizes(), t.options()) : new_like(t);
+      if (idle) continue;
+      p[i] = g[i].data_ptr();
+      sums = sums || i >= 2;
+    }
+    if (none) return g;
+    const On on(x);
+    Tensor ws;
+    if (sums)
+      ws = at::empty({lbw_gated_norm_bwd_workspace_bytes(o->batch, o->len, o->width, o->groups, o->group_len)},
+                     x.options().dtype(at::kByte));
+    done(lbw_gated_norm_bwd(ptr(ds), ptr(dh), x.data_ptr(), ptr(y), o->dtype, o->vec_dtype, o->batch, o->len, o->width,
+                            x.stride(0), x.stride(1), y_stride(0), y_stride(1), ptr(v[GATE]), stride(GATE, 0), stride(GATE, 1),
+                            ptr(v[SCALE]), stride(SCALE, 0), stride(SCALE, 1), o->rowwise, o->groups, o->group_len,
+                            ptr(v[WEIGHT]), ptr(v[BIAS]), ptr(v[POST_WEIGHT]), o->norm, o->post, o->eps, o->a, o->b, p[0], p[1],
+                            p[2 + GATE], p[2 + SHIFT], p[2 + SCALE], p[2 + WEIGHT], p[2 + BIAS], p[2 + POST_WEIGHT], ptr(ws),
+                            on.stream),
+         "lbw_gated_norm_bwd", python);
+    return g;
+  }
 };
 
-PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  count(n, Norm::ARGS + 1);
-  const Norm a(args);
-  const bool want_stream = args[Norm::ARGS] == Py_True || !a.norm;
-  Tensor s = want_stream ? new_like(a.x) : Tensor(), h = a.norm ? new_like(a.x) : Tensor();
-  if (!a.empty()) {
-    const On on(a.x);
-    done(lbw_gated_norm(a.x.data_ptr(), ptr(a.y), a.dtype, a.vec_dtype, a.batch, a.len, a.width, a.x.stride(0), a.x.stride(1),
-                        a.y.defined() ? a.y.stride(0) : 0, a.y.defined() ? a.y.stride(1) : 0, ptr(*a.v[GATE]), a.stride(GATE, 0),
-                        a.stride(GATE, 1), ptr(*a.v[SHIFT]), a.stride(SHIFT, 0), a.stride(SHIFT, 1), ptr(*a.v[SCALE]),
-                        a.stride(SCALE, 0), a.stride(SCALE, 1), a.group_len, ptr(*a.v[WEIGHT]), ptr(*a.v[BIAS]),
-                        ptr(*a.v[POST_WEIGHT]), a.norm, a.post, a.eps, a.a, a.b, ptr(s), ptr(h), on.stream),
-         "lbw_gated_norm");
+struct NormFunction : torch::autograd::Function<NormFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& y, const Maybe&, const Maybe&, const Maybe&,
+                               const Maybe&, const Maybe&, const Maybe&, const Norm* a) {
+    ctx->set_materialize_grads(false);
+    variable_list kept = {a->x, a->y};
+    kept.insert(kept.end(), a->v, a->v + VECTORS);
+    ctx->save_for_backward(kept);
+    ctx->saved_data["options"] = c10::IValue::make_capsule(a->o);
+    variable_list out;
+    for (const Tensor& t : a->forward(a->y.defined()))
+      if (t.defined()) out.push_back(t);
+    return out;
   }
-  return wrap_all(std::array<Tensor, 2>{s, h});
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!c10::GradMode::is_enabled(), "gated_norm has no second derivative");
+    const variable_list kept = ctx->get_saved_variables();
+    Norm a;
+    a.x = kept[0], a.y = kept[1];
+    for (int i = 0; i < VECTORS; ++i) a.v[i] = kept[2 + i];
+    a.o = c10::static_intrusive_pointer_cast<NormOptions>(ctx->saved_data["options"].toCapsule());
+    int64_t wants = 0, edge = 0;
+    for (int i = 0; i < 2 + VECTORS; ++i)
+      if (kept[i].defined() && ctx->needs_input_grad(edge++)) wants |= 1 << i;
+    for (Tensor& d : grads)
+      if (d.defined()) d = d.contiguous();
+    const bool both = grads.size() == 2;
+    const Tensor ds = both || !a.o->norm ? grads[0] : Tensor(), dh = both ? grads[1] : a.o->norm ? grads[0] : Tensor();
+    const auto g = a.backward(ds, dh, wants, false);
+    variable_list out(g.begin(), g.end());
+    out.emplace_back();   // the call itself
+    return out;
+  }
+};
+
+// The operator as users call it: (s or None, h or None), with a gradient where one is recorded. Vectors of different types are taken
+// in fp32.
+PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, Norm::ARGS);
+  std::array<PyObject*, Norm::ARGS> own;
+  std::array<THPObjectPtr, VECTORS> held;
+  std::copy(args, args + Norm::ARGS, own.begin());
+  const auto type = tensor("x", args[0]).scalar_type();
+  bool half = false, full = false;
+  for (int i = 2; i < 2 + VECTORS; ++i) {
+    if (!THPVariable_Check(args[i])) continue;
+    const auto d = THPVariable_Unpack(args[i]).scalar_type();
+    half = half || d == type;
+    full = full || d == at::kFloat;
+  }
+  for (int i = 2; half && full && i < 2 + VECTORS; ++i) {   // (other types stay, and are refused below)
+    if (!THPVariable_Check(args[i]) || THPVariable_Unpack(args[i]).scalar_type() != type) continue;
+    held[i - 2] = THPVariable_Wrap(THPVariable_Unpack(args[i]).to(at::kFloat));
+    own[i] = held[i - 2].get();
+  }
+  const Norm a(own.data());
+  if (!records_gradient({a.x, a.y, a.v[0], a.v[1], a.v[2], a.v[3], a.v[4], a.v[5]}))
+    return wrap_all(a.forward(a.y.defined()));
+  const auto out = NormFunction::apply(a.x, maybe(a.y), maybe(a.v[0]), maybe(a.v[1]), maybe(a.v[2]), maybe(a.v[3]),
+                                       maybe(a.v[4]), maybe(a.v[5]), &a);
+  return wrap_all(std::array<Tensor, 2>{a.y.defined() ? out.front() : Tensor(), a.o->norm ? out.back() : Tensor()});
   END_HANDLE_TH_ERRORS
 }
 
-// After the norm's arguments: ds, dh, and which of x, y and the vectors want a gradient (a bit each). A tuple of those, None
-// for the others.
+// The forward alone: the norm's arguments, and whether the stream is wanted.
+PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, Norm::ARGS + 1);
+  return wrap_all(Norm(args).forward(args[Norm::ARGS] == Py_True));
+  END_HANDLE_TH_ERRORS
+}
+
+// The gradients alone: the norm's arguments, ds, dh, and a bit for each of x, y and the vectors. A tuple of those, None for the
+// others.
 PyObject* gated_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, Norm::ARGS + 3);
@@ -257,93 +381,164 @@ PyObject* gated_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (d.defined() && (d.scalar_type() != a.x.scalar_type() || d.sizes() != a.x.sizes() || !d.is_contiguous()))
       value_error(name, " must be contiguous ", a.x.scalar_type(), " ", dims(a.x.sizes()), ", got ", d.scalar_type(), " ",
                   dims(d.sizes()));
-  if (dh.defined() && !a.norm) value_error("dh without a norm");
+  if (dh.defined() && !a.o->norm) value_error("dh without a norm");
   same_device("gated_norm_bwd", a.x, ds, dh);
-  std::array<Tensor, 2 + VECTORS> g;
-  void* p[2 + VECTORS] = {};
-  bool sums = false;
-  const bool none = (!ds.defined() && !dh.defined()) || a.empty();
-  for (int i = 0; i < 2 + VECTORS; ++i) {
-    const Tensor& t = i == 0 ? a.x : i == 1 ? a.y : *a.v[i - 2];
-    if (!(wants >> i & 1) || !t.defined()) continue;
-    // what only the norm's output depends on has a gradient of zero without dh
-    const bool idle = none || (!dh.defined() && i >= 2 + SHIFT && i <= 2 + BIAS);
-    g[i] = idle ? at::zeros(t.sizes(), t.options()) : new_like(t);
-    if (idle) continue;
-    p[i] = g[i].data_ptr();
-    sums = sums || i >= 2;
-  }
-  if (!none) {
-    const On on(a.x);
-    Tensor ws;
-    if (sums)
-      ws = at::empty({lbw_gated_norm_bwd_workspace_bytes(a.batch, a.len, a.width, a.groups, a.group_len)},
-                     a.x.options().dtype(at::kByte));
-    done(lbw_gated_norm_bwd(ptr(ds), ptr(dh), a.x.data_ptr(), ptr(a.y), a.dtype, a.vec_dtype, a.batch, a.len, a.width, a.x.stride(0),
-                            a.x.stride(1), a.y.defined() ? a.y.stride(0) : 0, a.y.defined() ? a.y.stride(1) : 0, ptr(*a.v[GATE]),
-                            a.stride(GATE, 0), a.stride(GATE, 1), ptr(*a.v[SCALE]), a.stride(SCALE, 0), a.stride(SCALE, 1),
-                            a.rowwise, a.groups, a.group_len, ptr(*a.v[WEIGHT]), ptr(*a.v[BIAS]), ptr(*a.v[POST_WEIGHT]), a.norm,
-                            a.post, a.eps, a.a, a.b, p[0], p[1], p[2 + GATE], p[2 + SHIFT], p[2 + SCALE], p[2 + WEIGHT],
-                            p[2 + BIAS], p[2 + POST_WEIGHT], ptr(ws), on.stream),
-         "lbw_gated_norm_bwd");
-  }
-  return wrap_all(g);
+  return wrap_all(a.backward(ds, dh, wants, true));
   END_HANDLE_TH_ERRORS
 }
 
 // ---------------------------------------------------------------- rotary
 
-// q, k, positions, freq, axis, pairs, factor, layout, inverse, q_out, k_out
+struct RotaryOptions : torch::CustomClassHolder {
+  int64_t start = 0;
+  double factor = 1.0;
+  bool interleaved = true, nhd = true;
+};
+
+struct Rotary {
+  Tensor q, k, pos, freq, axis;
+  c10::intrusive_ptr<RotaryOptions> o;
+
+  Rotary() = default;
+  // q, k, positions, freq, axis, pairs, factor, layout, checked
+  explicit Rotary(PyObject* const* args)
+      : q(tensor("q", args[0])), k(tensor("k", args[1], true)), freq(tensor("freq", args[3])), axis(tensor("axis", args[4], true)),
+        o(c10::make_intrusive<RotaryOptions>()) {
+    row_format("q", q);
+    const std::string layout = word("layout", args[7]), pairs = word("pairs", args[5]);
+    if (layout != "NHD" && layout != "HND") value_error("tensor_layout must be 'NHD' or 'HND', got '", layout, "'");
+    o->nhd = layout == "NHD";
+    if (pairs != "interleaved" && pairs != "half") value_error("pairs must be 'interleaved' or 'half', got '", pairs, "'");
+    o->interleaved = pairs == "interleaved";
+    o->factor = number("factor", args[6]);
+    for (const Tensor* t : {&q, &k}) {
+      if (!t->defined()) continue;
+      if (t->dim() != 4) value_error("expected a 4-d tensor, got shape ", dims(t->sizes()));
+      if (!unit_stride(*t)) value_error("q and k must have contiguous channels");
+    }
+    const int64_t b = q.size(0), len = q.size(tok()), d = q.size(3);
+    if (k.defined()) {
+      if (k.scalar_type() != q.scalar_type())
+        type_error("q (", q.scalar_type(), ") and k (", k.scalar_type(), ") must have one dtype");
+      if (k.size(0) != b || k.size(tok()) != len || k.size(3) != d)
+        value_error("q ", dims(q.sizes()), " and k ", dims(k.sizes()), " do not match");
+    }
+    if (q.numel() + (k.defined() ? k.numel() : 0) > 0 && (q.size(head()) < 1 || (k.defined() && k.size(head()) < 1)))
+      value_error("q and k need a head at least");
+    if (freq.scalar_type() != at::kDouble || freq.dim() != 1 || !freq.is_contiguous() || freq.size(0) < 1)
+      value_error("freq must be contiguous float64 [pairs], got ", freq.scalar_type(), " ", dims(freq.sizes()));
+    if (2 * freq.size(0) > d || d > LBW_ROTARY_MAX_DIM)
+      value_error(freq.size(0), " pairs do not fit heads of ", d, " (of ", LBW_ROTARY_MAX_DIM, " at most)");
+    if (axis.defined() && (axis.scalar_type() != at::kInt || axis.sizes() != freq.sizes() || !axis.is_contiguous()))
+      value_error("axis must be contiguous int32 ", dims(freq.sizes()), ", got ", axis.scalar_type(), " ", dims(axis.sizes()));
+    if (THPVariable_Check(args[2])) {
+      pos = tensor("positions", args[2]);
+      if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong)
+        type_error("positions must be int32 or int64, got ", pos.scalar_type());
+      const int64_t own = own_dims();
+      if (!((own == 1 && pos.size(0) == len) || (own == 2 && pos.size(0) == b && pos.size(1) == len)))
+        value_error("positions must be [", len, "] or [", b, ", ", len, "]", axis.defined() ? " x axes" : "", ", got ",
+                    dims(pos.sizes()));
+      if (axis.defined() && pos.size(own) < 1) value_error("positions need an axis at least");
+    } else {
+      if (axis.defined()) value_error("several axes need a positions tensor");
+      o->start = integer("positions", args[2]);
+    }
+    same_device("rotary", q, k, pos, freq, axis);
+  }
+  int tok() const { return o->nhd ? 1 : 2; }
+  int head() const { return o->nhd ? 2 : 1; }
+  int64_t own_dims() const { return pos.dim() - (axis.defined() ? 1 : 0); }   // of positions, without an axis dimension behind
+
+  void run(const Tensor& qo, const Tensor& ko, bool inverse, bool python) const {
+    if (q.numel() + (k.defined() ? k.numel() : 0) == 0) return;
+    const int64_t own = pos.defined() ? own_dims() : 0;
+    const auto st = [&](const Tensor& t, int dim) { return t.defined() ? t.stride(dim) : 0; };
+    const On on(q);
+    done(lbw_rotary(q.data_ptr(), ptr(k), row_format("q", q), q.size(0), q.size(tok()), q.size(head()),
+                    k.defined() ? k.size(head()) : 0, q.size(3), freq.size(0), st(q, 0), st(q, tok()), st(q, head()), st(k, 0),
+                    st(k, tok()), st(k, head()), ptr(pos), pos.defined() && pos.scalar_type() == at::kLong,
+                    own == 2 ? pos.stride(0) : 0, own ? pos.stride(own - 1) : 0, own && axis.defined() ? pos.stride(own) : 0,
+                    o->start, (const double*)freq.data_ptr(), (const int32_t*)ptr(axis),
+                    own && axis.defined() ? pos.size(own) : 1, o->interleaved, inverse, (float)o->factor, qo.data_ptr(), ptr(ko),
+                    st(qo, 0), st(qo, tok()), st(qo, head()), st(ko, 0), st(ko, tok()), st(ko, head()), on.stream),
+         "lbw_rotary", python);
+  }
+  // into new tensors
+  std::array<Tensor, 2> fresh(bool inverse, bool python) const {
+    const std::array<Tensor, 2> out = {new_like(q), k.defined() ? new_like(k) : Tensor()};
+    run(out[0], out[1], inverse, python);
+    return out;
+  }
+};
+
+// A tensor written in place: a graph that kept it notices.
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Maybe& k, const Rotary* a) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({a->pos, a->freq, a->axis});
+    ctx->saved_data["options"] = c10::IValue::make_capsule(a->o);
+    ctx->saved_data["k"] = a->k.defined();
+    const auto out = a->fresh(false, true);
+    return a->k.defined() ? variable_list{out[0], out[1]} : variable_list{out[0]};
+  }
+  // the opposite rotation of whichever gradients there are (one rotation takes any number of heads)
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!c10::GradMode::is_enabled(), "rotary_embed has no second derivative");
+    const variable_list kept = ctx->get_saved_variables();
+    Rotary a;
+    a.pos = kept[0], a.freq = kept[1], a.axis = kept[2];
+    a.o = c10::static_intrusive_pointer_cast<RotaryOptions>(ctx->saved_data["options"].toCapsule());
+    Tensor d[2];
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined() && ctx->needs_input_grad(i)) d[i] = unit_stride(grads[i]) ? grads[i] : grads[i].contiguous();
+    variable_list out(3);
+    if (!d[0].defined() && !d[1].defined()) return out;
+    const bool q = d[0].defined();
+    a.q = q ? d[0] : d[1];
+    if (q) a.k = d[1];
+    const auto g = a.fresh(true, false);
+    if (q) out[0] = g[0];
+    out[1] = q ? g[1] : g[0];
+    return out;
+  }
+};
+
+// The operator as users call it: q, k, positions, freq, axis, pairs, factor, layout, inplace. (q, k or None), with a gradient where
+// one is recorded.
+PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 9);
+  const Rotary a(args);
+  const bool grad = records_gradient({a.q, a.k});
+  if (args[8] == Py_True) {
+    if (grad) value_error("q and k cannot be rotated in place where a gradient is recorded");
+    for (const Tensor* t : {&a.q, &a.k})
+      for (int j = 0; t->defined() && j < 4; ++j)
+        if (t->stride(j) == 0 && t->size(j) > 1) value_error("q or k has elements that share their memory");
+    a.run(a.q, a.k, false, true);
+    written(a.q);
+    written(a.k);
+    return wrap_all(std::array<Tensor, 2>{a.q, a.k});
+  }
+  if (!grad) return wrap_all(a.fresh(false, true));
+  const auto out = RotaryFunction::apply(a.q, maybe(a.k), &a);
+  return wrap_all(std::array<Tensor, 2>{out[0], a.k.defined() ? out[1] : Tensor()});
+  END_HANDLE_TH_ERRORS
+}
+
+// The rotation alone: q, k, positions, freq, axis, pairs, factor, layout, inverse, q_out, k_out.
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 11);
-  const Tensor &q = tensor("q", args[0]), &k = tensor("k", args[1], true);
-  const Tensor &freq = tensor("freq", args[3]), &axis = tensor("axis", args[4], true);
-  const int dtype = row_format("q", q);
-  const std::string layout = word("layout", args[7]), pairs = word("pairs", args[5]);
-  if (layout != "NHD" && layout != "HND") value_error("tensor_layout must be 'NHD' or 'HND', got '", layout, "'");
-  const int tok = layout == "NHD" ? 1 : 2, head = 3 - tok;
-  for (const Tensor* t : {&q, &k}) {
-    if (!t->defined()) continue;
-    if (t->dim() != 4) value_error("expected a 4-d tensor, got shape ", dims(t->sizes()));
-    if (!unit_stride(*t)) value_error("q and k must have contiguous channels");
-  }
-  const int64_t b = q.size(0), len = q.size(tok), d = q.size(3);
-  if (k.defined()) {
-    if (k.scalar_type() != q.scalar_type()) type_error("q (", q.scalar_type(), ") and k (", k.scalar_type(), ") must have one dtype");
-    if (k.size(0) != b || k.size(tok) != len || k.size(3) != d)
-      value_error("q ", dims(q.sizes()), " and k ", dims(k.sizes()), " do not match");
-  }
-  if (pairs != "interleaved" && pairs != "half") value_error("pairs must be 'interleaved' or 'half', got '", pairs, "'");
-  if (freq.scalar_type() != at::kDouble || freq.dim() != 1 || !freq.is_contiguous() || freq.size(0) < 1)
-    value_error("freq must be contiguous float64 [pairs], got ", freq.scalar_type(), " ", dims(freq.sizes()));
-  if (2 * freq.size(0) > d || d > LBW_ROTARY_MAX_DIM)
-    value_error(freq.size(0), " pairs do not fit heads of ", d, " (of ", LBW_ROTARY_MAX_DIM, " at most)");
-  if (axis.defined() && (axis.scalar_type() != at::kInt || axis.sizes() != freq.sizes() || !axis.is_contiguous()))
-    value_error("axis must be contiguous int32 ", dims(freq.sizes()), ", got ", axis.scalar_type(), " ", dims(axis.sizes()));
-  const bool given = THPVariable_Check(args[2]);
-  const Tensor& pos = given ? tensor("positions", args[2]) : absent;
-  int64_t ps[3] = {0, 0, 0}, start = 0, axes = 1;
-  if (given) {
-    if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong)
-      type_error("positions must be int32 or int64, got ", pos.scalar_type());
-    const int64_t own = pos.dim() - (axis.defined() ? 1 : 0);   // [L] or [B, L], with an axis dimension behind
-    if (!((own == 1 && pos.size(0) == len) || (own == 2 && pos.size(0) == b && pos.size(1) == len)))
-      value_error("positions must be [", len, "] or [", b, ", ", len, "]", axis.defined() ? " x axes" : "", ", got ", dims(pos.sizes()));
-    ps[0] = own == 2 ? pos.stride(0) : 0;
-    ps[1] = pos.stride(own - 1);
-    if (axis.defined()) {
-      ps[2] = pos.stride(own);
-      axes = pos.size(own);
-      if (axes < 1) value_error("positions need an axis at least");
-    }
-  } else {
-    if (axis.defined()) value_error("several axes need a positions tensor");
-    start = integer("positions", args[2]);
-  }
+  const Rotary a(args);
   std::array<Tensor, 2> out;
   for (int i = 0; i < 2; ++i) {
-    const Tensor &x = i ? k : q, &o = tensor(i ? "k_out" : "q_out", args[9 + i], true);
+    const Tensor &x = i ? a.k : a.q, &o = tensor(i ? "k_out" : "q_out", args[9 + i], true);
     const char* name = i ? "k_out" : "q_out";
     if (!x.defined()) {
       if (o.defined()) value_error("k_out without k");
@@ -358,19 +553,10 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (o.numel() && o.data_ptr() == x.data_ptr() && o.strides() != x.strides())
       value_error(name, " overlaps its input in another order");
   }
-  same_device("rotary", q, k, pos, freq, axis, out[0], out[1]);
-  if (q.numel() + (k.defined() ? k.numel() : 0) > 0) {
-    if (q.size(head) < 1 || (k.defined() && k.size(head) < 1)) value_error("q and k need a head at least");
-    const On on(q);
-    const auto st = [&](const Tensor& t, int dim) { return t.defined() ? t.stride(dim) : 0; };
-    done(lbw_rotary(q.data_ptr(), ptr(k), dtype, b, len, q.size(head), k.defined() ? k.size(head) : 0, d, freq.size(0), st(q, 0),
-                    st(q, tok), st(q, head), st(k, 0), st(k, tok), st(k, head), ptr(pos), given && pos.scalar_type() == at::kLong,
-                    ps[0], ps[1], ps[2], start, (const double*)freq.data_ptr(), (const int32_t*)ptr(axis), axes,
-                    pairs == "interleaved", PyObject_IsTrue(args[8]), (float)number("factor", args[6]), out[0].data_ptr(),
-                    ptr(out[1]), st(out[0], 0), st(out[0], tok), st(out[0], head), st(out[1], 0), st(out[1], tok),
-                    st(out[1], head), on.stream),
-         "lbw_rotary");
-  }
+  same_device("rotary", a.q, out[0], out[1]);
+  a.run(out[0], out[1], PyObject_IsTrue(args[8]), true);
+  written(out[0]);
+  written(out[1]);
   return wrap_all(out);
   END_HANDLE_TH_ERRORS
 }
@@ -440,20 +626,6 @@ PyObject* plain(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// Whether these tensors (None: absent) are of different types.
-PyObject* mixed(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  const Tensor* first = nullptr;
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    if (!THPVariable_Check(args[i])) continue;
-    const Tensor& t = THPVariable_Unpack(args[i]);
-    if (first && first->scalar_type() != t.scalar_type()) Py_RETURN_TRUE;
-    first = &t;
-  }
-  Py_RETURN_FALSE;
-  END_HANDLE_TH_ERRORS
-}
-
 PyObject* on_status(PyObject*, PyObject* f) {
   Py_INCREF(f);
   Py_XSETREF(status_handler, f);
@@ -461,7 +633,8 @@ PyObject* on_status(PyObject*, PyObject* f) {
 }
 
 #define FAST(f) {#f, (PyCFunction)(void*)f, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(gated_norm), FAST(gated_norm_bwd), FAST(rotary), FAST(gemm_w4), FAST(plain), FAST(mixed),
+PyMethodDef methods[] = {FAST(norm), FAST(gated_norm), FAST(gated_norm_bwd), FAST(rotary_embed), FAST(rotary), FAST(gemm_w4),
+                         FAST(plain),
                          {"on_status", on_status, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_block", nullptr, -1, methods};
 

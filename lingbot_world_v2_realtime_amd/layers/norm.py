@@ -5,28 +5,9 @@ and modulates it for the next one (lingbot/models/lingbot_world/transformer.py:2
 latent frame. Written with torch operations that is a dozen passes over [B, L, C]; here it is one pass, and one more for all
 gradients.
 """
-import torch
-from torch.autograd.function import once_differentiable
-
 from .. import kernels
 
 __all__ = ["gated_norm"]
-
-class _GatedNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, opts, *args):
-        ctx.opts = opts
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*args)
-        return kernels.block_binding().gated_norm(*args, *opts, args[1] is not None)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, ds, dh):
-        wants = sum(1 << i for i, needed in enumerate(ctx.needs_input_grad[1:]) if needed)
-        ds, dh = (d if d is None else d.contiguous() for d in (ds, dh))
-        return None, *kernels.block_binding().gated_norm_bwd(*ctx.saved_tensors, *ctx.opts, ds, dh, wants)
-
 
 def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=None, post_weight=None, norm="layer",
                post_norm=None, eps=1e-6, residual_scale=1.0, branch_scale=1.0, group_len=None):
@@ -45,15 +26,6 @@ def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=N
     Differentiable in x, y and every vector (once: there is no second derivative). The backward reads x and y again and
     keeps nothing else; the sums over rows are in fp32 and in a fixed order.
     """
-    block = kernels.block_binding()
-    if block.mixed(gate, shift, scale, weight, bias, post_weight):
-        gate, shift, scale, weight, bias, post_weight = (
-            v if v is None or v.dtype == torch.float32 else v.float()
-            for v in (gate, shift, scale, weight, bias, post_weight))
-    args = (x, y, gate, shift, scale, weight, bias, post_weight)
-    opts = (norm, post_norm, eps, residual_scale, branch_scale, group_len)
-    if block.plain(*args):
-        s, h = block.gated_norm(*args, *opts, y is not None)
-    else:
-        s, h = _GatedNorm.apply(opts, *args)
+    s, h = kernels.block_binding().norm(x, y, gate, shift, scale, weight, bias, post_weight, norm, post_norm, eps,
+                                        residual_scale, branch_scale, group_len)
     return h if s is None else s if h is None else (s, h)

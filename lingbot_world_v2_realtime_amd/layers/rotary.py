@@ -10,7 +10,6 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import kernels
 
@@ -76,30 +75,6 @@ def grid_positions(grid_size, start_frame=0, device="cuda"):
     return torch.stack((start_frame + t // (h * w), t // w % h, t % w), dim=1)
 
 
-class _RotaryEmbed(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, rope, layout):
-        tensor = isinstance(positions, torch.Tensor)
-        ctx.save_for_backward(rope.freq, rope.axis, positions if tensor else None)
-        ctx.start, ctx.plan = None if tensor else positions, (rope.pairs, rope.factor, layout)
-        ctx.set_materialize_grads(False)
-        return kernels.rotary(q, k, positions, rope.freq, rope.axis, *ctx.plan)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        freq, axis, positions = ctx.saved_tensors
-        need_q, need_k = ctx.needs_input_grad[:2]
-        dq, dk = dq if need_q else None, dk if need_k else None
-        if dq is None and dk is None:
-            return None, None, None, None, None
-        dq, dk = (d if d is None or d.shape[-1] <= 1 or d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
-        one = (dq, dk) if dq is not None else (dk, None)   # one rotation takes any number of heads
-        one = kernels.rotary(*one, ctx.start if positions is None else positions, freq, axis, *ctx.plan, inverse=True)
-        dq, dk = one if dq is not None else (None, one[0])
-        return dq, dk, None, None, None
-
-
 def rotary_embed(q, k, positions, rope, tensor_layout="NHD", inplace=False):
     """q [B, L, Hq, D] and k [B, L, Hk, D] (or None) rotated by the plan `rope` ("HND": [B, H, L, D]; bf16, fp16 or fp32
     on the GPU, any strides with contiguous channels, any head counts). positions: int32 or int64 tensor [L] or [B, L]
@@ -107,10 +82,5 @@ def rotary_embed(q, k, positions, rope, tensor_layout="NHD", inplace=False):
     Channels past the plan's are copied. Angles are formed in 64 bits, the rotation in fp32, with one rounding.
     inplace: q and k are overwritten and returned (not where a gradient is recorded; every element must have memory of
     its own). Returns (q, k); differentiable in both."""
-    block = kernels.block_binding()
-    if block.plain(q, k):
-        return block.rotary(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor, tensor_layout, False,
-                            q if inplace else None, k if inplace else None)
-    if inplace:
-        raise ValueError("q and k cannot be rotated in place where a gradient is recorded")
-    return _RotaryEmbed.apply(q, k, positions, rope, tensor_layout)
+    return kernels.block_binding().rotary_embed(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor,
+                                                tensor_layout, inplace)

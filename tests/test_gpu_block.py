@@ -275,6 +275,41 @@ def test_gated_norm_refusals():
         gated_norm(x, y, gate=torch.ones(64, dtype=torch.bfloat16))
 
 
+def test_gradients_once_and_transforms():
+    """A second derivative, forward-mode tangents and torch.func transforms are refused, not answered wrongly; a tensor changed
+    after the call is noticed by the gradient."""
+    from lingbot_world_v2_realtime_amd import Rotary, gated_norm, rotary_embed
+    x = torch.randn(1, 4, 64, device=DEV, requires_grad=True)
+    rope = Rotary.build(64, DEV)
+    calls = (lambda t: gated_norm(t), lambda t: rotary_embed(t.view(1, 4, 1, 64), None, 0, rope)[0].view(1, 4, 64))
+    for f in calls:
+        (g,) = torch.autograd.grad(f(x).sum(), x)
+        assert bool(g.isfinite().all())
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(f(x).square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x.detach(),), (torch.ones_like(x),))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(x.detach())
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(lambda t: f(t))(torch.randn(3, 1, 4, 64, device=DEV))
+    y = x * 1.0
+    out = gated_norm(y)
+    y.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    q = torch.randn(1, 4, 2, 64, device=DEV, requires_grad=True)
+    z = q * 1.0
+    w = z.square().sum()
+    with torch.no_grad():
+        rotary_embed(z, None, 0, rope, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        w.backward()
+    with torch.inference_mode():
+        t = torch.randn(1, 4, 2, 64, device=DEV)
+        assert rotary_embed(t, None, 0, rope, inplace=True)[0] is not None and gated_norm(t.view(1, 8, 64)).shape == (1, 8, 64)
+
+
 # ---------------------------------------------------------------- rotary
 
 
@@ -350,7 +385,7 @@ def test_rotary_layouts_strides_and_inplace():
     want = rotary_embed(qv, kv, 9, rope)
     rest = fused[..., 1024:].clone()
     got = rotary_embed(qv, kv, 9, rope, inplace=True)
-    assert got[0] is qv and all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(fused[..., 1024:], rest)
+    assert got[0].data_ptr() == qv.data_ptr() and all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(fused[..., 1024:], rest)
     with pytest.raises(ValueError):
         rotary_embed(shared, None, 9, rope, inplace=True)
     with pytest.raises(ValueError):
