@@ -25,7 +25,8 @@ namespace {
 
 constexpr int MAX_TEAM = 512;
 constexpr int SUM_ROWS = 3;         // A, B, C of a workgroup's rows
-constexpr int SLICES = 16;          // waves of the two summing kernels
+constexpr int SUM_COLS = 32;        // channels of a workgroup of the two summing kernels, and the slices of the summed rows
+constexpr int SLICES = 32;
 
 struct Vec {
   const void* p;
@@ -100,6 +101,32 @@ struct Span {
   }
 };
 
+// A vector that the forward multiplies or adds. With one chunk a thread (few rows: the call is as long as its longest chain of
+// loads) it is loaded at the row's start, with all the others; with more where it is used, for the registers.
+template <int DT, int NCH, bool VEC>
+struct Factor {
+  const void* p;
+  Raw8<DT, VEC> w[NCH];
+  __device__ __forceinline__ Factor(const Span<NCH, VEC>& span, const void* at) : p(at) {
+    if constexpr (NCH == 1) {
+      if (p) span.load(w, p);
+    }
+  }
+  // op(f, the vector's value at the same channel) over the span, unless there is no such vector
+  template <typename F>
+  __device__ __forceinline__ void apply(const Span<NCH, VEC>& span, float (*f)[8], F op) {
+    if (!p) return;
+    if constexpr (NCH > 1) span.load(w, p);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      float v[8];
+      w[c].get(v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) op(f[c][e], v[e]);
+    }
+  }
+};
+
 // Sums over a team, the same bits in all its threads. One wave: no LDS. Else every wave leaves its sums in `red`, which
 // nobody may write again before another barrier has been passed.
 template <int N>
@@ -164,19 +191,23 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_kernel(NormArgs a, int te
   const int64_t row = one ? (int64_t)blockIdx.x * (blockDim.x >> 6) + wave : blockIdx.x;
   if (row >= a.rows) return;   // whole waves, and only where a wave is a team: nobody waits for them
   const int64_t b = row / a.len, t = row - b * a.len, g = t / a.group_len;
-  Raw8<DT, VEC> xw[NCH];
+  Raw8<DT, VEC> xw[NCH], yw[NCH];
   float s[NCH][8];
   span.load(xw, at<DT>(a.x, b * a.x_s_batch + t * a.x_s_tok));
+  if (a.y) span.load(yw, at<DT>(a.y, b * a.y_s_batch + t * a.y_s_tok));
+  using V = Factor<VDT, NCH, VEC>;
+  V post_weight(span, a.post_weight), gate(span, vec_row(a.gate, b, g, elem_size(VDT)));
+  V weight(span, a.weight), bias(span, a.bias), scale(span, vec_row(a.scale, b, g, elem_size(VDT)));
+  V shift(span, vec_row(a.shift, b, g, elem_size(VDT)));
+  const auto mul = [](float& f, float w) { f *= w; };
+  const auto add = [](float& f, float w) { f += w; };
   if (a.y) {
-    Raw8<DT, VEC> yw[NCH];
-    span.load(yw, at<DT>(a.y, b * a.y_s_batch + t * a.y_s_tok));
     float v[NCH][8];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) yw[c].get(v[c]);
     if (a.post_norm != LBW_NORM_NONE) normalise(v, a.post_norm, span, a.eps, red);
-    const auto mul = [](float& f, float w) { f *= w; };
-    span.template with<VDT>(v, a.post_weight, mul);
-    span.template with<VDT>(v, vec_row(a.gate, b, g, elem_size(VDT)), mul);
+    post_weight.apply(span, v, mul);
+    gate.apply(span, v, mul);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       xw[c].get(s[c]);
@@ -194,10 +225,10 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_kernel(NormArgs a, int te
   if (s_out) span.template store<DT>(at<DT>(s_out, row * a.width), s);
   if (a.norm == LBW_NORM_NONE) return;
   normalise(s, a.norm, span, a.eps, red + 2 * RED);
-  span.template with<VDT>(s, a.weight, [](float& f, float w) { f *= w; });
-  span.template with<VDT>(s, a.bias, [](float& f, float w) { f += w; });
-  span.template with<VDT>(s, vec_row(a.scale, b, g, elem_size(VDT)), [](float& f, float w) { f *= 1.f + w; });
-  span.template with<VDT>(s, vec_row(a.shift, b, g, elem_size(VDT)), [](float& f, float w) { f += w; });
+  weight.apply(span, s, mul);
+  bias.apply(span, s, add);
+  scale.apply(span, s, [](float& f, float w) { f *= 1.f + w; });
+  shift.apply(span, s, add);
   span.template store<DT>(at<DT>(h_out, row * a.width), s);
 }
 
@@ -373,18 +404,31 @@ __device__ __forceinline__ void weigh(const NormArgs& a, int64_t b, int64_t g, i
   for (int k = 0; k < SUM_ROWS; ++k) t[SUM_ROWS + k] += s[k];
 }
 
-// The workgroups' sums of one modulation row (blockIdx.y), 64 channels a workgroup, its waves taking every SLICES-th: the
-// row's own gradients, and its sums left where its first workgroup's were for the kernel below (which a single
+// The workgroups' sums of one modulation row (blockIdx.y), SUM_COLS channels a workgroup, its half-waves taking every SLICES-th, four
+// in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which a single
 // modulation row does not need: `last`).
 template <int VDT>
-__global__ __launch_bounds__(64 * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int last) {
-  __shared__ float part[SLICES][SUM_ROWS][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t ch = 64 * (int64_t)blockIdx.x + lane, bg = blockIdx.y, b = bg / o.groups, g = bg - b * o.groups;
+__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int last) {
+  __shared__ float part[SLICES][SUM_ROWS][SUM_COLS];
+  const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS;
+  const int64_t ch = SUM_COLS * (int64_t)blockIdx.x + lane, bg = blockIdx.y, b = bg / o.groups, g = bg - b * o.groups;
   float* base = o.sums + bg * o.chunks * SUM_ROWS * a.width;
   float s[SUM_ROWS] = {};
   if (ch < a.width) {
-    for (int64_t i = w; i < o.chunks; i += SLICES)
+    constexpr int U = 4;
+    int64_t i = w;
+    for (; i + (U - 1) * SLICES < o.chunks; i += U * SLICES) {
+      float f[U][SUM_ROWS];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < SUM_ROWS; ++k) f[u][k] = base[((i + u * SLICES) * SUM_ROWS + k) * a.width + ch];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < SUM_ROWS; ++k) s[k] += f[u][k];
+    }
+    for (; i < o.chunks; i += SLICES)
 #pragma unroll
       for (int k = 0; k < SUM_ROWS; ++k) s[k] += base[(i * SUM_ROWS + k) * a.width + ch];
   }
@@ -416,10 +460,10 @@ __global__ __launch_bounds__(64 * SLICES) void norm_group_sums_kernel(NormArgs a
 
 // The modulation rows' sums, weighted and added: the gradients of what they share.
 template <int VDT>
-__global__ __launch_bounds__(64 * SLICES) void norm_shared_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int64_t rows) {
-  __shared__ float part[SLICES][2 * SUM_ROWS][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t ch = 64 * (int64_t)blockIdx.x + lane;
+__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_shared_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int64_t rows) {
+  __shared__ float part[SLICES][2 * SUM_ROWS][SUM_COLS];
+  const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS;
+  const int64_t ch = SUM_COLS * (int64_t)blockIdx.x + lane;
   float t[2 * SUM_ROWS] = {};
   if (ch < a.width) {
     for (int64_t bg = w; bg < rows; bg += SLICES) {
@@ -493,8 +537,11 @@ int check(const NormArgs& a, int dtype, int vec_dtype, int64_t batch, bool& vec,
 
 template <int DT, int VDT, bool VEC>
 void forward(const NormArgs& a, void* s_out, void* h_out, hipStream_t stream) {
+  // Few rows are a matter of latency: one chunk a thread and more threads a row (1536 channels, LayerNorm and post norm: 1 row 4.7 ->
+  // 3.7 us, 64 rows 5.6 -> 4.1, 1024 rows 6.0 -> 5.6; but 2048 rows 8.1 -> 8.2, and with 4096 channels 14.2 -> 15.9).
+  constexpr int FEW = 1024;
   int nch = 0, team = 0;
-  pick(a.width, 3, nch, team);
+  pick(a.width, a.rows <= FEW && a.width <= 8 * MAX_TEAM ? 1 : 3, nch, team);
   const int threads = team == 64 ? 256 : team;
   const dim3 grid((unsigned)(team == 64 ? (a.rows + 3) / 4 : a.rows));
   if (nch == 1) gated_norm_kernel<DT, VDT, 1, VEC><<<grid, threads, 0, stream>>>(a, team, s_out, h_out);
@@ -502,11 +549,14 @@ void forward(const NormArgs& a, void* s_out, void* h_out, hipStream_t stream) {
   else gated_norm_kernel<DT, VDT, 3, VEC><<<grid, threads, 0, stream>>>(a, team, s_out, h_out);
 }
 
-// Rows of a workgroup of the backward, for `team` and the modulation rows' length: about one workgroup of eight waves a CU, since each
-// leaves three fp32 rows behind that are written and read again (against six of `dtype` for every row of the tensors).
-void split(int64_t rows, int64_t len, int64_t group_len, int team, int64_t& chunk_rows, int64_t& chunks) {
+// Rows of a workgroup of the backward. More workgroups keep more rows in flight, but each leaves three fp32 rows behind that are
+// written and read again (against six of `dtype` for every row of the tensors). With one chunk a thread 12 waves a CU are the best
+// (6032 x 1536 bf16, all gradients: 8 waves 41.4 us, 12 39.1, 16 39.8), with two 8, the registers' bound (4524 x 2048: 38.8,
+// 47.7, 47.6: a second round).
+void split(int64_t rows, int64_t len, int64_t group_len, int nch, int team, int64_t& chunk_rows, int64_t& chunks) {
   const int64_t gl = group_len < len ? group_len : len;
-  const int64_t blocks = team == 64 ? 256 : 256 * 8 / (team >> 6);
+  const int waves = team == 64 ? 8 : team >> 6, room = nch == 1 ? (team == 64 ? 16 : 12) : 8;   // of a workgroup, and of a CU
+  const int64_t blocks = 256 * (room > waves ? room / waves : 1);
   const int64_t step = team == 64 ? 8 : 1;
   int64_t r = (rows + blocks - 1) / blocks;
   r = (r + step - 1) / step * step;
@@ -575,7 +625,7 @@ extern "C" int64_t lbw_gated_norm_bwd_workspace_bytes(int64_t batch, int64_t len
   int nch = 0, team = 0;
   pick_bwd(width, nch, team);
   int64_t chunk_rows, chunks;
-  split(batch * len, len, group_len, team, chunk_rows, chunks);
+  split(batch * len, len, group_len, nch, team, chunk_rows, chunks);
   return batch * groups * chunks * SUM_ROWS * width * (int64_t)sizeof(float);
 }
 
@@ -618,20 +668,20 @@ extern "C" int lbw_gated_norm_bwd(const void* ds, const void* dh, const void* x,
   int nch = 0, team = 0;
   pick_bwd(width, nch, team);
   GradArgs o = {ds, dh, dx, dy, sums ? (float*)workspace : nullptr, groups, 0, 0};
-  split(a.rows, len, group_len, team, o.chunk_rows, o.chunks);
+  split(a.rows, len, group_len, nch, team, o.chunk_rows, o.chunks);
   if (batch * groups * o.chunks > (1 << 30) || (sums && batch * groups > 65535)) return LBW_E_SHAPE;
   if (const int st = check_device()) return st;
   by_type(dtype, vec_dtype, vec, [&](auto dt, auto vt, auto w) {
     backward<dt.value, vt.value, w.value>(a, o, nch, team, (hipStream_t)stream);
     if (!sums) return;
     const int64_t mrows = batch * groups;
-    const unsigned tiles = (unsigned)((width + 63) / 64);
-    norm_group_sums_kernel<vt.value><<<dim3(tiles, (unsigned)mrows), 64 * SLICES, 0, (hipStream_t)stream>>>(
+    const unsigned tiles = (unsigned)((width + SUM_COLS - 1) / SUM_COLS);
+    norm_group_sums_kernel<vt.value><<<dim3(tiles, (unsigned)mrows), SUM_COLS * SLICES, 0, (hipStream_t)stream>>>(
         a, o, d, mrows == 1);
     const bool shared = dweight || dbias || dpost_weight || (dgate && !d.gate_rows) ||
                         (dscale && !d.scale_rows) || (dshift && !d.shift_rows);
     if (shared && mrows > 1)
-      norm_shared_sums_kernel<vt.value><<<tiles, 64 * SLICES, 0, (hipStream_t)stream>>>(a, o, d, mrows);
+      norm_shared_sums_kernel<vt.value><<<tiles, SUM_COLS * SLICES, 0, (hipStream_t)stream>>>(a, o, d, mrows);
   });
   return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
 }
