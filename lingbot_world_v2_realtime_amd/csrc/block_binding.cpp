@@ -7,6 +7,7 @@
 // take. A status from the library goes to the function that `on_status` was given, which raises.
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
@@ -472,6 +473,14 @@ struct Rotary {
   }
 };
 
+// Tensors of which one is written while the other is read or written, by different threads.
+void apart(const Tensor& a, const Tensor& b, const char* what) {
+  if (!a.defined() || !b.defined()) return;
+  const auto o = at::get_overlap_status(a, b);
+  if (o == at::MemOverlapStatus::Full || o == at::MemOverlapStatus::Partial || (a.numel() && b.numel() && a.data_ptr() == b.data_ptr()))
+    value_error(what, " share their memory");
+}
+
 // A tensor written in place: a graph that kept it notices.
 void written(const Tensor& t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -520,6 +529,7 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (const Tensor* t : {&a.q, &a.k})
       for (int j = 0; t->defined() && j < 4; ++j)
         if (t->stride(j) == 0 && t->size(j) > 1) value_error("q or k has elements that share their memory");
+    apart(a.q, a.k, "q and k, to be rotated in place,");
     a.run(a.q, a.k, false, true);
     written(a.q);
     written(a.k);
@@ -554,6 +564,9 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
       value_error(name, " overlaps its input in another order");
   }
   same_device("rotary", a.q, out[0], out[1]);
+  apart(out[0], out[1], "q_out and k_out");
+  apart(out[0], a.k, "q_out and k");
+  apart(out[1], a.q, "k_out and q");
   a.run(out[0], out[1], PyObject_IsTrue(args[8]), true);
   written(out[0]);
   written(out[1]);

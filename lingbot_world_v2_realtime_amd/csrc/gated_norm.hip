@@ -25,7 +25,7 @@ namespace {
 
 constexpr int MAX_TEAM = 512;
 constexpr int SUM_ROWS = 3;         // A, B, C of a workgroup's rows
-constexpr int SUM_COLS = 32;        // channels of a workgroup of the two summing kernels, and the slices of the summed rows
+constexpr int SUM_COLS = 32;        // channels of a workgroup of the two summing kernels, and the slices of the summed rows at most
 constexpr int SLICES = 32;
 
 struct Vec {
@@ -404,31 +404,31 @@ __device__ __forceinline__ void weigh(const NormArgs& a, int64_t b, int64_t g, i
   for (int k = 0; k < SUM_ROWS; ++k) t[SUM_ROWS + k] += s[k];
 }
 
-// The workgroups' sums of one modulation row (blockIdx.y), SUM_COLS channels a workgroup, its half-waves taking every SLICES-th, four
-// in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which a single
+// The workgroups' sums of one modulation row (blockIdx.x / tiles), SUM_COLS channels a workgroup, its half-waves taking them in turn,
+// four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which a single
 // modulation row does not need: `last`).
 template <int VDT>
-__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int last) {
+__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int tiles, int last) {
   __shared__ float part[SLICES][SUM_ROWS][SUM_COLS];
-  const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS;
-  const int64_t ch = SUM_COLS * (int64_t)blockIdx.x + lane, bg = blockIdx.y, b = bg / o.groups, g = bg - b * o.groups;
+  const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS, slices = blockDim.x / SUM_COLS;
+  const int64_t bg = blockIdx.x / tiles, ch = SUM_COLS * (blockIdx.x - bg * tiles) + lane, b = bg / o.groups, g = bg - b * o.groups;
   float* base = o.sums + bg * o.chunks * SUM_ROWS * a.width;
   float s[SUM_ROWS] = {};
   if (ch < a.width) {
     constexpr int U = 4;
     int64_t i = w;
-    for (; i + (U - 1) * SLICES < o.chunks; i += U * SLICES) {
+    for (; i + (U - 1) * slices < o.chunks; i += U * slices) {
       float f[U][SUM_ROWS];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int k = 0; k < SUM_ROWS; ++k) f[u][k] = base[((i + u * SLICES) * SUM_ROWS + k) * a.width + ch];
+        for (int k = 0; k < SUM_ROWS; ++k) f[u][k] = base[((i + u * slices) * SUM_ROWS + k) * a.width + ch];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int k = 0; k < SUM_ROWS; ++k) s[k] += f[u][k];
     }
-    for (; i < o.chunks; i += SLICES)
+    for (; i < o.chunks; i += slices)
 #pragma unroll
       for (int k = 0; k < SUM_ROWS; ++k) s[k] += base[(i * SUM_ROWS + k) * a.width + ch];
   }
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(Norm
 #pragma unroll
   for (int k = 0; k < SUM_ROWS; ++k) {
     s[k] = 0.f;
-    for (int i = 0; i < SLICES; ++i) s[k] += part[i][k][lane];
+    for (int i = 0; i < slices; ++i) s[k] += part[i][k][lane];
   }
   const int64_t at = bg * a.width + ch;
   if (d.shift && d.shift_rows) store1<VDT>(d.shift, at, s[1]);
@@ -567,7 +567,7 @@ void split(int64_t rows, int64_t len, int64_t group_len, int nch, int team, int6
 
 template <int DT, int VDT, bool VEC>
 void backward(const NormArgs& a, const GradArgs& o, int nch, int team, hipStream_t stream) {
-  const int threads = team == 64 ? 512 : team;
+  const int threads = team == 64 ? (int)(64 * (o.chunk_rows < 8 ? o.chunk_rows : 8)) : team;
   const dim3 grid((unsigned)(a.rows / a.len * o.groups * o.chunks));
   if (nch == 1) gated_norm_bwd_kernel<DT, VDT, 1, VEC><<<grid, threads, 0, stream>>>(a, o, team);
   else if (nch == 2) gated_norm_bwd_kernel<DT, VDT, 2, VEC><<<grid, threads, 0, stream>>>(a, o, team);
@@ -669,15 +669,17 @@ extern "C" int lbw_gated_norm_bwd(const void* ds, const void* dh, const void* x,
   pick_bwd(width, nch, team);
   GradArgs o = {ds, dh, dx, dy, sums ? (float*)workspace : nullptr, groups, 0, 0};
   split(a.rows, len, group_len, nch, team, o.chunk_rows, o.chunks);
-  if (batch * groups * o.chunks > (1 << 30) || (sums && batch * groups > 65535)) return LBW_E_SHAPE;
+  if (batch * groups * o.chunks > (1 << 30) || batch * groups * ((width + SUM_COLS - 1) / SUM_COLS) > (1 << 30))
+    return LBW_E_SHAPE;
   if (const int st = check_device()) return st;
   by_type(dtype, vec_dtype, vec, [&](auto dt, auto vt, auto w) {
     backward<dt.value, vt.value, w.value>(a, o, nch, team, (hipStream_t)stream);
     if (!sums) return;
     const int64_t mrows = batch * groups;
     const unsigned tiles = (unsigned)((width + SUM_COLS - 1) / SUM_COLS);
-    norm_group_sums_kernel<vt.value><<<dim3(tiles, (unsigned)mrows), SUM_COLS * SLICES, 0, (hipStream_t)stream>>>(
-        a, o, d, mrows == 1);
+    const int64_t slices = o.chunks < SLICES ? (o.chunks + 1) / 2 * 2 : SLICES;   // (whole waves)
+    norm_group_sums_kernel<vt.value><<<(unsigned)(tiles * mrows), (unsigned)(SUM_COLS * slices), 0, (hipStream_t)stream>>>(
+        a, o, d, (int)tiles, mrows == 1);
     const bool shared = dweight || dbias || dpost_weight || (dgate && !d.gate_rows) ||
                         (dscale && !d.scale_rows) || (dshift && !d.shift_rows);
     if (shared && mrows > 1)

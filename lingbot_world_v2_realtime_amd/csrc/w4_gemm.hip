@@ -259,7 +259,7 @@ __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int r = lane & 15, q = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.y * ROWS, nt0 = (int64_t)blockIdx.x * NT, nts = (a.n + TN - 1) / TN;
+  const int64_t m0 = (int64_t)blockIdx.x * ROWS, nt0 = (int64_t)blockIdx.y * NT, nts = (a.n + TN - 1) / TN;
   char* mine = lds + wave * (ROWS * 256);
   const RowsOfX<VEC> rows(a, m0);
   const uint32_t off0 = rows.offset(q), four = rows.offset(4);
@@ -463,7 +463,7 @@ void launch_rows(const GemmArgs& a, int most, hipStream_t stream) {
   // the fewest rounds of K tiles that `most` waves allow, in as few waves
   const int64_t rounds = (a.kt + most - 1) / most;
   const int waves = (int)((a.kt + rounds - 1) / rounds);
-  const dim3 grid((unsigned)((a.n + TN * NT - 1) / (TN * NT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
+  const dim3 grid((unsigned)((a.m + 16 * MT - 1) / (16 * MT)), (unsigned)((a.n + TN * NT - 1) / (TN * NT)));
   const int each = MT * (NT > 4 ? NT : 4) * 1024;   // bytes of LDS a wave needs
   w4_rows_kernel<DT, F, GROUP, MT, NT, MOST, VEC><<<grid, 64 * waves, waves * each, stream>>>(a);
 }
@@ -495,9 +495,10 @@ void launch_format(const GemmArgs& a, int64_t group, bool vec, hipStream_t strea
   else launch_group<DT, F, 128>(a, vec, stream);
 }
 
+constexpr int64_t MAX_N = 65535 * TN;   // (column tiles are a second grid dimension)
+
 bool sizes_ok(int64_t n, int64_t k, int fmt, int64_t group) {
-  // (tiles along K and N are grid dimensions of at most 65535)
-  return n >= 1 && k >= 1 && n <= (1 << 20) && k <= (1 << 20) && (fmt == LBW_W4_INT4 || fmt == LBW_W4_FP4) &&
+  return n >= 1 && k >= 1 && n <= MAX_N && k <= (1 << 20) && (fmt == LBW_W4_INT4 || fmt == LBW_W4_FP4) &&
          (group == 32 || group == 64 || group == 128);
 }
 
@@ -514,7 +515,6 @@ extern "C" int lbw_quant_w4(const void* w, int w_is_fp32, int64_t n, int64_t k, 
     return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const dim3 grid((unsigned)((k + TK - 1) / TK), (unsigned)((n + TN - 1) / TN));
-  if (grid.y > 65535) return LBW_E_SHAPE;
   if (w_is_fp32) quant_w4_kernel<true><<<grid, 256, 0, (hipStream_t)stream>>>(w, n, k, s_row, fmt, (int)group, w4, scale, zero);
   else quant_w4_kernel<false><<<grid, 256, 0, (hipStream_t)stream>>>(w, n, k, s_row, fmt, (int)group, w4, scale, zero);
   return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
@@ -524,7 +524,7 @@ extern "C" int lbw_gemm_w4(const void* x, int dtype, int64_t m, int64_t k, int64
                            const uint16_t* scale, const uint8_t* zero, int fmt, int64_t group, int64_t n,
                            const void* bias, void* out, void* stream) {
   if (!x || !w4 || !scale || !out) return LBW_E_NULL;
-  if (!sizes_ok(n, k, fmt, group) || (zero && fmt == LBW_W4_FP4) || m < 1 || m > (1 << 20) ||
+  if (!sizes_ok(n, k, fmt, group) || (zero && fmt == LBW_W4_FP4) || m < 1 || m > (1 << 24) ||
       (dtype != LBW_DTYPE_BF16 && dtype != LBW_DTYPE_FP16))
     return LBW_E_SHAPE;
   if ((uintptr_t)x % 2 || (uintptr_t)w4 % 16 || (uintptr_t)scale % 16 || (uintptr_t)zero % 16 || (uintptr_t)bias % 2 || (uintptr_t)out % 8)

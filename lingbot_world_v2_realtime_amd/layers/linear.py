@@ -201,6 +201,14 @@ class W4Linear(torch.nn.Module):
         self.bias = lin.bias
         self.in_features, self.out_features, self.fmt = lin.in_features, lin.out_features, fmt
 
+    def _apply(self, fn, recurse=True):
+        # a module's .half() or .float() is for its parameters: the scales stay bf16 and move with the module
+        scale = self.w4_scale
+        super()._apply(fn, recurse)
+        if self.w4_scale.dtype != scale.dtype:
+            self.w4_scale = scale.to(self.w4.device)
+        return self
+
     def forward(self, x):
         shape = x.shape
         block = kernels.block_binding()

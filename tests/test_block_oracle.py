@@ -188,7 +188,7 @@ def test_gated_norm_entry_point_refusals():
     assert _norm_bwd(dpost_weight=FAKE) == E_NULL
     assert _norm_bwd(groups=2, group_len=4) == E_SHAPE                # tokens 8, 9 have no row
     assert _norm_bwd(groups=0) == E_SHAPE
-    assert _norm_bwd(batch=1 << 17, len=1, dgate=FAKE) == E_SHAPE     # more modulation rows than the grid has
+    assert _norm_bwd(batch=1 << 30, len=1, width=4096, dgate=FAKE) == E_SHAPE   # more workgroups than a grid has
     assert _norm_bwd(dgate=FAKE, ws=FAKE + 8) == E_ALIGN
     lib = _lib.load()
     assert lib.lbw_gated_norm_bwd_workspace_bytes(0, 1, 64, 1, 1) == 0
@@ -222,7 +222,7 @@ def _gemm(**kw):
 
 def test_w4_entry_point_refusals():
     assert _gemm(x=None) == E_NULL and _gemm(w4=None) == E_NULL and _gemm(scale=None) == E_NULL and _gemm(out=None) == E_NULL
-    assert _gemm(dtype=2) == E_SHAPE and _gemm(m=0) == E_SHAPE and _gemm(m=(1 << 20) + 1) == E_SHAPE
+    assert _gemm(dtype=2) == E_SHAPE and _gemm(m=0) == E_SHAPE and _gemm(m=(1 << 24) + 1) == E_SHAPE
     assert _gemm(k=0) == E_SHAPE and _gemm(n=0) == E_SHAPE and _gemm(group=16) == E_SHAPE and _gemm(fmt=2) == E_SHAPE
     assert _gemm(fmt=1, zero=FAKE) == E_SHAPE
     assert _gemm(x=FAKE + 1) == E_ALIGN and _gemm(w4=FAKE + 8) == E_ALIGN and _gemm(scale=FAKE + 1) == E_ALIGN
@@ -230,7 +230,7 @@ def test_w4_entry_point_refusals():
     assert q(None, 0, 8, 8, 8, 0, 64, FAKE, FAKE, None, None) == E_NULL
     assert q(FAKE, 0, 8, 8, 8, 1, 64, FAKE, FAKE, FAKE, None) == E_SHAPE
     assert q(FAKE, 0, 8, 0, 8, 0, 64, FAKE, FAKE, None, None) == E_SHAPE
-    assert q(FAKE, 0, (1 << 20), 8, 8, 0, 64, FAKE, FAKE, None, None) in (E_SHAPE, E_DEVICE)
+    assert q(FAKE, 0, (1 << 20), 8, 8, 0, 64, FAKE, FAKE, None, None) == E_SHAPE
     assert q(FAKE + 2, 1, 8, 8, 8, 0, 64, FAKE, FAKE, None, None) == E_ALIGN
 
 

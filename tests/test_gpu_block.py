@@ -150,6 +150,17 @@ def test_gated_norm_strides_and_ragged_rows():
     assert one.grad.shape == (c,) and bool(one.grad.isfinite().all())
 
 
+def test_gated_norm_a_row_for_each_token():
+    """Modulation rows of one token each, more of them (with the batch) than a grid's second dimension has."""
+    a = _norm_inputs(24, 3, 37, 520, "bf16", "fp32", rows=37)
+    g = _rand(25)
+    ds, dh = (torch.randn(3, 37, 520, device=DEV, generator=g).bfloat16() for _ in range(2))
+    _check_norm(a, "a row a token", ds, dh)
+    a = _norm_inputs(26, 300, 250, 16, "fp32", rows=250)
+    ds, dh = (torch.randn(300, 250, 16, device=DEV, generator=g) for _ in range(2))
+    _check_norm({k: v for k, v in a.items() if k in ("x", "y", "gate", "shift", "scale")}, "75000 rows", ds, dh)
+
+
 def test_gated_norm_unaligned_rows():
     """Rows that start at any element: the value-by-value form."""
     g = _rand(15)
@@ -237,6 +248,20 @@ def test_gated_norm_in_a_graph():
         return [*kernels.gated_norm(**a), *kernels.gated_norm_bwd(a["x"], ds, dh, **rest).values()]
 
     _replays(make, lambda i: a["x"].add_(0.25))
+
+
+def test_training_step_in_a_graph():
+    """Forward and backward through autograd, captured and replayed."""
+    from lingbot_world_v2_realtime_amd import Rotary, gated_norm, rotary_embed
+    a = {k: v.requires_grad_() for k, v in _norm_inputs(27, 1, 70, 512, "bf16", "fp32").items()}
+    rope, pos = Rotary.build(128, DEV, pairs="half"), torch.arange(70, device=DEV)
+
+    def make():
+        s, h = gated_norm(**a)
+        q, _ = rotary_embed(h.view(1, 70, 4, 128), None, pos, rope)
+        return torch.autograd.grad((s, q), list(a.values()), (torch.ones_like(s), torch.ones_like(q)))
+
+    _replays(make, lambda i: a["x"].detach().add_(0.25))
 
 
 def test_calls_on_another_stream():
@@ -388,6 +413,13 @@ def test_rotary_layouts_strides_and_inplace():
     assert got[0].data_ptr() == qv.data_ptr() and all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(fused[..., 1024:], rest)
     with pytest.raises(ValueError):
         rotary_embed(shared, None, 9, rope, inplace=True)
+    from lingbot_world_v2_realtime_amd import kernels
+    with pytest.raises(ValueError, match="share their memory"):
+        rotary_embed(q, q, 9, rope, inplace=True)
+    with pytest.raises(ValueError, match="share their memory"):
+        kernels.rotary(q, q.clone(), 9, rope.freq, q_out=q, k_out=q)
+    with pytest.raises(ValueError, match="share their memory"):
+        kernels.rotary(q, k, 9, rope.freq, k_out=q[:, :, :2])
     with pytest.raises(ValueError):
         rotary_embed(q.detach().requires_grad_(), k, 9, rope, inplace=True)
 
@@ -597,6 +629,14 @@ def test_w4_linear(fmt, zeros):
         mod(x.requires_grad_())
     net = torch.nn.Sequential(torch.nn.Linear(1536, 1024), torch.nn.Linear(1024, 8)).to(DEV)
     assert convert_to_w4(net, fmt=fmt, zeros=zeros) == (1, 2)
+    # casts of the module leave the weights alone; a copy through its state is the same module
+    scale, x = net[0].w4_scale.clone(), torch.randn(5, 1536, device=DEV).half()
+    with torch.no_grad():
+        want = net.half()[0](x)
+        assert torch.equal(net[0].w4_scale, scale) and want.dtype == torch.float16
+        other = W4Linear(torch.nn.Linear(1536, 1024).to(DEV), 128, fmt, zeros).half()
+        other.load_state_dict(net[0].state_dict())
+        assert torch.equal(other(x), want)
 
 
 def test_w4_refusals():
