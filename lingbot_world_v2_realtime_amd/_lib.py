@@ -61,16 +61,20 @@ BLOCK_SIGNATURES = {
 }
 
 
+# the block operators' own sources: translation units (and headers) that no kernel of the attention path includes
+_BLOCK_SOURCES = ("gated_norm.hip", "lbw_rows.h", "rotary.hip", "w4_gemm.hip")
+
+
 def sources_sha16():
-    """First 16 hex digits of a sha256 over what liblbw_attn.so is built from: the HIP sources and headers (csrc/,
-    include/) and the compiler flags. A measurement stored with this fingerprint describes this build when the
-    fingerprints match."""
+    """First 16 hex digits of a sha256 over what the attention path of liblbw_attn.so (attention, quantisers, prologue,
+    cross-attention, FP8 linears) is built from: its HIP sources and headers (csrc/, include/) and the compiler flags. A
+    measurement stored with this fingerprint describes this build when the fingerprints match."""
     import hashlib
     from . import build
     here = os.path.dirname(os.path.abspath(__file__))
     files = [os.path.join(here, "csrc", f) for f in sorted(os.listdir(os.path.join(here, "csrc")))
-             if f.endswith((".hip", ".h", ".cpp"))]
-    files += [os.path.join(os.path.dirname(here), "include", f) for f in ("lbw_attn.h", "lbw_block.h", "lbw_gemm.h")]
+             if f.endswith((".hip", ".h")) and f not in _BLOCK_SOURCES]
+    files += [os.path.join(os.path.dirname(here), "include", f) for f in ("lbw_attn.h", "lbw_gemm.h")]
     h = hashlib.sha256(" ".join(build.HIPCC_FLAGS).encode())
     for f in files:
         with open(f, "rb") as fh:
