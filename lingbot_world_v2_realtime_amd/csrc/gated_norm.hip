@@ -404,6 +404,30 @@ __device__ __forceinline__ void weigh(const NormArgs& a, int64_t b, int64_t g, i
   for (int k = 0; k < SUM_ROWS; ++k) t[SUM_ROWS + k] += s[k];
 }
 
+// The slices' sums of K values into those of slice 0, in halves (one slice adding all took 32 K reads in turn: 6.3 us for a kernel of
+// two rows). slices: a power of two, blockDim.x / SUM_COLS.
+template <int K>
+__device__ __forceinline__ void add_slices(float (*part)[K][SUM_COLS], int w, int lane, int slices, float* s) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) part[w][k][lane] = s[k];
+  for (int half = slices >> 1; half; half >>= 1) {
+    __syncthreads();
+    if (w < half) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        s[k] += part[w + half][k][lane];
+        part[w][k][lane] = s[k];
+      }
+    }
+  }
+}
+
+int slices_for(int64_t rows) {   // (two at least: whole waves)
+  int n = 2;
+  while (n < SLICES && n < rows) n *= 2;
+  return n;
+}
+
 // The workgroups' sums of one modulation row (blockIdx.x / tiles), SUM_COLS channels a workgroup, its half-waves taking them in turn,
 // four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which a single
 // modulation row does not need: `last`).
@@ -432,15 +456,8 @@ __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(Norm
 #pragma unroll
       for (int k = 0; k < SUM_ROWS; ++k) s[k] += base[(i * SUM_ROWS + k) * a.width + ch];
   }
-#pragma unroll
-  for (int k = 0; k < SUM_ROWS; ++k) part[w][k][lane] = s[k];
-  __syncthreads();   // (also: every read of this row's sums is over before they are written below)
+  add_slices<SUM_ROWS>(part, w, lane, slices, s);   // (past its first barrier every read of this row's sums is over)
   if (w || ch >= a.width) return;
-#pragma unroll
-  for (int k = 0; k < SUM_ROWS; ++k) {
-    s[k] = 0.f;
-    for (int i = 0; i < slices; ++i) s[k] += part[i][k][lane];
-  }
   const int64_t at = bg * a.width + ch;
   if (d.shift && d.shift_rows) store1<VDT>(d.shift, at, s[1]);
   if (d.scale && d.scale_rows)
@@ -462,26 +479,19 @@ __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(Norm
 template <int VDT>
 __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_shared_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int64_t rows) {
   __shared__ float part[SLICES][2 * SUM_ROWS][SUM_COLS];
-  const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS;
+  const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS, slices = blockDim.x / SUM_COLS;
   const int64_t ch = SUM_COLS * (int64_t)blockIdx.x + lane;
   float t[2 * SUM_ROWS] = {};
   if (ch < a.width) {
-    for (int64_t bg = w; bg < rows; bg += SLICES) {
+    for (int64_t bg = w; bg < rows; bg += slices) {
       const int64_t b = bg / o.groups;
       const float* p = o.sums + bg * o.chunks * SUM_ROWS * a.width + ch;
       const float s[SUM_ROWS] = {p[0], p[a.width], p[2 * a.width]};
       weigh<VDT>(a, b, bg - b * o.groups, ch, s, t);
     }
   }
-#pragma unroll
-  for (int k = 0; k < 2 * SUM_ROWS; ++k) part[w][k][lane] = t[k];
-  __syncthreads();
+  add_slices<2 * SUM_ROWS>(part, w, lane, slices, t);
   if (w || ch >= a.width) return;
-#pragma unroll
-  for (int k = 0; k < 2 * SUM_ROWS; ++k) {
-    t[k] = 0.f;
-    for (int i = 0; i < SLICES; ++i) t[k] += part[i][k][lane];
-  }
   finish<VDT>(a, d, ch, t);
 }
 
@@ -677,13 +687,12 @@ extern "C" int lbw_gated_norm_bwd(const void* ds, const void* dh, const void* x,
     if (!sums) return;
     const int64_t mrows = batch * groups;
     const unsigned tiles = (unsigned)((width + SUM_COLS - 1) / SUM_COLS);
-    const int64_t slices = o.chunks < SLICES ? (o.chunks + 1) / 2 * 2 : SLICES;   // (whole waves)
-    norm_group_sums_kernel<vt.value><<<(unsigned)(tiles * mrows), (unsigned)(SUM_COLS * slices), 0, (hipStream_t)stream>>>(
+    norm_group_sums_kernel<vt.value><<<(unsigned)(tiles * mrows), SUM_COLS * slices_for(o.chunks), 0, (hipStream_t)stream>>>(
         a, o, d, (int)tiles, mrows == 1);
     const bool shared = dweight || dbias || dpost_weight || (dgate && !d.gate_rows) ||
                         (dscale && !d.scale_rows) || (dshift && !d.shift_rows);
     if (shared && mrows > 1)
-      norm_shared_sums_kernel<vt.value><<<tiles, SUM_COLS * SLICES, 0, (hipStream_t)stream>>>(a, o, d, mrows);
+      norm_shared_sums_kernel<vt.value><<<tiles, SUM_COLS * slices_for(mrows), 0, (hipStream_t)stream>>>(a, o, d, mrows);
   });
   return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
 }
