@@ -65,10 +65,13 @@ const Tensor absent;
 const Tensor& tensor(const char* name, PyObject* o, bool optional = false) {
   if (optional && o == Py_None) return absent;
   if (!THPVariable_Check(o)) type_error(name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (t.is_neg()) value_error(name, " is a lazily negated view: give its resolve_neg()");
+  return t;
 }
 
 double number(const char* name, PyObject* o) {
+  if (THPVariable_Check(o)) type_error(name, " must be a number, got a tensor (whose gradient would be lost)");
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) {
     PyErr_Clear();
@@ -87,6 +90,12 @@ int64_t integer(const char* name, PyObject* o) {
   const int64_t v = PyLong_AsLongLongAndOverflow(i, &overflow);
   Py_DECREF(i);
   if (overflow) value_error(name, " is out of range");
+  return v;
+}
+
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
   return v;
 }
 
@@ -322,7 +331,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     for (int i = 0; i < 2 + VECTORS; ++i)
       if (kept[i].defined() && ctx->needs_input_grad(edge++)) wants |= 1 << i;
     for (Tensor& d : grads)
-      if (d.defined()) d = d.contiguous();
+      if (d.defined()) d = d.resolve_neg().contiguous();
     const bool both = grads.size() == 2;
     const Tensor ds = both || !a.o->norm ? grads[0] : Tensor(), dh = both ? grads[1] : a.o->norm ? grads[0] : Tensor();
     const auto g = a.backward(ds, dh, wants, false);
@@ -366,7 +375,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, Norm::ARGS + 1);
-  return wrap_all(Norm(args).forward(args[Norm::ARGS] == Py_True));
+  return wrap_all(Norm(args).forward(truth(args[Norm::ARGS])));
   END_HANDLE_TH_ERRORS
 }
 
@@ -428,6 +437,7 @@ struct Rotary {
       value_error("q and k need a head at least");
     if (freq.scalar_type() != at::kDouble || freq.dim() != 1 || !freq.is_contiguous() || freq.size(0) < 1)
       value_error("freq must be contiguous float64 [pairs], got ", freq.scalar_type(), " ", dims(freq.sizes()));
+    if (records_gradient({freq})) value_error("freq has no gradient: detach it");
     if (2 * freq.size(0) > d || d > LBW_ROTARY_MAX_DIM)
       value_error(freq.size(0), " pairs do not fit heads of ", d, " (of ", LBW_ROTARY_MAX_DIM, " at most)");
     if (axis.defined() && (axis.scalar_type() != at::kInt || axis.sizes() != freq.sizes() || !axis.is_contiguous()))
@@ -504,7 +514,10 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     a.o = c10::static_intrusive_pointer_cast<RotaryOptions>(ctx->saved_data["options"].toCapsule());
     Tensor d[2];
     for (size_t i = 0; i < grads.size(); ++i)
-      if (grads[i].defined() && ctx->needs_input_grad(i)) d[i] = unit_stride(grads[i]) ? grads[i] : grads[i].contiguous();
+      if (grads[i].defined() && ctx->needs_input_grad(i)) {
+        d[i] = grads[i].resolve_neg();
+        if (!unit_stride(d[i])) d[i] = d[i].contiguous();
+      }
     variable_list out(3);
     if (!d[0].defined() && !d[1].defined()) return out;
     const bool q = d[0].defined();
@@ -524,7 +537,7 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   count(n, 9);
   const Rotary a(args);
   const bool grad = records_gradient({a.q, a.k});
-  if (args[8] == Py_True) {
+  if (truth(args[8])) {
     if (grad) value_error("q and k cannot be rotated in place where a gradient is recorded");
     for (const Tensor* t : {&a.q, &a.k})
       for (int j = 0; t->defined() && j < 4; ++j)
@@ -560,14 +573,15 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
       value_error(name, " must be ", x.scalar_type(), " ", dims(x.sizes()), " with contiguous channels");
     for (int j = 0; j < 4; ++j)
       if (o.stride(j) == 0 && o.size(j) > 1) value_error(name, " has elements that share their memory");
-    if (o.numel() && o.data_ptr() == x.data_ptr() && o.strides() != x.strides())
-      value_error(name, " overlaps its input in another order");
+    if (o.numel() && (o.data_ptr() == x.data_ptr() ? o.strides() != x.strides()
+                                                   : at::get_overlap_status(o, x) == at::MemOverlapStatus::Partial))
+      value_error(name, " overlaps its input, but is not the input itself");
   }
   same_device("rotary", a.q, out[0], out[1]);
   apart(out[0], out[1], "q_out and k_out");
   apart(out[0], a.k, "q_out and k");
   apart(out[1], a.q, "k_out and q");
-  a.run(out[0], out[1], PyObject_IsTrue(args[8]), true);
+  a.run(out[0], out[1], truth(args[8]), true);
   written(out[0]);
   written(out[1]);
   return wrap_all(out);

@@ -46,7 +46,7 @@ struct GradArgs {
   const void *ds, *dh;
   void *dx, *dy;
   float* sums;                      // [batch * groups][chunks][SUM_ROWS][width], or null: no vector's gradient is asked for
-  int64_t groups, chunks, chunk_rows;
+  int64_t groups, mrows, chunks, chunk_rows;   // mrows: modulation rows, those of every entry of the batch
 };
 
 struct VecGrads {
@@ -188,8 +188,8 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_kernel(NormArgs a, int te
   const bool one = team == 64;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const Span<NCH, VEC> span = {one ? (int)(threadIdx.x & 63) : (int)threadIdx.x, team, a.width};
-  const int64_t row = one ? (int64_t)blockIdx.x * (blockDim.x >> 6) + wave : blockIdx.x;
-  if (row >= a.rows) return;   // whole waves, and only where a wave is a team: nobody waits for them
+  const int64_t row = one ? (int64_t)group_id() * (blockDim.x >> 6) + wave : group_id();
+  if (row >= a.rows) return;   // whole workgroups, or whole waves where a wave is a team: nobody waits for them
   const int64_t b = row / a.len, t = row - b * a.len, g = t / a.group_len;
   Raw8<DT, VEC> xw[NCH], yw[NCH];
   float s[NCH][8];
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_kernel(NormArgs a, int te
   span.template store<DT>(at<DT>(h_out, row * a.width), s);
 }
 
-// A workgroup takes the rows chunk * chunk_rows .. of modulation row blockIdx / chunks: one after another with a team of
+// A workgroup takes the rows chunk * chunk_rows .. of modulation row workgroup / chunks: one after another with a team of
 // several waves, one a wave where a wave is a team.
 template <int DT, int VDT, int NCH, bool VEC>
 __global__ __launch_bounds__(MAX_TEAM) void gated_norm_bwd_kernel(NormArgs a, GradArgs o, int team) {
@@ -242,7 +242,8 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_bwd_kernel(NormArgs a, Gr
   const bool one = team == 64;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const Span<NCH, VEC> span = {one ? (int)(threadIdx.x & 63) : (int)threadIdx.x, team, a.width};
-  const int64_t bg = blockIdx.x / o.chunks, chunk = blockIdx.x - bg * o.chunks;
+  const int64_t id = group_id(), bg = id / o.chunks, chunk = id - bg * o.chunks;
+  if (bg >= o.mrows) return;
   const int64_t b = bg / o.groups, g = bg - b * o.groups;
   int64_t t0 = g * a.group_len, t1 = min(t0 + a.group_len, a.len);
   t0 += chunk * o.chunk_rows;
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_bwd_kernel(NormArgs a, Gr
     span.template store<DT>(at<DT>(o.dy, row * a.width), d);
   }
   if (!o.sums) return;
-  float* out = o.sums + (int64_t)blockIdx.x * SUM_ROWS * a.width;
+  float* out = o.sums + id * SUM_ROWS * a.width;
   if (one && blockDim.x > 64) {   // the waves' sums into one, in their order
     for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
       if (w == wave) {
@@ -428,14 +429,15 @@ int slices_for(int64_t rows) {   // (two at least: whole waves)
   return n;
 }
 
-// The workgroups' sums of one modulation row (blockIdx.x / tiles), SUM_COLS channels a workgroup, its half-waves taking them in turn,
+// The workgroups' sums of one modulation row (workgroup / tiles), SUM_COLS channels a workgroup, its half-waves taking them in turn,
 // four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which a single
 // modulation row does not need: `last`).
 template <int VDT>
 __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int tiles, int last) {
   __shared__ float part[SLICES][SUM_ROWS][SUM_COLS];
   const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS, slices = blockDim.x / SUM_COLS;
-  const int64_t bg = blockIdx.x / tiles, ch = SUM_COLS * (blockIdx.x - bg * tiles) + lane, b = bg / o.groups, g = bg - b * o.groups;
+  const int64_t id = group_id(), bg = id / tiles, ch = SUM_COLS * (id - bg * tiles) + lane, b = bg / o.groups, g = bg - b * o.groups;
+  if (bg >= o.mrows) return;
   float* base = o.sums + bg * o.chunks * SUM_ROWS * a.width;
   float s[SUM_ROWS] = {};
   if (ch < a.width) {
@@ -477,13 +479,13 @@ __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(Norm
 
 // The modulation rows' sums, weighted and added: the gradients of what they share.
 template <int VDT>
-__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_shared_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int64_t rows) {
+__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_shared_sums_kernel(NormArgs a, GradArgs o, VecGrads d) {
   __shared__ float part[SLICES][2 * SUM_ROWS][SUM_COLS];
   const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS, slices = blockDim.x / SUM_COLS;
   const int64_t ch = SUM_COLS * (int64_t)blockIdx.x + lane;
   float t[2 * SUM_ROWS] = {};
   if (ch < a.width) {
-    for (int64_t bg = w; bg < rows; bg += slices) {
+    for (int64_t bg = w; bg < o.mrows; bg += slices) {
       const int64_t b = bg / o.groups;
       const float* p = o.sums + bg * o.chunks * SUM_ROWS * a.width + ch;
       const float s[SUM_ROWS] = {p[0], p[a.width], p[2 * a.width]};
@@ -553,7 +555,7 @@ void forward(const NormArgs& a, void* s_out, void* h_out, hipStream_t stream) {
   int nch = 0, team = 0;
   pick(a.width, a.rows <= FEW && a.width <= 8 * MAX_TEAM ? 1 : 3, nch, team);
   const int threads = team == 64 ? 256 : team;
-  const dim3 grid((unsigned)(team == 64 ? (a.rows + 3) / 4 : a.rows));
+  const dim3 grid = grid_of(team == 64 ? (a.rows + 3) / 4 : a.rows);
   if (nch == 1) gated_norm_kernel<DT, VDT, 1, VEC><<<grid, threads, 0, stream>>>(a, team, s_out, h_out);
   else if (nch == 2) gated_norm_kernel<DT, VDT, 2, VEC><<<grid, threads, 0, stream>>>(a, team, s_out, h_out);
   else gated_norm_kernel<DT, VDT, 3, VEC><<<grid, threads, 0, stream>>>(a, team, s_out, h_out);
@@ -578,7 +580,7 @@ void split(int64_t rows, int64_t len, int64_t group_len, int nch, int team, int6
 template <int DT, int VDT, bool VEC>
 void backward(const NormArgs& a, const GradArgs& o, int nch, int team, hipStream_t stream) {
   const int threads = team == 64 ? (int)(64 * (o.chunk_rows < 8 ? o.chunk_rows : 8)) : team;
-  const dim3 grid((unsigned)(a.rows / a.len * o.groups * o.chunks));
+  const dim3 grid = grid_of(o.mrows * o.chunks);
   if (nch == 1) gated_norm_bwd_kernel<DT, VDT, 1, VEC><<<grid, threads, 0, stream>>>(a, o, team);
   else if (nch == 2) gated_norm_bwd_kernel<DT, VDT, 2, VEC><<<grid, threads, 0, stream>>>(a, o, team);
   else gated_norm_bwd_kernel<DT, VDT, 3, VEC><<<grid, threads, 0, stream>>>(a, o, team);
@@ -677,22 +679,21 @@ extern "C" int lbw_gated_norm_bwd(const void* ds, const void* dh, const void* x,
   if (sums && !good(workspace, 16)) return LBW_E_ALIGN;
   int nch = 0, team = 0;
   pick_bwd(width, nch, team);
-  GradArgs o = {ds, dh, dx, dy, sums ? (float*)workspace : nullptr, groups, 0, 0};
+  GradArgs o = {ds, dh, dx, dy, sums ? (float*)workspace : nullptr, groups, batch * groups, 0, 0};
   split(a.rows, len, group_len, nch, team, o.chunk_rows, o.chunks);
-  if (batch * groups * o.chunks > (1 << 30) || batch * groups * ((width + SUM_COLS - 1) / SUM_COLS) > (1 << 30))
+  if (o.mrows * o.chunks > (1 << 30) || o.mrows * ((width + SUM_COLS - 1) / SUM_COLS) > (1 << 30))
     return LBW_E_SHAPE;
   if (const int st = check_device()) return st;
   by_type(dtype, vec_dtype, vec, [&](auto dt, auto vt, auto w) {
     backward<dt.value, vt.value, w.value>(a, o, nch, team, (hipStream_t)stream);
     if (!sums) return;
-    const int64_t mrows = batch * groups;
     const unsigned tiles = (unsigned)((width + SUM_COLS - 1) / SUM_COLS);
-    norm_group_sums_kernel<vt.value><<<(unsigned)(tiles * mrows), SUM_COLS * slices_for(o.chunks), 0, (hipStream_t)stream>>>(
-        a, o, d, (int)tiles, mrows == 1);
+    norm_group_sums_kernel<vt.value><<<grid_of(tiles * o.mrows), SUM_COLS * slices_for(o.chunks), 0, (hipStream_t)stream>>>(
+        a, o, d, (int)tiles, o.mrows == 1);
     const bool shared = dweight || dbias || dpost_weight || (dgate && !d.gate_rows) ||
                         (dscale && !d.scale_rows) || (dshift && !d.shift_rows);
-    if (shared && mrows > 1)
-      norm_shared_sums_kernel<vt.value><<<tiles, SUM_COLS * slices_for(mrows), 0, (hipStream_t)stream>>>(a, o, d, mrows);
+    if (shared && o.mrows > 1)
+      norm_shared_sums_kernel<vt.value><<<tiles, SUM_COLS * slices_for(o.mrows), 0, (hipStream_t)stream>>>(a, o, d);
   });
   return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
 }

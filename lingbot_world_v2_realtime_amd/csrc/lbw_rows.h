@@ -7,6 +7,14 @@
 
 namespace lbw {
 
+// Workgroups in any number up to 2^36: a grid dimension holds fewer than 2^32 threads, so past 2^20 workgroups there is a
+// second one, whose last part may have workgroups past the end.
+constexpr unsigned GRID_X = 1u << 20;
+inline dim3 grid_of(int64_t n) {
+  return dim3((unsigned)(n < GRID_X ? n : GRID_X), (unsigned)((n + GRID_X - 1) / GRID_X));
+}
+__device__ __forceinline__ uint32_t group_id() { return blockIdx.x + blockIdx.y * GRID_X; }
+
 constexpr int elem_size(int dt) { return dt == LBW_DTYPE_FP32 ? 4 : 2; }
 
 // One value.

@@ -82,7 +82,8 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
   constexpr int U = N == 1 ? 4 : 1;
   __shared__ float2 cs[MAX_TOKENS * MAX_PAIRS];
   __shared__ int64_t at_tok[MAX_TOKENS][4];   // where a token's rows start: q, k, and in the outputs
-  const int64_t tok0 = (int64_t)blockIdx.x * a.per_group;
+  const int64_t tok0 = (int64_t)group_id() * a.per_group;
+  if (tok0 >= a.tokens) return;
   const int ntok = (int)min((int64_t)a.per_group, a.tokens - tok0);
   if (threadIdx.x < ntok) {
     const uint32_t tok = (uint32_t)(tok0 + threadIdx.x), b = tok / (uint32_t)a.len, t = tok - b * (uint32_t)a.len;
@@ -158,8 +159,8 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
 
 template <int DT, int N>
 void launch(const RotaryArgs& a, bool inter, int64_t grid, hipStream_t stream) {
-  if (inter) rotary_kernel<DT, N, true><<<(unsigned)grid, THREADS, 0, stream>>>(a);
-  else rotary_kernel<DT, N, false><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  if (inter) rotary_kernel<DT, N, true><<<grid_of(grid), THREADS, 0, stream>>>(a);
+  else rotary_kernel<DT, N, false><<<grid_of(grid), THREADS, 0, stream>>>(a);
 }
 
 template <int DT>

@@ -556,7 +556,7 @@ W4_NIBBLES = {"int4": (0, 2, 4, 6, 1, 3, 5, 7), "fp4": (0, 1, 2, 3, 4, 5, 6, 7)}
 
 def pack_w4(codes, scale, zero=None, fmt="int4"):
     """Codes a checkpoint holds (uint8 [N, K], values 0 .. 15), with their scales (and zeros) [N, ceil(K / group)], in the
-    tiles gemm_w4 takes: (w4, scale bf16, zero uint8 or None) as quant_w4 makes them. Runs once at load, on any device."""
+    tiles gemm_w4 takes: (w4, scale rounded to bf16, zero uint8 or None) as quant_w4 makes them. Runs once at load, on any device."""
     if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.numel() == 0:
         raise ValueError(f"codes must be uint8 [N, K], got {codes.dtype} {tuple(codes.shape)}")
     if fmt not in W4_FORMATS or (zero is not None and fmt != "int4"):

@@ -19,8 +19,8 @@ from torch.autograd import forward_ad
 
 from .. import kernels
 
-__all__ = ["FP8Linear", "MXFP8Linear", "W4Linear", "convert_to_fp8", "convert_to_w4", "fp8_eligible", "use_tuned_gemms", "tune_gemms",
-           "GEMM_TABLE"]
+__all__ = ["FP8Linear", "MXFP8Linear", "W4Linear", "convert_to_fp8", "convert_to_w4", "fp8_eligible",
+           "use_tuned_gemms", "tune_gemms", "GEMM_TABLE"]
 
 # hipBLASLt solutions for the DiT's rowwise FP8 GEMMs at the chunk shape (6032 tokens), as a TunableOp results file (what
 # torch._scaled_mm takes; lbw_gemm_fp8_rows does not look at it):
@@ -217,6 +217,8 @@ class W4Linear(torch.nn.Module):
                                "a detached input")
         x2 = x.reshape(-1, shape[-1])
         if x2.dtype not in (torch.bfloat16, torch.float16):
+            if not x2.is_floating_point():
+                raise TypeError(f"W4Linear takes floating-point activations, got {x2.dtype}")
             x2 = x2.to(torch.bfloat16)
         if x2.shape[1] > 1 and x2.stride(1) != 1:
             x2 = x2.contiguous()
@@ -232,14 +234,19 @@ class W4Linear(torch.nn.Module):
 
 
 def convert_to_w4(blocks, group=128, fmt="int4", zeros=False, min_features=1024):
-    """Replace every nn.Linear below `blocks` with both dimensions at least min_features by W4Linear, in place. Returns
+    """Replace every nn.Linear below `blocks` with both dimensions at least min_features by W4Linear, in place: one that
+    stands in several places in all of them; subclasses of nn.Linear stay, as their owners may read their weight. Returns
     (replaced, linears seen)."""
-    found = [(path, m) for path, m in blocks.named_modules() if path and isinstance(m, torch.nn.Linear)]
-    chosen = [(path, m) for path, m in found if min(m.in_features, m.out_features) >= min_features]
-    for path, m in chosen:
+    found = [(path, m) for path, m in blocks.named_modules(remove_duplicate=False) if path and type(m) is torch.nn.Linear]
+    made = {}
+    for path, m in found:
+        if min(m.in_features, m.out_features) < min_features:
+            continue
+        if m not in made:
+            made[m] = W4Linear(m, group, fmt, zeros)
         owner, _, attr = path.rpartition(".")
-        setattr(blocks.get_submodule(owner), attr, W4Linear(m, group, fmt, zeros))
-    return len(chosen), len(found)
+        setattr(blocks.get_submodule(owner), attr, made[m])
+    return len(made), len({m for _, m in found})
 
 
 def fp8_eligible(lin, mx=False):

@@ -9,6 +9,7 @@ from .. import kernels
 
 __all__ = ["gated_norm"]
 
+
 def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=None, post_weight=None, norm="layer",
                post_norm=None, eps=1e-6, residual_scale=1.0, branch_scale=1.0, group_len=None):
     """The stream and the next sub-layer's input, in one pass:

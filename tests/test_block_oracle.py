@@ -252,6 +252,15 @@ def test_host_tensors_are_refused():
         kernels.gemm_w4(torch.zeros(2, 128), None, None)
 
 
+def test_lazy_and_learned_arguments_are_refused():
+    """A negation that is not in memory yet, and a factor given as a tensor, whose gradient a number would lose."""
+    x = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="negated"):
+        gated_norm(torch._neg_view(x))
+    with pytest.raises(ValueError, match="negated"):
+        rotary_embed(torch._neg_view(x.view(1, 4, 1, 64)), None, 0, Rotary.build(64, "cpu"))
+
+
 def test_pack_w4_refusals():
     codes, scale = torch.zeros(4, 128, dtype=torch.uint8), torch.ones(4, 1)
     for bad in (dict(codes=codes.int()), dict(codes=codes[0]), dict(scale=torch.ones(4, 3)), dict(scale=torch.ones(3, 1)),
@@ -267,3 +276,15 @@ def test_convert_to_w4_selects(monkeypatch):
     net = torch.nn.Sequential(torch.nn.Linear(1024, 1536), torch.nn.Linear(1536, 512), torch.nn.GELU())
     assert convert_to_w4(net) == (1, 2)
     assert isinstance(net[0], W4Linear) and type(net[1]) is torch.nn.Linear and net[0].out_features == 1536
+
+
+def test_convert_to_w4_shared_and_derived(monkeypatch):
+    """A linear that stands in two places is replaced in both by one module; a subclass (its owner may read its weight, as
+    nn.MultiheadAttention does) stays."""
+    monkeypatch.setattr(kernels, "quant_w4", lambda w, group, fmt, zeros: (
+        torch.zeros(1, dtype=torch.uint8), torch.zeros(1, dtype=torch.bfloat16), None))
+    lin = torch.nn.Linear(1024, 1024)
+    net = torch.nn.ModuleDict({"a": torch.nn.Sequential(lin, torch.nn.GELU(), lin), "b": torch.nn.MultiheadAttention(1024, 8)})
+    assert convert_to_w4(net) == (1, 1)
+    assert isinstance(net["a"][0], W4Linear) and net["a"][2] is net["a"][0]
+    assert isinstance(net["b"].out_proj, torch.nn.Linear)

@@ -685,3 +685,79 @@ def test_block_step():
         ws, wh, _ = block.gated_norm(x, y, **kw)
         _within(s, ws, "stream", 96)
         _within(h2, wh, "second norm", 96)
+
+
+# ---------------------------------------------------------------- the largest launches
+
+
+def _tail(t, rows):
+    return t[:, -rows:]
+
+
+def test_gated_norm_more_threads_than_a_grid_dimension():
+    """2^26 + 5 narrow rows, a wave each: more than the 2^32 threads that one grid dimension holds. A modulation row for every
+    token, so its gradient's workgroups are as many."""
+    from lingbot_world_v2_realtime_amd import kernels
+    n, c, last = 2 ** 26 + 5, 8, 4099
+    g = _rand(60)
+    x, shift, dh = (torch.randn(1, n, c, device=DEV, generator=g, dtype=torch.bfloat16) for _ in range(3))
+    print("rows", n, "forward", flush=True)
+    h = kernels.gated_norm(x, shift=shift, norm="rms")[1]
+    for part in (slice(0, last), slice(n - last, n), slice(2 ** 22 - 70, 2 ** 22 + 70)):
+        _within(h[:, part], block.gated_norm(x[:, part], shift=shift[:, part], norm="rms")[1], f"h {part}", 96)
+    del h
+    print("rows", n, "backward", flush=True)
+    d = kernels.gated_norm_bwd(x, None, dh, shift=shift, norm="rms", wants=("x", "shift"))
+    assert torch.equal(d["shift"], dh)   # each the sum of one row
+    one = kernels.gated_norm_bwd(_tail(x, last), None, _tail(dh, last).contiguous(), shift=_tail(shift, last), norm="rms",
+                                 wants=("x",))
+    assert torch.equal(_tail(d["x"], last), one["x"])
+
+
+def test_rotary_more_threads_than_a_grid_dimension():
+    from lingbot_world_v2_realtime_amd import kernels
+    n, last = 2 ** 27 + 11, 4099
+    q = torch.randn(1, n, 1, 2, device=DEV, generator=_rand(61), dtype=torch.bfloat16)
+    freq = torch.tensor([0.7], dtype=torch.float64, device=DEV)
+    print("tokens", n, flush=True)
+    out = kernels.rotary(q, None, 5, freq)[0]
+    for part in (slice(0, last), slice(n - last, n)):
+        pos = torch.arange(5 + part.start, 5 + part.stop, device=DEV)
+        _within(out[:, part], block.rotary(q[:, part], pos, freq), f"{part}", 13)
+
+
+def test_flags_numbers_and_overlaps():
+    """Flags of any truth value; factors and frequencies that would lose their gradient, and outputs that overlap their input,
+    are refused."""
+    from lingbot_world_v2_realtime_amd import Rotary, gated_norm, kernels, rotary_embed
+    rope = Rotary.build(64, DEV)
+    q, _ = _qk(62, 1, 9, 2, 1, 64)
+    want = rotary_embed(q, None, 0, rope)[0]
+    buf = torch.zeros(1, 10, 2, 64, device=DEV, dtype=q.dtype)
+    buf[:, :9] = q
+    with pytest.raises(ValueError, match="overlaps"):
+        kernels.rotary(buf[:, :9], None, 0, rope.freq, q_out=buf[:, 1:])
+    assert rotary_embed(q, None, 0, rope, inplace=1)[0].data_ptr() == q.data_ptr() and torch.equal(q, want)
+    learned = Rotary(rope.freq.clone().requires_grad_())
+    with pytest.raises(ValueError, match="freq"):
+        rotary_embed(q, None, 0, learned)
+    with torch.no_grad():
+        assert torch.equal(rotary_embed(q, None, 0, learned)[0], rotary_embed(q, None, 0, rope)[0])
+    x = torch.randn(1, 4, 64, device=DEV)
+    for name in ("residual_scale", "branch_scale", "eps"):
+        with pytest.raises(TypeError, match="gradient"):
+            gated_norm(x, x, **{name: torch.ones((), requires_grad=True)})
+    assert kernels.gated_norm(x, x, want_stream=1)[0] is not None and kernels.gated_norm(x, x, want_stream=0)[0] is None
+    grad = torch._neg_view(torch.randn(1, 4, 64, device=DEV))
+    leaf = x.clone().requires_grad_()
+    got = torch.autograd.grad(gated_norm(leaf), leaf, grad)[0]
+    assert torch.equal(got, torch.autograd.grad(gated_norm(leaf), leaf, grad.resolve_neg())[0])
+
+
+def test_w4_linear_takes_floating_point_rows():
+    from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
+    mod = W4Linear(torch.nn.Linear(128, 16).to(DEV))
+    with torch.no_grad():
+        with pytest.raises(TypeError, match="floating-point"):
+            mod(torch.ones(2, 128, device=DEV, dtype=torch.int64))
+        assert mod(torch.ones(0, 128, device=DEV)).shape == (0, 16)
