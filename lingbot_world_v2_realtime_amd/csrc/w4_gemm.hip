@@ -4,7 +4,7 @@
 // A code enters the products exactly. fp4 converts by the hardware's own instruction. An integer code c becomes 1 + c / 16 in
 // the 16-bit format: its four bits placed in the mantissa of 1, a shift and a mask for two codes (converting to the signed integer
 // instead takes three more operations a pair). With v = c - z the group's sum is then
-//   sum x v = 16 sum x (1 + c / 16) - (16 + z) sum x,
+//   sum x v = 16 (sum x (1 + c / 16) - (1 + z / 16) sum x),
 // sum x from one more matrix instruction a step (x times ones) whose result stands where the products' do. Group sums are
 // scaled in fp32: out += s (...) for every group, so neither scale nor zero is ever rounded into a 16-bit weight.
 #include "lbw_rows.h"
@@ -90,9 +90,18 @@ __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c) {
 template <int DT>
 constexpr uint32_t ONES = DT == LBW_DTYPE_FP16 ? 0x3C003C00u : 0x3F803F80u;
 
+// Those in a vector register: mask and ones then enter one instruction (which takes a single scalar or literal), not two. With the
+// factor of 16 left to the end a K tile takes 357 vector instructions beside its 68 products, not 437 (2048 x 8192 x 6144 with zeros: 238 -> 229 us).
+template <int DT>
+__device__ __forceinline__ uint32_t vector_ones() {
+  uint32_t r;
+  asm("v_mov_b32 %0, %1" : "=v"(r) : "i"(ONES<DT>));
+  return r;
+}
+
 // The 8 codes of a word as 16-bit operands: integer codes as 1 + c / 16, fp4 codes as their values.
 template <int DT, Form F>
-__device__ __forceinline__ v4i operand(uint32_t w) {
+__device__ __forceinline__ v4i operand(uint32_t w, uint32_t ones) {
   v4i r;
   if constexpr (F == FP4) {
     if constexpr (DT == LBW_DTYPE_FP16) {
@@ -111,7 +120,7 @@ __device__ __forceinline__ v4i operand(uint32_t w) {
     constexpr int S = DT == LBW_DTYPE_FP16 ? 6 : 3;
     constexpr uint32_t M = 0x000F000Fu << S;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) r[t] = (int)(((4 * t < S ? w << (S - 4 * t) : w >> (4 * t - S)) & M) | ONES<DT>);
+    for (int t = 0; t < 4; ++t) r[t] = (int)(((4 * t < S ? w << (S - 4 * t) : w >> (4 * t - S)) & M) | ones);
   }
   return r;
 }
@@ -164,19 +173,35 @@ struct RowsOfX {
   }
 };
 
-// Four columns of the output from n on (a multiple of 4), with the bias: 8 bytes at once where the output's rows allow it.
-template <int DT>
-__device__ __forceinline__ void store_out(const GemmArgs& a, int64_t m, int64_t n, v4f y) {
-  if (a.n % 4 == 0) {
-    if (a.bias) {
+// The bias of four columns of the output from n on, in its own format: without a branch around a load (past the last column the
+// last is read again), so that all are in flight together.
+struct Bias {
+  uint16_t w[4];
+  __device__ __forceinline__ Bias(const GemmArgs& a, int64_t n) : w{0, 0, 0, 0} {
+    if (!a.bias) return;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += load1<DT>(a.bias, n + e);
-    }
+    for (int e = 0; e < 4; ++e) w[e] = ((const uint16_t*)a.bias)[min(n + e, a.n - 1)];
+  }
+};
+
+// Sums of four columns with their bias. Integer codes were taken as sixteenths.
+template <int DT, Form F>
+__device__ __forceinline__ v4f finished(v4f y, const Bias& bias) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = fmaf(F == FP4 ? 1.f : 16.f, y[e], load1<DT>(bias.w, e));
+  return y;
+}
+
+// Four columns of the output from n on (a multiple of 4), 8 bytes at once where the output's rows allow it.
+template <int DT, Form F>
+__device__ __forceinline__ void store_out(const GemmArgs& a, int64_t m, int64_t n, v4f y, const Bias& bias) {
+  y = finished<DT, F>(y, bias);
+  if (a.n % 4 == 0) {
     *(v2i*)((uint16_t*)a.out + m * a.n + n) = v2i{(int)pack2<DT>(y[0], y[1]), (int)pack2<DT>(y[2], y[3])};
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (n + e < a.n) store1<DT>(a.out, m * a.n + n + e, y[e] + (a.bias ? load1<DT>(a.bias, n + e) : 0.f));
+      if (n + e < a.n) store1<DT>(a.out, m * a.n + n + e, y[e]);
   }
 }
 
@@ -214,7 +239,7 @@ struct Scales {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = PER * e + g;
-      r[e] = __uint_as_float(i & 1 ? s[i >> 1] & 0xFFFF0000u : s[i >> 1] << 16) * (F == FP4 ? 1.f : 16.f);
+      r[e] = __uint_as_float(i & 1 ? s[i >> 1] & 0xFFFF0000u : s[i >> 1] << 16);
     }
     return r;
   }
@@ -271,6 +296,7 @@ __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) out[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
   }
+  const uint32_t one = vector_ones<DT>();
   v4i w[NT], x[4 * MT];
   Scales<F, PER> sc[NT];
   const auto load = [&](int64_t t) {
@@ -315,7 +341,7 @@ __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
         for (int i = 0; i < MT; ++i) acc[i] = cc[n].start(g, sum[i]);
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
-          const v4i b = operand<DT, F>((uint32_t)wc[n][g * STEPS + j]);
+          const v4i b = operand<DT, F>((uint32_t)wc[n][g * STEPS + j], one);
 #pragma unroll
           for (int i = 0; i < MT; ++i) acc[i] = mfma<DT>(b, xo[i][j], acc[i]);
         }
@@ -339,22 +365,25 @@ __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
     if (m >= a.m || n >= a.n) continue;
     v4f y = *(const v4f*)(part + i);
     for (int w = 1; w < waves; ++w) y += *(const v4f*)(part + w * (ROWS * COLS) + i);
-    store_out<DT>(a, m, n, y);
+    store_out<DT, F>(a, m, n, y, Bias(a, n));
   }
 }
 
 // Many rows: 64 rows x 256 columns a workgroup, four waves of 64 x 64, two workgroups a CU (which drift apart, so that one's
-// matrix work runs under the other's conversions: 57.5 us for 1508 x 8960 x 1536 against 62.7 with eight waves in step on 128 rows).
+// matrix work runs under the other's conversions: 57.5 us for 1508 x 8960 x 1536 against 62.7 with eight waves in step on 128 rows,
+// both before the last steps; now 51.3, 810 TFLOP/s, and 1000 where K is 6144 and the grid fills whole rounds).
 // x passes through LDS, a K tile at a time in two buffers (rows and pieces as above): wave w loads rows 16 w .. 16 w + 15 in the
 // operands' own order, forms their sums over each group while they are in registers, and leaves both there. Codes go from
-// memory to registers, a tile ahead.
+// memory to registers, a tile ahead. The output leaves through LDS, so that a store holds whole rows of 128 bytes (1508 x 8960 x
+// 1536, zeros and bias: 68.1 -> 64.9 us; with no store at all 61.2). The conversions bound it: vector instructions take about
+// 1.3 times the matrix core's cycles, and two waves a SIMD overlap the two in part.
 constexpr int GM = 64, GN = 256;
 constexpr int X_TILE = GM * TK * 2;   // bytes
 
 template <int DT, Form F, int GROUP>
 __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(GemmArgs a, int m_tiles) {
   constexpr int PER = TK / GROUP, STEPS = GROUP / 32;
-  __shared__ __align__(16) char xs[2][X_TILE];
+  __shared__ __align__(16) char xs[2][X_TILE];   // (afterwards the output, GM * 128 bytes a wave)
   __shared__ float sums[2][PER][GM];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -376,6 +405,7 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(GemmArgs a, int m_tiles
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
 
+  const uint32_t one = vector_ones<DT>();
   v4i xr[4], w[4];
   Scales<F, PER> sc[4];
   const auto load = [&](int64_t t) {
@@ -423,7 +453,7 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(GemmArgs a, int m_tiles
         for (int i = 0; i < 4; ++i) acc[i] = sc[n].start(g, sum[i]);
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
-          const v4i b = operand<DT, F>((uint32_t)w[n][g * STEPS + j]);
+          const v4i b = operand<DT, F>((uint32_t)w[n][g * STEPS + j], one);
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[i] = mfma<DT>(b, x[i][j], acc[i]);
         }
@@ -445,14 +475,37 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(GemmArgs a, int m_tiles
     leave(buf ^ 1);
     __syncthreads();
   }
+  const int64_t col0 = nt0 * TN + 4 * q;
+  const Bias bias[4] = {{a, col0}, {a, col0 + TN}, {a, col0 + 2 * TN}, {a, col0 + 3 * TN}};
+  if (a.n % 8 == 0 && (uintptr_t)a.out % 16 == 0) {
+    char* mine = xs[0] + wave * (GM * 128);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const v4f y = finished<DT, F>(out[n][i], bias[n]);
+        *(v2i*)(mine + (16 * i + r) * 128 + (((2 * n + (q >> 1)) ^ (r & 7)) << 4) + 8 * (q & 1)) =
+            v2i{(int)pack2<DT>(y[0], y[1]), (int)pack2<DT>(y[2], y[3])};
+      }
+    __builtin_amdgcn_wave_barrier();
+    const int piece = lane & 7;
+    const int64_t col = nt0 * TN + 8 * piece;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 8 * i + (lane >> 3);
+      const v4i y = *(const v4i*)(mine + row * 128 + ((piece ^ (row & 7)) << 4));
+      if (m0 + row < a.m && col < a.n) *(v4i*)((uint16_t*)a.out + (m0 + row) * a.n + col) = y;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t m = m0 + 16 * i + r;
     if (m >= a.m) continue;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const int64_t col = (nt0 + n) * TN + 4 * q;
-      if (col < a.n) store_out<DT>(a, m, col, out[n][i]);
+      const int64_t col = col0 + n * TN;
+      if (col < a.n) store_out<DT, F>(a, m, col, out[n][i], bias[n]);
     }
   }
 }
@@ -474,8 +527,9 @@ void launch_rows(const GemmArgs& a, int most, hipStream_t stream) {
 //   24 x 1536 x 8960:   16 x 16 tiles 7.3,  32 x 16 9.8,  32 x 48 19.6     32 x 8960 x 1536: 32 x 16 7.6, 32 x 48 6.0
 //   128 x 1536 x 8960:  32 x 16 17.3, 16 x 48 12.3, 32 x 48 17.8          256 x 1536 x 8960: 16 x 48 20.6, 32 x 48 18.1
 // With 32 x 48 tiles past one round two workgroups of four waves share a CU better than one of six (512 x 1536 x 8960: 28.6
-// against 34.4). Whole tiles of 64 x 256 win from more than half a tile a CU on: 256 x 8960 x 1536 (140 tiles) 20.7 against 22.1,
-// 512 x 8960 x 1536 (280) 30.7 against 40.0, but 1508 x 1536 x 8960 (144) 96 against 79.
+// against 34.4). Whole tiles of 64 x 256 win from about half a tile a CU on: 256 x 8960 x 1536 (140 tiles) 18.0 against 20.9,
+// 1508 x 1536 x 1536 (144) 17.8 against 19.8, 512 x 8960 x 1536 (280) 26.3 against 36.5, about even for 1508 x 1536 x 8960 (144)
+// 84 against 81; but 1024 x 1536 x 1536 (96) 17.4 against 14.5.
 template <int DT, Form F, int GROUP>
 void launch_group(const GemmArgs& a, bool vec, hipStream_t stream) {
   const auto grid = [&](int rows, int cols) { return ((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols); };
@@ -484,7 +538,7 @@ void launch_group(const GemmArgs& a, bool vec, hipStream_t stream) {
   else if (a.m <= 16) launch_rows<DT, F, GROUP, 1, 1, 8, true>(a, 8, stream);
   else if (grid(32, 16) <= CUS) launch_rows<DT, F, GROUP, 2, 1, 8, true>(a, 8, stream);
   else if (grid(16, 48) <= CUS) launch_rows<DT, F, GROUP, 1, 3, 8, true>(a, 8, stream);
-  else if (grid(GM, GN) < 160) launch_rows<DT, F, GROUP, 2, 3, 6, true>(a, grid(32, 48) <= CUS ? 6 : 4, stream);
+  else if (grid(GM, GN) < CUS / 2) launch_rows<DT, F, GROUP, 2, 3, 6, true>(a, grid(32, 48) <= CUS ? 6 : 4, stream);
   else w4_gemm_kernel<DT, F, GROUP><<<(unsigned)((grid(GM, GN) + 7) / 8 * 8), 4 * GM, 0, stream>>>(a, (int)grid(GM, 1 << 30));
 }
 
