@@ -1,10 +1,10 @@
-// The block operators' calls from Python: tensors checked, outputs allocated and the C-ABI of include/lbw_block.h called in
-// one native step. A call of these is bound by its host side (a token's norm takes 4 us on the GPU); the same checks and the
-// 33 arguments of a ctypes call took 15-19 us in Python, against 5 here.
+// The block operators' calls from Python: tensors checked, outputs allocated and the C-ABI of include/lbw_block.h
+// called in one native step. A call of these is bound by its host side (a token's norm takes 4 us on the GPU); the
+// same checks and the 33 arguments of a ctypes call took 15-19 us in Python, against 5 here.
 //
-// Every function takes its arguments by position (kernels.py holds the signatures that users see), runs on the current
-// stream of its first tensor's device, with that device current, and raises ValueError / TypeError for what it does not
-// take. A status from the library goes to the function that `on_status` was given, which raises.
+// Every function takes its arguments by position (kernels.py holds the signatures that users see), runs on the
+// current stream of its first tensor's device, with that device current, and raises ValueError / TypeError for what
+// it does not take. A status from the library goes to the function that `on_status` was given, which raises.
 #include <Python.h>
 
 #include <ATen/MemoryOverlap.h>
@@ -134,7 +134,8 @@ struct On {
   explicit On(const Tensor& t) : guard(t.device().index()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-// A bad status: raised by the Python side's function, or, in a backward pass (which runs without the interpreter), as torch's error.
+// A bad status: raised by the Python side's function, or, in a backward pass (which runs without the interpreter), as
+// torch's error.
 void done(int status, const char* what, bool python = true) {
   if (status == LBW_OK) return;
   TORCH_CHECK(python, what, " failed: status ", status, " (", lbw_status_string(status), ")");
@@ -146,7 +147,8 @@ void done(int status, const char* what, bool python = true) {
 
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
-// Whether autograd has to see the call: a gradient is recorded, or an input carries a forward-mode tangent (which it refuses).
+// Whether autograd has to see the call: a gradient is recorded, or an input carries a forward-mode tangent (which it
+// refuses).
 bool records_gradient(std::initializer_list<Tensor> ts) {
   for (const Tensor& t : ts)
     if (t.defined() && ((c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())) return true;
@@ -274,7 +276,8 @@ struct Norm {
     return {s, h};
   }
 
-  // The gradients of x, y and the vectors, those with their bit in `wants`. ds and dh are packed, of x's type and shape.
+  // The gradients of x, y and the vectors, those with their bit in `wants`. ds and dh are packed, of x's type and
+  // shape.
   std::array<Tensor, 2 + VECTORS> backward(const Tensor& ds, const Tensor& dh, int64_t wants, bool python) const {
     std::array<Tensor, 2 + VECTORS> g;
     void* p[2 + VECTORS] = {};
@@ -341,8 +344,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
   }
 };
 
-// The operator as users call it: (s or None, h or None), with a gradient where one is recorded. Vectors of different types are taken
-// in fp32.
+// The operator as users call it: (s or None, h or None), with a gradient where one is recorded. Vectors of different
+// types are taken in fp32.
 PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, Norm::ARGS);
@@ -379,8 +382,8 @@ PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The gradients alone: the norm's arguments, ds, dh, and a bit for each of x, y and the vectors. A tuple of those, None for the
-// others.
+// The gradients alone: the norm's arguments, ds, dh, and a bit for each of x, y and the vectors. A tuple of those,
+// None for the others.
 PyObject* gated_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, Norm::ARGS + 3);
@@ -530,8 +533,8 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   }
 };
 
-// The operator as users call it: q, k, positions, freq, axis, pairs, factor, layout, inplace. (q, k or None), with a gradient where
-// one is recorded.
+// The operator as users call it: q, k, positions, freq, axis, pairs, factor, layout, inplace. (q, k or None), with a
+// gradient where one is recorded.
 PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 9);
@@ -634,8 +637,8 @@ PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// Whether a kernel may take these tensors (None: absent) by their address: none records a gradient, carries a forward-mode
-// tangent, stands for others inside a torch.func transform, or is of a subclass.
+// Whether a kernel may take these tensors (None: absent) by their address: none records a gradient, carries a
+// forward-mode tangent, stands for others inside a torch.func transform, or is of a subclass.
 PyObject* plain(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const bool grad = c10::GradMode::is_enabled();

@@ -1,11 +1,12 @@
 // The gated norm between two sub-layers of a block (include/lbw_block.h), forward and backward.
 //
-// Both directions are bound by memory: a row's inputs are read once into registers, where its statistics, its
-// outputs and its gradients are formed, and nothing but the results goes back. A row belongs to a team of 64 lanes
-// (a wave; no barrier) or of more waves of one workgroup (sums through LDS); thread i of a team of T holds the 8-value
-// chunks i, i + T, ... of the row.
+// Both directions are bound by memory: a row's inputs are read once into registers, where its statistics, its outputs
+// and its gradients are formed, and nothing but the results goes back. A row belongs to a team of 64 lanes (a wave;
+// no barrier) or of more waves of one workgroup (sums through LDS); thread i of a team of T holds the 8-value chunks
+// i, i + T, ... of the row.
 //
-// Norm statistics take two passes over the registers (mean, then the mean square of the differences): no cancellation.
+// Norm statistics take two passes over the registers (mean, then the mean square of the differences): no
+// cancellation.
 //
 // Backward, with u = norm(s), lin = u w + c, h = lin (1 + scale) + shift, s = a x + b gate pw v, v = post(y):
 //   du = dh (1 + scale) w;  g = ds + r (du - [mean du] - u mean(du u))     (the bracket for LayerNorm)
@@ -15,9 +16,9 @@
 //   A = sum dh u,  B = sum dh,  C = sum g v:
 //   dshift = B, dscale = w A + c B, dgate = b pw C;  dweight = sum_rows (1 + scale) A, dbias = sum_rows (1 + scale) B,
 //   dpost_weight = b sum_rows gate C
-// A workgroup adds them over its rows (all of one modulation row) in registers and leaves one fp32 row each; a second kernel
-// adds the workgroups of a modulation row, a third the modulation rows where a vector is shared by several. No atomics: the order
-// of every sum is fixed by the sizes.
+// A workgroup adds them over its rows (all of one modulation row) in registers and leaves one fp32 row each; a second
+// kernel adds the workgroups of a modulation row, a third the modulation rows where a vector is shared by several. No
+// atomics: the order of every sum is fixed by the sizes.
 #include "lbw_rows.h"
 
 namespace lbw {
@@ -25,8 +26,8 @@ namespace {
 
 constexpr int MAX_TEAM = 512;
 constexpr int SUM_ROWS = 3;         // A, B, C of a workgroup's rows
-constexpr int SUM_COLS = 32;        // channels of a workgroup of the two summing kernels, and the slices of the summed rows at most
-constexpr int SLICES = 32;
+constexpr int SUM_COLS = 32;        // channels of a workgroup of the two summing kernels
+constexpr int SLICES = 32;          // and the slices of the rows that it sums, at most
 
 struct Vec {
   const void* p;
@@ -101,8 +102,9 @@ struct Span {
   }
 };
 
-// A vector that the forward multiplies or adds. With one chunk a thread (few rows: the call is as long as its longest chain of
-// loads) it is loaded at the row's start, with all the others; with more where it is used, for the registers.
+// A vector that the forward multiplies or adds. With one chunk a thread (few rows: the call is as long as its longest
+// chain of loads) it is loaded at the row's start, with all the others; with more where it is used, for the
+// registers.
 template <int DT, int NCH, bool VEC>
 struct Factor {
   const void* p;
@@ -127,8 +129,8 @@ struct Factor {
   }
 };
 
-// Sums over a team, the same bits in all its threads. One wave: no LDS. Else every wave leaves its sums in `red`, which
-// nobody may write again before another barrier has been passed.
+// Sums over a team, the same bits in all its threads. One wave: no LDS. Else every wave leaves its sums in `red`,
+// which nobody may write again before another barrier has been passed.
 template <int N>
 __device__ __forceinline__ void team_sum(float* v, int team, float* red) {
 #pragma unroll
@@ -152,8 +154,8 @@ constexpr int RED = 2 * (MAX_TEAM / 64);   // floats of a reduction's slot
 // f <- (f - mean) / sqrt(. + eps), zero past the width; returns the factor.
 template <int NCH, bool VEC>
 __device__ __forceinline__ float normalise(float (*f)[8], int kind, const Span<NCH, VEC>& at, float eps, float* red) {
-  // (divided, not multiplied by a rounded 1 / width: the mean of equal values is that value, and u = 0, wherever their sum is
-  // exact)
+  // (divided, not multiplied by a rounded 1 / width: the mean of equal values is that value, and u = 0, wherever
+  // their sum is exact)
   const float width = (float)at.width;
   if (kind == LBW_NORM_LAYER) {
     float s = 0.f;
@@ -232,8 +234,8 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_kernel(NormArgs a, int te
   span.template store<DT>(at<DT>(h_out, row * a.width), s);
 }
 
-// A workgroup takes the rows chunk * chunk_rows .. of modulation row workgroup / chunks: one after another with a team of
-// several waves, one a wave where a wave is a team.
+// A workgroup takes the rows chunk * chunk_rows .. of modulation row workgroup / chunks: one after another with a
+// team of several waves, one a wave where a wave is a team.
 template <int DT, int VDT, int NCH, bool VEC>
 __global__ __launch_bounds__(MAX_TEAM) void gated_norm_bwd_kernel(NormArgs a, GradArgs o, int team) {
   constexpr int ONE_WIDTH = 64 * 8 * NCH;   // the widest row of a one-wave team
@@ -379,8 +381,8 @@ __global__ __launch_bounds__(MAX_TEAM) void gated_norm_bwd_kernel(NormArgs a, Gr
   }
 }
 
-// The gradients of what all modulation rows share, from sums over them: sum (1 + scale) A, sum (1 + scale) B, sum gate C,
-// sum A, sum B, sum C.
+// The gradients of what all modulation rows share, from sums over them: sum (1 + scale) A, sum (1 + scale) B, sum
+// gate C, sum A, sum B, sum C.
 template <int VDT>
 __device__ __forceinline__ void finish(const NormArgs& a, const VecGrads& d, int64_t ch, const float* t) {
   if (d.weight) store1<VDT>(d.weight, ch, t[0]);
@@ -405,8 +407,8 @@ __device__ __forceinline__ void weigh(const NormArgs& a, int64_t b, int64_t g, i
   for (int k = 0; k < SUM_ROWS; ++k) t[SUM_ROWS + k] += s[k];
 }
 
-// The slices' sums of K values into those of slice 0, in halves (one slice adding all took 32 K reads in turn: 6.3 us for a kernel of
-// two rows). slices: a power of two, blockDim.x / SUM_COLS.
+// The slices' sums of K values into those of slice 0, in halves (one slice adding all took 32 K reads in turn: 6.3 us
+// for a kernel of two rows). slices: a power of two, blockDim.x / SUM_COLS.
 template <int K>
 __device__ __forceinline__ void add_slices(float (*part)[K][SUM_COLS], int w, int lane, int slices, float* s) {
 #pragma unroll
@@ -429,14 +431,17 @@ int slices_for(int64_t rows) {   // (two at least: whole waves)
   return n;
 }
 
-// The workgroups' sums of one modulation row (workgroup / tiles), SUM_COLS channels a workgroup, its half-waves taking them in turn,
-// four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which a single
-// modulation row does not need: `last`).
+// The workgroups' sums of one modulation row (workgroup / tiles), SUM_COLS channels a workgroup, its half-waves
+// taking them in turn, four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one
+// at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which
+// a single modulation row does not need: `last`).
 template <int VDT>
-__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int tiles, int last) {
+__global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int tiles,
+                                                                            int last) {
   __shared__ float part[SLICES][SUM_ROWS][SUM_COLS];
   const int lane = threadIdx.x % SUM_COLS, w = threadIdx.x / SUM_COLS, slices = blockDim.x / SUM_COLS;
-  const int64_t id = group_id(), bg = id / tiles, ch = SUM_COLS * (id - bg * tiles) + lane, b = bg / o.groups, g = bg - b * o.groups;
+  const int64_t id = group_id(), bg = id / tiles, ch = SUM_COLS * (id - bg * tiles) + lane;
+  const int64_t b = bg / o.groups, g = bg - b * o.groups;
   if (bg >= o.mrows) return;
   float* base = o.sums + bg * o.chunks * SUM_ROWS * a.width;
   float s[SUM_ROWS] = {};
@@ -497,8 +502,8 @@ __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_shared_sums_kernel(Nor
   finish<VDT>(a, d, ch, t);
 }
 
-// Chunks a thread holds and threads a row's team has: the fewest idle lanes, and of those the smallest team (one wave needs
-// no barrier; a tenth is added for those that do).
+// Chunks a thread holds and threads a row's team has: the fewest idle lanes, and of those the smallest team (one wave
+// needs no barrier; a tenth is added for those that do).
 void pick(int64_t width, int most, int& nch, int& team) {
   int64_t best = INT64_MAX;
   for (int c = most; c >= 1; --c) {
@@ -513,8 +518,8 @@ void pick(int64_t width, int most, int& nch, int& team) {
   }
 }
 
-// The backward holds three sums, two vectors and four rows of each: a third chunk spills (130 registers), and only the widest rows
-// need it.
+// The backward holds three sums, two vectors and four rows of each: a third chunk spills (130 registers), and only
+// the widest rows need it.
 void pick_bwd(int64_t width, int& nch, int& team) { pick(width, width <= 2 * 8 * MAX_TEAM ? 2 : 3, nch, team); }
 
 bool good(const void* p, int size) { return ((uintptr_t)p & (size - 1)) == 0; }
@@ -549,8 +554,9 @@ int check(const NormArgs& a, int dtype, int vec_dtype, int64_t batch, bool& vec,
 
 template <int DT, int VDT, bool VEC>
 void forward(const NormArgs& a, void* s_out, void* h_out, hipStream_t stream) {
-  // Few rows are a matter of latency: one chunk a thread and more threads a row (1536 channels, LayerNorm and post norm: 1 row 4.7 ->
-  // 3.7 us, 64 rows 5.6 -> 4.1, 1024 rows 6.0 -> 5.6; but 2048 rows 8.1 -> 8.2, and with 4096 channels 14.2 -> 15.9).
+  // Few rows are a matter of latency: one chunk a thread and more threads a row (1536 channels, LayerNorm and post
+  // norm: 1 row 4.7 -> 3.7 us, 64 rows 5.6 -> 4.1, 1024 rows 6.0 -> 5.6; but 2048 rows 8.1 -> 8.2, and with 4096
+  // channels 14.2 -> 15.9).
   constexpr int FEW = 1024;
   int nch = 0, team = 0;
   pick(a.width, a.rows <= FEW && a.width <= 8 * MAX_TEAM ? 1 : 3, nch, team);
@@ -561,10 +567,10 @@ void forward(const NormArgs& a, void* s_out, void* h_out, hipStream_t stream) {
   else gated_norm_kernel<DT, VDT, 3, VEC><<<grid, threads, 0, stream>>>(a, team, s_out, h_out);
 }
 
-// Rows of a workgroup of the backward. More workgroups keep more rows in flight, but each leaves three fp32 rows behind that are
-// written and read again (against six of `dtype` for every row of the tensors). With one chunk a thread 12 waves a CU are the best
-// (6032 x 1536 bf16, all gradients: 8 waves 41.4 us, 12 39.1, 16 39.8), with two 8, the registers' bound (4524 x 2048: 38.8,
-// 47.7, 47.6: a second round).
+// Rows of a workgroup of the backward. More workgroups keep more rows in flight, but each leaves three fp32 rows
+// behind that are written and read again (against six of `dtype` for every row of the tensors). With one chunk a
+// thread 12 waves a CU are the best (6032 x 1536 bf16, all gradients: 8 waves 41.4 us, 12 39.1, 16 39.8), with two 8,
+// the registers' bound (4524 x 2048: 38.8, 47.7, 47.6: a second round).
 void split(int64_t rows, int64_t len, int64_t group_len, int nch, int team, int64_t& chunk_rows, int64_t& chunks) {
   const int64_t gl = group_len < len ? group_len : len;
   const int waves = team == 64 ? 8 : team >> 6, room = nch == 1 ? (team == 64 ? 16 : 12) : 8;   // of a workgroup, and of a CU
@@ -647,7 +653,8 @@ extern "C" int lbw_gated_norm_bwd(const void* ds, const void* dh, const void* x,
                                   int64_t gate_s_batch, int64_t gate_s_group, const void* scale,
                                   int64_t scale_s_batch, int64_t scale_s_group, int rowwise,
                                   int64_t groups, int64_t group_len, const void* weight, const void* bias,
-                                  const void* post_weight, int norm, int post_norm, float eps, float residual_scale, float branch_scale, void* dx, void* dy, void* dgate,
+                                  const void* post_weight, int norm, int post_norm, float eps,
+                                  float residual_scale, float branch_scale, void* dx, void* dy, void* dgate,
                                   void* dshift, void* dscale, void* dweight, void* dbias, void* dpost_weight,
                                   void* workspace, void* stream) {
   NormArgs a = {x, y, 0, len, width, x_s_batch, x_s_tok, y_s_batch, y_s_tok, group_len,

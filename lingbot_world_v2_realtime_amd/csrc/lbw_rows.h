@@ -7,8 +7,8 @@
 
 namespace lbw {
 
-// Workgroups in any number up to 2^36: a grid dimension holds fewer than 2^32 threads, so past 2^20 workgroups there is a
-// second one, whose last part may have workgroups past the end.
+// Workgroups in any number up to 2^36: a grid dimension holds fewer than 2^32 threads, so past 2^20 workgroups there
+// is a second one, whose last part may have workgroups past the end.
 constexpr unsigned GRID_X = 1u << 20;
 inline dim3 grid_of(int64_t n) {
   return dim3((unsigned)(n < GRID_X ? n : GRID_X), (unsigned)((n + GRID_X - 1) / GRID_X));
@@ -45,8 +45,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// The 8 values p[i .. i + 8) as they lie in memory. VEC: i is a multiple of 8 and p 16-byte aligned (two loads of 16 bytes for
-// fp32); else value by value, those at or past `end` read as zero.
+// The 8 values p[i .. i + 8) as they lie in memory. VEC: i is a multiple of 8 and p 16-byte aligned (two loads of 16
+// bytes for fp32); else value by value, those at or past `end` read as zero.
 template <int DT, bool VEC>
 struct Raw8 {
   v4i w[DT == LBW_DTYPE_FP32 ? 2 : 1];

@@ -1,10 +1,11 @@
 // Rotary positions (include/lbw_block.h): q and k read once, rotated in registers, written once. Bound by memory.
 //
-// A workgroup takes a few tokens. Their angles are formed once for all heads: position * frequency in 64 bits, reduced to
-// (-1/2, 1/2] turns there (far positions lose nothing: an angle of 1e6 radians is still good to 1e-10), then sine and cosine of
-// the reduced angle in fp32, into LDS. The heads' values then pass through registers, 16 bytes a load: with neighbouring pairs
-// a load holds whole pairs; with halves a thread takes the 16 bytes of both partners. 6032 tokens of 24 heads of 128 in bf16 take
-// 13.4 us (5.5 TB/s; a copy of 1 GiB reaches 5.1), 24 of their 96 channels turned 11.6 with 8-byte units (53 value by value).
+// A workgroup takes a few tokens. Their angles are formed once for all heads: position * frequency in 64 bits,
+// reduced to (-1/2, 1/2] turns there (far positions lose nothing: an angle of 1e6 radians is still good to 1e-10),
+// then sine and cosine of the reduced angle in fp32, into LDS. The heads' values then pass through registers, 16
+// bytes a load: with neighbouring pairs a load holds whole pairs; with halves a thread takes the 16 bytes of both
+// partners. 6032 tokens of 24 heads of 128 in bf16 take 13.4 us (5.5 TB/s; a copy of 1 GiB reaches 5.1), 24 of their
+// 96 channels turned 11.6 with 8-byte units (53 value by value).
 #include "lbw_rows.h"
 
 namespace lbw {
@@ -72,13 +73,14 @@ struct Unit {
   }
 };
 
-// N: values of a unit (16 bytes of the format, 8, or one value, as strides, sizes and addresses allow). An item is two units:
-// those of partners (with INTER N pairs, 2 N channels in a row, else N channels in each half), or two neighbouring ones of the
-// channels past the pairs, which are copied.
+// N: values of a unit (16 bytes of the format, 8, or one value, as strides, sizes and addresses allow). An item is
+// two units: those of partners (with INTER N pairs, 2 N channels in a row, else N channels in each half), or two
+// neighbouring ones of the channels past the pairs, which are copied.
 template <int DT, int N, bool INTER>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
-  // Items whose loads are in flight together: with whole units more waves do better than more loads a wave (bf16, 6032 tokens of 24
-  // heads of 128: 13.4 us with one, 13.9 with two, 16.4 with four), single values need them (8 heads of 80: 10.7 with four, 15.2).
+  // Items whose loads are in flight together: with whole units more waves do better than more loads a wave (bf16,
+  // 6032 tokens of 24 heads of 128: 13.4 us with one, 13.9 with two, 16.4 with four), single values need them (8
+  // heads of 80: 10.7 with four, 15.2).
   constexpr int U = N == 1 ? 4 : 1;
   __shared__ float2 cs[MAX_TOKENS * MAX_PAIRS];
   __shared__ int64_t at_tok[MAX_TOKENS][4];   // where a token's rows start: q, k, and in the outputs

@@ -1,12 +1,12 @@
 // Linears with 4-bit weights (include/lbw_block.h): their quantisation, and x w^T with codes that become matrix-core
 // operands in registers.
 //
-// A code enters the products exactly. fp4 converts by the hardware's own instruction. An integer code c becomes 1 + c / 16 in
-// the 16-bit format: its four bits placed in the mantissa of 1, a shift and a mask for two codes (converting to the signed integer
-// instead takes three more operations a pair). With v = c - z the group's sum is then
+// A code enters the products exactly. fp4 converts by the hardware's own instruction. An integer code c becomes 1 + c
+// / 16 in the 16-bit format: its four bits placed in the mantissa of 1, a shift and a mask for two codes (converting
+// to the signed integer instead takes three more operations a pair). With v = c - z the group's sum is then
 //   sum x v = 16 (sum x (1 + c / 16) - (1 + z / 16) sum x),
-// sum x from one more matrix instruction a step (x times ones) whose result stands where the products' do. Group sums are
-// scaled in fp32: out += s (...) for every group, so neither scale nor zero is ever rounded into a 16-bit weight.
+// sum x from one more matrix instruction a step (x times ones) whose result stands where the products' do. Group sums
+// are scaled in fp32: out += s (...) for every group, so neither scale nor zero is ever rounded into a 16-bit weight.
 #include "lbw_rows.h"
 
 namespace lbw {
@@ -90,8 +90,9 @@ __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c) {
 template <int DT>
 constexpr uint32_t ONES = DT == LBW_DTYPE_FP16 ? 0x3C003C00u : 0x3F803F80u;
 
-// Those in a vector register: mask and ones then enter one instruction (which takes a single scalar or literal), not two. With the
-// factor of 16 left to the end a K tile takes 357 vector instructions beside its 68 products, not 437 (2048 x 8192 x 6144 with zeros: 238 -> 229 us).
+// Those in a vector register: mask and ones then enter one instruction (which takes a single scalar or literal), not
+// two. With the factor of 16 left to the end a K tile takes 357 vector instructions beside its 68 products, not 437
+// (2048 x 8192 x 6144 with zeros: 238 -> 229 us).
 template <int DT>
 __device__ __forceinline__ uint32_t vector_ones() {
   uint32_t r;
@@ -136,9 +137,10 @@ struct GemmArgs {
   void* out;
 };
 
-// x from row m0 on, read 8 columns at a time. VEC: by buffer loads, a base for the workgroup and 32 bits of offset a lane (64-bit
-// addresses of 16 rows took 32 registers, spills, and more clocks than the products); what lies past the last row or past K
-// reads as zero by the buffer's bounds. Else value by value. Zero past K is needed: the tiles hold anything there.
+// x from row m0 on, read 8 columns at a time. VEC: by buffer loads, a base for the workgroup and 32 bits of offset a
+// lane (64-bit addresses of 16 rows took 32 registers, spills, and more clocks than the products); what lies past the
+// last row or past K reads as zero by the buffer's bounds. Else value by value. Zero past K is needed: the tiles hold
+// anything there.
 template <bool VEC>
 struct RowsOfX {
   __amdgpu_buffer_rsrc_t rsrc;
@@ -173,8 +175,8 @@ struct RowsOfX {
   }
 };
 
-// The bias of four columns of the output from n on, in its own format: without a branch around a load (past the last column the
-// last is read again), so that all are in flight together.
+// The bias of four columns of the output from n on, in its own format: without a branch around a load (past the last
+// column the last is read again), so that all are in flight together.
 struct Bias {
   uint16_t w[4];
   __device__ __forceinline__ Bias(const GemmArgs& a, int64_t n) : w{0, 0, 0, 0} {
@@ -243,8 +245,8 @@ struct Scales {
     }
     return r;
   }
-  // where they start, from the sum of x: the codes' offset -(16 + z) / 16 comes off (for z = 8 it has already been multiplied
-  // in, once for all columns)
+  // where they start, from the sum of x: the codes' offset -(16 + z) / 16 comes off (for z = 8 it has already been
+  // multiplied in, once for all columns)
   __device__ __forceinline__ v4f start(int g, float sum) const {
     v4f r;
 #pragma unroll
@@ -256,8 +258,8 @@ struct Scales {
   }
 };
 
-// The sum of each of 16 rows of x over a group, from its operands (ones times them: every row of the result is the sums), as
-// Scales::start takes it.
+// The sum of each of 16 rows of x over a group, from its operands (ones times them: every row of the result is the
+// sums), as Scales::start takes it.
 template <int DT, Form F, int STEPS>
 __device__ __forceinline__ float group_sum(const v4i* x) {
   if constexpr (F == FP4) return 0.f;
@@ -268,15 +270,15 @@ __device__ __forceinline__ float group_sum(const v4i* x) {
   return F == INT4 ? -1.5f * sum[0] : sum[0];
 }
 
-// Both kernels multiply weights by x transposed: a lane then holds 4 neighbouring columns of a row of the output, which
-// it stores at once, and one sum of x for them.
+// Both kernels multiply weights by x transposed: a lane then holds 4 neighbouring columns of a row of the output,
+// which it stores at once, and one sum of x for them.
 
-// Few rows: 16 MT rows and 16 NT columns a workgroup. Its waves share out the K tiles (so that the few workgroups of a
-// narrow output still have loads in flight on every SIMD) and add their sums through LDS at the end. x comes in rows of 256
-// bytes, four a load, and is turned into operands through LDS, each wave in a part of its own (no barrier): loads in the
-// operands' own order, 16 rows of 64 bytes each, took 120 clocks apiece, all rows in one bank of the cache's tags. A row's
-// 16-byte pieces are exchanged by its number, so that 16 rows' pieces lie in all banks. The next tile's x and codes are in
-// flight while a tile is multiplied.
+// Few rows: 16 MT rows and 16 NT columns a workgroup. Its waves share out the K tiles (so that the few workgroups of
+// a narrow output still have loads in flight on every SIMD) and add their sums through LDS at the end. x comes in
+// rows of 256 bytes, four a load, and is turned into operands through LDS, each wave in a part of its own (no
+// barrier): loads in the operands' own order, 16 rows of 64 bytes each, took 120 clocks apiece, all rows in one bank
+// of the cache's tags. A row's 16-byte pieces are exchanged by its number, so that 16 rows' pieces lie in all banks.
+// The next tile's x and codes are in flight while a tile is multiplied.
 template <int DT, Form F, int GROUP, int MT, int NT, int MOST, bool VEC>
 __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
   constexpr int PER = TK / GROUP, STEPS = GROUP / 32, ROWS = 16 * MT, COLS = TN * NT;
@@ -369,14 +371,15 @@ __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
   }
 }
 
-// Many rows: 64 rows x 256 columns a workgroup, four waves of 64 x 64, two workgroups a CU (which drift apart, so that one's
-// matrix work runs under the other's conversions: 57.5 us for 1508 x 8960 x 1536 against 62.7 with eight waves in step on 128 rows,
-// both before the last steps; now 51.3, 810 TFLOP/s, and 1000 where K is 6144 and the grid fills whole rounds).
-// x passes through LDS, a K tile at a time in two buffers (rows and pieces as above): wave w loads rows 16 w .. 16 w + 15 in the
-// operands' own order, forms their sums over each group while they are in registers, and leaves both there. Codes go from
-// memory to registers, a tile ahead. The output leaves through LDS, so that a store holds whole rows of 128 bytes (1508 x 8960 x
-// 1536, zeros and bias: 68.1 -> 64.9 us; with no store at all 61.2). The conversions bound it: vector instructions take about
-// 1.3 times the matrix core's cycles, and two waves a SIMD overlap the two in part.
+// Many rows: 64 rows x 256 columns a workgroup, four waves of 64 x 64, two workgroups a CU (which drift apart, so
+// that one's matrix work runs under the other's conversions: 57.5 us for 1508 x 8960 x 1536 against 62.7 with eight
+// waves in step on 128 rows, both before the last steps; now 51.3, 810 TFLOP/s, and 1000 where K is 6144 and the grid
+// fills whole rounds). x passes through LDS, a K tile at a time in two buffers (rows and pieces as above): wave w
+// loads rows 16 w .. 16 w + 15 in the operands' own order, forms their sums over each group while they are in
+// registers, and leaves both there. Codes go from memory to registers, a tile ahead. The output leaves through LDS,
+// so that a store holds whole rows of 128 bytes (1508 x 8960 x 1536, zeros and bias: 68.1 -> 64.9 us; with no store
+// at all 61.2). The conversions bound it: vector instructions take about 1.3 times the matrix core's cycles, and two
+// waves a SIMD overlap the two in part.
 constexpr int GM = 64, GN = 256;
 constexpr int X_TILE = GM * TK * 2;   // bytes
 
@@ -463,7 +466,8 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(GemmArgs a, int m_tiles
           for (int e = 0; e < 4; ++e) out[n][i][e] = fmaf(s[e], acc[i][e], out[n][i][e]);
         if (g == PER - 1) load_w(n, next);   // into the registers just read: no second set
         if (g == 0 && n == 0) {
-          // (not earlier, for its registers; and held here: the scheduler moves the loads down to where they are waited for)
+          // (not earlier, for its registers; and held here: the scheduler moves the loads down to where they are
+          // waited for)
           __builtin_amdgcn_sched_barrier(0);
           load(next);
           __builtin_amdgcn_sched_barrier(0);
@@ -521,15 +525,15 @@ void launch_rows(const GemmArgs& a, int most, hipStream_t stream) {
   w4_rows_kernel<DT, F, GROUP, MT, NT, MOST, VEC><<<grid, 64 * waves, waves * each, stream>>>(a);
 }
 
-// Which kernel. Few rows are a matter of latency: the smallest tile whose workgroups all run at once, one a CU, since a second
-// round costs more than a larger tile, and a larger tile more than a part of the first round left empty (bf16, int4, groups of
-// 128; rows x columns x K, us):
+// Which kernel. Few rows are a matter of latency: the smallest tile whose workgroups all run at once, one a CU, since
+// a second round costs more than a larger tile, and a larger tile more than a part of the first round left empty
+// (bf16, int4, groups of 128; rows x columns x K, us):
 //   24 x 1536 x 8960:   16 x 16 tiles 7.3,  32 x 16 9.8,  32 x 48 19.6     32 x 8960 x 1536: 32 x 16 7.6, 32 x 48 6.0
 //   128 x 1536 x 8960:  32 x 16 17.3, 16 x 48 12.3, 32 x 48 17.8          256 x 1536 x 8960: 16 x 48 20.6, 32 x 48 18.1
-// With 32 x 48 tiles past one round two workgroups of four waves share a CU better than one of six (512 x 1536 x 8960: 28.6
-// against 34.4). Whole tiles of 64 x 256 win from about half a tile a CU on: 256 x 8960 x 1536 (140 tiles) 18.0 against 20.9,
-// 1508 x 1536 x 1536 (144) 17.8 against 19.8, 512 x 8960 x 1536 (280) 26.3 against 36.5, about even for 1508 x 1536 x 8960 (144)
-// 84 against 81; but 1024 x 1536 x 1536 (96) 17.4 against 14.5.
+// With 32 x 48 tiles past one round two workgroups of four waves share a CU better than one of six (512 x 1536 x
+// 8960: 28.6 against 34.4). Whole tiles of 64 x 256 win from about half a tile a CU on: 256 x 8960 x 1536 (140 tiles)
+// 18.0 against 20.9, 1508 x 1536 x 1536 (144) 17.8 against 19.8, 512 x 8960 x 1536 (280) 26.3 against 36.5, about
+// even for 1508 x 1536 x 8960 (144) 84 against 81; but 1024 x 1536 x 1536 (96) 17.4 against 14.5.
 template <int DT, Form F, int GROUP>
 void launch_group(const GemmArgs& a, bool vec, hipStream_t stream) {
   const auto grid = [&](int rows, int cols) { return ((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols); };
