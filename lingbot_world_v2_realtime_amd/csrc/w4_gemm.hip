@@ -527,22 +527,31 @@ void launch_rows(const GemmArgs& a, int most, hipStream_t stream) {
 
 // Which kernel. Few rows are a matter of latency: the smallest tile whose workgroups all run at once, one a CU, since
 // a second round costs more than a larger tile, and a larger tile more than a part of the first round left empty
-// (bf16, int4, groups of 128; rows x columns x K, us):
-//   24 x 1536 x 8960:   16 x 16 tiles 7.3,  32 x 16 9.8,  32 x 48 19.6     32 x 8960 x 1536: 32 x 16 7.6, 32 x 48 6.0
-//   128 x 1536 x 8960:  32 x 16 17.3, 16 x 48 12.3, 32 x 48 17.8          256 x 1536 x 8960: 16 x 48 20.6, 32 x 48 18.1
+// (bf16, groups of 128, int4 / groups of 64, int4 with zeros; rows x columns x K, us in graphs):
+//                        16 x 16 tiles   16 x 32         16 x 48         32 x 48
+//   24 x  1536 x 8960     6.9 /  7.8      9.4 / 11.6     11.3 / 14.8     17.0 / 21.0
+//   77 x  1536 x 1536     4.5 /  4.9      4.3 /  4.8      4.8 /  5.7      5.9 /  6.8
+//    1 x  9216 x 1536     5.3 /  5.9      5.6 /  6.5      4.7 /  5.6      5.9 /  6.8
+//   32 x  8960 x 1536     7.8 /  8.5      7.9 /  9.1      7.1 /  9.6      6.1 /  7.0
+//    5 x 20480 x 8960    29.9 / 32.9     23.3 / 28.6     21.7 / 28.7     27.3 / 34.0
+// (the last: up to 16 rows never fill two row blocks). A CU with a single 16 x 16 tile has 12 waves, against 8
+// (5 x 1536 x 8960: fp4 7.15 -> 7.05, int4 with zeros 7.95 -> 7.55; 16 waves 7.45 and 7.9).
 // With 32 x 48 tiles past one round two workgroups of four waves share a CU better than one of six (512 x 1536 x
 // 8960: 28.6 against 34.4). Whole tiles of 64 x 256 win from about half a tile a CU on: 256 x 8960 x 1536 (140 tiles)
-// 18.0 against 20.9, 1508 x 1536 x 1536 (144) 17.8 against 19.8, 512 x 8960 x 1536 (280) 26.3 against 36.5, about
-// even for 1508 x 1536 x 8960 (144) 84 against 81; but 1024 x 1536 x 1536 (96) 17.4 against 14.5.
+// 18.0 against 20.9, 1508 x 1536 x 1536 (144) 17.8 against 19.8, 512 x 8960 x 1536 (280) 26.3 against 36.5, about even
+// for 1508 x 1536 x 8960 (144) 84 against 81; but 1024 x 1536 x 1536 (96) 17.4 against 14.5, and half empty ones never:
+// 32 x 40960 x 1536 (160) 17.5 against 15.4.
 template <int DT, Form F, int GROUP>
 void launch_group(const GemmArgs& a, bool vec, hipStream_t stream) {
   const auto grid = [&](int rows, int cols) { return ((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols); };
   constexpr int CUS = 256;
   if (!vec) launch_rows<DT, F, GROUP, 2, 1, 8, false>(a, 8, stream);
-  else if (a.m <= 16) launch_rows<DT, F, GROUP, 1, 1, 8, true>(a, 8, stream);
-  else if (grid(32, 16) <= CUS) launch_rows<DT, F, GROUP, 2, 1, 8, true>(a, 8, stream);
+  else if (grid(16, 16) <= CUS) launch_rows<DT, F, GROUP, 1, 1, 12, true>(a, 12, stream);
+  else if (grid(16, 32) <= CUS) launch_rows<DT, F, GROUP, 1, 2, 8, true>(a, 8, stream);
   else if (grid(16, 48) <= CUS) launch_rows<DT, F, GROUP, 1, 3, 8, true>(a, 8, stream);
-  else if (grid(GM, GN) < CUS / 2) launch_rows<DT, F, GROUP, 2, 3, 6, true>(a, grid(32, 48) <= CUS ? 6 : 4, stream);
+  else if (a.m <= 16) launch_rows<DT, F, GROUP, 1, 2, 8, true>(a, 8, stream);
+  else if (a.m <= 32 || grid(GM, GN) < CUS / 2)
+    launch_rows<DT, F, GROUP, 2, 3, 6, true>(a, grid(32, 48) <= CUS ? 6 : 4, stream);
   else w4_gemm_kernel<DT, F, GROUP><<<(unsigned)((grid(GM, GN) + 7) / 8 * 8), 4 * GM, 0, stream>>>(a, (int)grid(GM, 1 << 30));
 }
 

@@ -541,11 +541,12 @@ def _check_w4(m, n, k, group, fmt, zeros, dtype, bias, x=None):
     _within(out, (want, mag + want.abs()), f"{m}x{n}x{k} group {group} {fmt} {zeros} {dtype}", k / 16 + 24)
 
 
-# every kernel and tile, with rows, columns and K that end inside a tile: 16 x 16 (to 16 rows), 32 x 16, 16 x 48 and 32 x 48
-# (by the workgroups they give), 64 x 256 (from 160 of those on)
+# every kernel and tile, with rows, columns and K that end inside a tile: 16 x 16, 16 x 32, 16 x 48 and 32 x 48 (by the
+# workgroups they give, and by the rows), 64 x 256 (from 128 of those on)
 W4_SIZES = [(1, 16, 128), (1, 1, 1), (3, 37, 300), (16, 64, 1536), (17, 48, 256), (33, 100, 520), (65, 130, 384),
             (130, 257, 640), (300, 144, 1000), (2, 1536, 8960), (129, 16, 128), (100, 1203, 264), (70, 4004, 392),
-            (300, 1601, 136), (450, 5204, 520), (1030, 2310, 256)]
+            (300, 1601, 136), (450, 5204, 520), (1030, 2310, 256), (100, 700, 264), (65, 1000, 1536),
+            (9, 12400, 136), (20, 32800, 128)]
 
 
 @pytest.mark.parametrize("m,n,k", W4_SIZES)
