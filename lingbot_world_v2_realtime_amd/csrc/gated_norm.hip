@@ -408,7 +408,7 @@ __device__ __forceinline__ void weigh(const NormArgs& a, int64_t b, int64_t g, i
 }
 
 // The slices' sums of K values into those of slice 0, in halves (one slice adding all took 32 K reads in turn: 6.3 us
-// for a kernel of two rows). slices: a power of two, blockDim.x / SUM_COLS.
+// for a kernel of two rows, 3.9 now). slices: a power of two, blockDim.x / SUM_COLS.
 template <int K>
 __device__ __forceinline__ void add_slices(float (*part)[K][SUM_COLS], int w, int lane, int slices, float* s) {
 #pragma unroll
@@ -432,9 +432,9 @@ int slices_for(int64_t rows) {   // (two at least: whole waves)
 }
 
 // The workgroups' sums of one modulation row (workgroup / tiles), SUM_COLS channels a workgroup, its half-waves
-// taking them in turn, four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 5.7 us with 64 channels and one
-// at a time): the row's own gradients, and its sums left where its first workgroup's were for the kernel below (which
-// a single modulation row does not need: `last`).
+// taking them in turn, four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 6.1 us; with eight in flight 6.9,
+// with 64 channels and one at a time 8.0, with 16 channels 10.6): the row's own gradients, and its sums left where
+// its first workgroup's were for the kernel below (which a single modulation row does not need: `last`).
 template <int VDT>
 __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int tiles,
                                                                             int last) {
@@ -569,8 +569,10 @@ void forward(const NormArgs& a, void* s_out, void* h_out, hipStream_t stream) {
 
 // Rows of a workgroup of the backward. More workgroups keep more rows in flight, but each leaves three fp32 rows
 // behind that are written and read again (against six of `dtype` for every row of the tensors). With one chunk a
-// thread 12 waves a CU are the best (6032 x 1536 bf16, all gradients: 8 waves 41.4 us, 12 39.1, 16 39.8), with two 8,
-// the registers' bound (4524 x 2048: 38.8, 47.7, 47.6: a second round).
+// thread 12 waves a CU are the best over widths (bf16, all gradients with their sums over rows: 6032 x 1536 8 waves
+// 43.9 us, 12 36.5, 16 36.0, but 3016 x 2304 33.3 with 12, 40.2 with 16), where a wave is a team 16 (24000 x 512: 8
+// waves 43.0, 16 37.8, 24 45.4), with two chunks 8, the registers' bound (4524 x 2048: 38.8, with 12 and 16 47.7: a
+// second round).
 void split(int64_t rows, int64_t len, int64_t group_len, int nch, int team, int64_t& chunk_rows, int64_t& chunks) {
   const int64_t gl = group_len < len ? group_len : len;
   const int waves = team == 64 ? 8 : team >> 6, room = nch == 1 ? (team == 64 ? 16 : 12) : 8;   // of a workgroup, and of a CU
