@@ -5,6 +5,9 @@
 // no barrier) or of more waves of one workgroup (sums through LDS); thread i of a team of T holds the 8-value chunks
 // i, i + T, ... of the row.
 //
+// 6032 x 1536 in bf16, LayerNorm, gate, shift and scale in 4 rows of fp32: forward 13.9 us (5.3 TB/s; a copy of 1 GiB
+// reaches 5.1), backward 30.5 (3.6 TB/s, its fp32 sums left aside) and 6.1 for the sums over workgroups; one row 3.2.
+//
 // Norm statistics take two passes over the registers (mean, then the mean square of the differences): no
 // cancellation.
 //

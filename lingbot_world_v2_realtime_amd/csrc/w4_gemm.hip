@@ -278,7 +278,8 @@ __device__ __forceinline__ float group_sum(const v4i* x) {
 // rows of 256 bytes, four a load, and is turned into operands through LDS, each wave in a part of its own (no
 // barrier): loads in the operands' own order, 16 rows of 64 bytes each, took 120 clocks apiece, all rows in one bank
 // of the cache's tags. A row's 16-byte pieces are exchanged by its number, so that 16 rows' pieces lie in all banks.
-// The next tile's x and codes are in flight while a tile is multiplied.
+// The next tile's x and codes are in flight while a tile is multiplied. Latency bounds it: 5 x 1536 x 8960 in fp4 6.8
+// us, 61 x 8960 x 1536 in int4 with zeros 9.7, one row x 9216 x 1536 5.0, where the weights' bytes take 1.4 to 1.7.
 template <int DT, Form F, int GROUP, int MT, int NT, int MOST, bool VEC>
 __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
   constexpr int PER = TK / GROUP, STEPS = GROUP / 32, ROWS = 16 * MT, COLS = TN * NT;
@@ -534,13 +535,13 @@ void launch_rows(const GemmArgs& a, int most, hipStream_t stream) {
 //    1 x  9216 x 1536     5.3 /  5.9      5.6 /  6.5      4.7 /  5.6      5.9 /  6.8
 //   32 x  8960 x 1536     7.8 /  8.5      7.9 /  9.1      7.1 /  9.6      6.1 /  7.0
 //    5 x 20480 x 8960    29.9 / 32.9     23.3 / 28.6     21.7 / 28.7     27.3 / 34.0
-// (the last: up to 16 rows never fill two row blocks). A CU with a single 16 x 16 tile has 12 waves, against 8
-// (5 x 1536 x 8960: fp4 7.15 -> 7.05, int4 with zeros 7.95 -> 7.55; 16 waves 7.45 and 7.9).
-// With 32 x 48 tiles past one round two workgroups of four waves share a CU better than one of six (512 x 1536 x
-// 8960: 28.6 against 34.4). Whole tiles of 64 x 256 win from about half a tile a CU on: 256 x 8960 x 1536 (140 tiles)
-// 18.0 against 20.9, 1508 x 1536 x 1536 (144) 17.8 against 19.8, 512 x 8960 x 1536 (280) 26.3 against 36.5, about even
-// for 1508 x 1536 x 8960 (144) 84 against 81; but 1024 x 1536 x 1536 (96) 17.4 against 14.5, and half empty ones never:
-// 32 x 40960 x 1536 (160) 17.5 against 15.4.
+// (the last: up to 16 rows never fill two row blocks). A CU with a single 16 x 16 tile has 12 waves, against 8 (5 x
+// 1536 x 8960: fp4 7.15 -> 7.05, int4 with zeros 7.95 -> 7.55; 16 waves 7.45 and 7.9). With 32 x 48 tiles past one
+// round two workgroups of four waves share a CU better than one of six (512 x 1536 x 8960: 28.6 against 34.4). Whole
+// tiles of 64 x 256 win from about half a tile a CU on: 256 x 8960 x 1536 (140 tiles) 18.0 against 20.9, 1508 x 1536
+// x 1536 (144) 17.8 against 19.8, 512 x 8960 x 1536 (280) 26.3 against 36.5, about even for 1508 x 1536 x 8960 (144)
+// 84 against 81; but 1024 x 1536 x 1536 (96) 17.4 against 14.5, and half empty ones never: 32 x 40960 x 1536 (160)
+// 17.5 against 15.4.
 template <int DT, Form F, int GROUP>
 void launch_group(const GemmArgs& a, bool vec, hipStream_t stream) {
   const auto grid = [&](int rows, int cols) { return ((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols); };
