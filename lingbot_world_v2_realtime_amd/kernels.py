@@ -583,7 +583,8 @@ def pack_w4(codes, scale, zero=None, fmt="int4"):
 def gemm_w4(x, w4, scale, zero=None, bias=None, out_features=None, fmt="int4"):
     """x [M, K] (bf16 or fp16, unit column stride) times 4-bit weights [N, K] in the tiles of quant_w4 / pack_w4
     (lbw_gemm_w4), bias of x's dtype [N] or None -> [M, N] of x's dtype: codes exact, sums, scales and bias in fp32, one
-    rounding. out_features: N where it is not a multiple of 16 (default: every row the tiles hold)."""
+    rounding. out_features: N where it is not a multiple of 16 (default: every row the tiles hold). K has to end in the
+    tiles' last 128 columns; which of them, the caller knows (W4Linear checks it)."""
     return block_binding().gemm_w4(x, w4, scale, zero, bias, out_features, fmt)
 
 

@@ -215,6 +215,8 @@ class W4Linear(torch.nn.Module):
         if not block.plain(x):
             raise RuntimeError("W4Linear has no gradient with respect to its input: call it under torch.no_grad(), or on "
                                "a detached input")
+        if not shape or shape[-1] != self.in_features:   # (the tiles hold 128 columns each and cannot tell)
+            raise ValueError(f"x must have {self.in_features} columns, got {tuple(shape)}")
         x2 = x.reshape(-1, shape[-1])
         if x2.dtype not in (torch.bfloat16, torch.float16):
             if not x2.is_floating_point():
