@@ -155,6 +155,16 @@ bool records_gradient(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// For the calls that have no gradient of their own: a tensor among the arguments that would record one is refused (the
+// result would be detached).
+void no_gradient(const char* what, PyObject* const* args, Py_ssize_t n) {
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!THPVariable_Check(args[i]) || !records_gradient({THPVariable_Unpack(args[i])})) continue;
+    PyErr_Format(PyExc_RuntimeError, "%s records no gradient: call it under torch.no_grad(), or on detached tensors", what);
+    throw python_error();
+  }
+}
+
 Tensor new_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }   // (packed, whatever t's strides)
 
 PyObject* wrap(const Tensor& t) {
@@ -378,6 +388,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, Norm::ARGS + 1);
+  no_gradient("kernels.gated_norm", args, n);
   return wrap_all(Norm(args).forward(truth(args[Norm::ARGS])));
   END_HANDLE_TH_ERRORS
 }
@@ -387,6 +398,7 @@ PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* gated_norm_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, Norm::ARGS + 3);
+  no_gradient("kernels.gated_norm_bwd", args, n);
   const Norm a(args);
   const Tensor &ds = tensor("ds", args[Norm::ARGS], true), &dh = tensor("dh", args[Norm::ARGS + 1], true);
   const int64_t wants = integer("wants", args[Norm::ARGS + 2]);
@@ -561,6 +573,7 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 11);
+  no_gradient("kernels.rotary", args, n);
   const Rotary a(args);
   std::array<Tensor, 2> out;
   for (int i = 0; i < 2; ++i) {
@@ -597,6 +610,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   count(n_args, 7);
+  no_gradient("gemm_w4", args, n_args);
   const Tensor& x = tensor("x", args[0]);
   const auto dt = x.scalar_type();
   if (dt != at::kBFloat16 && dt != at::kHalf) type_error("x must be bfloat16 or float16, got ", dt);

@@ -492,7 +492,8 @@ def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=N
     """s = residual_scale * x + branch_scale * gate * (post_norm(y) * post_weight), h = (norm(s) * weight + bias) *
     (1 + scale) + shift in one pass (lbw_gated_norm): (s or None, h or None). x, y [B, L, C] bf16, fp16 or fp32 with any
     strides of B and L; vectors of x's dtype or fp32, [C], the modulations also [B, rows, C] with group_len tokens a row
-    (default: the rows share the tokens evenly). s is made where want_stream, h where there is a norm."""
+    (default: ceil(L / rows)). s is made where want_stream, h where there is a norm. No gradient: a call that would
+    record one is refused (layers/norm.py records it)."""
     return block_binding().gated_norm(x, y, gate, shift, scale, weight, bias, post_weight, norm, post_norm, eps,
                                       residual_scale, branch_scale, group_len, want_stream)
 
@@ -514,7 +515,8 @@ def rotary(q, k, positions, freq, axis=None, pairs="interleaved", factor=1.0, la
     channels) rotated by the positions of their tokens (lbw_rotary): (q_out, k_out). positions: int32 or int64 [L] or
     [B, L], with several axes [L, axes] or [B, L, axes], or an int, the first token's position. freq: float64 [pairs],
     radians a position; axis: int32 [pairs], or None with one axis. pairs: 'interleaved' (channels 2 i, 2 i + 1) or
-    'half' (i, pairs + i). inverse: the opposite rotation. The outputs may be the inputs themselves."""
+    'half' (i, pairs + i). inverse: the opposite rotation. The outputs may be the inputs themselves. No gradient: a call
+    that would record one is refused (layers/rotary.py records it)."""
     return block_binding().rotary(q, k, positions, freq, axis, pairs, factor, layout, inverse, q_out, k_out)
 
 
@@ -584,7 +586,7 @@ def gemm_w4(x, w4, scale, zero=None, bias=None, out_features=None, fmt="int4"):
     """x [M, K] (bf16 or fp16, unit column stride) times 4-bit weights [N, K] in the tiles of quant_w4 / pack_w4
     (lbw_gemm_w4), bias of x's dtype [N] or None -> [M, N] of x's dtype: codes exact, sums, scales and bias in fp32, one
     rounding. out_features: N where it is not a multiple of 16 (default: every row the tiles hold). K has to end in the
-    tiles' last 128 columns; which of them, the caller knows (W4Linear checks it)."""
+    tiles' last 128 columns; which of them, the caller knows (W4Linear checks it). No gradient: a call that would record one is refused."""
     return block_binding().gemm_w4(x, w4, scale, zero, bias, out_features, fmt)
 
 

@@ -18,8 +18,8 @@ def gated_norm(x, y=None, gate=None, shift=None, scale=None, weight=None, bias=N
         h = (norm(s) * weight + bias) * (1 + scale) + shift
 
     x, y: [B, L, C] bf16, fp16 or fp32 on the GPU, any strides of B and L. norm, post_norm: 'layer', 'rms' or None, with
-    `eps`. gate, shift, scale: [C], or [B, rows, C] with `group_len` tokens a row (default: the rows share the L tokens
-    evenly), e.g. slices of one projection's output. weight, bias, post_weight: [C]. Vectors are of x's dtype or fp32;
+    `eps`. gate, shift, scale: [C], or [B, rows, C] with `group_len` tokens a row (default: ceil(L / rows)),
+    e.g. slices of one projection's output. weight, bias, post_weight: [C]. Vectors are of x's dtype or fp32;
     where they differ among themselves all are taken in fp32. Every step is fp32 and each output is rounded once: the norm reads
     s before its rounding. C is at most 12288; the rows may be none.
 

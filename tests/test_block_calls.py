@@ -2,6 +2,7 @@
 looks for a device."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from lingbot_world_v2_realtime_amd import kernels
 from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
@@ -22,3 +23,49 @@ def test_w4_linear_refuses_another_width(w4_module, width):
     """1409 to 1535 columns end in the weights' last tile of 128: the tiles alone do not tell them from 1536."""
     with torch.no_grad(), pytest.raises(ValueError, match=f"1536 .*{width}"):
         w4_module(torch.zeros(2, width, dtype=torch.bfloat16))
+
+
+def _recording(t, how):
+    if how == "gradient":
+        return t.clone().requires_grad_()
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.parametrize("how", ["gradient", "tangent"])
+def test_raw_calls_do_not_lose_a_gradient(how):
+    """The functions of kernels.py that have no gradient of their own refuse a call that would record one, whichever tensor
+    asks for it: their results would be detached without a word."""
+    x = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    norm = dict(x=x, y=x.clone(), gate=x[0, 0].clone(), weight=x[0, 0].clone())
+    q = x.view(1, 4, 1, 128)
+    freq = torch.ones(8, dtype=torch.float64)
+    gemm = dict(x=x[0], w4=torch.zeros(1, 1, 1024, dtype=torch.uint8), scale=torch.zeros(1, 1, 16, 1, dtype=torch.bfloat16),
+                bias=torch.zeros(16, dtype=torch.bfloat16))
+    with forward_ad.dual_level():
+        for name in ("x", "bias", "scale"):
+            with pytest.raises(RuntimeError, match="gemm_w4.*gradient"):
+                kernels.gemm_w4(**{**gemm, name: _recording(gemm[name], how)})
+        for name in norm:
+            args = {**norm, name: _recording(norm[name], how)}
+            with pytest.raises(RuntimeError, match="gated_norm.*gradient"):
+                kernels.gated_norm(**args)
+            with pytest.raises(RuntimeError, match="gated_norm_bwd.*gradient"):
+                kernels.gated_norm_bwd(args.pop("x"), x, x, **args)
+        with pytest.raises(RuntimeError, match="gated_norm_bwd.*gradient"):
+            kernels.gated_norm_bwd(x, _recording(x, how), x)
+        for args in (dict(q=_recording(q, how), k=None), dict(q=q, k=_recording(q, how)),
+                     dict(q=q, k=None, q_out=_recording(q, how))):
+            with pytest.raises(RuntimeError, match="rotary.*gradient"):
+                kernels.rotary(**args, positions=0, freq=freq)
+
+
+def test_raw_calls_without_grad_mode_go_on():
+    """As the forward of a user's own autograd function has them: what is refused then is the host tensor."""
+    x = torch.zeros(1, 4, 128, dtype=torch.bfloat16, requires_grad=True)
+    with torch.no_grad():
+        for call in (lambda: kernels.gated_norm(x), lambda: kernels.gated_norm_bwd(x, None, x),
+                     lambda: kernels.rotary(x.view(1, 4, 1, 128), None, 0, torch.ones(8, dtype=torch.float64)),
+                     lambda: kernels.gemm_w4(x[0], torch.zeros(1, 1, 1024, dtype=torch.uint8),
+                                             torch.zeros(1, 1, 16, 1, dtype=torch.bfloat16))):
+            with pytest.raises(ValueError, match="device tensor"):
+                call()
