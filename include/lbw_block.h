@@ -79,10 +79,10 @@ int64_t lbw_gated_norm_bwd_workspace_bytes(int64_t batch, int64_t len, int64_t w
  * the others copied. interleaved: pair i is channels (2 i, 2 i + 1), else (i, pairs + i). inverse: w negated (the
  * gradient's rotation). The angle is formed in 64 bits and reduced to a turn before the sine and cosine are taken in
  * fp32, so far positions keep theirs; one rounding to `dtype`. freq: float64 [pairs], radians a position. axis: int32
- * [pairs] with values in 0 .. axes - 1, or null (all 0). positions: int64 (pos_is_i64) or int32 with strides
- * p_s_batch, p_s_tok, p_s_axis, or null: token t of every entry is at pos_start + t on every axis. q_out, k_out as q,
- * k (strides qo_*, ko_*); a call in place passes the same pointer and strides twice, any other overlap is an error of
- * the caller. k may be null with k_heads 0. dim even is not required; 2 * pairs <= dim <= LBW_ROTARY_MAX_DIM,
+ * [pairs] with values in 0 .. axes - 1, or null (all 0); a pair of another axis comes out as NaN. positions: int64
+ * (pos_is_i64) or int32 with strides p_s_batch, p_s_tok, p_s_axis, or null: token t of every entry is at pos_start + t
+ * on every axis. q_out, k_out as q, k (strides qo_*, ko_*); a call in place passes the same pointer and strides twice,
+ * any other overlap is an error of the caller. k may be null with k_heads 0. dim even is not required; 2 * pairs <= dim <= LBW_ROTARY_MAX_DIM,
  * batch * len <= 2^30, 4096 heads at most.
  */
 int lbw_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t len, int64_t q_heads, int64_t k_heads,

@@ -106,11 +106,20 @@ std::string word(const char* name, PyObject* o) {
   return s;
 }
 
-int row_format(const char* name, const Tensor& t) {
+int element_format(const char* name, const Tensor& t) {
   const auto d = t.scalar_type();
   const int code = d == at::kBFloat16 ? LBW_DTYPE_BF16 : d == at::kHalf ? LBW_DTYPE_FP16 : d == at::kFloat ? LBW_DTYPE_FP32 : -1;
   if (code < 0) type_error(name, " must be bfloat16, float16 or float32, got ", d);
+  return code;
+}
+
+void on_device(const char* name, const Tensor& t) {
   if (!t.is_cuda()) value_error(name, " must be a device tensor (the block operators have no CPU implementation)");
+}
+
+int row_format(const char* name, const Tensor& t) {
+  const int code = element_format(name, t);
+  on_device(name, t);
   return code;
 }
 
@@ -425,11 +434,12 @@ struct Rotary {
   c10::intrusive_ptr<RotaryOptions> o;
 
   Rotary() = default;
-  // q, k, positions, freq, axis, pairs, factor, layout, checked
+  // q, k, positions, freq, axis, pairs, factor, layout, axes, checked (but for the device: that comes last, so that
+  // every other refusal can be seen without one)
   explicit Rotary(PyObject* const* args)
       : q(tensor("q", args[0])), k(tensor("k", args[1], true)), freq(tensor("freq", args[3])), axis(tensor("axis", args[4], true)),
         o(c10::make_intrusive<RotaryOptions>()) {
-    row_format("q", q);
+    element_format("q", q);
     const std::string layout = word("layout", args[7]), pairs = word("pairs", args[5]);
     if (layout != "NHD" && layout != "HND") value_error("tensor_layout must be 'NHD' or 'HND', got '", layout, "'");
     o->nhd = layout == "NHD";
@@ -457,6 +467,9 @@ struct Rotary {
       value_error(freq.size(0), " pairs do not fit heads of ", d, " (of ", LBW_ROTARY_MAX_DIM, " at most)");
     if (axis.defined() && (axis.scalar_type() != at::kInt || axis.sizes() != freq.sizes() || !axis.is_contiguous()))
       value_error("axis must be contiguous int32 ", dims(freq.sizes()), ", got ", axis.scalar_type(), " ", dims(axis.sizes()));
+    const int64_t axes = args[8] == Py_None ? 1 : integer("axes", args[8]);   // (None: not known here)
+    if (axes < 1 || (axes > 1 && !axis.defined()))
+      value_error("a plan of ", axes, " axes", axes > 1 ? " needs the axis of each pair" : "");
     if (THPVariable_Check(args[2])) {
       pos = tensor("positions", args[2]);
       if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong)
@@ -465,7 +478,8 @@ struct Rotary {
       if (!((own == 1 && pos.size(0) == len) || (own == 2 && pos.size(0) == b && pos.size(1) == len)))
         value_error("positions must be [", len, "] or [", b, ", ", len, "]", axis.defined() ? " x axes" : "", ", got ",
                     dims(pos.sizes()));
-      if (axis.defined() && pos.size(own) < 1) value_error("positions need an axis at least");
+      if (axis.defined() && pos.size(own) < axes)
+        value_error("positions ", dims(pos.sizes()), " have ", pos.size(own), " axes, the plan has ", axes, " axes");
     } else {
       if (axis.defined()) value_error("several axes need a positions tensor");
       o->start = integer("positions", args[2]);
@@ -477,11 +491,12 @@ struct Rotary {
   int64_t own_dims() const { return pos.dim() - (axis.defined() ? 1 : 0); }   // of positions, without an axis dimension behind
 
   void run(const Tensor& qo, const Tensor& ko, bool inverse, bool python) const {
+    if (python) on_device("q", q);
     if (q.numel() + (k.defined() ? k.numel() : 0) == 0) return;
     const int64_t own = pos.defined() ? own_dims() : 0;
     const auto st = [&](const Tensor& t, int dim) { return t.defined() ? t.stride(dim) : 0; };
     const On on(q);
-    done(lbw_rotary(q.data_ptr(), ptr(k), row_format("q", q), q.size(0), q.size(tok()), q.size(head()),
+    done(lbw_rotary(q.data_ptr(), ptr(k), element_format("q", q), q.size(0), q.size(tok()), q.size(head()),
                     k.defined() ? k.size(head()) : 0, q.size(3), freq.size(0), st(q, 0), st(q, tok()), st(q, head()), st(k, 0),
                     st(k, tok()), st(k, head()), ptr(pos), pos.defined() && pos.scalar_type() == at::kLong,
                     own == 2 ? pos.stride(0) : 0, own ? pos.stride(own - 1) : 0, own && axis.defined() ? pos.stride(own) : 0,
@@ -545,14 +560,14 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   }
 };
 
-// The operator as users call it: q, k, positions, freq, axis, pairs, factor, layout, inplace. (q, k or None), with a
-// gradient where one is recorded.
+// The operator as users call it: q, k, positions, freq, axis, pairs, factor, layout, axes, inplace. (q, k or None), with
+// a gradient where one is recorded.
 PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 9);
+  count(n, 10);
   const Rotary a(args);
   const bool grad = records_gradient({a.q, a.k});
-  if (truth(args[8])) {
+  if (truth(args[9])) {
     if (grad) value_error("q and k cannot be rotated in place where a gradient is recorded");
     for (const Tensor* t : {&a.q, &a.k})
       for (int j = 0; t->defined() && j < 4; ++j)
@@ -569,15 +584,15 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The rotation alone: q, k, positions, freq, axis, pairs, factor, layout, inverse, q_out, k_out.
+// The rotation alone: q, k, positions, freq, axis, pairs, factor, layout, axes, inverse, q_out, k_out.
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 11);
+  count(n, 12);
   no_gradient("kernels.rotary", args, n);
   const Rotary a(args);
   std::array<Tensor, 2> out;
   for (int i = 0; i < 2; ++i) {
-    const Tensor &x = i ? a.k : a.q, &o = tensor(i ? "k_out" : "q_out", args[9 + i], true);
+    const Tensor &x = i ? a.k : a.q, &o = tensor(i ? "k_out" : "q_out", args[10 + i], true);
     const char* name = i ? "k_out" : "q_out";
     if (!x.defined()) {
       if (o.defined()) value_error("k_out without k");
@@ -597,7 +612,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   apart(out[0], out[1], "q_out and k_out");
   apart(out[0], a.k, "q_out and k");
   apart(out[1], a.q, "k_out and q");
-  a.run(out[0], out[1], truth(args[8]), true);
+  a.run(out[0], out[1], truth(args[9]), true);
   written(out[0]);
   written(out[1]);
   return wrap_all(out);

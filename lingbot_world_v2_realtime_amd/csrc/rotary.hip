@@ -97,13 +97,15 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
   for (int i = threadIdx.x; i < ntok * a.pairs; i += THREADS) {
     const int j = i / a.pairs, p = i - j * a.pairs;
     const uint32_t tok = (uint32_t)(tok0 + j), b = tok / (uint32_t)a.len, t = tok - b * (uint32_t)a.len;
-    // an axis outside the positions' would read past them: held inside
-    const int64_t ax = a.axis ? max((int64_t)0, min((int64_t)a.axis[p], a.axes - 1)) : 0;
+    // an axis that the positions do not have: nothing is read there, and the pair becomes NaN
+    const int64_t want = a.axis ? a.axis[p] : 0, ax = max((int64_t)0, min(want, a.axes - 1));
+    const bool missing = a.pos && ax != want;
     const int64_t at = b * a.p_s_batch + t * a.p_s_tok + ax * a.p_s_axis;
     const int64_t pos = !a.pos ? a.pos_start + t : a.pos_is_i64 ? ((const int64_t*)a.pos)[at] : ((const int32_t*)a.pos)[at];
     const double turns = (double)pos * a.freq[p] * 0.15915494309189533577;   // 1 / (2 pi)
     float s, c;
     sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    if (missing) s = c = __int_as_float(0x7FC00000);
     cs[i] = make_float2(a.factor * c, a.sign * a.factor * s);
   }
   __syncthreads();

@@ -510,14 +510,15 @@ def gated_norm_bwd(x, ds, dh, y=None, gate=None, shift=None, scale=None, weight=
 
 
 def rotary(q, k, positions, freq, axis=None, pairs="interleaved", factor=1.0, layout="NHD", inverse=False,
-           q_out=None, k_out=None):
+           q_out=None, k_out=None, axes=None):
     """q [B, L, Hq, D] and k [B, L, Hk, D] or None (HND: [B, H, L, D]; bf16, fp16 or fp32, any strides with contiguous
     channels) rotated by the positions of their tokens (lbw_rotary): (q_out, k_out). positions: int32 or int64 [L] or
     [B, L], with several axes [L, axes] or [B, L, axes], or an int, the first token's position. freq: float64 [pairs],
     radians a position; axis: int32 [pairs], or None with one axis. pairs: 'interleaved' (channels 2 i, 2 i + 1) or
-    'half' (i, pairs + i). inverse: the opposite rotation. The outputs may be the inputs themselves. No gradient: a call
+    'half' (i, pairs + i). axes: how many axes the plan has, where it is known: positions of fewer are refused then, while
+    pairs of an axis that they do not hold come out as NaN without it. inverse: the opposite rotation. The outputs may be the inputs themselves. No gradient: a call
     that would record one is refused (layers/rotary.py records it)."""
-    return block_binding().rotary(q, k, positions, freq, axis, pairs, factor, layout, inverse, q_out, k_out)
+    return block_binding().rotary(q, k, positions, freq, axis, pairs, factor, layout, axes, inverse, q_out, k_out)
 
 
 def _w4_shapes(n, k, group):

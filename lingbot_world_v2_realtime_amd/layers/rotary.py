@@ -19,11 +19,14 @@ __all__ = ["Rotary", "rotary_embed", "grid_positions"]
 @dataclass
 class Rotary:
     """A rotation's plan, on the device: float64 frequencies [pairs] (radians a position), the axis of each pair (int32, None
-    with one axis), which channels are partners, and the factor that cos and sin are multiplied by."""
+    with one axis), which channels are partners, the factor that cos and sin are multiplied by, and how many axes there
+    are, so that positions of fewer can be refused (None: not known; a pair whose axis the positions do not hold comes out
+    as NaN)."""
     freq: torch.Tensor
     axis: Optional[torch.Tensor] = None
     pairs: str = "interleaved"
     factor: float = 1.0
+    axes: Optional[int] = None
 
     @classmethod
     def build(cls, dim, device, base=10000.0, pairs="interleaved", sections=None, scaling=None, stretch=1.0,
@@ -65,7 +68,7 @@ class Rotary:
             axis += [i] * n
         return cls(torch.cat(freq).to(device),
                    torch.tensor(axis, dtype=torch.int32, device=device) if len(parts) > 1 else None, pairs,
-                   1.0 + 0.1 * math.log(stretch) if scaling == "ramp" else 1.0)
+                   1.0 + 0.1 * math.log(stretch) if scaling == "ramp" else 1.0, len(parts))
 
 
 def grid_positions(grid_size, start_frame=0, device="cuda"):
@@ -83,4 +86,4 @@ def rotary_embed(q, k, positions, rope, tensor_layout="NHD", inplace=False):
     inplace: q and k are overwritten and returned (not where a gradient is recorded; every element must have memory of
     its own). Returns (q, k); differentiable in both."""
     return kernels.block_binding().rotary_embed(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor,
-                                                tensor_layout, inplace)
+                                                tensor_layout, rope.axes, inplace)

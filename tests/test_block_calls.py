@@ -6,6 +6,7 @@ from torch.autograd import forward_ad
 
 from lingbot_world_v2_realtime_amd import kernels
 from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
+from lingbot_world_v2_realtime_amd.layers.rotary import Rotary, rotary_embed
 
 
 @pytest.fixture
@@ -69,3 +70,25 @@ def test_raw_calls_without_grad_mode_go_on():
                                              torch.zeros(1, 1, 16, 1, dtype=torch.bfloat16))):
             with pytest.raises(ValueError, match="device tensor"):
                 call()
+
+
+@pytest.mark.parametrize("axes", [1, 2])
+@pytest.mark.parametrize("batch", [False, True])
+def test_rotary_positions_need_every_axis_of_the_plan(axes, batch):
+    """A plan of frame, row and column with positions of two columns (or one) has nothing to turn the last section by."""
+    rope = Rotary.build(128, "cpu", sections=(22, 21, 21))
+    q = torch.zeros(2, 6, 1, 128, dtype=torch.bfloat16)
+    pos = torch.zeros((2, 6, axes) if batch else (6, axes), dtype=torch.int64)
+    assert rope.axes == 3 and Rotary.build(128, "cpu").axes == 1
+    with pytest.raises(ValueError, match="3 axes"):
+        rotary_embed(q, None, pos, rope)
+    with pytest.raises(ValueError, match="3 axes"):
+        kernels.rotary(q, None, pos, rope.freq, rope.axis, axes=rope.axes)
+
+
+def test_a_plan_built_by_hand_may_leave_its_axes_open():
+    rope = Rotary.build(128, "cpu", sections=(22, 21, 21))
+    by_hand = Rotary(rope.freq, rope.axis, rope.pairs, rope.factor)
+    assert by_hand.axes is None
+    with pytest.raises(ValueError, match="axes"):
+        rotary_embed(torch.zeros(1, 6, 1, 128), None, torch.zeros(6, 3, dtype=torch.int64), Rotary(rope.freq, rope.axis, axes=0))
