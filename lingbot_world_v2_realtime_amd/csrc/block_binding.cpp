@@ -7,7 +7,6 @@
 // it does not take. A status from the library goes to the function that `on_status` was given, which raises.
 #include <Python.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
@@ -513,12 +512,86 @@ struct Rotary {
   }
 };
 
+// Memory that tensors share, found exactly for strided views too (torch's own check answers for packed ones only). Two
+// elements share a byte where sum x_k step_k = target has a solution with lo_k <= x_k <= hi_k: a term for every
+// dimension of either, and one of single bytes for the elements' size.
+class Overlap {
+  struct Term {
+    int64_t step, lo, hi;
+  };
+  static constexpr int MOST = 2 * 4 + 1;      // (4-d tensors)
+  Term terms[MOST];                           // steps falling, the bytes last
+  int64_t low[MOST + 1], high[MOST + 1];      // least and largest sum of the terms from k on
+  int n = 0, budget = 1 << 16;                // looks, after which the answer is that they might
+
+  void add(const Tensor& t, bool first, bool second) {
+    const int64_t size = t.element_size();
+    for (int i = 0; i < 4; ++i) {
+      const int64_t most = t.size(i) - 1;
+      if (most > 0) terms[n++] = {t.stride(i) * size, second ? -most : 0, first ? most : 0};
+    }
+  }
+  void sort(int64_t size) {
+    std::sort(terms, terms + n, [](const Term& a, const Term& b) { return a.step > b.step; });
+    terms[n++] = {1, 1 - size, size - 1};
+    low[n] = high[n] = 0;
+    for (int k = n; k-- > 0;) {
+      low[k] = low[k + 1] + terms[k].lo * terms[k].step;
+      high[k] = high[k + 1] + terms[k].hi * terms[k].step;
+    }
+  }
+  static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+  // whether the terms from k on reach `target`
+  bool reach(int k, int64_t target) {
+    if (target < low[k] || target > high[k]) return false;
+    // (nothing but bytes, and steps of zero, left: they reach all of their range)
+    if (k + 1 == n || terms[k].step == 0 || --budget < 0) return true;
+    const Term& t = terms[k];
+    const int64_t x0 = std::max(t.lo, -floor_div(high[k + 1] - target, t.step)), x1 = std::min(t.hi, floor_div(target - low[k + 1], t.step));
+    for (int64_t x = x0; x <= x1; ++x)
+      if (reach(k + 1, target - x * t.step)) return true;
+    return false;
+  }
+
+ public:
+  static bool of(const Tensor& a, const Tensor& b) {
+    if (!a.defined() || !b.defined() || !a.numel() || !b.numel() || a.device() != b.device()) return false;
+    Overlap o;
+    o.add(a, true, false);
+    o.add(b, false, true);
+    o.sort(a.element_size());
+    return o.reach(0, (const char*)b.data_ptr() - (const char*)a.data_ptr());
+  }
+  // whether two elements of `t` share memory: two places that differ, by more in the k-th term than by nothing
+  static bool within(const Tensor& t) {
+    if (!t.defined() || !t.numel()) return false;
+    Overlap o;
+    o.add(t, true, true);
+    o.sort(t.element_size());
+    for (int k = 0; k + 1 < o.n; ++k) {
+      const Term& d = o.terms[k];
+      if (d.step == 0) return true;
+      for (int64_t x = 1; x <= d.hi && x * d.step <= o.high[k + 1]; ++x)
+        if (o.reach(k + 1, -x * d.step)) return true;
+    }
+    return false;
+  }
+};
+
 // Tensors of which one is written while the other is read or written, by different threads.
 void apart(const Tensor& a, const Tensor& b, const char* what) {
-  if (!a.defined() || !b.defined()) return;
-  const auto o = at::get_overlap_status(a, b);
-  if (o == at::MemOverlapStatus::Full || o == at::MemOverlapStatus::Partial || (a.numel() && b.numel() && a.data_ptr() == b.data_ptr()))
-    value_error(what, " share their memory");
+  if (Overlap::of(a, b)) value_error(what, " share their memory");
+}
+
+// An output: every element has memory of its own.
+void own_memory(const Tensor& t, const char* name) {
+  if (Overlap::within(t)) value_error(name, " has elements that share their memory");
+}
+
+bool same_memory(const Tensor& a, const Tensor& b) {   // (of one shape)
+  bool same = a.data_ptr() == b.data_ptr();
+  for (int64_t i = 0; i < a.dim(); ++i) same = same && (a.size(i) <= 1 || a.stride(i) == b.stride(i));
+  return same;
 }
 
 // A tensor written in place: a graph that kept it notices.
@@ -569,9 +642,8 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool grad = records_gradient({a.q, a.k});
   if (truth(args[9])) {
     if (grad) value_error("q and k cannot be rotated in place where a gradient is recorded");
-    for (const Tensor* t : {&a.q, &a.k})
-      for (int j = 0; t->defined() && j < 4; ++j)
-        if (t->stride(j) == 0 && t->size(j) > 1) value_error("q or k has elements that share their memory");
+    own_memory(a.q, "q");
+    own_memory(a.k, "k");
     apart(a.q, a.k, "q and k, to be rotated in place,");
     a.run(a.q, a.k, false, true);
     written(a.q);
@@ -602,11 +674,8 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!o.defined()) continue;
     if (o.scalar_type() != x.scalar_type() || o.sizes() != x.sizes() || !unit_stride(o))
       value_error(name, " must be ", x.scalar_type(), " ", dims(x.sizes()), " with contiguous channels");
-    for (int j = 0; j < 4; ++j)
-      if (o.stride(j) == 0 && o.size(j) > 1) value_error(name, " has elements that share their memory");
-    if (o.numel() && (o.data_ptr() == x.data_ptr() ? o.strides() != x.strides()
-                                                   : at::get_overlap_status(o, x) == at::MemOverlapStatus::Partial))
-      value_error(name, " overlaps its input, but is not the input itself");
+    own_memory(o, name);
+    if (!same_memory(o, x) && Overlap::of(o, x)) value_error(name, " overlaps its input, but is not the input itself");
   }
   same_device("rotary", a.q, out[0], out[1]);
   apart(out[0], out[1], "q_out and k_out");

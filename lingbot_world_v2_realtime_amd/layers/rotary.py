@@ -83,7 +83,7 @@ def rotary_embed(q, k, positions, rope, tensor_layout="NHD", inplace=False):
     on the GPU, any strides with contiguous channels, any head counts). positions: int32 or int64 tensor [L] or [B, L]
     (with several axes [L, axes] or [B, L, axes]), or an int: the first token's position, the others following.
     Channels past the plan's are copied. Angles are formed in 64 bits, the rotation in fp32, with one rounding.
-    inplace: q and k are overwritten and returned (not where a gradient is recorded; every element must have memory of
-    its own). Returns (q, k); differentiable in both."""
+    inplace: q and k are overwritten and returned (refused where a gradient is recorded, or where two elements of them
+    share memory). Returns (q, k); differentiable in both."""
     return kernels.block_binding().rotary_embed(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor,
                                                 tensor_layout, rope.axes, inplace)

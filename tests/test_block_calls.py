@@ -92,3 +92,81 @@ def test_a_plan_built_by_hand_may_leave_its_axes_open():
     assert by_hand.axes is None
     with pytest.raises(ValueError, match="axes"):
         rotary_embed(torch.zeros(1, 6, 1, 128), None, torch.zeros(6, 3, dtype=torch.int64), Rotary(rope.freq, rope.axis, axes=0))
+
+
+def _answer(call):
+    """'ok' where only the host tensors are refused, else what the call said."""
+    with pytest.raises(ValueError) as e:
+        call()
+    said = str(e.value)
+    return "ok" if "device tensor" in said else said
+
+
+def _addresses(t):
+    at = torch.tensor(t.storage_offset())
+    for n, s in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    return at.flatten().tolist()
+
+
+FREQ = torch.ones(1, dtype=torch.float64)
+
+
+def test_rotary_outputs_that_share_memory_are_refused():
+    """Views with gaps, of which the channels, heads or tokens of one lie in the other: their threads would write over what
+    others read. Views that only lie between each other are taken."""
+    fused = torch.zeros(2, 5, 10, 8, dtype=torch.bfloat16)
+    rope = Rotary(FREQ)
+
+    def inplace(q, k=None):
+        return _answer(lambda: rotary_embed(q, k, 0, rope, inplace=True))
+
+    assert inplace(fused[:, :, :6], fused[:, :, 6:8]) == "ok"                 # q and k of one projection
+    assert inplace(fused[:, :, ::2], fused[:, :, 1::2]) == "ok"               # alternating heads
+    assert inplace(fused[:, :3], fused[:, 2:][:, :3]) != "ok"                 # a token of both
+    assert inplace(fused[:, :, :6], fused[:, :, 5:7]) != "ok"                 # a head of both
+    assert inplace(fused[..., :4], fused[..., 3:7]) != "ok"                   # a channel of both
+    assert inplace(fused[..., :4], fused[..., 4:]) == "ok"
+    flat = torch.zeros(400, dtype=torch.bfloat16)
+    assert inplace(flat.as_strided((1, 20, 1, 8), (400, 8, 8, 1))) == "ok"
+    assert "share" in inplace(flat.as_strided((1, 20, 1, 8), (400, 7, 8, 1)))      # windows one channel into the next
+    assert "share" in inplace(flat.as_strided((2, 5, 3, 8), (40, 8, 40, 1)))       # two ways to the same head
+    assert inplace(flat.as_strided((2, 3, 5, 8), (120, 40, 8, 1)).transpose(1, 2)) == "ok"
+
+    def out(q, q_out, **kw):
+        return _answer(lambda: kernels.rotary(q, None, 0, FREQ, q_out=q_out, **kw))
+
+    assert out(fused[:, :, :6], fused[:, :, :6]) == "ok"                      # the input itself
+    assert "overlaps" in out(fused[:, :, :6], fused[:, :, 1:7])
+    assert "overlaps" in out(fused[..., :4], fused[..., 2:6])
+    assert out(fused[:, :, :4], fused[:, :, 4:8]) == "ok"
+    assert "overlaps" in out(fused[:, :2], fused[:, :2].transpose(0, 1))      # its memory in another order
+    assert "share" in out(fused[:, :, :1], flat.as_strided((2, 5, 1, 8), (35, 7, 7, 1)))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_rotary_overlaps_against_every_address(seed):
+    """Two strided views of one buffer, of random sizes and steps, against the sets of their elements' addresses."""
+    g = torch.Generator().manual_seed(seed)
+    rope, seen = Rotary(FREQ), set()
+
+    def draw(*of):
+        return of[int(torch.randint(len(of), (), generator=g))]
+
+    buf = torch.zeros(4096)
+    for _ in range(300):
+        b, n, h = draw(1, 2), draw(1, 2, 3), draw(1, 2, 3)
+        d = draw(2, 3, 4)
+        shape = (b, n, h, d)
+        q, k = (buf.as_strided(shape, (draw(0, 5, 12, 24, 36, 72), draw(3, 4, 12, 13, 24), draw(2, 3, 4, 6, 8, 24), 1),
+                               draw(0, 1, 2, 4, 6, 12, 16, 40, 100)) for _ in range(2))
+        at = [_addresses(t) for t in (q, k)]
+        own = [len(set(a)) == len(a) for a in at]
+        apart = not set(at[0]) & set(at[1])
+        same = at[0] == at[1]
+        said = _answer(lambda: rotary_embed(q, k, 0, rope, inplace=True))
+        assert (said == "ok") == (all(own) and apart), (shape, q.stride(), k.stride(), said)
+        said = _answer(lambda: kernels.rotary(q, None, 0, FREQ, q_out=k))
+        assert (said == "ok") == (own[1] and (apart or same)), (shape, q.stride(), k.stride(), said)
+        seen.add((all(own), apart, same))
+    assert len(seen) >= 4
