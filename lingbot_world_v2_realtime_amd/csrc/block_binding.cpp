@@ -157,17 +157,20 @@ Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
 // Whether autograd has to see the call: a gradient is recorded, or an input carries a forward-mode tangent (which it
 // refuses).
-bool records_gradient(std::initializer_list<Tensor> ts) {
-  for (const Tensor& t : ts)
-    if (t.defined() && ((c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())) return true;
-  return false;
+bool records_gradient(const Tensor& t) {
+  if (!t.defined() || !t.unsafeGetTensorImpl()->autograd_meta()) return false;   // (a plain tensor has none)
+  return (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
+}
+template <typename... T>
+bool records_gradient(const Tensor& t, const T&... rest) {
+  return records_gradient(t) || records_gradient(rest...);
 }
 
 // For the calls that have no gradient of their own: a tensor among the arguments that would record one is refused (the
 // result would be detached).
 void no_gradient(const char* what, PyObject* const* args, Py_ssize_t n) {
   for (Py_ssize_t i = 0; i < n; ++i) {
-    if (!THPVariable_Check(args[i]) || !records_gradient({THPVariable_Unpack(args[i])})) continue;
+    if (!THPVariable_Check(args[i]) || !records_gradient(THPVariable_Unpack(args[i]))) continue;
     PyErr_Format(PyExc_RuntimeError, "%s records no gradient: call it under torch.no_grad(), or on detached tensors", what);
     throw python_error();
   }
@@ -384,7 +387,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     own[i] = held[i - 2].get();
   }
   const Norm a(own.data());
-  if (!records_gradient({a.x, a.y, a.v[0], a.v[1], a.v[2], a.v[3], a.v[4], a.v[5]}))
+  if (!records_gradient(a.x, a.y, a.v[0], a.v[1], a.v[2], a.v[3], a.v[4], a.v[5]))
     return wrap_all(a.forward(a.y.defined()));
   const auto out = NormFunction::apply(a.x, maybe(a.y), maybe(a.v[0]), maybe(a.v[1]), maybe(a.v[2]), maybe(a.v[3]),
                                        maybe(a.v[4]), maybe(a.v[5]), &a);
@@ -461,7 +464,7 @@ struct Rotary {
       value_error("q and k need a head at least");
     if (freq.scalar_type() != at::kDouble || freq.dim() != 1 || !freq.is_contiguous() || freq.size(0) < 1)
       value_error("freq must be contiguous float64 [pairs], got ", freq.scalar_type(), " ", dims(freq.sizes()));
-    if (records_gradient({freq})) value_error("freq has no gradient: detach it");
+    if (records_gradient(freq)) value_error("freq has no gradient: detach it");
     if (2 * freq.size(0) > d || d > LBW_ROTARY_MAX_DIM)
       value_error(freq.size(0), " pairs do not fit heads of ", d, " (of ", LBW_ROTARY_MAX_DIM, " at most)");
     if (axis.defined() && (axis.scalar_type() != at::kInt || axis.sizes() != freq.sizes() || !axis.is_contiguous()))
@@ -639,7 +642,7 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 10);
   const Rotary a(args);
-  const bool grad = records_gradient({a.q, a.k});
+  const bool grad = records_gradient(a.q, a.k);
   if (truth(args[9])) {
     if (grad) value_error("q and k cannot be rotated in place where a gradient is recorded");
     own_memory(a.q, "q");
