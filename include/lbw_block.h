@@ -115,11 +115,15 @@ int lbw_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t l
 int lbw_quant_w4(const void* w, int w_is_fp32, int64_t n, int64_t k, int64_t s_row, int fmt, int64_t group,
                  uint8_t* w4, uint16_t* scale, uint8_t* zero, void* stream);
 
+/* Beside the element format of lbw_gemm_w4: the bias is fp32. */
+#define LBW_W4_BIAS_FP32 256
+
 /*
  * out[m][n] = x w^T + bias: x [m][k] of `dtype` (bf16 or fp16; row stride x_s_row; the k that w was packed for), w
- * as above, bias [n] of `dtype` or null, out [m][n] packed of `dtype`. Codes enter the products exactly; sums, the
- * group scales and the bias are fp32, with one rounding at the end. m <= 2^24, n <= 1048560, k <= 2^20. With
- * LBW_W4_INT4 a row of x that holds an infinity gives NaN (the codes' offset is taken off the sums).
+ * as above, bias [n] of `dtype` (of fp32 where dtype has LBW_W4_BIAS_FP32 added) or null, out [m][n] packed of `dtype`.
+ * Codes enter the products exactly; sums and group scales are fp32, the bias is added in fp32, with one rounding at the
+ * end. m <= 2^24, n <= 1048560, k <= 2^20. With LBW_W4_INT4 a row of x that holds an infinity gives NaN (the codes'
+ * offset is taken off the sums).
  */
 int lbw_gemm_w4(const void* x, int dtype, int64_t m, int64_t k, int64_t x_s_row, const uint8_t* w4,
                 const uint16_t* scale, const uint8_t* zero, int fmt, int64_t group, int64_t n, const void* bias,

@@ -693,15 +693,14 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---------------------------------------------------------------- 4-bit linears
 
-// x, w4, scale, zero, bias, out_features, fmt
+// x, w4, scale, zero, bias, out_features, fmt, whether the bias may be fp32 (else it has x's type)
 PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  count(n_args, 7);
+  count(n_args, 8);
   no_gradient("gemm_w4", args, n_args);
   const Tensor& x = tensor("x", args[0]);
   const auto dt = x.scalar_type();
   if (dt != at::kBFloat16 && dt != at::kHalf) type_error("x must be bfloat16 or float16, got ", dt);
-  if (!x.is_cuda()) value_error("x must be a device tensor (the 4-bit path has no CPU implementation)");
   if (x.dim() != 2 || !unit_stride(x) || x.size(1) < 1)
     value_error("x must be [M, K] with contiguous rows, got ", dims(x.sizes()), " / ", dims(x.strides()));
   Tensor w4 = tensor("w4", args[1]), scale = tensor("scale", args[2]), zero = tensor("zero", args[3], true);
@@ -721,8 +720,10 @@ PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     value_error("scale must be contiguous bfloat16 ", dims(groups), ", got ", scale.scalar_type(), " ", dims(scale.sizes()));
   if (zero.defined() && (zero.scalar_type() != at::kByte || zero.sizes() != at::IntArrayRef(groups) || !zero.is_contiguous()))
     value_error("zero must be contiguous uint8 ", dims(groups), ", got ", zero.scalar_type(), " ", dims(zero.sizes()));
-  if (bias.defined() && (bias.scalar_type() != dt || bias.dim() != 1 || bias.size(0) != n || !bias.is_contiguous()))
+  const bool bias_fp32 = bias.defined() && bias.scalar_type() == at::kFloat && truth(args[7]);
+  if (bias.defined() && ((bias.scalar_type() != dt && !bias_fp32) || bias.dim() != 1 || bias.size(0) != n || !bias.is_contiguous()))
     value_error("bias must be contiguous ", dt, " (", n, ",), got ", bias.scalar_type(), " ", dims(bias.sizes()));
+  if (!x.is_cuda()) value_error("x must be a device tensor (the 4-bit path has no CPU implementation)");
   same_device("gemm_w4", x, w4, scale, zero, bias);
   const On on(x);
   // weights at an address the kernel does not load from (views of a larger buffer) as copies
@@ -730,7 +731,7 @@ PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (t->defined() && (uintptr_t)t->data_ptr() % 16) *t = t->clone();
   Tensor out = at::empty({m, n}, x.options());
   if (m)
-    done(lbw_gemm_w4(x.data_ptr(), dt == at::kHalf ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16, m, k, x.stride(0), (const uint8_t*)w4.data_ptr(),
+    done(lbw_gemm_w4(x.data_ptr(), (dt == at::kHalf ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16) + (bias_fp32 ? LBW_W4_BIAS_FP32 : 0), m, k, x.stride(0), (const uint8_t*)w4.data_ptr(),
                      (const uint16_t*)scale.data_ptr(), (const uint8_t*)ptr(zero), fmt == "fp4" ? LBW_W4_FP4 : LBW_W4_INT4,
                      128 / per, n, ptr(bias), out.data_ptr(), on.stream),
          "lbw_gemm_w4");

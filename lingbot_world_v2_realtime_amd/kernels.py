@@ -588,7 +588,7 @@ def gemm_w4(x, w4, scale, zero=None, bias=None, out_features=None, fmt="int4"):
     (lbw_gemm_w4), bias of x's dtype [N] or None -> [M, N] of x's dtype: codes exact, sums, scales and bias in fp32, one
     rounding. out_features: N where it is not a multiple of 16 (default: every row the tiles hold). K has to end in the
     tiles' last 128 columns; which of them, the caller knows (W4Linear checks it). No gradient: a call that would record one is refused."""
-    return block_binding().gemm_w4(x, w4, scale, zero, bias, out_features, fmt)
+    return block_binding().gemm_w4(x, w4, scale, zero, bias, out_features, fmt, False)
 
 
 _ATTN_WS = {}

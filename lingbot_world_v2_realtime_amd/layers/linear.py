@@ -186,8 +186,9 @@ class W4Linear(torch.nn.Module):
     embedding and the modulation it gives), a few sequences, a context's tokens. Codes of 4 bits with a bf16 scale for each `group`
     columns (32, 64 or 128): fmt 'int4', with `zeros` a zero point for each group too, or 'fp4' (e2m1). Weights are
     quantised once (lbw_quant_w4), a call is one kernel (lbw_gemm_w4) on bf16 or fp16 activations, other types cast to
-    bf16; out in that type. Codes are exact in the products and every scale, sum and the bias fp32. No gradient reaches the
-    input: a call that would record one is refused. A bias that records one is added after the kernel."""
+    bf16; out in that type. Codes are exact in the products, every scale and sum is fp32, and the bias, of x's type or fp32, is
+    added in fp32 before the one rounding. No gradient reaches the input: a call that would record one is refused. A bias
+    that records one is added after the kernel, to the rounded product."""
 
     def __init__(self, lin, group=128, fmt="int4", zeros=False):
         super().__init__()
@@ -225,13 +226,13 @@ class W4Linear(torch.nn.Module):
         if x2.shape[1] > 1 and x2.stride(1) != 1:
             x2 = x2.contiguous()
         bias = self.bias
-        if bias is not None:
-            bias = bias.to(x2.dtype)
+        if bias is not None and bias.dtype is not torch.float32 and bias.dtype is not x2.dtype:
+            bias = bias.float()
         fused = bias is None or (block.plain(bias) and bias.is_contiguous())
         y = block.gemm_w4(x2, self.w4, self.w4_scale, self.w4_zero, bias if fused else None, self.out_features,
-                          self.fmt)
+                          self.fmt, True)
         if not fused:
-            y = y + bias
+            y = (y + bias).to(x2.dtype)
         return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)
 
 

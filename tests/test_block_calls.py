@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from lingbot_world_v2_realtime_amd import kernels
+from lingbot_world_v2_realtime_amd import _lib, kernels
 from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
 from lingbot_world_v2_realtime_amd.layers.rotary import Rotary, rotary_embed
 
@@ -170,3 +170,19 @@ def test_rotary_overlaps_against_every_address(seed):
         assert (said == "ok") == (own[1] and (apart or same)), (shape, q.stride(), k.stride(), said)
         seen.add((all(own), apart, same))
     assert len(seen) >= 4
+
+
+def test_gemm_w4_takes_a_bias_of_its_own_type_only():
+    x = torch.zeros(2, 128, dtype=torch.bfloat16)
+    tiles = torch.zeros(1, 1, 1024, dtype=torch.uint8), torch.zeros(1, 1, 16, 1, dtype=torch.bfloat16)
+    for bias in (torch.zeros(16), torch.zeros(16, dtype=torch.float16)):
+        with pytest.raises(ValueError, match="bias must be"):
+            kernels.gemm_w4(x, *tiles, bias=bias)
+
+
+def test_w4_entry_point_takes_an_fp32_bias():
+    """Its flag beside the format: alignment of four bytes, and no other bit."""
+    def gemm(dtype, bias):
+        return _lib.load().lbw_gemm_w4(1 << 20, dtype, 3, 100, 100, 1 << 20, 1 << 20, None, 0, 64, 30, bias, 1 << 20, None)
+    assert gemm(0, (1 << 20) + 1) == 3 and gemm(256, (1 << 20) + 2) == 3
+    assert gemm(2, None) == 2 and gemm(256 + 2, None) == 2 and gemm(512, None) == 2

@@ -26,3 +26,36 @@ def test_rotary_axis_that_the_positions_do_not_hold():
             # (positions up to 500 of a frequency of 1: the 64-bit angle adds nothing to the 12 roundings)
             _within(o[..., held], (want[..., held], mag[..., held]), pairs, 13)
             assert bool(o[..., first[10:]].isnan().all()) and bool(o[..., second[10:]].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (5, 1001, 256), (3, 37, 300), (70, 4004, 392), (1030, 2320, 256),
+                                   (1030, 2310, 256)])
+def test_w4_linear_adds_an_fp32_bias_unrounded(m, n, k, dtype):
+    """nn.Linear's own parameters are fp32. With a bias far larger than the products the output is the bias, rounded once:
+    rounded to x's type first it would be off by up to a whole step where half of one is allowed."""
+    from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
+    torch.manual_seed(m + n)
+    lin = torch.nn.Linear(k, n).to(DEV)
+    with torch.no_grad():
+        lin.bias.normal_(std=30.0)
+    for fmt, zeros in (("int4", True), ("fp4", False)):
+        mod = W4Linear(lin, 64, fmt, zeros)
+        sc, z = block.unpack_scale(mod.w4_scale), None if mod.w4_zero is None else block.unpack_scale(mod.w4_zero)
+        value = block.w4_values(block.unpack_w4(mod.w4, fmt), sc, z, fmt)[:n, :k]
+        x = torch.randn(m, k, device=DEV, generator=_rand(m)).to(DT[dtype])
+        mag = x.double().abs() @ (sc.double().repeat_interleave(64, 1)[:n, :k] * 62).t().contiguous()
+        want = x.double() @ value.t().contiguous() + lin.bias.double()
+        with torch.no_grad():
+            got = mod(x)
+        assert got.dtype == x.dtype
+        _within(got, (want, mag + want.abs()), f"{m}x{n}x{k} {fmt} {dtype}", k / 16 + 24)
+        # a bias that records a gradient is added after the kernel: one more rounding, of the product alone
+        y = mod(x)
+        assert y.dtype == x.dtype
+        half = torch.finfo(x.dtype).eps / 2
+        err = (y.detach().double() - want).abs()
+        tol = half * want.abs() + half * (want - lin.bias.double()).abs() + (k / 16 + 24) * 2.0 ** -24 * (mag + want.abs())
+        assert bool((err <= 1.02 * tol).all())   # (a rounding of what a rounding gave: products of two halves, under 2^-8)
+        (g,) = torch.autograd.grad(y, lin.bias, torch.ones_like(y))
+        assert torch.equal(g, torch.full_like(lin.bias, m))
