@@ -94,7 +94,7 @@ int lbw_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t l
                int64_t ko_s_head, void* stream);
 
 /* Code formats of the 4-bit weights. */
-#define LBW_W4_INT4 0   /* value code - zero, zero 0 .. 15 for each group (8 without zeros) */
+#define LBW_W4_INT4 0   /* value code - zero, a zero for each group (8 without zeros) */
 #define LBW_W4_FP4 1    /* e2m1: sign, two exponent bits, one mantissa bit: +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} */
 
 /*
@@ -103,7 +103,7 @@ int lbw_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t l
  *   w4     uint8 [nt][kt][1024]: word j (0 .. 3) of lane 16 q + r holds the codes of row r at columns 32 j + 8 q + i,
  *          i = 0 .. 7; its nibble s holds i = s for LBW_W4_FP4 and i = 2 s (s < 4), 2 s - 7 (s >= 4) for LBW_W4_INT4
  *   scale  bf16  [nt][kt][16][128 / group]
- *   zero   uint8 [nt][kt][16][128 / group], LBW_W4_INT4 only, or null
+ *   zero   uint8 [nt][kt][16][128 / group], LBW_W4_INT4 only, or null (8); lbw_quant_w4 makes 0 .. 15, any is taken
  * (All 16-byte aligned.) A weight is scale * value. Rows and columns past n and k hold scale 0 where a whole group
  * lies there, and any code.
  *

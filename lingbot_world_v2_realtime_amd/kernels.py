@@ -558,8 +558,9 @@ W4_NIBBLES = {"int4": (0, 2, 4, 6, 1, 3, 5, 7), "fp4": (0, 1, 2, 3, 4, 5, 6, 7)}
 
 
 def pack_w4(codes, scale, zero=None, fmt="int4"):
-    """Codes a checkpoint holds (uint8 [N, K], values 0 .. 15), with their scales (and zeros) [N, ceil(K / group)], in the
-    tiles gemm_w4 takes: (w4, scale rounded to bf16, zero uint8 or None) as quant_w4 makes them. Runs once at load, on any device."""
+    """Codes a checkpoint holds (uint8 [N, K], values 0 .. 15), with their scales (and zeros: whole numbers of any type, 0 ..
+    255) [N, ceil(K / group)], in the tiles gemm_w4 takes: (w4, scale rounded to bf16, zero uint8 or None) as quant_w4 makes
+    them. Runs once at load, on any device; it reads the values to check them, so not into a graph."""
     if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.numel() == 0:
         raise ValueError(f"codes must be uint8 [N, K], got {codes.dtype} {tuple(codes.shape)}")
     if fmt not in W4_FORMATS or (zero is not None and fmt != "int4"):
@@ -568,6 +569,12 @@ def pack_w4(codes, scale, zero=None, fmt="int4"):
     fits = [g for g in W4_GROUPS if tuple(scale.shape) == (n, -(-k // g))]
     if not fits or (zero is not None and zero.shape != scale.shape):
         raise ValueError(f"scale {tuple(scale.shape)} does not hold {n} rows of groups of {W4_GROUPS}")
+    if int(codes.max()) > 15:
+        raise ValueError(f"codes must be 0 .. 15, got {int(codes.max())}")
+    if zero is not None and zero.dtype != torch.uint8:
+        z = zero.double()   # (a narrow integer type cannot be compared with 255)
+        if not bool(((z >= 0) & (z <= 255) & (z % 1 == 0)).all()):
+            raise ValueError("zeros must be whole numbers of 0 .. 255")
     group = fits[-1]
     (nt, kt, _), scales = _w4_shapes(n, k, group)
     full = codes.new_zeros(nt * 16, kt * 128)

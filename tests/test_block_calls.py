@@ -7,6 +7,7 @@ from torch.autograd import forward_ad
 from lingbot_world_v2_realtime_amd import _lib, kernels
 from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
 from lingbot_world_v2_realtime_amd.layers.rotary import Rotary, rotary_embed
+from oracle import block
 
 
 @pytest.fixture
@@ -186,3 +187,22 @@ def test_w4_entry_point_takes_an_fp32_bias():
         return _lib.load().lbw_gemm_w4(1 << 20, dtype, 3, 100, 100, 1 << 20, 1 << 20, None, 0, 64, 30, bias, 1 << 20, None)
     assert gemm(0, (1 << 20) + 1) == 3 and gemm(256, (1 << 20) + 2) == 3
     assert gemm(2, None) == 2 and gemm(256 + 2, None) == 2 and gemm(512, None) == 2
+
+
+def test_pack_w4_refuses_what_its_bytes_cannot_hold():
+    """Zeros that a cast to a byte would change, and codes of more than four bits, which would lose their upper ones."""
+    codes, scale = torch.zeros(4, 128, dtype=torch.uint8), torch.ones(4, 2)
+    for bad in (7.5, -1.0, 256.0, float("nan"), float("inf")):
+        zero = torch.full((4, 2), 8.0)
+        zero[3, 1] = bad
+        with pytest.raises(ValueError, match="zeros must be whole numbers"):
+            kernels.pack_w4(codes, scale, zero)
+    for bad in (torch.full((4, 2), -1, dtype=torch.int8), torch.full((4, 2), 300)):
+        with pytest.raises(ValueError, match="zeros must be whole numbers"):
+            kernels.pack_w4(codes, scale, bad)
+    for kind in (torch.float32, torch.float16, torch.int8, torch.int64, torch.uint8):
+        z = kernels.pack_w4(codes, scale, torch.full((4, 2), 9, dtype=kind))[2]
+        assert z.dtype == torch.uint8 and bool((block.unpack_scale(z)[:4, :2] == 9).all())
+    codes[2, 77] = 16
+    with pytest.raises(ValueError, match="0 .. 15"):
+        kernels.pack_w4(codes, scale)

@@ -59,3 +59,19 @@ def test_w4_linear_adds_an_fp32_bias_unrounded(m, n, k, dtype):
         assert bool((err <= 1.02 * tol).all())   # (a rounding of what a rounding gave: products of two halves, under 2^-8)
         (g,) = torch.autograd.grad(y, lin.bias, torch.ones_like(y))
         assert torch.equal(g, torch.full_like(lin.bias, m))
+
+
+@pytest.mark.parametrize("m", [1, 40, 1030])
+def test_gemm_w4_zeros_past_the_codes(m):
+    """Zeros of any byte, as checkpoints that count them from one hold 16: the value is code - zero all the same."""
+    from lingbot_world_v2_realtime_amd import kernels
+    g, n, k = _rand(72), 2320, 256
+    codes = torch.randint(0, 16, (n, k), device=DEV, generator=g, dtype=torch.uint8)
+    scale = (torch.rand(n, 4, device=DEV, generator=g) + 0.1).bfloat16()
+    zero = torch.randint(0, 256, (n, 4), device=DEV, generator=g, dtype=torch.uint8)
+    zero[0] = 16
+    x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    want = x.double() @ block.w4_values(codes, scale, zero, "int4").t().contiguous()
+    # what the products and their offset add: codes up to 31 steps, zeros up to 255 + 16
+    mag = x.double().abs() @ (scale.double().repeat_interleave(64, 1) * 302).t().contiguous()
+    _within(kernels.gemm_w4(x, *kernels.pack_w4(codes, scale, zero.float())), (want, mag + want.abs()), f"{m} rows", k / 16 + 24)
