@@ -503,6 +503,9 @@ def gated_norm_bwd(x, ds, dh, y=None, gate=None, shift=None, scale=None, weight=
                    wants=_NORM_INPUTS):
     """The gradients of gated_norm (lbw_gated_norm_bwd) from those of its outputs (ds, dh [B, L, C] of x's dtype, either
     None): a dict name -> gradient of each given input named in `wants`, in its shape and dtype."""
+    wants = wants if isinstance(wants, str) else tuple(wants)
+    if isinstance(wants, str) or any(name not in _NORM_INPUTS for name in wants):
+        raise ValueError(f"wants must be a sequence of names out of {_NORM_INPUTS}, got {wants!r}")
     bits = sum(1 << i for i, name in enumerate(_NORM_INPUTS) if name in wants)
     grads = block_binding().gated_norm_bwd(x, y, gate, shift, scale, weight, bias, post_weight, norm, post_norm, eps,
                                            residual_scale, branch_scale, group_len, ds, dh, bits)

@@ -206,3 +206,15 @@ def test_pack_w4_refuses_what_its_bytes_cannot_hold():
     codes[2, 77] = 16
     with pytest.raises(ValueError, match="0 .. 15"):
         kernels.pack_w4(codes, scale)
+
+
+def test_gated_norm_bwd_names_its_gradients():
+    """wants holds names of inputs: a plain string would be searched letter by letter (and 'weight' be found in
+    'post_weight'), an unknown name would ask for nothing."""
+    x = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    for bad in ("post_weight", "x", ("gat",), ("x", "wieght"), (0,)):
+        with pytest.raises((ValueError, TypeError), match="wants"):
+            kernels.gated_norm_bwd(x, None, x, wants=bad)
+    for good in ((), ["x"], ("x", "gate"), {"x"}):
+        with pytest.raises(ValueError, match="device tensor"):
+            kernels.gated_norm_bwd(x, None, x, wants=good)
