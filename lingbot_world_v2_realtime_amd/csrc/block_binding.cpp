@@ -739,20 +739,41 @@ PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+bool in_transform(const Tensor& t) {
+  const auto keys = t.key_set();
+  return keys.has(c10::DispatchKey::FuncTorchBatched) || keys.has(c10::DispatchKey::FuncTorchGradWrapper) ||
+         keys.has(c10::DispatchKey::Functionalize);
+}
+
+// The input of a 4-bit linear, refused where the kernel may not take it by its address or would lose its gradient.
+PyObject* linear_input(PyObject*, PyObject* x) {
+  HANDLE_TH_ERRORS
+  if (!THPVariable_Check(x)) type_error("W4Linear takes a tensor, got ", Py_TYPE(x)->tp_name);
+  if (!THPVariable_CheckExact(x)) type_error("W4Linear takes no tensor subclass, got ", Py_TYPE(x)->tp_name);
+  const Tensor& t = THPVariable_Unpack(x);
+  const char* why = in_transform(t) ? "W4Linear does not run inside a torch.func transform"
+      : c10::GradMode::is_enabled() && t.requires_grad()
+          ? "W4Linear has no gradient with respect to its input: call it under torch.no_grad(), or on a detached input"
+      : records_gradient(t) ? "W4Linear has no derivative for a forward-mode tangent: call it on a detached input"
+                            : nullptr;
+  if (why) {
+    PyErr_SetString(PyExc_RuntimeError, why);
+    throw python_error();
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // Whether a kernel may take these tensors (None: absent) by their address: none records a gradient, carries a
 // forward-mode tangent, stands for others inside a torch.func transform, or is of a subclass.
 PyObject* plain(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  const bool grad = c10::GradMode::is_enabled();
   for (Py_ssize_t i = 0; i < n; ++i) {
     if (args[i] == Py_None) continue;
     if (!THPVariable_Check(args[i])) continue;   // (the call itself says what it wanted)
     if (!THPVariable_CheckExact(args[i])) Py_RETURN_FALSE;
     const Tensor& t = THPVariable_Unpack(args[i]);
-    const auto keys = t.key_set();
-    if ((grad && t.requires_grad()) || keys.has(c10::DispatchKey::FuncTorchBatched) ||
-        keys.has(c10::DispatchKey::FuncTorchGradWrapper) || keys.has(c10::DispatchKey::Functionalize) || t._fw_grad(0).defined())
-      Py_RETURN_FALSE;
+    if (in_transform(t) || records_gradient(t)) Py_RETURN_FALSE;
   }
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
@@ -767,6 +788,7 @@ PyObject* on_status(PyObject*, PyObject* f) {
 #define FAST(f) {#f, (PyCFunction)(void*)f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(norm), FAST(gated_norm), FAST(gated_norm_bwd), FAST(rotary_embed), FAST(rotary), FAST(gemm_w4),
                          FAST(plain),
+                         {"linear_input", linear_input, METH_O, nullptr},
                          {"on_status", on_status, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_block", nullptr, -1, methods};
 

@@ -211,11 +211,9 @@ class W4Linear(torch.nn.Module):
         return self
 
     def forward(self, x):
-        shape = x.shape
         block = kernels.block_binding()
-        if not block.plain(x):
-            raise RuntimeError("W4Linear has no gradient with respect to its input: call it under torch.no_grad(), or on "
-                               "a detached input")
+        block.linear_input(x)
+        shape = x.shape
         if not shape or shape[-1] != self.in_features:   # (the tiles hold 128 columns each and cannot tell)
             raise ValueError(f"x must have {self.in_features} columns, got {tuple(shape)}")
         x2 = x.reshape(-1, shape[-1])

@@ -218,3 +218,22 @@ def test_gated_norm_bwd_names_its_gradients():
     for good in ((), ["x"], ("x", "gate"), {"x"}):
         with pytest.raises(ValueError, match="device tensor"):
             kernels.gated_norm_bwd(x, None, x, wants=good)
+
+
+def test_w4_linear_says_what_it_cannot_take(w4_module):
+    """A gradient, a tangent, a transform's stand-in and a tensor subclass are four reasons, not one."""
+    class Marked(torch.Tensor):
+        pass
+
+    x = torch.zeros(2, 1536, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        w4_module(x.clone().requires_grad_())
+    with torch.no_grad():
+        with pytest.raises(TypeError, match="Marked"):
+            w4_module(x.as_subclass(Marked))
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.func.vmap(w4_module)(x[None])
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangent"):
+            w4_module(forward_ad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(TypeError, match="tensor"):
+        w4_module([1.0] * 1536)
