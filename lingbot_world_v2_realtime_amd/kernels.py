@@ -536,6 +536,8 @@ def quant_w4(w, group=128, fmt="int4", zeros=False):
     (32, 64 or 128), in the tiles gemm_w4 takes (lbw_quant_w4): (w4 uint8 [N/16, K/128, 1024], scale bf16
     [N/16, K/128, 16, 128/group], zero uint8 like scale or None). fmt 'int4' (codes less 8, or with `zeros` less a zero
     of the group's own) or 'fp4' (e2m1)."""
+    if w.is_neg():
+        raise ValueError("w is a lazily negated view: give its resolve_neg()")
     if not w.is_cuda:
         raise ValueError("w must be a device tensor (the 4-bit path has no CPU implementation)")
     if w.dtype not in (torch.bfloat16, torch.float32):

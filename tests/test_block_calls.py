@@ -5,7 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 from lingbot_world_v2_realtime_amd import _lib, kernels
-from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
+from lingbot_world_v2_realtime_amd.layers.linear import W4Linear, convert_to_w4
 from lingbot_world_v2_realtime_amd.layers.rotary import Rotary, rotary_embed
 from oracle import block
 
@@ -237,3 +237,9 @@ def test_w4_linear_says_what_it_cannot_take(w4_module):
             w4_module(forward_ad.make_dual(x, torch.ones_like(x)))
     with pytest.raises(TypeError, match="tensor"):
         w4_module([1.0] * 1536)
+
+
+def test_quant_w4_refuses_a_lazy_negation():
+    """It is not in memory yet, and would be read without its sign."""
+    with pytest.raises(ValueError, match="negated"):
+        kernels.quant_w4(torch._neg_view(torch.ones(16, 128)))
