@@ -534,7 +534,8 @@ def _w4_shapes(n, k, group):
 def quant_w4(w, group=128, fmt="int4", zeros=False):
     """4-bit codes of a weight [N, K] (bf16 or fp32, unit column stride) with a bf16 scale for each `group` columns
     (32, 64 or 128), in the tiles gemm_w4 takes (lbw_quant_w4): (w4 uint8 [N/16, K/128, 1024], scale bf16
-    [N/16, K/128, 16, 128/group], zero uint8 like scale or None). fmt 'int4' (codes less 8, or with `zeros` less a zero
+    [N/16, K/128, 16, 128/group], zero uint8 like scale or None). Weights are finite (a NaN would become an ordinary code;
+    W4Linear looks). fmt 'int4' (codes less 8, or with `zeros` less a zero
     of the group's own) or 'fp4' (e2m1)."""
     if w.is_neg():
         raise ValueError("w is a lazily negated view: give its resolve_neg()")

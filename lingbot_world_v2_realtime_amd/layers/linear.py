@@ -195,6 +195,8 @@ class W4Linear(torch.nn.Module):
         w = lin.weight.detach()
         if w.dtype not in (torch.bfloat16, torch.float32):
             w = w.float()
+        if not bool(w.isfinite().all()):
+            raise ValueError("a linear's weight must be finite to be quantised")
         w4, scale, zero = kernels.quant_w4(w.contiguous(), group, fmt, zeros)
         self.register_buffer("w4", w4)
         self.register_buffer("w4_scale", scale)
@@ -239,12 +241,10 @@ def convert_to_w4(blocks, group=128, fmt="int4", zeros=False, min_features=1024)
     stands in several places in all of them; subclasses of nn.Linear stay, as their owners may read their weight. Returns
     (replaced, linears seen)."""
     found = [(path, m) for path, m in blocks.named_modules(remove_duplicate=False) if path and type(m) is torch.nn.Linear]
-    made = {}
-    for path, m in found:
-        if min(m.in_features, m.out_features) < min_features:
-            continue
-        if m not in made:
-            made[m] = W4Linear(m, group, fmt, zeros)
+    # (all are made before any is put in: a weight that is refused leaves the module as it was)
+    fits = [(path, m) for path, m in found if min(m.in_features, m.out_features) >= min_features]
+    made = {m: W4Linear(m, group, fmt, zeros) for m in dict.fromkeys(m for _, m in fits)}
+    for path, m in fits:
         owner, _, attr = path.rpartition(".")
         setattr(blocks.get_submodule(owner), attr, made[m])
     return len(made), len({m for _, m in found})

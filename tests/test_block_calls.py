@@ -243,3 +243,19 @@ def test_quant_w4_refuses_a_lazy_negation():
     """It is not in memory yet, and would be read without its sign."""
     with pytest.raises(ValueError, match="negated"):
         kernels.quant_w4(torch._neg_view(torch.ones(16, 128)))
+
+
+def test_w4_linear_refuses_weights_that_are_not_finite(monkeypatch):
+    """A NaN would become an ordinary code."""
+    monkeypatch.setattr(kernels, "quant_w4", lambda *a: (torch.zeros(1, dtype=torch.uint8), torch.zeros(1), None))
+    for bad in (float("nan"), float("inf")):
+        lin = torch.nn.Linear(128, 16)
+        with torch.no_grad():
+            lin.weight[3, 5] = bad
+        with pytest.raises(ValueError, match="finite"):
+            W4Linear(lin)
+        net = torch.nn.Sequential(torch.nn.Linear(128, 16), lin)
+        with pytest.raises(ValueError, match="finite"):
+            convert_to_w4(net, min_features=16)
+        assert type(net[0]) is torch.nn.Linear   # nothing is replaced by a conversion that fails
+    W4Linear(torch.nn.Linear(128, 16))
