@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import block
-from test_gpu_block import DEV, DT, _qk, _rand, _within
+from test_gpu_block import DEV, DT, _check_norm, _check_rotary, _norm_inputs, _qk, _rand, _replays, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +75,132 @@ def test_gemm_w4_zeros_past_the_codes(m):
     # what the products and their offset add: codes up to 31 steps, zeros up to 255 + 16
     mag = x.double().abs() @ (scale.double().repeat_interleave(64, 1) * 302).t().contiguous()
     _within(kernels.gemm_w4(x, *kernels.pack_w4(codes, scale, zero.float())), (want, mag + want.abs()), f"{m} rows", k / 16 + 24)
+
+
+# ---------------------------------------------------------------- the forms that a chunk's sizes take
+
+
+# forward, more than 1024 rows: one wave a row with one, two and three pieces of 8 values a thread (up to 512, 1024 and
+# 1536 channels), several waves with two and three, whole units and value by value
+@pytest.mark.parametrize("c,dtype,vec", [(512, "fp16", "fp32"), (768, "bf16", "fp32"), (1536, "bf16", "fp32"),
+                                         (1536, "fp16", "fp16"), (1536, "fp32", "fp32"), (771, "bf16", "bf16"),
+                                         (1531, "fp16", "fp32"), (2048, "bf16", "bf16"), (4096, "fp16", "fp16"),
+                                         (12288, "bf16", "fp32")])
+def test_gated_norm_many_rows(c, dtype, vec):
+    for norm, post, b, n, rows in (("layer", None, 1, 1100, 4), ("rms", "rms", 3, 371, 2), ("layer", "layer", 1, 1037, 5)):
+        a = _norm_inputs(c + n, b, n, c, dtype, vec, norm, post, rows=rows)
+        _check_norm(a, f"{b}x{n}x{c} {dtype}/{vec} {norm}/{post}", norm=norm, post_norm=post)
+
+
+# backward with a norm on both sides and both outputs' gradients: every count of pieces a thread and of waves a row, few
+# rows and a chunk's, of which a workgroup takes more than its least of four (bounds as in test_gpu_block.py: at most 8
+# rows in a thread's turn and 300 workgroups' sums over 32 slices, far under 160 additions)
+@pytest.mark.parametrize("norm,post", [("rms", "rms"), ("layer", "layer"), ("rms", "layer"), ("layer", "rms")])
+@pytest.mark.parametrize("b,n,c,dtype,mod", [(1, 1500, 512, "bf16", "rows"), (1, 1500, 1024, "fp16", "shared"),
+                                             (2, 777, 1536, "bf16", "rows"), (1, 300, 2048, "bf16", "rows"),
+                                             (2, 259, 4096, "fp16", "shared"), (2, 70, 4090, "bf16", "rows"),
+                                             (1, 66, 5120, "fp32", "shared"), (1, 37, 8192, "bf16", "rows"),
+                                             (2, 19, 8200, "fp16", "shared"), (1, 41, 12288, "bf16", "rows"),
+                                             (1, 13, 12285, "fp32", "rows"), (1, 6032, 1536, "bf16", "rows"),
+                                             (1, 1100, 12288, "bf16", "shared"), (1, 4500, 2048, "fp16", "shared")])
+def test_gated_norm_gradients_with_norms_on_both_sides(b, n, c, dtype, mod, norm, post):
+    a = _norm_inputs(n + c, b, n, c, dtype, None, norm, post, mod, 4)
+    g = _rand(c)
+    ds, dh = (torch.randn(b, n, c, device=DEV, generator=g).to(DT[dtype]) for _ in range(2))
+    _check_norm(a, f"{b}x{n}x{c} {dtype} {norm}/{post}/{mod}", ds, dh, norm=norm, post_norm=post)
+
+
+# several tokens a workgroup (2, 4 and 8), the entries of a batch ending inside one, k beside q; units of 16 bytes, of 8
+# and single values
+@pytest.mark.parametrize("pairs", ["interleaved", "half"])
+@pytest.mark.parametrize("b,n,hq,hk,d,rot,dtype", [(3, 1001, 12, 2, 128, 128, "bf16"), (3, 1001, 3, 1, 128, 64, "fp32"),
+                                                   (3, 2749, 4, 4, 128, 64, "fp16"), (5, 3333, 1, 1, 64, 64, "bf16"),
+                                                   (5, 3333, 2, 1, 96, 24, "fp16"), (7, 2347, 1, 0, 7, 6, "bf16"),
+                                                   (3, 1001, 2, 2, 80, 70, "bf16")])
+def test_rotary_several_tokens_a_workgroup(b, n, hq, hk, d, rot, dtype, pairs):
+    from lingbot_world_v2_realtime_amd import Rotary
+    q, k = _qk(n + d, b, n, hq, hk, d, dtype)
+    rope = Rotary.build(rot, DEV, pairs=pairs)
+    pos = torch.randint(0, 5000, (b, n), device=DEV, generator=_rand(2))
+    _check_rotary(q, k, pos, rope, f"{dtype} {pairs} {b}x{n}x{hq}/{hk}x{d}/{rot}")
+    _check_rotary(q.transpose(1, 2), None if k is None else k.transpose(1, 2), 77, rope, "HND, one position", "HND")
+
+
+def test_rotary_three_axes_of_a_chunk():
+    """A chunk's grid at its start frame, two entries of the batch at different ones."""
+    from lingbot_world_v2_realtime_amd import Rotary, grid_positions
+    rope = Rotary.build(128, DEV, sections=(22, 21, 21))
+    q, k = _qk(73, 2, 4 * 29 * 13, 3, 1, 128)
+    pos = torch.stack([grid_positions((4, 29, 13), f, DEV) for f in (0, 1000)])
+    _check_rotary(q, k, pos, rope, "chunk")
+
+
+def test_rotary_needs_a_head():
+    from lingbot_world_v2_realtime_amd import Rotary, rotary_embed
+    rope = Rotary.build(128, DEV)
+    q, k = _qk(74, 1, 5, 4, 2, 128)
+    for bad in ((q[:, :, :0], k), (q, k[:, :, :0])):
+        with pytest.raises(ValueError, match="a head at least"):
+            rotary_embed(*bad, 0, rope)
+    oq, ok = rotary_embed(q[:, :, :0], k[:, :, :0], 0, rope)   # nothing at all is no error
+    assert oq.numel() == ok.numel() == 0
+
+
+# ---------------------------------------------------------------- calls in a graph, in place, from several threads
+
+
+def test_module_and_inplace_rotation_in_a_graph():
+    """A 4-bit linear with an fp32 bias and a rotation in place, captured together and replayed with other inputs; eager calls
+    run between the replays."""
+    from lingbot_world_v2_realtime_amd import Rotary, rotary_embed
+    from lingbot_world_v2_realtime_amd.layers.linear import W4Linear
+    torch.manual_seed(5)
+    mod, rope = W4Linear(torch.nn.Linear(256, 6 * 128).to(DEV), 64, "int4", True), Rotary.build(128, DEV, pairs="half")
+    x = torch.randn(9, 256, device=DEV, generator=_rand(75)).bfloat16()
+    pos = torch.arange(9, device=DEV)
+
+    def make():
+        with torch.no_grad():
+            y = mod(x).view(1, 9, 6, 128)
+            rotary_embed(y[:, :, :4], y[:, :, 4:5], pos, rope, inplace=True)
+        return [y]
+
+    _replays(make, lambda i: (x.add_(0.25), pos.add_(3)))
+
+
+def test_two_threads_on_two_streams():
+    """Two host threads, each with a stream and inputs of its own, forward and backward, fifty calls each: every result is the
+    bits of a call alone."""
+    import threading
+
+    from lingbot_world_v2_realtime_amd import Rotary, gated_norm, rotary_embed
+    rope, results = Rotary.build(128, DEV), {}
+
+    def step(a, pos):
+        s, h = gated_norm(**a)
+        q, _ = rotary_embed(h.view(1, 90, 4, 128), None, pos, rope)
+        return [s.detach(), q.detach(), *torch.autograd.grad((s, q), list(a.values()), (torch.ones_like(s), torch.ones_like(q)))]
+
+    inputs = []
+    for seed in (76, 77):
+        a = {k: v.requires_grad_() for k, v in _norm_inputs(seed, 1, 90, 512, "bf16", "fp32").items()}
+        pos = torch.randint(0, 9999, (90,), device=DEV, generator=_rand(seed))
+        inputs.append((a, pos, [t.clone() for t in step(a, pos)]))
+    torch.cuda.synchronize()
+
+    def work(i):
+        a, pos, want = inputs[i]
+        stream, same = torch.cuda.Stream(), True
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got = step(a, pos)
+                same = same and all(torch.equal(x, y) for x, y in zip(got, want))
+            stream.synchronize()
+        results[i] = same
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert results == {0: True, 1: True}
