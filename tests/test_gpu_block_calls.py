@@ -204,3 +204,27 @@ def test_two_threads_on_two_streams():
     for t in threads:
         t.join(60)
     assert results == {0: True, 1: True}
+
+
+@pytest.mark.parametrize("m", [1, 40, 1030])
+@pytest.mark.parametrize("fmt,zeros", [("int4", False), ("int4", True), ("fp4", False)])
+def test_gemm_w4_small_and_large_rows(m, fmt, zeros):
+    """Rows below the format's normal numbers, rows near fp16's largest, and rows of one sign, whose codes' offset is far larger
+    than what remains of it."""
+    from lingbot_world_v2_realtime_amd import kernels
+    n, k = 2320, 256
+    for dtype, size, std in (("fp16", 2.0 ** -20, 200.0), ("bf16", 2.0 ** -130, 1.0), ("fp16", 3e4, 2.0 ** -12),
+                             ("bf16", 2.0 ** 100, 1.0), ("bf16", 1.0, 1.0)):
+        g = _rand(78)
+        codes = torch.randint(0, 16, (n, k), device=DEV, generator=g, dtype=torch.uint8)
+        scale = ((torch.rand(n, 4, device=DEV, generator=g) + 0.1) * std).bfloat16()
+        zero = torch.randint(0, 16, (n, 4), device=DEV, generator=g, dtype=torch.uint8) if zeros else None
+        x = (torch.rand(m, k, device=DEV, generator=g, dtype=torch.float64) * 0.9 + 0.1) * size
+        if size != 1.0:
+            x = x * (1 - 2 * torch.randint(0, 2, (m, k), device=DEV, generator=g))
+        x = x.to(DT[dtype])
+        want = x.double() @ block.w4_values(codes, scale, zero, fmt).t().contiguous()
+        steps = 62 if fmt == "int4" else 6
+        mag = x.double().abs() @ (scale.double().repeat_interleave(64, 1) * steps).t().contiguous()
+        _within(kernels.gemm_w4(x, *kernels.pack_w4(codes, scale, zero, fmt), fmt=fmt), (want, mag + want.abs()),
+                f"{m} rows of {dtype} around {size}", k / 16 + 24)
