@@ -77,8 +77,8 @@ int64_t lbw_gated_norm_bwd_workspace_bytes(int64_t batch, int64_t len, int64_t w
  * [batch][len][k_heads][dim] (`dtype`; strides *_s_batch, *_s_tok, *_s_head; channels contiguous) are rotated,
  *   (a, b) -> factor * (a cos w - b sin w, b cos w + a sin w),   w = position[axis of the pair] * freq[pair],
  * the others copied. interleaved: pair i is channels (2 i, 2 i + 1), else (i, pairs + i). inverse: w negated (the
- * gradient's rotation). The angle is formed in 64 bits and reduced to a turn before the sine and cosine are taken in
- * fp32, so far positions keep theirs; one rounding to `dtype`. freq: float64 [pairs], radians a position. axis: int32
+ * gradient's rotation). The angle is formed in 64 bits and reduced to a turn there, so far positions keep theirs; sine
+ * and cosine are fp32 (rounded once from 64 bits for fp32 tensors); one rounding to `dtype`. freq: float64 [pairs], radians a position. axis: int32
  * [pairs] with values in 0 .. axes - 1, or null (all 0); a pair of another axis comes out as NaN. positions: int64
  * (pos_is_i64) or int32 with strides p_s_batch, p_s_tok, p_s_axis, or null: token t of every entry is at pos_start + t
  * on every axis. q_out, k_out as q, k (strides qo_*, ko_*); a call in place passes the same pointer and strides twice,

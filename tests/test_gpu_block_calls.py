@@ -228,3 +228,23 @@ def test_gemm_w4_small_and_large_rows(m, fmt, zeros):
         mag = x.double().abs() @ (scale.double().repeat_interleave(64, 1) * steps).t().contiguous()
         _within(kernels.gemm_w4(x, *kernels.pack_w4(codes, scale, zero, fmt), fmt=fmt), (want, mag + want.abs()),
                 f"{m} rows of {dtype} around {size}", k / 16 + 24)
+
+
+@pytest.mark.parametrize("pairs", ["interleaved", "half"])
+def test_rotary_fp32_sine_and_cosine_are_rounded_once(pairs):
+    """fp32 q: each factor is off by its one rounding and each product by another, so 2 * 2^-24 of what is added, beside the
+    sum's own (positions up to 5000: the 64-bit angle is good to 2e-12). On the whole no further off than the same products
+    by torch, with sine and cosine taken in 64 bits and rounded: those round as often, or once more."""
+    from lingbot_world_v2_realtime_amd import Rotary, rotary_embed
+    q, _ = _qk(79, 1, 5000, 4, 0, 128, "fp32")
+    rope, pos = Rotary.build(128, DEV, pairs=pairs), torch.arange(5000, device=DEV)
+    want = block.rotary(q, pos, rope.freq, pairs=pairs)
+    got = rotary_embed(q, None, pos, rope)[0]
+    _within(got, want, pairs, 2.001)
+    angle = pos.double()[:, None] * rope.freq
+    cos, sin = angle.cos().float()[None, :, None], angle.sin().float()[None, :, None]
+    a, b = (q[..., 0::2], q[..., 1::2]) if pairs == "interleaved" else (q[..., :64], q[..., 64:])
+    parts = (a * cos - b * sin, b * cos + a * sin)
+    plain = torch.stack(parts, -1).flatten(-2) if pairs == "interleaved" else torch.cat(parts, -1)
+    rms = [(t.double() - want[0]).square().mean().sqrt().item() for t in (got, plain)]
+    assert rms[0] <= rms[1], rms
