@@ -62,9 +62,9 @@ int lbw_gated_norm_bwd(const void* ds, const void* dh, const void* x, const void
                        const void* gate, int64_t gate_s_batch, int64_t gate_s_group,
                        const void* scale, int64_t scale_s_batch, int64_t scale_s_group, int rowwise,
                        int64_t groups, int64_t group_len, const void* weight, const void* bias,
-                       const void* post_weight, int norm, int post_norm, float eps, float residual_scale, float branch_scale, void* dx, void* dy, void* dgate,
-                       void* dshift, void* dscale, void* dweight, void* dbias, void* dpost_weight, void* workspace,
-                       void* stream);
+                       const void* post_weight, int norm, int post_norm, float eps, float residual_scale,
+                       float branch_scale, void* dx, void* dy, void* dgate, void* dshift, void* dscale, void* dweight,
+                       void* dbias, void* dpost_weight, void* workspace, void* stream);
 
 /* Bytes of scratch lbw_gated_norm_bwd needs for its sums over rows. */
 int64_t lbw_gated_norm_bwd_workspace_bytes(int64_t batch, int64_t len, int64_t width, int64_t groups,
@@ -77,13 +77,13 @@ int64_t lbw_gated_norm_bwd_workspace_bytes(int64_t batch, int64_t len, int64_t w
  * [batch][len][k_heads][dim] (`dtype`; strides *_s_batch, *_s_tok, *_s_head; channels contiguous) are rotated,
  *   (a, b) -> factor * (a cos w - b sin w, b cos w + a sin w),   w = position[axis of the pair] * freq[pair],
  * the others copied. interleaved: pair i is channels (2 i, 2 i + 1), else (i, pairs + i). inverse: w negated (the
- * gradient's rotation). The angle is formed in 64 bits and reduced to a turn there, so far positions keep theirs; sine
- * and cosine are fp32 (rounded once from 64 bits for fp32 tensors); one rounding to `dtype`. freq: float64 [pairs], radians a position. axis: int32
+ * gradient's rotation). The angle is formed in 64 bits and reduced to a turn before the sine and cosine are taken in
+ * fp32, so far positions keep theirs; one rounding to `dtype`. freq: float64 [pairs], radians a position. axis: int32
  * [pairs] with values in 0 .. axes - 1, or null (all 0); a pair of another axis comes out as NaN. positions: int64
  * (pos_is_i64) or int32 with strides p_s_batch, p_s_tok, p_s_axis, or null: token t of every entry is at pos_start + t
  * on every axis. q_out, k_out as q, k (strides qo_*, ko_*); a call in place passes the same pointer and strides twice,
- * any other overlap is an error of the caller. k may be null with k_heads 0. dim even is not required; 2 * pairs <= dim <= LBW_ROTARY_MAX_DIM,
- * batch * len <= 2^30, 4096 heads at most.
+ * any other overlap is an error of the caller. k may be null with k_heads 0. dim even is not required; 2 * pairs <= dim
+ * <= LBW_ROTARY_MAX_DIM, batch * len <= 2^30, 4096 heads at most.
  */
 int lbw_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t len, int64_t q_heads, int64_t k_heads,
                int64_t dim, int64_t pairs, int64_t q_s_batch, int64_t q_s_tok, int64_t q_s_head, int64_t k_s_batch,
@@ -123,7 +123,7 @@ int lbw_quant_w4(const void* w, int w_is_fp32, int64_t n, int64_t k, int64_t s_r
  * as above, bias [n] of `dtype` (of fp32 where dtype has LBW_W4_BIAS_FP32 added) or null, out [m][n] packed of `dtype`.
  * Codes enter the products exactly; sums and group scales are fp32, the bias is added in fp32, with one rounding at the
  * end. m <= 2^24, n <= 1048560, k <= 2^20. With LBW_W4_INT4 a row of x that holds an infinity gives NaN (the codes'
- * offset is taken off the sums).
+ * offset is taken off the sums), and one of bf16 values of 2^115 and more may (the offset's part leaves fp32's range).
  */
 int lbw_gemm_w4(const void* x, int dtype, int64_t m, int64_t k, int64_t x_s_row, const uint8_t* w4,
                 const uint16_t* scale, const uint8_t* zero, int fmt, int64_t group, int64_t n, const void* bias,

@@ -2,11 +2,11 @@
 //
 // A workgroup takes a few tokens. Their angles are formed once for all heads: position * frequency in 64 bits,
 // reduced to (-1/2, 1/2] turns there (far positions lose nothing: an angle of 1e6 radians is still good to 1e-10),
-// then sine and cosine, into LDS: for 16-bit values in fp32 of the reduced angle rounded to fp32 (off by a few 2^-24,
-// which their own rounding hides), for fp32 values in 64 bits, rounded once (error of standard normal values 3.7e-8 rms,
-// 5.6e-8 with the fp32 functions; on a bf16 chunk 64 bits cost 13.7 us against 13.4). The heads' values then pass through
-// registers, 16 bytes a load: with neighbouring pairs a load holds whole pairs; with halves a thread takes the 16 bytes
-// of both partners. 6032 tokens of 24 heads of 128 in bf16 take 13.4 us (5.5 TB/s; a copy of 1 GiB reaches 5.1), 24 of
+// then sine and cosine in fp32 of the reduced angle rounded to fp32, into LDS. 16-bit values do not see that rounding;
+// for fp32 values both are moved by what it took off (standard normal values: 4.1e-8 rms off, 5.4e-8 without; sine and
+// cosine in 64 bits 3.7e-8, but 64 tokens of 14 heads 3.27 us against 3.07). The heads' values then pass through
+// registers, 16 bytes a load: with neighbouring pairs a load holds whole pairs; with halves a thread takes the 16
+// bytes of both partners. 6032 tokens of 24 heads of 128 in bf16 take 13.4 us (5.5 TB/s; a copy of 1 GiB reaches 5.1), 24 of
 // their 96 channels turned 11.6 with 8-byte units (53 value by value).
 #include "lbw_rows.h"
 
@@ -99,17 +99,26 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
   for (int i = threadIdx.x; i < ntok * a.pairs; i += THREADS) {
     const int j = i / a.pairs, p = i - j * a.pairs;
     const uint32_t tok = (uint32_t)(tok0 + j), b = tok / (uint32_t)a.len, t = tok - b * (uint32_t)a.len;
-    // an axis that the positions do not have: nothing is read there, and the pair becomes NaN
-    const int64_t want = a.axis ? a.axis[p] : 0, ax = max((int64_t)0, min(want, a.axes - 1));
-    const bool missing = a.pos && ax != want;
+    int64_t ax = 0;
+    double freq = a.freq[p];
+    if (a.axis) {   // an axis that the positions do not have: they are read inside, and the pair becomes NaN
+      const int want = a.axis[p];
+      ax = max((int64_t)0, min((int64_t)want, a.axes - 1));
+      if (a.pos && ax != want) freq = __longlong_as_double(0x7FF8000000000000ll);
+    }
     const int64_t at = b * a.p_s_batch + t * a.p_s_tok + ax * a.p_s_axis;
     const int64_t pos = !a.pos ? a.pos_start + t : a.pos_is_i64 ? ((const int64_t*)a.pos)[at] : ((const int32_t*)a.pos)[at];
-    const double turns = (double)pos * a.freq[p] * 0.15915494309189533577;   // 1 / (2 pi)
-    std::conditional_t<DT == LBW_DTYPE_FP32, double, float> s, c;
-    if constexpr (DT == LBW_DTYPE_FP32) sincospi(2.0 * (turns - rint(turns)), &s, &c);
-    else sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    if (missing) s = c = __int_as_float(0x7FC00000);
-    cs[i] = make_float2((float)(a.factor * c), (float)(a.sign * a.factor * s));
+    const double turns = (double)pos * freq * 0.15915494309189533577;   // 1 / (2 pi)
+    const double half = 2.0 * (turns - rint(turns));
+    const float near = (float)half;
+    float s, c;
+    sincospif(near, &s, &c);
+    if constexpr (DT == LBW_DTYPE_FP32) {
+      const float rest = (float)(half - near) * 3.14159265358979f, s0 = s;
+      s = fmaf(c, rest, s);
+      c = fmaf(-s0, rest, c);
+    }
+    cs[i] = make_float2(a.factor * c, a.sign * a.factor * s);
   }
   __syncthreads();
   const int pair_items = a.pairs / N, rest = a.copy ? (a.dim - 2 * a.pairs) / N : 0;   // (units of the rest)
