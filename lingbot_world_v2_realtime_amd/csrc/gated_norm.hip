@@ -435,8 +435,8 @@ int slices_for(int64_t rows) {   // (two at least: whole waves)
 }
 
 // The workgroups' sums of one modulation row (workgroup / tiles), SUM_COLS channels a workgroup, its half-waves
-// taking them in turn, four in flight (6032 x 1536 in 4 rows, 503 workgroups' sums: 6.1 us; with eight in flight 6.9,
-// with 64 channels and one at a time 8.0, with 16 channels 10.6): the row's own gradients, and its sums left where
+// taking them in turn, four in flight (6032 x 1536 in 4 rows, 252 workgroups' sums each: 6.1 us; with eight in flight
+// 6.9, with 64 channels 6.4, with 16 channels 10.6): the row's own gradients, and its sums left where
 // its first workgroup's were for the kernel below (which a single modulation row does not need: `last`).
 template <int VDT>
 __global__ __launch_bounds__(SUM_COLS * SLICES) void norm_group_sums_kernel(NormArgs a, GradArgs o, VecGrads d, int tiles,

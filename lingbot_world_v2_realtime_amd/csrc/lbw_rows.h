@@ -7,8 +7,9 @@
 
 namespace lbw {
 
-// Workgroups in any number up to 2^36: a grid dimension holds fewer than 2^32 threads, so past 2^20 workgroups there
-// is a second one, whose last part may have workgroups past the end.
+// Workgroups in any number below 2^32, which group_id() counts in 32 bits (the entry points take 2^30 at most): a grid
+// dimension holds fewer than 2^32 threads, so past 2^20 workgroups there is a second one, whose last part may have
+// workgroups past the end.
 constexpr unsigned GRID_X = 1u << 20;
 inline dim3 grid_of(int64_t n) {
   return dim3((unsigned)(n < GRID_X ? n : GRID_X), (unsigned)((n + GRID_X - 1) / GRID_X));

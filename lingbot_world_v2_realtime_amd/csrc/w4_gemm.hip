@@ -28,7 +28,8 @@ __device__ __forceinline__ void dpp_max_min(float& hi, float& lo) {
   lo = fminf(lo, dpp<DPP>(lo));
 }
 
-// A workgroup makes one tile: 16 lanes a row, each 8 columns in a row; a group's extremes by DPP within its lanes.
+// A workgroup makes one tile: 16 lanes a row, each 8 columns in a row; a group's extremes by DPP within its lanes. Runs
+// once, at load, and reads value by value: 8960 x 1536 from bf16 in 18.6 us (1.9 TB/s), fp4 22.4, from fp32 27.
 template <bool F32>
 __global__ __launch_bounds__(256) void quant_w4_kernel(const void* w, int64_t n, int64_t k, int64_t s_row, int fmt,
                                                        int group, uint8_t* w4, uint16_t* scale, uint8_t* zero) {
@@ -384,15 +385,17 @@ __global__ __launch_bounds__(64 * MOST) void w4_rows_kernel(GemmArgs a) {
   }
 }
 
-// Many rows: 64 rows x 256 columns a workgroup, four waves of 64 x 64, two workgroups a CU (which drift apart, so
-// that one's matrix work runs under the other's conversions: 57.5 us for 1508 x 8960 x 1536 against 62.7 with eight
-// waves in step on 128 rows, both before the last steps; now 51.3, 810 TFLOP/s, and 1000 where K is 6144 and the grid
-// fills whole rounds). x passes through LDS, a K tile at a time in two buffers (rows and pieces as above): wave w
+// Many rows: 64 rows x 256 columns a workgroup, four waves of 64 x 64, two workgroups a CU, which drift apart, so
+// that one's matrix work runs under the other's conversions (eight such waves in step on 128 rows took 62.7 us where
+// this took 57.5, before the steps that made it 51). With a bias, groups of 128, bf16, int4 / int4 with zeros / fp4:
+//   1508 x 8960 x 1536    51.1 us (813 TFLOP/s) / 56.6 (733) / 47.2 (879); 64 columns a group with zeros 66.9
+//   2048 x 8192 x 6144   195.2   (1056)         / 216.0 (954) / 184.2 (1119); the grid fills whole rounds
+// x passes through LDS, a K tile at a time in two buffers (rows and pieces as above): wave w
 // loads rows 16 w .. 16 w + 15 in the operands' own order, forms their sums over each group while they are in
 // registers, and leaves both there. Codes go from memory to registers, a tile ahead. The output leaves through LDS,
-// so that a store holds whole rows of 128 bytes (1508 x 8960 x 1536, zeros and bias: 68.1 -> 64.9 us; with no store
-// at all 61.2). The conversions bound it: vector instructions take about 1.3 times the matrix core's cycles, and two
-// waves a SIMD overlap the two in part.
+// so that a store holds whole rows of 128 bytes (1508 x 8960 x 1536, zeros and bias, at that step: 68.1 -> 64.9 us;
+// with no store at all 61.2). The conversions bound it: each wave makes its columns' operands for its own 64 rows, and
+// vector instructions take about 1.3 times the matrix core's cycles, which two waves a SIMD overlap in part.
 constexpr int GM = 64, GN = 256;
 constexpr int X_TILE = GM * TK * 2;   // bytes
 
