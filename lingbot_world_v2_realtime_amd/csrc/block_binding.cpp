@@ -66,6 +66,8 @@ const Tensor& tensor(const char* name, PyObject* o, bool optional = false) {
   if (!THPVariable_Check(o)) type_error(name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
   const Tensor& t = THPVariable_Unpack(o);
   if (t.is_neg()) value_error(name, " is a lazily negated view: give its resolve_neg()");
+  // (an address of zero means that the tensor is absent)
+  if (t.numel() && !t.const_data_ptr()) type_error(name, " has no memory of its own, got ", Py_TYPE(o)->tp_name);
   return t;
 }
 

@@ -6,6 +6,7 @@ from torch.autograd import forward_ad
 
 from lingbot_world_v2_realtime_amd import _lib, kernels
 from lingbot_world_v2_realtime_amd.layers.linear import W4Linear, convert_to_w4
+from lingbot_world_v2_realtime_amd.layers.norm import gated_norm
 from lingbot_world_v2_realtime_amd.layers.rotary import Rotary, rotary_embed
 from oracle import block
 
@@ -259,3 +260,40 @@ def test_w4_linear_refuses_weights_that_are_not_finite(monkeypatch):
             convert_to_w4(net, min_features=16)
         assert type(net[0]) is torch.nn.Linear   # nothing is replaced by a conversion that fails
     W4Linear(torch.nn.Linear(128, 16))
+
+
+class _StandIn(torch.Tensor):
+    """A tensor that stands for another and has no memory of its own, as distributed tensors do."""
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device, strides=t.stride())
+
+    def __init__(self, t):
+        pass
+
+    @classmethod
+    def __torch_dispatch__(cls, *a, **kw):
+        raise AssertionError("the operators look at tensors only")
+
+
+def test_tensors_without_memory_are_refused():
+    """An address of zero means 'absent' to the kernels: a weight, a branch or positions held by such a tensor would be left
+    out of the result."""
+    x = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    v, freq = x[0, 0].clone(), torch.ones(8, dtype=torch.float64)
+    args = dict(x=x, y=x.clone(), gate=v, shift=v, scale=v, weight=v, bias=v, post_weight=v, post_norm="rms")
+    for name in ("x", "y", "gate", "shift", "scale", "weight", "bias", "post_weight"):
+        with pytest.raises(TypeError, match=f"^{name} has no memory"):
+            gated_norm(**{**args, name: _StandIn(args[name])})
+    q, axis = x.view(1, 4, 1, 128), torch.zeros(8, dtype=torch.int32)
+    rotary = dict(q=q, k=q.clone(), positions=torch.zeros(4, 1, dtype=torch.int64), freq=freq, axis=axis)
+    for name in rotary:
+        with pytest.raises(TypeError, match=f"^{name} has no memory"):
+            kernels.rotary(**{**rotary, name: _StandIn(rotary[name])})
+    gemm = dict(x=x[0], w4=torch.zeros(1, 1, 1024, dtype=torch.uint8), scale=torch.zeros(1, 1, 16, 1, dtype=torch.bfloat16),
+                zero=torch.zeros(1, 1, 16, 1, dtype=torch.uint8), bias=torch.zeros(16, dtype=torch.bfloat16))
+    for name in gemm:
+        with pytest.raises(TypeError, match=f"^{name} has no memory"):
+            kernels.gemm_w4(**{**gemm, name: _StandIn(gemm[name])})
+    with pytest.raises(ValueError, match="device tensor"):   # nothing to hold needs no memory
+        gated_norm(torch.zeros(1, 0, 128))
