@@ -168,14 +168,16 @@ bool records_gradient(const Tensor& t, const T&... rest) {
   return records_gradient(t) || records_gradient(rest...);
 }
 
-// For the calls that have no gradient of their own: a tensor among the arguments that would record one is refused (the
-// result would be detached).
-void no_gradient(const char* what, PyObject* const* args, Py_ssize_t n) {
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    if (!THPVariable_Check(args[i]) || !records_gradient(THPVariable_Unpack(args[i]))) continue;
-    PyErr_Format(PyExc_RuntimeError, "%s records no gradient: call it under torch.no_grad(), or on detached tensors", what);
-    throw python_error();
-  }
+// For the calls that have no gradient of their own: a tensor that would record one is refused (the result would be
+// detached).
+void no_gradient(const char* what, bool recorded) {
+  if (!recorded) return;
+  PyErr_Format(PyExc_RuntimeError, "%s records no gradient: call it under torch.no_grad(), or on detached tensors", what);
+  throw python_error();
+}
+void no_gradient(const char* what, PyObject* const* args, Py_ssize_t n) {   // (before anything else looks at them)
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (args[i] != Py_None && THPVariable_Check(args[i])) no_gradient(what, records_gradient(THPVariable_Unpack(args[i])));
 }
 
 Tensor new_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }   // (packed, whatever t's strides)
@@ -699,7 +701,6 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   count(n_args, 8);
-  no_gradient("gemm_w4", args, n_args);
   const Tensor& x = tensor("x", args[0]);
   const auto dt = x.scalar_type();
   if (dt != at::kBFloat16 && dt != at::kHalf) type_error("x must be bfloat16 or float16, got ", dt);
@@ -707,6 +708,7 @@ PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     value_error("x must be [M, K] with contiguous rows, got ", dims(x.sizes()), " / ", dims(x.strides()));
   Tensor w4 = tensor("w4", args[1]), scale = tensor("scale", args[2]), zero = tensor("zero", args[3], true);
   const Tensor& bias = tensor("bias", args[4], true);
+  no_gradient("gemm_w4", records_gradient(x, scale, bias));
   const std::string fmt = word("fmt", args[6]);
   if ((fmt != "int4" && fmt != "fp4") || (zero.defined() && fmt != "int4"))
     value_error("fmt must be 'int4' or 'fp4' (zeros: 'int4' only), got '", fmt, "'");
