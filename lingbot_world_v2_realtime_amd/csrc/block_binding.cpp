@@ -135,7 +135,13 @@ void same_device(const char* what, const Tensor& first, const T&... rest) {
   (check(rest), ...);
 }
 
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// (a gradient that a hook replaced by a tensor without memory must not count as absent either)
+void* ptr(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  void* p = t.data_ptr();
+  TORCH_CHECK(p || !t.numel(), "a tensor without memory of its own");
+  return p;
+}
 
 // The device of a call made current, and its current stream.
 struct On {

@@ -248,3 +248,102 @@ def test_rotary_fp32_values_keep_the_angle(pairs):
     plain = torch.stack(parts, -1).flatten(-2) if pairs == "interleaved" else torch.cat(parts, -1)
     rms = [(t.double() - want[0]).square().mean().sqrt().item() for t in (got, plain)]
     assert rms[0] <= rms[1], rms
+
+
+# ---------------------------------------------------------------- gradients by halves
+
+
+@pytest.mark.parametrize("shapes", [("rows", "shared", "none"), ("shared", "rows", "rows"), ("none", "rows", "shared"),
+                                    ("rows", "none", "rows"), ("shared", "shared", "rows")])
+def test_gated_norm_modulations_of_different_shapes(shapes):
+    """gate, shift and scale each with rows of its own, shared or absent."""
+    b, n, c, rows = 2, 61, 520, 4
+    a = _norm_inputs(80, b, n, c, "bf16", "fp32", "layer", "rms", "rows", rows)
+    for name, shape in zip(("gate", "shift", "scale"), shapes):
+        if shape == "shared":
+            a[name] = a[name][0, 1].clone()
+        elif shape == "none":
+            del a[name]
+    g = _rand(81)
+    ds, dh = (torch.randn(b, n, c, device=DEV, generator=g).bfloat16() for _ in range(2))
+    kw = dict(post_norm="rms", group_len=17)
+    _check_norm(a, f"{shapes}", ds, dh, **kw)
+
+
+@pytest.mark.parametrize("branch", [False, True])
+def test_gated_norm_each_gradient_alone(branch):
+    """Only one input records a gradient, whichever others are there: the bits it has among all."""
+    from lingbot_world_v2_realtime_amd import gated_norm
+    a = _norm_inputs(82, 2, 37, 520, "fp16", "fp32", rows=3)
+    if not branch:
+        a = {k: v for k, v in a.items() if k not in ("y", "gate", "post_weight")}
+    g = _rand(83)
+    d = [torch.randn(2, 37, 520, device=DEV, generator=g).half() for _ in range(2 if branch else 1)]
+
+    def grads(names):
+        leaf = {k: v.detach().requires_grad_(k in names) for k, v in a.items()}
+        out = gated_norm(**leaf)
+        return dict(zip(names, torch.autograd.grad(out, [leaf[k] for k in names], d)))
+
+    every = grads(list(a))
+    for name in a:
+        assert torch.equal(grads([name])[name], every[name]), name
+
+
+def test_gradients_of_a_batch_of_gradients_are_refused():
+    from lingbot_world_v2_realtime_amd import Rotary, gated_norm, rotary_embed
+    x = torch.randn(1, 4, 64, device=DEV, requires_grad=True)
+    rope = Rotary.build(64, DEV)
+    for f in (lambda t: gated_norm(t), lambda t: rotary_embed(t.view(1, 4, 1, 64), None, 0, rope)[0]):
+        y = f(x)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, x, torch.randn(3, *y.shape, device=DEV), is_grads_batched=True)
+
+
+def test_gradients_by_saved_tensor_hooks_and_checkpoints():
+    """Saved tensors moved to the host and back, and a forward run again by a checkpoint: the same bits."""
+    from torch.utils.checkpoint import checkpoint
+
+    from lingbot_world_v2_realtime_amd import Rotary, gated_norm, rotary_embed
+    a = {k: v.requires_grad_() for k, v in _norm_inputs(84, 1, 30, 512, "bf16", "fp32").items()}
+    rope, pos = Rotary.build(128, DEV), torch.arange(30, device=DEV)
+
+    def step(*ts):
+        s, h = gated_norm(**dict(zip(a, ts)))
+        return s, rotary_embed(h.view(1, 30, 4, 128), None, pos, rope)[0]
+
+    def grads(out):
+        return torch.autograd.grad(out, list(a.values()), [torch.ones_like(o) for o in out])
+
+    want = grads(step(*a.values()))
+    with torch.autograd.graph.save_on_cpu():
+        got = step(*a.values())
+    assert all(torch.equal(x, y) for x, y in zip(grads(got), want))
+    assert all(torch.equal(x, y) for x, y in zip(grads(checkpoint(step, *a.values(), use_reentrant=False)), want))
+
+
+def test_operators_in_a_compiled_function():
+    """Inside torch.compile the calls are made as they are, between the compiled pieces."""
+    from lingbot_world_v2_realtime_amd import Rotary, gated_norm, rotary_embed
+    rope = Rotary.build(64, DEV)
+    x = torch.randn(1, 6, 64, device=DEV, requires_grad=True)
+
+    def f(t):
+        h = gated_norm(t * 2, norm="rms") + 1
+        return rotary_embed(h.view(1, 6, 1, 64), None, 3, rope)[0] * 0.5
+
+    want = f(x)
+    got = torch.compile(f, backend="eager")(x)
+    assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(got.sum(), x)[0], torch.autograd.grad(want.sum(), x)[0])
+
+
+def test_a_gradient_without_memory_is_refused():
+    """A hook that puts a stand-in for another tensor in a gradient's place: it must not count as no gradient."""
+    from lingbot_world_v2_realtime_amd import gated_norm
+    from test_block_calls import _StandIn
+    x = torch.randn(1, 4, 64, device=DEV, requires_grad=True)
+    s, h = gated_norm(x, x.detach())
+    s.register_hook(_StandIn)
+    with pytest.raises(RuntimeError, match="without memory"):
+        torch.autograd.grad((s, h), x, (torch.ones_like(s), torch.ones_like(h)))
