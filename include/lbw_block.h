@@ -109,8 +109,8 @@ int lbw_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t l
  *
  * lbw_quant_w4 makes them from w [n][k] (bf16, or fp32 when w_is_fp32; row stride s_row): scale = amax / 6 (fp4),
  * amax / 7 (int4 without zeros) or (max(x, 0) - min(x, 0)) / 15 (with zeros), rounded to bf16, codes to the nearest
- * value of the rounded scale (ties to even codes for integers, to the smaller magnitude for fp4). Values are finite;
- * a group that holds none but zeros gets scale 0.
+ * value of the rounded scale by arithmetic in fp32 (integers: w * (1 / scale) + zero, ties to even codes; fp4: w / scale,
+ * ties to the smaller magnitude). Values are finite; a group that holds none but zeros gets scale 0.
  */
 int lbw_quant_w4(const void* w, int w_is_fp32, int64_t n, int64_t k, int64_t s_row, int fmt, int64_t group,
                  uint8_t* w4, uint16_t* scale, uint8_t* zero, void* stream);
