@@ -544,6 +544,22 @@ class Overlap {
       if (most > 0) terms[n++] = {t.stride(i) * size, second ? -most : 0, first ? most : 0};
     }
   }
+  // dimensions of one step as one: views of one projection share theirs, and each place of the one would be tried
+  // with the nearest of the other (a chunk's tokens would spend the budget)
+  void merge() {
+    int m = 0;
+    for (int i = 0; i < n; ++i) {
+      int j = 0;
+      while (j < m && terms[j].step != terms[i].step) ++j;
+      if (j < m) {
+        terms[j].lo += terms[i].lo;
+        terms[j].hi += terms[i].hi;
+      } else {
+        terms[m++] = terms[i];
+      }
+    }
+    n = m;
+  }
   void sort(int64_t size) {
     std::sort(terms, terms + n, [](const Term& a, const Term& b) { return a.step > b.step; });
     terms[n++] = {1, 1 - size, size - 1};
@@ -572,6 +588,7 @@ class Overlap {
     Overlap o;
     o.add(a, true, false);
     o.add(b, false, true);
+    o.merge();
     o.sort(a.element_size());
     return o.reach(0, (const char*)b.data_ptr() - (const char*)a.data_ptr());
   }

@@ -297,3 +297,33 @@ def test_tensors_without_memory_are_refused():
             kernels.gemm_w4(**{**gemm, name: _StandIn(gemm[name])})
     with pytest.raises(ValueError, match="device tensor"):   # nothing to hold needs no memory
         gated_norm(torch.zeros(1, 0, 128))
+
+
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_rotary_views_of_a_whole_projection_are_told_apart(layout):
+    """q and k of a chunk's fused projection, in place: thousands of tokens whose addresses interleave, and no element of
+    both; and the same with one head of both."""
+    fused = torch.zeros(2, 6032, 36, 128, dtype=torch.bfloat16)
+    if layout == "HND":
+        fused = fused.transpose(1, 2)
+    axis, rope = (2 if layout == "NHD" else 1), Rotary(torch.ones(64, dtype=torch.float64))
+    view = lambda start, heads: fused.narrow(axis, start, heads)   # noqa: E731
+
+    def inplace(q, k):
+        return _answer(lambda: rotary_embed(q, k, 0, rope, layout, inplace=True))
+
+    assert inplace(view(0, 12), view(12, 12)) == "ok"
+    assert inplace(view(0, 12), view(24, 2)) == "ok"
+    assert "share" in inplace(view(0, 12), view(11, 2))
+    halves = fused.unflatten(axis, (18, 2)).movedim(axis + 1, 0)   # heads in turn
+    assert inplace(halves[0], halves[1]) == "ok"
+
+
+def test_rotary_token_steps_without_a_common_factor():
+    flat = torch.zeros(4000000, dtype=torch.bfloat16)
+    a = flat.as_strided((1, 6032, 1, 128), (0, 300, 0, 1))
+    rope = Rotary(torch.ones(64, dtype=torch.float64))
+    for start, shares in ((150, True), (300 * 6031 + 128, False)):
+        b = flat.as_strided((1, 3000, 1, 128), (0, 701, 0, 1), start)
+        said = _answer(lambda: rotary_embed(a[:, :3000], b, 0, rope, inplace=True))
+        assert ("share" in said) == shares
