@@ -7,9 +7,12 @@ Python call surface (lingbot/layers/attention.py).
 """
 from . import _lib  # noqa: F401
 from .layers.attention import attention, flash_attention, sage_attention  # noqa: F401
-from .layers import kv_quant, linear, norm, prologue, rotary  # noqa: F401
+from .layers import kv4, kv_quant, linear, norm, packed, prologue, rotary  # noqa: F401
 from .layers.norm import gated_norm  # noqa: F401
-from .layers.rotary import Rotary, grid_positions, rotary_embed  # noqa: F401
+from .layers.kv4 import KV4Cache  # noqa: F401
+from .layers.packed import packed_attention  # noqa: F401
+from .layers.rotary import Rotary, grid_positions, norm_rotary_embed, rotary_embed  # noqa: F401
 
 __all__ = ["attention", "flash_attention", "sage_attention", "gated_norm", "Rotary", "grid_positions", "rotary_embed",
-           "kv_quant", "linear", "norm", "prologue", "rotary"]
+           "norm_rotary_embed", "packed_attention", "KV4Cache", "kv4", "kv_quant", "linear", "norm", "packed", "prologue",
+           "rotary"]

@@ -1,5 +1,5 @@
-"""ctypes binding of liblbw_attn.so (the C-ABI declared in include/lbw_attn.h, include/lbw_gemm.h and
-include/lbw_block.h)."""
+"""ctypes binding of liblbw_attn.so (the C-ABI declared in include/lbw_attn.h, include/lbw_gemm.h,
+include/lbw_block.h and include/lbw_causal.h)."""
 import ctypes
 import os
 
@@ -61,8 +61,27 @@ BLOCK_SIGNATURES = {
 }
 
 
-# the block operators' own sources: translation units (and headers) that no kernel of the attention path includes
-_BLOCK_SOURCES = ("gated_norm.hip", "lbw_rows.h", "rotary.hip", "w4_gemm.hip")
+# causal self-attention's entry points; mirrors include/lbw_causal.h
+CAUSAL_SIGNATURES = {
+    "lbw_norm_rotary": (_i32, [_p, _p, _i32, _i32] + [_i64] * 12 + [_p, _p, _f32, _p, _i32] + [_i64] * 4 +
+                        [_p, _p, _i64, _i32, _f32, _p, _p] + [_i64] * 6 + [_p]),
+    "lbw_norm_rotary_bwd": (_i32, [_p] * 4 + [_i32, _i32] + [_i64] * 18 + [_p, _p, _f32, _p, _i32] + [_i64] * 4 +
+                            [_p, _p, _i64, _i32, _f32, _p, _p] + [_i64] * 6 + [_p] * 4),
+    "lbw_norm_rotary_bwd_workspace_bytes": (_i64, [_i64]),
+    "lbw_packed_attn_fwd": (_i32, [_p] * 3 + [_i32] + [_i64] * 12 + [_p, _p, _i32, _f32] + [_p] * 4),
+    "lbw_packed_attn_bwd": (_i32, [_p] * 7 + [_i32] + [_i64] * 14 + [_p, _p, _i32, _f32] + [_p] * 5),
+    "lbw_packed_attn_bwd_workspace_bytes": (_i64, [_i64] * 4),
+    "lbw_kv4_write": (_i32, [_p, _p, _i32] + [_i64] * 8 + [_p] * 3 + [_i64] * 3 + [_p] * 5),
+    "lbw_kv4_read": (_i32, [_i64] * 4 + [_p] * 3 + [_i64] * 3 + [_p] * 7),
+    "lbw_kv4_attn": (_i32, [_p, _i32] + [_i64] * 7 + [_p] * 3 + [_i64] * 3 + [_p] * 4 + [_f32, _p, _p, _p]),
+    "lbw_kv4_attn_workspace_bytes": (_i64, [_i64] * 6 + [_i32]),
+}
+
+
+# the block operators' and causal attention's own sources: translation units (and headers) that no kernel of the attention
+# path includes
+_BLOCK_SOURCES = ("gated_norm.hip", "lbw_rows.h", "lbw_turn.h", "rotary.hip", "w4_gemm.hip", "norm_rotary.hip", "lbw_spans.h",
+                  "lbw_packed.h", "packed_attn.hip", "packed_attn_bwd.hip", "kv4.hip", "binding.h")
 
 
 def sources_sha16():
@@ -98,7 +117,7 @@ def load(path=LIB_PATH):
         raise ImportError(f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
                           "or `python lingbot_world_v2_realtime_amd/build.py`")
     lib = ctypes.CDLL(path)
-    for name, (res, args) in (*SIGNATURES.items(), *GEMM_SIGNATURES.items(), *BLOCK_SIGNATURES.items()):
+    for name, (res, args) in (*SIGNATURES.items(), *GEMM_SIGNATURES.items(), *BLOCK_SIGNATURES.items(), *CAUSAL_SIGNATURES.items()):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

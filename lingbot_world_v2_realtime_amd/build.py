@@ -9,7 +9,9 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "liblbw_attn.so")
 BLOCK = os.path.join(HERE, "_block.so")
 SOURCES = ["lbw_abi.hip", "kv_requant.hip", "quant_q.hip", "prologue.hip", "cross_attn.hip", "fp8_quant.hip", "fp8_gemm.hip",
-           "gated_norm.hip", "rotary.hip", "w4_gemm.hip", "attn_fwd.hip"]
+           "gated_norm.hip", "rotary.hip", "w4_gemm.hip", "norm_rotary.hip", "packed_attn.hip", "packed_attn_bwd.hip", "kv4.hip",
+           "attn_fwd.hip"]
+BINDING = ["block_binding.cpp", "causal_binding.cpp"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
@@ -40,7 +42,7 @@ def build_library(verbose=False):
 
 
 def build_binding(verbose=False):
-    """Compile csrc/block_binding.cpp against this Python and torch (always recompiles; liblbw_attn.so has to be built).
+    """Compile the bindings (csrc/*_binding.cpp) against this Python and torch (always recompiles; liblbw_attn.so has to be built).
     Returns the module's path."""
     import sysconfig
     from torch.utils import cpp_extension
@@ -51,7 +53,7 @@ def build_binding(verbose=False):
     for d in (os.path.join(ROOT, "include"), sysconfig.get_paths()["include"], *cpp_extension.include_paths(),
               os.path.join(rocm, "include")):
         cmd += ["-isystem" if d != os.path.join(ROOT, "include") else "-I", d]
-    cmd += [os.path.join(HERE, "csrc", "block_binding.cpp"), "-o", tmp, "-L", HERE, "-llbw_attn"]
+    cmd += [os.path.join(HERE, "csrc", s) for s in BINDING] + ["-o", tmp, "-L", HERE, "-llbw_attn"]
     for d in cpp_extension.library_paths():
         cmd += ["-L", d]
     cmd += ["-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]

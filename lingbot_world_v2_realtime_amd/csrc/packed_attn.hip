@@ -1,0 +1,193 @@
+// Attention over packed sequences, forward (include/lbw_causal.h): S = q k^T, softmax, times v, a tile of keys after
+// another with the running maximum and sum.
+//
+// A workgroup takes 128 queries of a head and sequence, 32 a wave, and walks the keys 64 at a time (two stages in LDS).
+// S^T = K Q^T on v_mfma_f32_32x32x16: a lane holds one query and 32 of the 64 keys, so the row's maximum and sum are
+// register work and one exchange between the wave's halves; P^T goes in the type of v from those registers into
+// O^T += V^T P^T, whose V^T comes from the rows of v by transposing LDS reads.
+#include "lbw_packed.h"
+
+namespace lbw {
+namespace packed {
+namespace {
+
+constexpr int QW = 32, WAVES = 4, QT = QW * WAVES, KT = 64, THREADS = 64 * WAVES;
+
+struct FwdArgs {
+  Shape s;
+  const uint16_t *q, *k, *v;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  uint16_t *out, *rest;
+  float* lse;
+  uint32_t tiles;
+};
+
+template <int DH, bool F16>
+__global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
+  constexpr int NS = DH / 16, MT = DH / 32, TILE = KT * row_bytes<DH>, STAGE = 2 * TILE;
+  constexpr int LDS = 2 * STAGE > WAVES * STAGING<DH> ? 2 * STAGE : WAVES * STAGING<DH>;
+  __shared__ __align__(16) uint8_t lds[LDS];
+  const int lane = threadIdx.x & 63, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t head, tile;
+  head_tile(group_id(), a.s.q_heads, head, tile);
+  if (tile >= a.tiles) return;
+  const int64_t o_tok = (int64_t)a.s.q_heads * DH;
+  zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.out + head * DH, o_tok, DH, tile, a.tiles);
+  const Place at = place(a.s.starts, a.s.seqs, a.s.q_rows, QT, tile);
+  if (at.seq < 0) return;
+  const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
+  const int n = qs.n, m = ks.n, shift = m - n;
+  const int q0 = (at.tiles - 1 - at.tile) * QT;   // the tiles with the most keys first
+  const int row0 = q0 + QW * w, row = row0 + (lane & 31);
+  // keys that the tile's last query sees, and the wave's last and first
+  const auto seen = [&](int r) { return a.s.causal ? max(0, min(m, min(r, n - 1) + shift + 1)) : m; };
+  const int upto = seen(q0 + QT - 1), w_upto = row0 < n ? seen(row0 + QW - 1) : 0, w_first = seen(row0), own = seen(row);
+  const int tiles = (upto + KT - 1) / KT;
+
+  const uint16_t* kb = a.k + ks.first * a.k_tok + (head / a.s.group) * a.k_head;
+  const uint16_t* vb = a.v + ks.first * a.v_tok + (head / a.s.group) * a.v_head;
+  Loader<DH, KT, WAVES> kl, vl;
+  kl.init(w, lane, a.k_tok);
+  vl.init(w, lane, a.v_tok);
+  const auto issue = [&](int t, int stage) {
+    const int64_t r = (int64_t)t * KT;
+    kl.issue(rows_buffer<DH>(kb + r * a.k_tok, a.k_tok, m - t * KT, KT), w, lds + stage * STAGE);
+    vl.issue(rows_buffer<DH>(vb + r * a.v_tok, a.v_tok, m - t * KT, KT), w, lds + stage * STAGE + TILE);
+  };
+  if (tiles > 0) issue(0, 0);
+  v4i qf[NS];
+  load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, lane, qf);
+  RowReads<DH> kr;
+  TurnedReads<DH> vr;
+  kr.init(lane);
+  vr.init(lane);
+
+  v16f o[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) o[mt] = zeros16();
+  float top = -INFINITY, total = 0.f;
+
+  const auto step = [&](int t, auto stage) {
+    const uint8_t* kt = lds + decltype(stage)::value * STAGE;
+    const uint8_t* vt = kt + TILE;
+    wait_dma();
+    __syncthreads();   // the tile is in LDS, and every wave is done with the other stage
+    if (t + 1 < tiles) issue(t + 1, 1 - decltype(stage)::value);
+    if (t * KT >= w_upto) return;
+    v16f s[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      s[x] = zeros16();
+#pragma unroll
+      for (int st = 0; st < NS; ++st) s[x] = mfma<F16>(kr.get(kt, x, st), qf[st], s[x]);
+    }
+    if ((t + 1) * KT > w_first) {   // keys that a query does not see
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (t * KT + 32 * x + 8 * (i >> 2) + 4 * hf + (i & 3) >= own) s[x][i] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
+    mx = max_xor32(mx) * a.s.sl2;
+    const float next = fmaxf(top, mx);
+    if (__any(next > top)) {
+      // a row that has seen nothing yet has sums of zero, whatever they are multiplied by
+      const float by = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[mt][i] *= by;
+      total *= by;
+      top = next;
+    }
+    const float off = (top == -INFINITY ? 0.f : -top) + LIFT<F16>;
+    v4i pf[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + j], a.s.sl2, off));
+      sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      pf[u] = v4i{(int)pack<F16>(p[0], p[1]), (int)pack<F16>(p[2], p[3]), (int)pack<F16>(p[4], p[5]), (int)pack<F16>(p[6], p[7])};
+    }
+    total += sum;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt] = mfma<F16>(vr.get(vt, u, mt), pf[u], o[mt]);
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    step(t, ic<0>{});
+    if (t + 1 < tiles) step(t + 1, ic<1>{});
+  }
+  total = sum_xor32(total);
+  __syncthreads();   // every wave is done with the stages
+  if (row0 >= n) return;
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  store_turned<DH, F16>(o, inv, lds + w * STAGING<DH>, lane, a.out + (qs.first + row0) * o_tok + head * DH, o_tok, n - row0);
+  if (a.rest) {
+    __builtin_amdgcn_wave_barrier();
+    store_turned<DH, F16, true>(o, inv, lds + w * STAGING<DH>, lane, a.rest + (qs.first + row0) * o_tok + head * DH, o_tok, n - row0);
+  }
+  if (a.lse && row < n && lane < 32)
+    a.lse[(int64_t)head * a.s.q_rows + qs.first + row] = own > 0 ? top + __builtin_amdgcn_logf(total) - LIFT<F16> : INFINITY;
+}
+
+template <int DH, bool F16>
+void launch(const FwdArgs& a, hipStream_t stream) {
+  packed_fwd_kernel<DH, F16><<<grid_of((int64_t)a.tiles * a.s.q_heads), THREADS, 0, stream>>>(a);
+}
+
+}  // namespace
+}  // namespace packed
+}  // namespace lbw
+
+using namespace lbw;
+
+namespace lbw {
+namespace packed {
+
+int check(int dtype, int64_t seqs, int64_t q_rows, int64_t k_rows, int64_t q_heads, int64_t k_heads, int64_t dim, float sm_scale) {
+  if ((dtype != LBW_DTYPE_BF16 && dtype != LBW_DTYPE_FP16) || seqs < 1 || seqs > 65535 || q_rows < 1 || q_rows >= 1ll << 31 ||
+      k_rows < 0 || k_rows >= 1ll << 31 || q_heads < 1 || q_heads > 4096 || k_heads < 1 || q_heads % k_heads ||
+      (dim != 64 && dim != 128) || !(sm_scale > 0.f) || !(sm_scale < INFINITY))
+    return LBW_E_SHAPE;
+  return LBW_OK;
+}
+// (the kernels tell rows past a sequence's end by their offsets: those of different tokens lie apart)
+bool aligned(const void* p, int64_t tok, int64_t head, int64_t dim) {
+  return (uintptr_t)p % 16 == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= dim && tok < 1 << 24 && head >= 0;
+}
+
+}  // namespace packed
+}  // namespace lbw
+
+extern "C" int lbw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, int64_t seqs, int64_t q_rows,
+                                   int64_t k_rows, int64_t q_heads, int64_t k_heads, int64_t dim, int64_t q_s_tok,
+                                   int64_t q_s_head, int64_t k_s_tok, int64_t k_s_head, int64_t v_s_tok, int64_t v_s_head,
+                                   const int32_t* starts, const int32_t* k_starts, int causal, float sm_scale, void* out,
+                                   void* rest, float* lse, void* stream) {
+  if (!q || (k_rows && (!k || !v)) || !starts || !k_starts || !out) return LBW_E_NULL;
+  if (const int st = packed::check(dtype, seqs, q_rows, k_rows, q_heads, k_heads, dim, sm_scale)) return st;
+  if (!packed::aligned(q, q_s_tok, q_s_head, dim) || !packed::aligned(k, k_s_tok, k_s_head, dim) || !packed::aligned(v, v_s_tok, v_s_head, dim) ||
+      ((uintptr_t)out | (uintptr_t)rest) % 16 || (uintptr_t)starts % 4 || (uintptr_t)k_starts % 4 || (uintptr_t)lse % 4)
+    return LBW_E_ALIGN;
+  const int64_t tiles = places_of(q_rows, seqs, packed::QT);
+  if (tiles * q_heads > 1 << 30) return LBW_E_SHAPE;
+  if (const int st = check_device()) return st;
+  packed::FwdArgs a = {{seqs, q_rows, k_rows, (int)q_heads, (int)k_heads, (int)(q_heads / k_heads), starts, k_starts, causal,
+                        sm_scale, sm_scale * packed::LOG2E},
+                       (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_s_tok, q_s_head, k_s_tok, k_s_head,
+                       v_s_tok, v_s_head, (uint16_t*)out, (uint16_t*)rest, lse, (uint32_t)tiles};
+  const bool f16 = dtype == LBW_DTYPE_FP16;
+  if (dim == 128) f16 ? packed::launch<128, true>(a, (hipStream_t)stream) : packed::launch<128, false>(a, (hipStream_t)stream);
+  else f16 ? packed::launch<64, true>(a, (hipStream_t)stream) : packed::launch<64, false>(a, (hipStream_t)stream);
+  return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
+}

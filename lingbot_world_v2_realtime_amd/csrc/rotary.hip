@@ -8,7 +8,7 @@
 // registers, 16 bytes a load: with neighbouring pairs a load holds whole pairs; with halves a thread takes the 16
 // bytes of both partners. 6032 tokens of 24 heads of 128 in bf16 take 13.4 us (5.5 TB/s; a copy of 1 GiB reaches 5.1), 24 of
 // their 96 channels turned 11.6 with 8-byte units (53 value by value).
-#include "lbw_rows.h"
+#include "lbw_turn.h"
 
 namespace lbw {
 namespace {
@@ -35,44 +35,6 @@ struct RotaryArgs {
   int64_t axes;
   float factor, sign;             // sign -1: the inverse rotation
   int copy;                       // whether the channels past the pairs have to be written (not in place)
-};
-
-// N consecutive values: 16 bytes, 8, or one value
-template <int DT, int N>
-struct Unit {
-  static constexpr int WORDS = N * elem_size(DT) / 4;
-  float f[N];
-  __device__ __forceinline__ void load(const void* p, int64_t i) {
-    if constexpr (N == 1) {
-      f[0] = load1<DT>(p, i);
-    } else {
-      typedef int vec __attribute__((ext_vector_type(WORDS)));
-      const vec w = *(const vec*)((const char*)p + i * elem_size(DT));
-#pragma unroll
-      for (int e = 0; e < WORDS; ++e) {
-        if constexpr (DT == LBW_DTYPE_FP32) {
-          f[e] = __int_as_float(w[e]);
-        } else {
-          f[2 * e] = lo16<DT == LBW_DTYPE_FP16>((uint32_t)w[e]);
-          f[2 * e + 1] = hi16<DT == LBW_DTYPE_FP16>((uint32_t)w[e]);
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ void store(void* p, int64_t i) const {
-    if constexpr (N == 1) {
-      store1<DT>(p, i, f[0]);
-    } else {
-      typedef int vec __attribute__((ext_vector_type(WORDS)));
-      vec w;
-#pragma unroll
-      for (int e = 0; e < WORDS; ++e) {
-        if constexpr (DT == LBW_DTYPE_FP32) w[e] = __float_as_int(f[e]);
-        else w[e] = (int)pack2<DT>(f[2 * e], f[2 * e + 1]);
-      }
-      *(vec*)((char*)p + i * elem_size(DT)) = w;
-    }
-  }
 };
 
 // N: values of a unit (16 bytes of the format, 8, or one value, as strides, sizes and addresses allow). An item is
@@ -108,16 +70,8 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
     }
     const int64_t at = b * a.p_s_batch + t * a.p_s_tok + ax * a.p_s_axis;
     const int64_t pos = !a.pos ? a.pos_start + t : a.pos_is_i64 ? ((const int64_t*)a.pos)[at] : ((const int32_t*)a.pos)[at];
-    const double turns = (double)pos * freq * 0.15915494309189533577;   // 1 / (2 pi)
-    const double half = 2.0 * (turns - rint(turns));
-    const float near = (float)half;
     float s, c;
-    sincospif(near, &s, &c);
-    if constexpr (DT == LBW_DTYPE_FP32) {
-      const float rest = (float)(half - near) * 3.14159265358979f, s0 = s;
-      s = fmaf(c, rest, s);
-      c = fmaf(-s0, rest, c);
-    }
+    turn_of<DT>(pos, freq, s, c);
     cs[i] = make_float2(a.factor * c, a.sign * a.factor * s);
   }
   __syncthreads();

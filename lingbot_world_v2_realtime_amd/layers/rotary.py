@@ -13,7 +13,7 @@ import torch
 
 from .. import kernels
 
-__all__ = ["Rotary", "rotary_embed", "grid_positions"]
+__all__ = ["Rotary", "rotary_embed", "norm_rotary_embed", "grid_positions"]
 
 
 @dataclass
@@ -87,3 +87,12 @@ def rotary_embed(q, k, positions, rope, tensor_layout="NHD", inplace=False):
     share memory). Returns (q, k); differentiable in both."""
     return kernels.block_binding().rotary_embed(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor,
                                                 tensor_layout, rope.axes, inplace)
+
+
+def norm_rotary_embed(q, k, positions, rope, q_weight=None, k_weight=None, eps=1e-6, tensor_layout="NHD"):
+    """The RMS norm of every head of q and k (x / sqrt(mean(x^2) + eps), times q_weight / k_weight [D]) and then the rotation
+    of rotary_embed, in one pass over them: arguments and layouts as there. Weights have q's type or fp32, both the same,
+    and may be left out. fp32 from the load to the one rounding. Returns new (q, k), packed; differentiable in q, k and both
+    weights."""
+    return kernels.block_binding().norm_rotary_embed(q, k, positions, rope.freq, rope.axis, rope.pairs, rope.factor,
+                                                     tensor_layout, rope.axes, q_weight, k_weight, eps)
