@@ -18,7 +18,7 @@ extern "C" {
 /*
  * Every head of q [batch][len][q_heads][dim] and k [batch][len][k_heads][dim] (`dtype`; strides *_s_batch, *_s_tok,
  * *_s_head; channels contiguous) divided by the root of its mean square (plus eps), multiplied by q_weight / k_weight
- * ([dim] of vec_dtype, `dtype` or fp32, or null: 1), and its first 2 * pairs channels turned as lbw_rotary turns them.
+ * ([dim] of vec_dtype, `dtype` or fp32, 16-byte aligned, or null: 1), and its first 2 * pairs channels turned as lbw_rotary turns them.
  * fp32 from the load to the one rounding. Outputs with strides qo_*, ko_*, apart from the inputs. k may be null with
  * k_heads 0. Limits of lbw_rotary.
  */
@@ -32,7 +32,7 @@ int lbw_norm_rotary(const void* q, const void* k, int dtype, int vec_dtype, int6
 
 /*
  * Gradients of lbw_norm_rotary from those of its outputs, dq and dk (strides dq_*, dk_*; either null: zero): dq_in and
- * dk_in of `dtype` (strides qo_*, ko_*), dq_weight and dk_weight [dim] of vec_dtype; any of the four may be null. The sums
+ * dk_in of `dtype` (strides qo_*, ko_*), dq_weight and dk_weight [dim] of vec_dtype (16-byte aligned); any of the four may be null. The sums
  * over tokens and heads are fp32 in a fixed order. `workspace`: lbw_norm_rotary_bwd_workspace_bytes(dim) bytes, 16-byte
  * aligned, used where a weight's gradient is asked for; calls that share it must not overlap.
  */

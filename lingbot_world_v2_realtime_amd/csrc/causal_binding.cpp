@@ -44,9 +44,10 @@ struct NormRotary : Rotary {
     const std::array<Tensor, 2> out = {new_like(q), k.defined() ? new_like(k) : Tensor()};
     if (empty()) return out;
     const On on(q);
+    const auto w = weights();
     done(lbw_norm_rotary(q.data_ptr(), ptr(k), element_format("q", q), vec_dtype, q.size(0), q.size(tok()), q.size(head()),
                          k.defined() ? k.size(head()) : 0, q.size(3), freq.size(0), st(q, 0), st(q, tok()), st(q, head()), st(k, 0),
-                         st(k, tok()), st(k, head()), ptr(weight[0]), ptr(weight[1]), eps, ptr(pos),
+                         st(k, tok()), st(k, head()), ptr(w[0]), ptr(w[1]), eps, ptr(pos),
                          pos.defined() && pos.scalar_type() == at::kLong, own() == 2 ? pos.stride(0) : 0, own() ? pos.stride(own() - 1) : 0,
                          own() && axis.defined() ? pos.stride(own()) : 0, o->start, (const double*)freq.data_ptr(),
                          (const int32_t*)ptr(axis), own() && axis.defined() ? pos.size(own()) : 1, o->interleaved, (float)o->factor,
@@ -54,6 +55,13 @@ struct NormRotary : Rotary {
                          st(out[1], tok()), st(out[1], head()), on.stream),
          "lbw_norm_rotary");
     return out;
+  }
+  // weights at an address that the kernels do not load from (views of a larger buffer) as copies
+  std::array<Tensor, 2> weights() const {
+    std::array<Tensor, 2> w = {weight[0], weight[1]};
+    for (Tensor& t : w)
+      if (t.defined() && (uintptr_t)t.const_data_ptr() % 16) t = t.clone();
+    return w;
   }
   // The gradients of q, k and the weights, those that are wanted, from the outputs' (either may be undefined).
   std::array<Tensor, 4> backward(const Tensor& dq, const Tensor& dk, const std::array<bool, 4>& wants) const {
@@ -64,6 +72,7 @@ struct NormRotary : Rotary {
       if (wants[i] && of[i]->defined()) g[i] = none ? at::zeros(of[i]->sizes(), of[i]->options()) : new_like(*of[i]);
     if (none) return g;
     const On on(q);
+    const auto w = weights();
     Tensor ws;
     if (g[2].defined() || g[3].defined())
       ws = at::empty({lbw_norm_rotary_bwd_workspace_bytes(q.size(3))}, q.options().dtype(at::kByte));
@@ -71,7 +80,7 @@ struct NormRotary : Rotary {
     done(lbw_norm_rotary_bwd(ptr(dq), ptr(dk), q.data_ptr(), ptr(k), element_format("q", q), vec_dtype, q.size(0), q.size(tok()),
                              q.size(head()), k.defined() ? k.size(head()) : 0, q.size(3), freq.size(0), st(dq, 0), st(dq, tok()),
                              st(dq, head()), st(dk, 0), st(dk, tok()), st(dk, head()), st(q, 0), st(q, tok()), st(q, head()), st(k, 0),
-                             st(k, tok()), st(k, head()), ptr(weight[0]), ptr(weight[1]), eps, ptr(pos),
+                             st(k, tok()), st(k, head()), ptr(w[0]), ptr(w[1]), eps, ptr(pos),
                              pos.defined() && pos.scalar_type() == at::kLong, own() == 2 ? pos.stride(0) : 0,
                              own() ? pos.stride(own() - 1) : 0, own() && axis.defined() ? pos.stride(own()) : 0, o->start,
                              (const double*)freq.data_ptr(), (const int32_t*)ptr(axis), own() && axis.defined() ? pos.size(own()) : 1,

@@ -2,21 +2,38 @@
 // position's angle.
 #pragma once
 
+#include <type_traits>
+
 #include "lbw_rows.h"
 
 namespace lbw {
 
-// N consecutive values: 16 bytes, 8, or one value
+// N consecutive values: 16 bytes, 8, or one value; as they lie in memory, too, for loads that run ahead
 template <int DT, int N>
 struct Unit {
   static constexpr int WORDS = N * elem_size(DT) / 4;
+  struct One {
+    float v;
+    __device__ __forceinline__ One() {}
+    __device__ __forceinline__ One(int x) : v((float)x) {}
+  };
+  typedef int vec __attribute__((ext_vector_type(WORDS > 0 ? WORDS : 1)));
+  typedef std::conditional_t<N == 1, One, vec> Raw;
   float f[N];
-  __device__ __forceinline__ void load(const void* p, int64_t i) {
+  static __device__ __forceinline__ Raw raw(const void* p, int64_t i) {
     if constexpr (N == 1) {
-      f[0] = load1<DT>(p, i);
+      One r;
+      r.v = load1<DT>(p, i);
+      return r;
     } else {
-      typedef int vec __attribute__((ext_vector_type(WORDS)));
-      const vec w = *(const vec*)((const char*)p + i * elem_size(DT));
+      return *(const vec*)((const char*)p + i * elem_size(DT));
+    }
+  }
+  __device__ __forceinline__ void load(const void* p, int64_t i) { set(raw(p, i)); }
+  __device__ __forceinline__ void set(const Raw w) {
+    if constexpr (N == 1) {
+      f[0] = w.v;
+    } else {
 #pragma unroll
       for (int e = 0; e < WORDS; ++e) {
         if constexpr (DT == LBW_DTYPE_FP32) {
@@ -32,7 +49,6 @@ struct Unit {
     if constexpr (N == 1) {
       store1<DT>(p, i, f[0]);
     } else {
-      typedef int vec __attribute__((ext_vector_type(WORDS)));
       vec w;
 #pragma unroll
       for (int e = 0; e < WORDS; ++e) {

@@ -8,6 +8,8 @@
 //   dx = r (g - u mean(g u)),   dw = sum over rows of d u,
 // where mean(g u) = r mean(g x) needs no second pass. A lane adds up its channels' weight gradients over its rows, a
 // workgroup its teams, and a second kernel the workgroups, in one order.
+#include <type_traits>
+
 #include "lbw_causal.h"
 #include "lbw_turn.h"
 
@@ -17,7 +19,10 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int MAX_TOKENS = 8;   // of a step of a workgroup
 constexpr int MAX_PAIRS = LBW_ROTARY_MAX_DIM / 2;
-constexpr int MAX_GROUPS = 1024;   // workgroups of a backward pass
+constexpr int MAX_GROUPS = 512;   // workgroups of a backward pass
+
+template <int N>
+using ic = std::integral_constant<int, N>;
 
 struct Rows {
   const void *in, *grad;          // grad: of the outputs (backward), or null
@@ -57,6 +62,26 @@ __device__ __forceinline__ float team_sum(float x, int team) {
   return x;
 }
 
+// N weights from channel c on, in a load of their own type or of fp32.
+template <int DT, int N>
+__device__ __forceinline__ void load_weights(const void* v, int fp32, int c, float* w) {
+  if (fp32) {
+    constexpr int M = N < 4 ? N : 4;
+#pragma unroll
+    for (int i = 0; i < N; i += M) {
+      Unit<LBW_DTYPE_FP32, M> u;
+      u.load(v, c + i);
+#pragma unroll
+      for (int e = 0; e < M; ++e) w[i + e] = u.f[e];
+    }
+  } else {
+    Unit<DT, N> u;
+    u.load(v, c);
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = u.f[e];
+  }
+}
+
 // N: values of a unit; U: items of a lane (4 where 64 lanes of one do not hold a row: single values of wide heads)
 template <int DT, int N, bool INTER, int U, bool BWD>
 __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormRotaryArgs a) {
@@ -64,26 +89,18 @@ __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormRotaryArgs a) 
   __shared__ int64_t at_tok[MAX_TOKENS][6];   // where a token's rows start: q, k, their gradients, the outputs
   const int team = a.team, it0 = threadIdx.x & (team - 1), mine = threadIdx.x / team, teams = THREADS / team;
   const int pair_items = a.pairs / N, rest = (a.dim - 2 * a.pairs) / N, items = pair_items + (rest + 1) / 2;
-  const uint32_t heads = (uint32_t)(a.q.heads + a.k.heads);
 
-  // a lane's channels: where its two units lie, and their weights for q and k
-  int c0[U], c1[U];   // -1: nothing there
-  float w[2][U][2 * N], sums[BWD ? 2 : 1][U][2 * N];
+  int c0[U], c1[U];   // where a lane's two units lie in a head; -1: nothing there
+  float sums[BWD ? 2 : 1][U][2 * N];
 #pragma unroll
   for (int n = 0; n < U; ++n) {
     const int it = it0 + n * team, p = it * N, r0 = 2 * a.pairs + 2 * (it - pair_items) * N;
     const bool turned = it < pair_items;
     c0[n] = it < items ? (turned ? (INTER ? 2 * p : p) : r0) : -1;
     c1[n] = turned ? (INTER ? 2 * p + N : a.pairs + p) : it < items && r0 + N < a.dim ? r0 + N : -1;
+    if constexpr (BWD) {
 #pragma unroll
-    for (int e = 0; e < 2 * N; ++e) {
-      const int c = e < N ? c0[n] : c1[n], at = c + e % N;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const void* v = x ? a.k.weight : a.q.weight;
-        w[x][n][e] = c < 0 || !v ? 1.f : a.vec_fp32 ? ((const float*)v)[at] : load1<DT>(v, at);
-        if constexpr (BWD) sums[x][n][e] = 0.f;
-      }
+      for (int e = 0; e < 2 * N; ++e) sums[0][n][e] = sums[1][n][e] = 0.f;
     }
   }
 
@@ -101,6 +118,40 @@ __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormRotaryArgs a) 
       at_tok[threadIdx.x][4] = b * a.q.o_batch + t * a.q.o_tok;
       at_tok[threadIdx.x][5] = b * a.k.o_batch + t * a.k.o_tok;
     }
+    __syncthreads();
+    // The rows of q, then those of k: a team's next row, loaded while the one before it is worked on (the first ones while the
+    // angles are formed).
+    typedef typename Unit<DT, N>::Raw Raw;
+    struct Ahead {
+      Raw x[U][2], d[BWD ? U : 1][2];
+      char* out;
+      uint32_t j;
+    };
+    const auto fetch = [&](auto which, uint32_t row) {
+      constexpr int X = decltype(which)::value;
+      const Rows& t = X ? a.k : a.q;
+      const uint32_t heads = (uint32_t)t.heads;
+      const bool live = row < ntok * heads;   // (lanes without a row take part in the exchanges)
+      Ahead r;
+      r.j = live ? row / heads : 0;
+      const uint32_t h = live ? row - r.j * heads : 0;
+      const char* in = (const char*)t.in + (at_tok[r.j][X] + h * t.s_head) * elem_size(DT);
+      const char* grad = BWD && t.grad ? (const char*)t.grad + (at_tok[r.j][2 + X] + h * t.g_head) * elem_size(DT) : nullptr;
+      r.out = t.out && live ? (char*)t.out + (at_tok[r.j][4 + X] + h * t.o_head) * elem_size(DT) : nullptr;
+#pragma unroll
+      for (int n = 0; n < U; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int c = k ? c1[n] : c0[n];
+          const bool there = live && c >= 0;
+          r.x[n][k] = there ? Unit<DT, N>::raw(in, c) : Raw(0);
+          if constexpr (BWD) r.d[n][k] = there && grad ? Unit<DT, N>::raw(grad, c) : Raw(0);
+        }
+      return r;
+    };
+    Ahead first[2];
+    first[0] = fetch(ic<0>{}, mine);
+    if (a.k.heads) first[1] = fetch(ic<1>{}, mine);
     for (int i = threadIdx.x; i < ntok * a.pairs; i += THREADS) {
       const int j = i / a.pairs, p = i - j * a.pairs;
       const uint32_t tok = (uint32_t)(tok0 + j), b = tok / (uint32_t)a.len, t = tok - b * (uint32_t)a.len;
@@ -118,93 +169,87 @@ __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormRotaryArgs a) 
       cs[i] = make_float2(a.factor * c, (BWD ? -a.factor : a.factor) * s);   // (the gradient's turn is the opposite one)
     }
     __syncthreads();
-    const uint32_t total = ntok * heads;
-    for (uint32_t row0 = 0; row0 < total; row0 += teams) {
-      const uint32_t row = row0 + mine;
-      const bool live = row < total;   // (lanes without a row take part in the exchanges)
-      const uint32_t j = live ? row / heads : 0, h = live ? row - j * heads : 0;
-      const bool is_q = h < (uint32_t)a.q.heads;
-      const Rows& t = is_q ? a.q : a.k;
-      const int64_t hh = is_q ? h : h - a.q.heads;
-      const char* in = (const char*)t.in + (at_tok[j][is_q ? 0 : 1] + hh * t.s_head) * elem_size(DT);
-      const char* grad = BWD && t.grad ? (const char*)t.grad + (at_tok[j][is_q ? 2 : 3] + hh * t.g_head) * elem_size(DT) : nullptr;
-      char* out = t.out ? (char*)t.out + (at_tok[j][is_q ? 4 : 5] + hh * t.o_head) * elem_size(DT) : nullptr;
-      Unit<DT, N> x[U][2], d[BWD ? U : 1][2];
-      float squares = 0.f, dots = 0.f;
+    const auto section = [&](auto which) {
+      constexpr int X = decltype(which)::value;
+      const Rows& t = X ? a.k : a.q;
+      float w[U][2 * N];
 #pragma unroll
       for (int n = 0; n < U; ++n)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int c = k ? c1[n] : c0[n];
-          if (live && c >= 0) {
-            x[n][k].load(in, c);
-            if constexpr (BWD) {
-              if (grad) d[n][k].load(grad, c);
-            }
-          }
-          if (!(live && c >= 0)) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[n][k].f[e] = 0.f;
-          }
-          if constexpr (BWD) {
-            if (!(live && c >= 0 && grad)) {
-#pragma unroll
-              for (int e = 0; e < N; ++e) d[n][k].f[e] = 0.f;
-            }
-          }
+          for (int e = 0; e < N; ++e) w[n][k * N + e] = 1.f;
+          if (c >= 0 && t.weight) load_weights<DT, N>(t.weight, a.vec_fp32, c, w[n] + k * N);
         }
-      // pair e of an item: in a row the values 2 e, 2 e + 1 of both units, else value e of each
-      const auto turn = [&](Unit<DT, N> (&u)[2], int n) {
-        if (c0[n] < 0 || it0 + n * team >= pair_items) return;
-        const float2* at = cs + j * a.pairs + (it0 + n * team) * N;
+      const uint32_t total = ntok * (uint32_t)t.heads;
+      Ahead next = first[X];
+      for (uint32_t row0 = 0; row0 < total; row0 += teams) {
+        const Ahead now = next;
+        const bool live = row0 + mine < total;
+        if (row0 + teams < total) next = fetch(which, row0 + teams + mine);
+        Unit<DT, N> x[U][2], d[BWD ? U : 1][2];
+        float squares = 0.f, dots = 0.f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          float& f0 = INTER && N > 1 ? (2 * e < N ? u[0].f[2 * e % N] : u[1].f[2 * e % N]) : u[0].f[e];
-          float& f1 = INTER && N > 1 ? (2 * e < N ? u[0].f[(2 * e + 1) % N] : u[1].f[(2 * e + 1) % N]) : u[1].f[e];
-          const float x0 = f0, x1 = f1;
-          const float2 v = at[e];
-          f0 = x0 * v.x - x1 * v.y;
-          f1 = x1 * v.x + x0 * v.y;
-        }
-      };
+        for (int n = 0; n < U; ++n)
 #pragma unroll
-      for (int n = 0; n < U; ++n) {
-        if constexpr (BWD) turn(d[n], n);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
+          for (int k = 0; k < 2; ++k) {
+            x[n][k].set(now.x[n][k]);
+            if constexpr (BWD) d[n][k].set(now.d[n][k]);
+          }
+        // pair e of an item: in a row the values 2 e, 2 e + 1 of both units, else value e of each
+        const auto turn = [&](Unit<DT, N> (&u)[2], int n) {
+          if (c0[n] < 0 || it0 + n * team >= pair_items) return;
+          const float2* at = cs + now.j * a.pairs + (it0 + n * team) * N;
 #pragma unroll
           for (int e = 0; e < N; ++e) {
-            const float v = x[n][k].f[e];
-            squares = fmaf(v, v, squares);
-            if constexpr (BWD) dots = fmaf(d[n][k].f[e] * (is_q ? w[0][n][k * N + e] : w[1][n][k * N + e]), v, dots);
+            float& f0 = INTER && N > 1 ? (2 * e < N ? u[0].f[2 * e % N] : u[1].f[2 * e % N]) : u[0].f[e];
+            float& f1 = INTER && N > 1 ? (2 * e < N ? u[0].f[(2 * e + 1) % N] : u[1].f[(2 * e + 1) % N]) : u[1].f[e];
+            const float x0 = f0, x1 = f1;
+            const float2 v = at[e];
+            f0 = x0 * v.x - x1 * v.y;
+            f1 = x1 * v.x + x0 * v.y;
           }
-      }
-      const float r = rsqrtf(team_sum(squares, team) / (float)a.dim + a.eps);
-      if constexpr (BWD) dots = team_sum(dots, team) / (float)a.dim * r * r;
+        };
 #pragma unroll
-      for (int n = 0; n < U; ++n) {
+        for (int n = 0; n < U; ++n) {
+          if constexpr (BWD) turn(d[n], n);
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            float& f = x[n][k].f[e];
-            const float wt = is_q ? w[0][n][k * N + e] : w[1][n][k * N + e];
-            if constexpr (!BWD) {
-              f = f * r * wt;
-            } else {
-              const float dv = d[n][k].f[e], du = live ? dv * (f * r) : 0.f;
-              sums[0][n][k * N + e] += is_q ? du : 0.f;
-              sums[1][n][k * N + e] += is_q ? 0.f : du;
-              f = r * (dv * wt - f * dots);
+            for (int e = 0; e < N; ++e) {
+              const float v = x[n][k].f[e];
+              squares = fmaf(v, v, squares);
+              if constexpr (BWD) dots = fmaf(d[n][k].f[e] * w[n][k * N + e], v, dots);
             }
+        }
+        const float r = rsqrtf(team_sum(squares, team) / (float)a.dim + a.eps);
+        if constexpr (BWD) dots = team_sum(dots, team) / (float)a.dim * r * r;
+#pragma unroll
+        for (int n = 0; n < U; ++n) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              float& f = x[n][k].f[e];
+              if constexpr (!BWD) {
+                f = f * r * w[n][k * N + e];
+              } else {
+                const float dv = d[n][k].f[e];
+                sums[X][n][k * N + e] += live ? dv * (f * r) : 0.f;
+                f = r * (dv * w[n][k * N + e] - f * dots);
+              }
+            }
+          if constexpr (!BWD) turn(x[n], n);
+          if (now.out) {
+            if (c0[n] >= 0) x[n][0].store(now.out, c0[n]);
+            if (c1[n] >= 0) x[n][1].store(now.out, c1[n]);
           }
-        if constexpr (!BWD) turn(x[n], n);
-        if (live && out) {
-          if (c0[n] >= 0) x[n][0].store(out, c0[n]);
-          if (c1[n] >= 0) x[n][1].store(out, c1[n]);
         }
       }
-    }
+    };
+    section(ic<0>{});
+    if (a.k.heads) section(ic<1>{});
   }
   if constexpr (BWD) {
     if (!a.partial) return;
@@ -229,24 +274,28 @@ __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormRotaryArgs a) 
   }
 }
 
-// The workgroups' sums of the weights' gradients: 16 columns of [2][dim] by 16 slices of the workgroups.
+// The workgroups' sums of the weights' gradients: 4 columns of [2][dim] by 64 slices of the workgroups.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void norm_rotary_sums_kernel(const float* partial, int groups, int dim, int vec_fp32, void* dq, void* dk) {
-  __shared__ float part[16][17];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+  __shared__ float part[64][5];
+  const int x = threadIdx.x & 3, col = blockIdx.x * 4 + x, slice = threadIdx.x >> 2;
   float s = 0.f;
-  if (col < 2 * dim)
-    for (int i = slice; i < groups; i += 16) s += partial[(int64_t)i * 2 * dim + col];
-  part[slice][threadIdx.x & 15] = s;
+  if (col < 2 * dim) {
+#pragma unroll
+    for (int i = 0; i < MAX_GROUPS / 64; ++i)
+      if (i * 64 + slice < groups) s += partial[(int64_t)(i * 64 + slice) * 2 * dim + col];
+  }
+  part[slice][x] = s;
   __syncthreads();
-  if (threadIdx.x >= 16 || col >= 2 * dim) return;
-  s = 0.f;
-  for (int i = 0; i < 16; ++i) s += part[i][threadIdx.x];
-  void* out = col < dim ? dq : dk;
-  const int c = col < dim ? col : col - dim;
-  if (!out) return;
-  if (vec_fp32) ((float*)out)[c] = s;
-  else store1<DT>(out, c, s);
+  if (threadIdx.x >= 64) return;   // (the first wave: 16 lanes a column, four slices each)
+  const int c = threadIdx.x >> 4, l = threadIdx.x & 15;
+  s = (part[l][c] + part[l + 16][c]) + (part[l + 32][c] + part[l + 48][c]);
+  s = row16_sum(s);
+  const int out_col = blockIdx.x * 4 + c, at = out_col < dim ? out_col : out_col - dim;
+  void* out = out_col < dim ? dq : dk;
+  if (l || out_col >= 2 * dim || !out) return;
+  if (vec_fp32) ((float*)out)[at] = s;
+  else store1<DT>(out, at, s);
 }
 
 template <int DT, int N, bool BWD>
@@ -294,7 +343,7 @@ int run(NormRotaryArgs a, int dtype, int vec_dtype, int64_t batch, bool inter, v
   };
   if (!fits(1) || (uintptr_t)a.freq % 8 || (uintptr_t)a.axis % 4 || (uintptr_t)a.pos % (a.pos_is_i64 ? 8 : 4)) return LBW_E_ALIGN;
   for (const void* p : {a.q.weight, a.k.weight, (const void*)dq_weight, (const void*)dk_weight})
-    if ((uintptr_t)p % elem_size(vec_dtype)) return LBW_E_ALIGN;
+    if ((uintptr_t)p % 16) return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const int unit = es == 2 && fits(8) ? 8 : fits(4) ? 4 : 1;
   const int items = a.pairs / unit + ((a.dim - 2 * a.pairs) / unit + 1) / 2;
@@ -302,16 +351,23 @@ int run(NormRotaryArgs a, int dtype, int vec_dtype, int64_t batch, bool inter, v
   a.vec_fp32 = vec_dtype == LBW_DTYPE_FP32;
   a.team = 4;
   while (a.team < 64 && a.team < items) a.team *= 2;
-  // a few rows a team, as long as there are workgroups for every CU
-  const int64_t rows = a.q.heads + a.k.heads;
+  // The tokens of a workgroup's step whose rows fill its teams best, q's and k's each by themselves, as long as there are
+  // workgroups for every CU (6032 tokens of 12 + 12 heads: 17 us with eight, 21 with four).
+  const int64_t teams = THREADS / a.team;
+  double best = 0;
   a.per_group = 1;
-  while (a.per_group < MAX_TOKENS && a.per_group * rows * a.team < 4 * THREADS && a.tokens / (2 * a.per_group) >= 1024) a.per_group *= 2;
+  for (int n = 1; n <= MAX_TOKENS; n *= 2) {
+    if (n > 1 && a.tokens / n < 512) break;
+    const int64_t passes = (n * a.q.heads + teams - 1) / teams + (n * a.k.heads + teams - 1) / teams;
+    const double filled = (double)(n * (a.q.heads + a.k.heads)) / (double)(passes * teams);
+    if (filled > 1.05 * best) best = filled, a.per_group = n;
+  }
   const int64_t groups = (a.tokens + a.per_group - 1) / a.per_group, grid = BWD ? std::min<int64_t>(groups, MAX_GROUPS) : groups;
   if (dtype == LBW_DTYPE_BF16) launch_by_unit<LBW_DTYPE_BF16, BWD>(a, unit, inter, grid, stream);
   else if (dtype == LBW_DTYPE_FP16) launch_by_unit<LBW_DTYPE_FP16, BWD>(a, unit, inter, grid, stream);
   else launch_by_unit<LBW_DTYPE_FP32, BWD>(a, unit, inter, grid, stream);
   if (BWD && a.partial) {
-    const unsigned n = (2 * a.dim + 15) / 16;
+    const unsigned n = (2 * a.dim + 3) / 4;
     if (dtype == LBW_DTYPE_BF16) norm_rotary_sums_kernel<LBW_DTYPE_BF16><<<n, THREADS, 0, stream>>>(a.partial, (int)grid, a.dim, a.vec_fp32, dq_weight, dk_weight);
     else if (dtype == LBW_DTYPE_FP16) norm_rotary_sums_kernel<LBW_DTYPE_FP16><<<n, THREADS, 0, stream>>>(a.partial, (int)grid, a.dim, a.vec_fp32, dq_weight, dk_weight);
     else norm_rotary_sums_kernel<LBW_DTYPE_FP32><<<n, THREADS, 0, stream>>>(a.partial, (int)grid, a.dim, a.vec_fp32, dq_weight, dk_weight);

@@ -556,3 +556,21 @@ def test_cache_attend_does_not_see_what_it_should_not():
         got = odd.attend(0, q, *args)
         seen = torch.tensor([0, 0, 0, 1, 1, 1, 0], dtype=torch.bool, device=DEV)
         assert torch.equal(got[~seen], want[~seen]) and bool(got[seen].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_norm_rotary_weights_of_a_larger_buffer(dtype):
+    """Weights that lie anywhere in a flat buffer, and their gradients."""
+    from lingbot_world_v2_realtime_amd import Rotary, norm_rotary_embed
+    g = _gen(60)
+    flat = _rand(g, 300, mean=1.0, dtype=DT[dtype]).requires_grad_()
+    q = _rand(g, 1, 9, 4, 128, dtype=torch.bfloat16)
+    plan, dy = Rotary.build(128, DEV), _rand(g, 1, 9, 4, 128, dtype=torch.bfloat16)
+    for at in (1, 3, 8):
+        out = norm_rotary_embed(q, q, 5, plan, flat[at:at + 128], flat[at + 128:at + 256])
+        (got,) = torch.autograd.grad(out, flat, (dy, dy))
+        for i in range(2):
+            part = slice(at + 128 * i, at + 128 * i + 128)
+            (y, mag), grads = causal.norm_rotary(q, flat[part], torch.arange(5, 14, device=DEV), plan.freq, d=dy)
+            _within(out[i].detach(), y, 36 * E * mag, f"at {at}")
+            _within(got[part], grads["weight"][0], 256 * E * grads["weight"][1], f"dw at {at}")
