@@ -121,7 +121,8 @@ __device__ __forceinline__ v4i decode8(uint32_t w, float scale) {
              (int)__builtin_bit_cast(uint32_t, (bf2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
              (int)__builtin_bit_cast(uint32_t, (bf2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
 }
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+// Byte i of a word as that operand: its exponent bits, and whatever falls around them.
+__device__ __forceinline__ float scale_at(uint32_t w, int i) { return __uint_as_float(i < 3 ? w << (23 - 8 * i) : w >> 1); }
 
 template <int DH>
 __global__ __launch_bounds__(THREADS) void kv4_read_kernel(Pages c, uint16_t* k, uint16_t* v) {
@@ -137,13 +138,13 @@ __global__ __launch_bounds__(THREADS) void kv4_read_kernel(Pages c, uint16_t* k,
     const int64_t h = is_k ? i : i - c.heads, tile = page * c.heads + h;
     v4i x = {0, 0, 0, 0};
     if (page >= 0 && is_k) {
-      x = decode8(*(const uint32_t*)(c.k4 + (tile * PAGE + t) * (DH / 2) + p * (DH / 8) + g * 4), scale_of(c.ks[(tile * PAGE + t) * (DH / 32) + g]));
+      x = decode8(*(const uint32_t*)(c.k4 + (tile * PAGE + t) * (DH / 2) + p * (DH / 8) + g * 4), scale_at(c.ks[(tile * PAGE + t) * (DH / 32) + g], 0));
     } else if (page >= 0) {
       const uint8_t* from = c.v4 + tile * (PAGE * DH / 2);
       uint32_t w = 0;
 #pragma unroll
       for (int n = 0; n < 8; ++n) w |= (uint32_t)(from[v_code_at<DH>(t, g, 8 * (p & 1) + n)] >> (p < 2 ? 0 : 4) & 15) << 4 * n;
-      x = decode8(w, scale_of(c.vs[tile * (PAGE * DH / 32) + v_scale_at<DH>(t, g)]));
+      x = decode8(w, scale_at(c.vs[tile * (PAGE * DH / 32) + v_scale_at<DH>(t, g)], 0));
     }
     *(v4i*)((is_k ? k : v) + (r * c.heads + h) * DH + 8 * c8) = x;
   }
@@ -157,13 +158,13 @@ struct AttnArgs {
   Pages c;
   const uint16_t* q;
   int64_t q_tok, q_head;
-  int q_heads, group, row_tiles;    // row_tiles: workgroups that share the heads of a group where those of one token are too many
-  int tokens;                       // tokens of a workgroup's rows
-  uint32_t places;
-  int chunk, splits;                // keys of a workgroup; workgroups of a row's keys (1: no partial sums)
+  int q_heads, group, row_tiles;    // row_tiles: waves that share the heads of a group where those of one token are too many
+  int tokens, tile_rows;            // tokens of a wave's rows, and how many rows those are at most
+  uint32_t places, shares;          // shares: waves that share a head's work evenly; 0: one for each place's rows
+  int64_t segments;                 // of a head, at most
   float sl2;
   uint16_t* out;
-  float *part, *stats;              // [rows][q_heads][splits][DH], [..][2]: sums, and the maximum and sum of the weights
+  float *part, *stats;              // [heads][segments][tile_rows][DH], [..][2]: sums, and the maximum and sum of the weights
 };
 
 __device__ __forceinline__ v4f mfma16(const v4i a, const v4i b, const v4f c) {
@@ -207,40 +208,130 @@ struct Step {
   }
 };
 
-// A workgroup: up to 16 RT rows (tokens x the heads that share a head of the cache) over a chunk of keys, 32 keys a wave and
-// step. S^T = K Q^T on v_mfma_f32_16x16x32_bf16: a lane holds one row and 8 of the 32 keys; the row's maximum needs two
-// exchanges; P^T goes from those registers into O^T += V^T P^T. fp16 q and P enter as two bf16 values each, high and low.
-template <int DH, bool F16, int RT>
-__global__ __launch_bounds__(THREADS) void kv4_attn_kernel(AttnArgs a) {
-  constexpr int G = DH / 32, NT = DH / 16;
-  __shared__ __align__(16) float part[WAVES][16][DH + 4];
-  __shared__ float stats[WAVES][16][2];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, p = lane >> 4;
-  const uint32_t id = group_id();
-  uint32_t split = id % a.splits, rest = id / a.splits;
-  const uint32_t row_tile = rest % a.row_tiles;
-  rest /= a.row_tiles;
-  const uint32_t head = rest % a.c.heads, at = rest / a.c.heads;
-  if (at >= a.places) return;
-  if (a.splits == 1 && a.c.starts && row_tile == 0)
-    zero_outside(a.c.starts, a.c.seqs, a.c.rows, a.out + (int64_t)head * a.group * DH, (int64_t)a.q_heads * DH, a.group * DH, at, a.places);
-  // the sequence, its rows in the call, and the first of this workgroup's tokens
-  int64_t seq = at, first = at;
-  int count = 1, token0 = 0;
-  if (a.c.starts) {
-    const Place pl = place(a.c.starts, a.c.seqs, a.c.rows, a.tokens, at);
-    if (pl.seq < 0) return;
-    const Span s = span(a.c.starts, pl.seq, a.c.rows);
-    seq = pl.seq, first = s.first, count = s.n, token0 = pl.tile * a.tokens;
+// A head's work as a line of units, each a tile of rows against a page: sequence by sequence its tiles of tokens, of each the
+// pages of its keys. Wave i of n takes the units from i U / n to (i + 1) U / n, wherever those end (n: no more than there are
+// units): all of them finish together, however different the sequences are. What a wave does of one tile is a segment; a
+// tile whose keys are cut has several, one behind the other, which a second kernel joins. Every head has a line of its own,
+// cut alike, and the waves of all heads at one place of it are neighbours: they read the same pages at the same time, which
+// memory likes (61 sequences of up to 6032 tokens, 8 heads, pages anywhere: 59 us, and 75 with one line of all heads, at four waves a tile).
+constexpr int UNIT = PAGE;
+
+struct Spot {
+  int64_t seq;
+  uint32_t units_before, tiles_before, tiles, units;   // of the line; of the sequence: its tiles, and units of each
+};
+struct Line {
+  const AttnArgs& a;
+  uint32_t total, n, all_w, all_t, w, t, l;   // a lane's sequence of 64: units and tiles up to it, its tiles' units
+  uint32_t own_w, own_t;
+
+  __device__ __forceinline__ void look(int64_t s0) {
+    const int64_t s = s0 + (threadIdx.x & 63);
+    l = own_t = 0;
+    if (s < a.c.seqs) {
+      const int count = a.c.starts ? span(a.c.starts, s, a.c.rows).n : 1;
+      own_t = (uint32_t)((count + a.tokens - 1) / a.tokens) * (uint32_t)a.row_tiles;
+      l = (uint32_t)((min(max((int64_t)a.c.lens[s], (int64_t)0), a.c.width * PAGE) + UNIT - 1) / UNIT);
+    }
+    w = own_w = own_t * l;
+    t = own_t;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t x = __shfl_up(w, o), y = __shfl_up(t, o);
+      if ((threadIdx.x & 63) >= o) w += x, t += y;
+    }
+    all_w = __shfl(w, 63), all_t = __shfl(t, 63);
   }
-  const int64_t len = min(max((int64_t)a.c.lens[seq], (int64_t)0), a.c.width * PAGE);
-  // row i of the workgroup: token token0 + i / group, head i % group of the group (heads from row_tile on where they are many)
+  __device__ __forceinline__ explicit Line(const AttnArgs& args) : a(args) {
+    total = 0;
+    for (int64_t s0 = 0; s0 < a.c.seqs; s0 += 64) {
+      look(s0);
+      total += all_w;
+    }
+    n = min(a.shares, total);
+  }
+  // the sequence at which f(its units up to and with it, its number) becomes true
+  template <typename F>
+  __device__ __forceinline__ Spot find(F f) {
+    uint32_t before = 0, tiles = 0;
+    for (int64_t s0 = 0; s0 < a.c.seqs; s0 += 64) {
+      if (a.c.seqs > 64) look(s0);
+      const uint64_t hit = __ballot(f(before + w, s0 + (threadIdx.x & 63)));
+      if (hit) {
+        const int at = __builtin_ctzll(hit);
+        const uint32_t ow = __shfl(own_w, at), ot = __shfl(own_t, at);
+        return {s0 + at, (uint32_t)__builtin_amdgcn_readfirstlane(before + __shfl(w, at) - ow),
+                (uint32_t)__builtin_amdgcn_readfirstlane(tiles + __shfl(t, at) - ot), (uint32_t)__builtin_amdgcn_readfirstlane(ot),
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)__shfl(l, at))};
+      }
+      before += all_w, tiles += all_t;
+    }
+    return {-1, 0, 0, 0, 0};
+  }
+  __device__ __forceinline__ uint32_t share(uint32_t i) const { return (uint32_t)((uint64_t)i * total / n); }
+  // the workgroup that has unit u
+  __device__ __forceinline__ uint32_t owner(uint32_t u) const { return (uint32_t)((((uint64_t)u + 1) * n - 1) / total); }
+};
+
+// A segment: up to 16 RT rows (tokens x the heads that share a head of the cache) over a run of keys, 32 a step, by one wave. S^T = K Q^T on v_mfma_f32_16x16x32_bf16: a lane holds one row and 8 of the 32 keys; the row's maximum needs two
+// exchanges; P^T goes from those registers into O^T += V^T P^T. fp16 q and P enter as two bf16 values each, high and low.
+template <int DH, int RT>
+constexpr int ATTN_WAVES = RT == 1 ? (DH == 128 ? 3 : 4) : RT == 2 ? (DH == 128 ? 2 : 3) : (DH == 128 ? 1 : 2);   // a SIMD
+
+template <int DH, bool F16, int RT>
+__global__ __launch_bounds__(THREADS, (ATTN_WAVES<DH, RT>)) void kv4_attn_kernel(AttnArgs a) {
+  constexpr int G = DH / 32, NT = DH / 16;
+  const uint32_t id = __builtin_amdgcn_readfirstlane(group_id() * WAVES + (threadIdx.x >> 6)), heads = (uint32_t)a.c.heads;
+  // where the wave is: a head, a sequence, a tile in it (tokens, part of the group), and the units of its keys
+  int64_t seq;
+  uint32_t head, tile = 0, unit = 0, units = 0, left = 1, tiles = 0, tiles_before = 0;   // left: units to go
+  if (a.shares) {
+    const uint32_t mine = id / heads;
+    head = id - mine * heads;
+    Line line(a);
+    if (mine >= line.n) return;
+    const uint32_t u = line.share(mine);
+    left = line.share(mine + 1) - u;
+    const Spot at = line.find([&](uint32_t upto, int64_t) { return upto > u; });
+    seq = at.seq, tiles = at.tiles, units = at.units, tiles_before = at.tiles_before;
+    tile = (u - at.units_before) / units;
+    unit = u - at.units_before - tile * units;
+  } else {
+    const uint32_t rest = id / heads, at = rest / a.row_tiles;
+    head = id - rest * heads;
+    tile = rest - at * a.row_tiles;
+    if (at >= a.places) return;
+    if (a.c.starts && tile == 0)
+      zero_outside(a.c.starts, a.c.seqs, a.c.rows, a.out + (int64_t)head * a.group * DH, (int64_t)a.q_heads * DH, a.group * DH, at, a.places,
+                   threadIdx.x & 63, 64);
+    seq = at;
+    if (a.c.starts) {
+      const Place pl = place(a.c.starts, a.c.seqs, a.c.rows, a.tokens, at);
+      if (pl.seq < 0) return;
+      seq = pl.seq;
+      tile += pl.tile * a.row_tiles;
+    }
+  }
+  while (true) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));   // (what is made of it is made here again for each segment: kept, it would take 30 registers)
+  const int n = lane & 15, p = lane >> 4;
+  seq = __builtin_amdgcn_readfirstlane((int)seq);
+  // (read by vector loads, for the kernel writes memory too: brought back to what one value of a wave is)
+  const Span of = a.c.starts ? span(a.c.starts, seq, a.c.rows) : Span{seq, 1};
+  const int64_t first = __builtin_amdgcn_readfirstlane((int)of.first);
+  const int count = __builtin_amdgcn_readfirstlane(of.n);
+  const uint32_t row_tile = tile % a.row_tiles;
+  const int token0 = (int)(tile / a.row_tiles) * a.tokens;
+  const int64_t len = min(max((int64_t)__builtin_amdgcn_readfirstlane(a.c.lens[seq]), (int64_t)0), a.c.width * PAGE);
+  // row i of the tile: token token0 + i / heads_here, head i % heads_here of the group (from row_tile on where they are many)
   const int group0 = row_tile * 16 * RT, heads_here = min(a.group - group0, a.row_tiles > 1 ? 16 * RT : a.group);
   const int rows = min(a.tokens, count - token0) * heads_here;
   const int64_t seen = len - count + token0 + 1;   // keys that the first token sees
   const int upto = (int)max((int64_t)0, min(len, seen + min(a.tokens, count - token0) - 1));
-  const int k0 = split * a.chunk, k1 = min(upto, k0 + a.chunk);
-  if (a.splits > 1 && k0 >= len) return;   // (nobody reads its part)
+  const uint32_t run = a.shares ? min(left, units - unit) : 0;
+  const int k0 = (int)unit * UNIT, k1 = a.shares ? min(upto, k0 + (int)run * UNIT) : upto;
+  const bool whole = !a.shares || run == units;
 
   v4i qh[RT][G], ql[F16 ? RT : 1][G];
   int own[RT];   // keys that the lane's row sees
@@ -277,46 +368,52 @@ __global__ __launch_bounds__(THREADS) void kv4_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[rt][i] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-  // the pages of the chunk (64 at most), one a lane
-  const int page0 = k0 / PAGE;
-  int64_t held = -1;
-  if (page0 + lane < a.c.width && (int64_t)(page0 + lane) * PAGE < k1) held = page_of(a.c, seq, (int64_t)(page0 + lane) * PAGE);
-  const int mine = (int)held;
-
-  for (int key = k0 + w * KB; key < k1; key += WAVES * KB) {
+  // the pages of the run, 64 at a time, one a lane
+  int page0 = k0 / PAGE, mine = -1;
+  const auto pages = [&] {
+    const int64_t t = page0 + lane;
+    mine = t * PAGE < k1 ? (int)page_of(a.c, seq, t * PAGE) : -1;
+  };
+  pages();
+  // a step's codes are loaded while the step before it is worked on
+  Step<DH> next;
+  const auto fetch = [&](int key) {
+    if (key / PAGE - page0 >= 64) {
+      page0 = key / PAGE;
+      pages();
+    }
     const int page = __builtin_amdgcn_readlane(mine, key / PAGE - page0);
+    if (page >= 0) next.load(a.c, (int64_t)page * heads + head, key / KB & 1, lane);
+    return page;
+  };
+  int next_page = -1;
+  if (k0 < k1) next_page = fetch(k0);
+  for (int key = k0; key < k1; key += KB) {
+    const int page = next_page;
+    Step<DH> st = next;
+    if (key + KB < k1) next_page = fetch(key + KB);
     if (page < 0) continue;
-    Step<DH> st;
-    st.load(a.c, (int64_t)page * a.c.heads + head, key / KB & 1, lane);
-    v4i kf[2][G], vf[G][2];
+    // Some row may not see all of these keys: those behind the last hold what they like, and a NaN must not reach the rows
+    // that do not see it through a weight of zero. Their scales become 1 (127), and the NaN is put where it belongs below.
+    const bool edge = key + KB > seen;
+    bool odd = false;
+    if (edge) {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at_key = key + 16 * (e >> 2) + 4 * p + (e & 3);
+          const bool nan = (st.vs[g][e >> 2] >> 8 * (e & 3) & 255) == 255;
+          if (at_key < seen || (at_key < k1 && !nan)) continue;
+          odd = odd || at_key < k1;
+          st.vs[g][e >> 2] = (st.vs[g][e >> 2] & ~(255u << 8 * (e & 3))) | 127u << 8 * (e & 3);
+        }
+    }
+    v4i kf[2][G], ph[RT], pl[F16 ? RT : 1];
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int j = 0; j < G; ++j) kf[x][j] = decode8(st.k[x][j], scale_of(st.ks[x] >> 8 * j & 255));
-    // Some row may not see all of these keys: those behind the last hold what they like, and a NaN must not reach the rows
-    // that do not see it through a weight of zero.
-    const bool edge = key + KB > seen;
-    bool odd = false;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      uint32_t two[8];   // channel 32 g + n low, 32 g + 16 + n high, of the lane's 8 keys
-#define LBW_KEY(e)                                                                                                         \
-  {                                                                                                                        \
-    uint32_t b = st.vs[g][e >> 2] >> 8 * (e & 3) & 255;                                                                    \
-    if (edge && key + 16 * (e >> 2) + 4 * p + (e & 3) >= seen && (b == 255 || key + 16 * (e >> 2) + 4 * p + (e & 3) >= k1)) {   \
-      odd = odd || key + 16 * (e >> 2) + 4 * p + (e & 3) < k1;                                                             \
-      b = 127;                                                                                                             \
-    }                                                                                                                      \
-    two[e] = __builtin_bit_cast(uint32_t, (bf2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(st.v[g][e >> 2], scale_of(b), e & 3)); \
-  }
-      LBW_KEY(0) LBW_KEY(1) LBW_KEY(2) LBW_KEY(3) LBW_KEY(4) LBW_KEY(5) LBW_KEY(6) LBW_KEY(7)
-#undef LBW_KEY
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        vf[g][0][e] = (int)__builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x05040100u);
-        vf[g][1][e] = (int)__builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x07060302u);
-      }
-    }
+      for (int j = 0; j < G; ++j) kf[x][j] = decode8(st.k[x][j], scale_at(st.ks[x], j));
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       v4f s[2];
@@ -345,7 +442,6 @@ __global__ __launch_bounds__(THREADS) void kv4_attn_kernel(AttnArgs a) {
         top[rt] = next;
       }
       const float off = top[rt] == -INFINITY ? 0.f : -top[rt];
-      v4i ph, pl;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         float pr[4];
@@ -355,16 +451,30 @@ __global__ __launch_bounds__(THREADS) void kv4_attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t hi = pack2<LBW_DTYPE_BF16>(pr[2 * i], pr[2 * i + 1]);
-          ph[2 * x + i] = (int)hi;
-          if constexpr (F16) pl[2 * x + i] = (int)pack2<LBW_DTYPE_BF16>(pr[2 * i] - lo16<false>(hi), pr[2 * i + 1] - hi16<false>(hi));
+          ph[rt][2 * x + i] = (int)hi;
+          if constexpr (F16) pl[rt][2 * x + i] = (int)pack2<LBW_DTYPE_BF16>(pr[2 * i] - lo16<false>(hi), pr[2 * i + 1] - hi16<false>(hi));
         }
       }
+    }
+    __builtin_amdgcn_sched_barrier(0);   // (V's values made before their weights are there only take registers)
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+    for (int g = 0; g < G; ++g) {
+      uint32_t two[8];   // channel 32 g + n low, 32 g + 16 + n high, of the lane's 8 keys
+#define LBW_KEY(e) two[e] = __builtin_bit_cast(uint32_t, (bf2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(st.v[g][e >> 2], scale_at(st.vs[g][e >> 2], e & 3), e & 3));
+      LBW_KEY(0) LBW_KEY(1) LBW_KEY(2) LBW_KEY(3) LBW_KEY(4) LBW_KEY(5) LBW_KEY(6) LBW_KEY(7)
+#undef LBW_KEY
+      v4i vf[2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        vf[0][e] = (int)__builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x05040100u);
+        vf[1][e] = (int)__builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x07060302u);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          o[rt][2 * g + x] = mfma16(vf[g][x], ph, o[rt][2 * g + x]);
-          if constexpr (F16) o[rt][2 * g + x] = mfma16(vf[g][x], pl, o[rt][2 * g + x]);
+          o[rt][2 * g + x] = mfma16(vf[x], ph[rt], o[rt][2 * g + x]);
+          if constexpr (F16) o[rt][2 * g + x] = mfma16(vf[x], pl[rt], o[rt][2 * g + x]);
         }
     }
     if (__any(odd)) {
@@ -384,99 +494,159 @@ __global__ __launch_bounds__(THREADS) void kv4_attn_kernel(AttnArgs a) {
     }
   }
 
-  // the waves' sums, a tile of 16 rows at a time: O^T's lane (p, n) holds channels 16 i + 4 p .. + 4 of row n
+  // O^T's lane (p, n) holds channels 16 i + 4 p .. + 4 of row n
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    if (rt * 16 >= rows) break;
-    if (rt) __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NT; ++i) *(v4f*)&part[w][n][16 * i + 4 * p] = o[rt][i];
+    const int i = rt * 16 + n;
     const float sum = sum_quarters(total[rt]);
-    if (p == 0) stats[w][n][0] = top[rt], stats[w][n][1] = sum;
-    __syncthreads();
-    constexpr int PER = 16 * DH / THREADS, LANES = DH / PER;   // channels of a thread
-    const int row = threadIdx.x / LANES, c0 = (threadIdx.x % LANES) * PER, i = rt * 16 + row;
     if (i < rows) {
-      float most = -INFINITY, sums = 0.f, x[PER] = {};
+      if (whole) {
+        const int tok = i / heads_here, h = i - tok * heads_here;
+        uint16_t* to = a.out + ((first + token0 + tok) * a.q_heads + (int64_t)head * a.group + group0 + h) * DH + 4 * p;
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
-      for (int v = 0; v < WAVES; ++v) most = fmaxf(most, stats[v][row][0]);
-#pragma unroll
-      for (int v = 0; v < WAVES; ++v) {
-        const float by = stats[v][row][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stats[v][row][0] - most);
-        sums = fmaf(by, stats[v][row][1], sums);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) x[e] = fmaf(by, part[v][row][c0 + e], x[e]);
-      }
-      const int tok = i / heads_here, h = i - tok * heads_here;
-      const int64_t r = (first + token0 + tok) * a.q_heads + (int64_t)head * a.group + group0 + h;
-      if (a.splits == 1) {
-        const float inv = sums > 0.f || sums != sums ? 1.f / sums : 0.f;
-#pragma unroll
-        for (int e = 0; e < PER; e += 2)
-          *(uint32_t*)(a.out + r * DH + c0 + e) = pack2<F16 ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16>(x[e] * inv, x[e + 1] * inv);
+        for (int x = 0; x < NT; ++x) {
+          constexpr int DT = F16 ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16;
+          *(uint2*)(to + 16 * x) = make_uint2(pack2<DT>(o[rt][x][0] * inv, o[rt][x][1] * inv), pack2<DT>(o[rt][x][2] * inv, o[rt][x][3] * inv));
+        }
       } else {
+        const int64_t at = ((int64_t)head * a.segments + id / heads + tiles_before + tile) * a.tile_rows + i;
 #pragma unroll
-        for (int e = 0; e < PER; e += 4) *(v4f*)(a.part + (r * a.splits + split) * DH + c0 + e) = v4f{x[e], x[e + 1], x[e + 2], x[e + 3]};
-        if (c0 == 0) a.stats[(r * a.splits + split) * 2] = most, a.stats[(r * a.splits + split) * 2 + 1] = sums;
+        for (int x = 0; x < NT; ++x) *(v4f*)(a.part + at * DH + 16 * x + 4 * p) = o[rt][x];
+        if (p == 0) *(float2*)(a.stats + at * 2) = make_float2(top[rt], sum);
       }
     }
   }
+  if (!a.shares || left == run) return;
+  left -= run;
+  unit = 0;
+  if (++tile == tiles) {   // the next sequence that has any work
+    tile = 0;
+    do {
+      tiles_before += tiles;
+      ++seq;
+      units = (uint32_t)((min(max((int64_t)__builtin_amdgcn_readfirstlane(a.c.lens[seq]), (int64_t)0), a.c.width * PAGE) + UNIT - 1) / UNIT);
+      const int rows_of = a.c.starts ? __builtin_amdgcn_readfirstlane(span(a.c.starts, seq, a.c.rows).n) : 1;
+      tiles = (uint32_t)((rows_of + a.tokens - 1) / a.tokens) * a.row_tiles;
+    } while (units * tiles == 0);
+  }
+  }
 }
 
-// The chunks of a row's keys joined: a wave a row and head, DH / 64 channels a lane.
-template <int DH, bool F16>
+// The segments of a row's tile joined, where it has several, and zeros where it has none: a workgroup a row and head, DH / 4
+// lanes a segment, so that 8 (16) segments are read at once, four times over; each group of lanes keeps a running maximum and
+// sum, and the groups' are joined in LDS.
+template <int DH, bool F16, int RT>
 __global__ __launch_bounds__(THREADS) void kv4_join_kernel(AttnArgs a) {
-  constexpr int PER = DH / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)group_id() * WAVES + (threadIdx.x >> 6);
+  constexpr int LANES = DH / 4, GROUPS = THREADS / LANES, AHEAD = 4, DT = F16 ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16;
+  __shared__ __align__(16) v4f sums[GROUPS][LANES];
+  __shared__ float2 stats[GROUPS];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int64_t i = group_id();
   if (i >= a.c.rows * a.q_heads) return;
-  int64_t seq = i / a.q_heads;
+  const int64_t row = i / a.q_heads;
+  const int hq = (int)(i - row * a.q_heads), head = hq / a.group, g = hq - head * a.group;
+  int64_t seq = row;
+  int token = 0;
   if (a.c.starts) {
-    seq = last_of(a.c.seqs + 1, seq, [&](int64_t s) { return (int64_t)a.c.starts[s]; });
+    seq = last_of(a.c.seqs + 1, row, [&](int64_t s) { return (int64_t)a.c.starts[s]; });
     if (seq >= a.c.seqs) seq = -1;
+    if (seq >= 0) token = (int)(row - span(a.c.starts, seq, a.c.rows).first);
   }
-  const int64_t len = seq < 0 ? 0 : min(max((int64_t)a.c.lens[seq], (int64_t)0), a.c.width * PAGE);
-  const int parts = (int)((len + a.chunk - 1) / a.chunk);
-  float most = -INFINITY, sums = 0.f, x[PER] = {};
-  for (int s = 0; s < parts; ++s) most = fmaxf(most, a.stats[(i * a.splits + s) * 2]);
-  for (int s = 0; s < parts; ++s) {
-    const float m = a.stats[(i * a.splits + s) * 2], by = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - most);
-    sums = fmaf(by, a.stats[(i * a.splits + s) * 2 + 1], sums);
+  int parts = 0;
+  int64_t at = 0;   // the first segment's row
+  if (seq >= 0) {
+    Line line(a);
+    const Spot s = line.find([&](uint32_t, int64_t x) { return x == seq; });
+    const int row_tile = a.row_tiles > 1 ? g / (16 * RT) : 0, heads_here = min(a.group - row_tile * 16 * RT, a.row_tiles > 1 ? 16 * RT : a.group);
+    const uint32_t tile = (uint32_t)(token / a.tokens * a.row_tiles + row_tile);
+    if (s.units && tile < s.tiles) {
+      const uint32_t u = s.units_before + tile * s.units, first = line.owner(u);
+      parts = (int)(line.owner(u + s.units - 1) - first) + 1;
+      if (parts == 1) return;   // (the one segment wrote the row)
+      at = (head * a.segments + first + s.tiles_before + tile) * a.tile_rows + token % a.tokens * heads_here + g - row_tile * 16 * RT;
+    }
+  }
+  float most = -INFINITY, total = 0.f;
+  v4f x = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = group; s0 < parts; s0 += GROUPS * AHEAD) {
+    float2 st[AHEAD];
+    v4f p[AHEAD];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) x[e] = fmaf(by, a.part[(i * a.splits + s) * DH + lane * PER + e], x[e]);
+    for (int k = 0; k < AHEAD; ++k) {
+      const int s = s0 + k * GROUPS;
+      const int64_t mine = at + (int64_t)s * a.tile_rows;
+      st[k] = s < parts ? *(const float2*)(a.stats + mine * 2) : make_float2(-INFINITY, 0.f);
+      p[k] = s < parts ? *(const v4f*)(a.part + mine * DH + lane * 4) : v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    float next = most;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) next = fmaxf(next, st[k].x);
+    const float before = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(most - next);
+    total *= before;
+    x *= before;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const float by = st[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[k].x - next);
+      total = fmaf(by, st[k].y, total);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = fmaf(by, p[k][e], x[e]);
+    }
+    most = next;
   }
-  const float inv = sums > 0.f || sums != sums ? 1.f / sums : 0.f;
-  if constexpr (PER == 2) *(uint32_t*)(a.out + i * DH + 2 * lane) = pack2<F16 ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16>(x[0] * inv, x[1] * inv);
-  else store1<F16 ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16>(a.out, i * DH + lane, x[0] * inv);
+  sums[group][lane] = x;
+  if (lane == 0) stats[group] = make_float2(most, total);
+  __syncthreads();
+  if (group) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) top = fmaxf(top, stats[k].x);
+  total = 0.f;
+  x = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    const float by = stats[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stats[k].x - top);
+    total = fmaf(by, stats[k].y, total);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = fmaf(by, sums[k][lane][e], x[e]);
+  }
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  *(uint2*)(a.out + i * DH + lane * 4) = make_uint2(pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv));
 }
 
-// How a call's work is cut: 16-row tiles of a workgroup, tokens of its rows, workgroups for a group's heads, keys of a chunk.
+// How a call's work is cut: 16-row tiles of a wave, tokens of its rows, waves for a group's heads; the waves that share a
+// head's work evenly (of all heads as many as run at once), or 0: each tile of rows has one of its own. That is so where its keys are one
+// unit at most (a second kernel would be there for nothing), and where the tiles are so many that they even out.
 struct Plan {
-  int rt, tokens, row_tiles, chunk, splits;
-  int64_t places;
+  int rt, tokens, tile_rows, row_tiles, shares;
+  int64_t places, segments;
 };
-Plan plan(int64_t seqs, int64_t rows, int64_t group, int64_t heads, bool single, int64_t width) {
+Plan plan(int64_t seqs, int64_t rows, int64_t group, int64_t heads, int64_t dim, bool single, int64_t width) {
   Plan p;
   const int64_t each = single ? group : group * ((rows + seqs - 1) / seqs);   // rows of a sequence, about
   p.rt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
   p.tokens = (int)std::max<int64_t>(1, 16 * p.rt / group);
+  p.tile_rows = (int)std::min<int64_t>(16 * p.rt, p.tokens * group);
   p.row_tiles = (int)((group + 16 * p.rt - 1) / (16 * p.rt));
   p.places = single ? seqs : places_of(rows, seqs, p.tokens);
-  const int64_t keys = width * PAGE, base = std::max<int64_t>(1, std::min(p.places, rows) * heads * p.row_tiles);
-  int64_t chunk = (keys * base / 2048 + 127) / 128 * 128;
-  chunk = std::min<int64_t>(std::max<int64_t>(chunk, 128), 4096 - PAGE);
-  p.chunk = (int)chunk;
-  p.splits = (int)std::max<int64_t>(1, (keys + chunk - 1) / chunk);
+  const int waves = dim == 128 ? (p.rt == 1 ? 3 : p.rt == 2 ? 2 : 1) : (p.rt == 1 ? 4 : p.rt == 2 ? 3 : 2);   // ATTN_WAVES
+  const int64_t tiles = p.places * p.row_tiles, most = (width * PAGE + UNIT - 1) / UNIT;
+  p.shares = most > 1 && tiles * heads < 16 * 1024 * waves && tiles * most < 1 << 30 ? (int)(1024 * waves / heads) : 0;
+  p.segments = p.shares ? p.shares + tiles : 0;
   return p;
 }
 
+template <int DH, bool F16, int RT>
+void launch_attn(const AttnArgs& a, hipStream_t stream) {
+  const int64_t grid = a.shares ? a.shares * a.c.heads : (int64_t)a.places * a.c.heads * a.row_tiles;
+  kv4_attn_kernel<DH, F16, RT><<<grid_of((grid + WAVES - 1) / WAVES), THREADS, 0, stream>>>(a);
+  if (a.shares) kv4_join_kernel<DH, F16, RT><<<grid_of(a.c.rows * a.q_heads), THREADS, 0, stream>>>(a);
+}
 template <int DH, bool F16>
 void launch_attn(const AttnArgs& a, int rt, hipStream_t stream) {
-  const dim3 grid = grid_of((int64_t)a.places * a.c.heads * a.row_tiles * a.splits);
-  if (rt == 1) kv4_attn_kernel<DH, F16, 1><<<grid, THREADS, 0, stream>>>(a);
-  else if (rt == 2) kv4_attn_kernel<DH, F16, 2><<<grid, THREADS, 0, stream>>>(a);
-  else kv4_attn_kernel<DH, F16, 4><<<grid, THREADS, 0, stream>>>(a);
-  if (a.splits > 1) kv4_join_kernel<DH, F16><<<grid_of((a.c.rows * a.q_heads + WAVES - 1) / WAVES), THREADS, 0, stream>>>(a);
+  if (rt == 1) launch_attn<DH, F16, 1>(a, stream);
+  else if (rt == 2) launch_attn<DH, F16, 2>(a, stream);
+  else launch_attn<DH, F16, 4>(a, stream);
 }
 
 int check_pages(int64_t seqs, int64_t rows, int64_t heads, int64_t dim, const int32_t* starts, const int32_t* lens,
@@ -540,8 +710,8 @@ extern "C" int lbw_kv4_read(int64_t seqs, int64_t rows, int64_t heads, int64_t d
 extern "C" int64_t lbw_kv4_attn_workspace_bytes(int64_t seqs, int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t width,
                                                 int single) {
   if (seqs < 1 || rows < 1 || heads < 1 || q_heads < heads) return 0;
-  const Plan p = plan(seqs, rows, q_heads / heads, heads, single, width);
-  return p.splits > 1 ? rows * q_heads * p.splits * (dim + 2) * 4 : 0;
+  const Plan p = plan(seqs, rows, q_heads / heads, heads, dim, single, width);
+  return heads * p.segments * p.tile_rows * (dim + 2) * 4;
 }
 
 extern "C" int lbw_kv4_attn(const void* q, int dtype, int64_t seqs, int64_t rows, int64_t q_heads, int64_t heads, int64_t dim,
@@ -553,16 +723,16 @@ extern "C" int lbw_kv4_attn(const void* q, int dtype, int64_t seqs, int64_t rows
   if ((dtype != LBW_DTYPE_BF16 && dtype != LBW_DTYPE_FP16) || q_heads < heads || q_heads > 4096 || q_heads % heads ||
       !(sm_scale > 0.f) || !(sm_scale < INFINITY))
     return LBW_E_SHAPE;
-  const Plan p = plan(seqs, rows, q_heads / heads, heads, !starts, width);
-  if (p.places * heads * p.row_tiles * p.splits > 1 << 30 || rows * q_heads > 1ll << 31) return LBW_E_SHAPE;
-  if (p.splits > 1 && !workspace) return LBW_E_NULL;
+  const Plan p = plan(seqs, rows, q_heads / heads, heads, dim, !starts, width);
+  if (p.places * heads * p.row_tiles > 1 << 30 || rows * q_heads > 1 << 30) return LBW_E_SHAPE;
+  if (p.shares && !workspace) return LBW_E_NULL;
   if (!aligned(q, q_s_tok, q_s_head) || ((uintptr_t)out | (uintptr_t)workspace) % 16) return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   float* part = (float*)workspace;
   const AttnArgs a = {{(uint8_t*)k4, (uint8_t*)ks, (uint8_t*)v4, (uint8_t*)vs, heads, pages, width, t_s_seq, seqs, rows, starts, lens, table},
-                      (const uint16_t*)q, q_s_tok, q_s_head, (int)q_heads, (int)(q_heads / heads), p.row_tiles, p.tokens,
-                      (uint32_t)p.places, p.chunk, p.splits, sm_scale * LOG2E, (uint16_t*)out, part,
-                      part ? part + rows * q_heads * p.splits * dim : nullptr};
+                      (const uint16_t*)q, q_s_tok, q_s_head, (int)q_heads, (int)(q_heads / heads), p.row_tiles, p.tokens, p.tile_rows,
+                      (uint32_t)p.places, (uint32_t)p.shares, p.segments, sm_scale * LOG2E, (uint16_t*)out, part,
+                      part ? part + heads * p.segments * p.tile_rows * dim : nullptr};
   const bool f16 = dtype == LBW_DTYPE_FP16;
   if (dim == 128) f16 ? launch_attn<128, true>(a, p.rt, (hipStream_t)stream) : launch_attn<128, false>(a, p.rt, (hipStream_t)stream);
   else f16 ? launch_attn<64, true>(a, p.rt, (hipStream_t)stream) : launch_attn<64, false>(a, p.rt, (hipStream_t)stream);

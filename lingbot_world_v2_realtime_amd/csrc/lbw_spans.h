@@ -53,15 +53,15 @@ __device__ __forceinline__ Place place(const int32_t* starts, int64_t seqs, int6
 }
 
 // Rows of the tensor that belong to no sequence (before the first and behind the last): zeros, a part of them for each of
-// `parts` workgroups. `width` 16-bit values (a multiple of 8) from base on in rows `stride` elements apart.
+// `parts` workgroups (or waves; `threads` of it). `width` 16-bit values (a multiple of 8) from base on in rows `stride` elements apart.
 __device__ __forceinline__ void zero_outside(const int32_t* starts, int64_t seqs, int64_t rows, uint16_t* base, int64_t stride,
-                                             int width, uint32_t part, uint32_t parts) {
+                                             int width, uint32_t part, uint32_t parts, int thread, int threads) {
   const int64_t a = min(max((int64_t)starts[0], (int64_t)0), rows), b = min(max((int64_t)starts[seqs], a), rows);
   const int64_t outside = a + rows - b;
   if (outside == 0) return;
   const int pieces = width / 8;
   for (int64_t i = part; i < outside; i += parts)
-    for (int c = threadIdx.x; c < pieces; c += blockDim.x)
+    for (int c = thread; c < pieces; c += threads)
       *(v4i*)(base + (i < a ? i : b + (i - a)) * stride + c * 8) = v4i{0, 0, 0, 0};
 }
 

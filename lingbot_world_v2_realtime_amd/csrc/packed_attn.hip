@@ -33,7 +33,7 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
   head_tile(group_id(), a.s.q_heads, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.q_heads * DH;
-  zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.out + head * DH, o_tok, DH, tile, a.tiles);
+  zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.out + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
   const Place at = place(a.s.starts, a.s.seqs, a.s.q_rows, QT, tile);
   if (at.seq < 0) return;
   const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);

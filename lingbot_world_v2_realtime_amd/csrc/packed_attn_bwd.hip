@@ -104,8 +104,8 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   head_tile(group_id(), a.s.k_heads, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.k_heads * DH;
-  zero_outside(a.s.k_starts, a.s.seqs, a.s.k_rows, a.dk + head * DH, o_tok, DH, tile, a.tiles);
-  zero_outside(a.s.k_starts, a.s.seqs, a.s.k_rows, a.dv + head * DH, o_tok, DH, tile, a.tiles);
+  zero_outside(a.s.k_starts, a.s.seqs, a.s.k_rows, a.dk + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
+  zero_outside(a.s.k_starts, a.s.seqs, a.s.k_rows, a.dv + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
   const Place at = place(a.s.k_starts, a.s.seqs, a.s.k_rows, KT, tile);
   if (at.seq < 0) return;
   const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   head_tile(group_id(), a.s.q_heads, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.q_heads * DH;
-  zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.dq + head * DH, o_tok, DH, tile, a.tiles);
+  zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.dq + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
   const Place at = place(a.s.starts, a.s.seqs, a.s.q_rows, QT, tile);
   if (at.seq < 0) return;
   const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
