@@ -150,6 +150,129 @@ __global__ __launch_bounds__(THREADS) void kv4_read_kernel(Pages c, uint16_t* k,
   }
 }
 
+// ---- prompts: a workgroup a head's 32 tokens between two multiples of 32, whose V codes are neighbours in memory
+
+constexpr int BLOCK = 32;
+
+// The tokens of a call in blocks: where sequence s holds positions [from, to), the blocks from / 32 to (to - 1) / 32, numbered
+// from starts[s] / 32 + 2 s on (n tokens lie in n / 32 + 2 blocks at most).
+struct Block {
+  int64_t seq, row;   // row: of the block's first token, were it one of the call
+  int64_t pos;        // its position
+  int first, end;     // tokens of the block that are the call's
+};
+inline int64_t blocks_of(int64_t rows, int64_t seqs) { return rows / BLOCK + 2 * seqs; }
+__device__ __forceinline__ Block block_of(const Pages& c, int64_t want) {
+  const int64_t s = last_of(c.seqs, want, [&](int64_t i) { return min(max((int64_t)c.starts[i], (int64_t)0), c.rows) / BLOCK + 2 * i; });
+  if (s < 0) return {-1, 0, 0, 0, 0};
+  const Span of = span(c.starts, s, c.rows);
+  const int64_t from = (int64_t)c.lens[s] - of.n, to = c.lens[s];   // (from below zero: tokens before the first, in no page)
+  const int64_t base = min(max((int64_t)c.starts[s], (int64_t)0), c.rows) / BLOCK + 2 * s;
+  const int64_t pos = ((from >> 5) + want - base) * BLOCK;
+  static_assert(BLOCK == 1 << 5, "the shift rounds down below zero too");
+  if (of.n == 0 || pos >= to) return {-1, 0, 0, 0, 0};
+  return {s, of.first + pos - from, pos, (int)max(from - pos, (int64_t)0), (int)min(to - pos, (int64_t)BLOCK)};
+}
+
+template <int DH, bool F16>
+__global__ __launch_bounds__(THREADS) void kv4_write_block_kernel(Pages c, const uint16_t* k, const uint16_t* v, int64_t k_tok, int64_t k_head,
+                                                                  int64_t v_tok, int64_t v_head) {
+  constexpr int LANES = DH / 8, G = DH / 32, ROWS = THREADS / LANES;   // tokens of a pass
+  __shared__ uint32_t codes[BLOCK][LANES + 1];
+  __shared__ uint8_t scales[BLOCK][G];
+  const uint32_t id = group_id(), head = id % (uint32_t)c.heads;
+  const Block b = block_of(c, id / (uint32_t)c.heads);
+  const int64_t page = page_of(c, b.seq, b.pos);
+  if (page < 0) return;
+  const int64_t tile = page * c.heads + head;
+  const int c8 = threadIdx.x % LANES, g = c8 >> 2, p = c8 & 3, t0 = (int)(b.pos & (PAGE - 1));
+#pragma unroll
+  for (int i = 0; i < BLOCK / ROWS; ++i) {
+    const int t = i * ROWS + threadIdx.x / LANES;
+    const bool live = t >= b.first && t < b.end;   // (lanes of a group together)
+    float x[8] = {}, y[8] = {};
+    if (live) {
+      unpack8t<F16>(*(const v4i*)(k + (b.row + t) * k_tok + head * k_head + 8 * c8), x);
+      unpack8t<F16>(*(const v4i*)(v + (b.row + t) * v_tok + head * v_head + 8 * c8), y);
+    }
+    uint32_t ks, vs;
+    const uint32_t kw = encode8(x, ks), vw = encode8(y, vs);
+    codes[t][c8] = vw;
+    if (p == 0) scales[t][g] = (uint8_t)vs;
+    if (!live) continue;
+    *(uint32_t*)(c.k4 + (tile * PAGE + t0 + t) * (DH / 2) + p * (DH / 8) + g * 4) = kw;
+    if (p == 0) c.ks[(tile * PAGE + t0 + t) * G + g] = (uint8_t)ks;
+  }
+  __syncthreads();
+  // 16 bytes of V: channel n of two groups, the 8 tokens of part p; then the scales of a part and group, 8 bytes
+  const bool all = b.first == 0 && b.end == BLOCK;
+  uint8_t *to = c.v4 + tile * (PAGE * DH / 2) + t0 * (DH / 2), *sc = c.vs + tile * (PAGE * G) + t0 * G;
+  for (int i = threadIdx.x; i < BLOCK * DH / 32; i += THREADS) {
+    const int n = i & 15, vp = i >> 4 & 3, g2 = i >> 6;
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {   // (half a group's channels, then the other's)
+      const int t = 16 * (e >> 2 & 1) + 4 * vp + (e & 3), at = 4 * (2 * g2 + (e >> 3)) + (n >> 3);
+      const uint32_t byte = (codes[t][at] >> 4 * (n & 7) & 15) | (codes[t][at + 2] >> 4 * (n & 7) & 15) << 4;
+      w[e >> 2] |= byte << 8 * (e & 3);
+    }
+    if (all) {
+      *(v4i*)(to + i * 16) = v4i{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int t = 16 * (e >> 2 & 1) + 4 * vp + (e & 3);
+        if (t >= b.first && t < b.end) to[i * 16 + e] = (uint8_t)(w[e >> 2] >> 8 * (e & 3));
+      }
+    }
+  }
+  for (int i = threadIdx.x; i < BLOCK * G; i += THREADS) {
+    const int e = i & 7, vg = i / 8 % G, vp = i / (8 * G), t = 16 * (e >> 2) + 4 * vp + (e & 3);
+    if (t >= b.first && t < b.end) sc[i] = scales[t][vg];
+  }
+}
+
+template <int DH>
+__global__ __launch_bounds__(THREADS) void kv4_read_block_kernel(Pages c, uint16_t* k, uint16_t* v, int64_t blocks) {
+  constexpr int LANES = DH / 8, G = DH / 32, ROWS = THREADS / LANES;
+  __shared__ __align__(16) uint8_t codes[BLOCK * DH / 2];
+  __shared__ uint8_t scales[BLOCK * G];
+  const uint32_t id = group_id(), head = id % (uint32_t)c.heads;
+  const int64_t want = id / (uint32_t)c.heads, o_tok = c.heads * DH;
+  if (want >= blocks) return;
+  for (uint16_t* out : {k, v})
+    zero_outside(c.starts, c.seqs, c.rows, out + head * DH, o_tok, DH, (uint32_t)want, (uint32_t)blocks, threadIdx.x, THREADS);
+  const Block b = block_of(c, want);
+  if (b.seq < 0) return;
+  const int64_t page = page_of(c, b.seq, b.pos), tile = page * c.heads + head;
+  const int c8 = threadIdx.x % LANES, g = c8 >> 2, p = c8 & 3, t0 = (int)(b.pos & (PAGE - 1));
+  if (page >= 0) {
+    const uint8_t *from = c.v4 + tile * (PAGE * DH / 2) + t0 * (DH / 2), *sc = c.vs + tile * (PAGE * G) + t0 * G;
+    for (int i = threadIdx.x; i < BLOCK * DH / 32; i += THREADS) *(v4i*)(codes + i * 16) = *(const v4i*)(from + i * 16);
+    for (int i = threadIdx.x; i < BLOCK * G; i += THREADS) scales[i] = sc[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < BLOCK / ROWS; ++i) {
+    const int t = i * ROWS + threadIdx.x / LANES;
+    if (t < b.first || t >= b.end) continue;
+    v4i x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+    if (page >= 0) {
+      const uint32_t kw = *(const uint32_t*)(c.k4 + (tile * PAGE + t0 + t) * (DH / 2) + p * (DH / 8) + g * 4);
+      uint32_t vw = 0;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) vw |= (uint32_t)(codes[v_code_at<DH>(t, g, 8 * (p & 1) + n)] >> (p < 2 ? 0 : 4) & 15) << 4 * n;
+      x = decode8(kw, scale_at(c.ks[(tile * PAGE + t0 + t) * G + g], 0));
+      y = decode8(vw, scale_at(scales[v_scale_at<DH>(t, g)], 0));
+    }
+    *(v4i*)(k + (b.row + t) * o_tok + head * DH + 8 * c8) = x;
+    *(v4i*)(v + (b.row + t) * o_tok + head * DH + 8 * c8) = y;
+  }
+}
+
+// Rows a sequence, about, from which on blocks are the better form (TODO).
+constexpr int64_t BLOCK_ROWS = 16;
+
 // ---------------------------------------------------------------- attention
 
 constexpr int KB = 32, WAVES = THREADS / 64;   // keys of a wave's step
@@ -679,11 +802,18 @@ extern "C" int lbw_kv4_write(const void* k, const void* v, int dtype, int64_t se
   if (!aligned(k, k_s_tok, k_s_head) || !aligned(v, v_s_tok, v_s_head)) return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const Pages c = {k4, ks, v4, vs, heads, pages, width, t_s_seq, seqs, rows, starts, lens, table};
-  const dim3 grid = grid_of((rows + 3) / 4);
+  const bool blocks = starts && rows >= BLOCK_ROWS * seqs && blocks_of(rows, seqs) * heads <= 1 << 30;
+  const dim3 grid = grid_of(blocks ? blocks_of(rows, seqs) * heads : (rows + 3) / 4);
   const uint16_t *kp = (const uint16_t*)k, *vp = (const uint16_t*)v;
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype == LBW_DTYPE_FP16;
-  if (dim == 128) {
+  if (blocks && dim == 128) {
+    if (f16) kv4_write_block_kernel<128, true><<<grid, THREADS, 0, s>>>(c, kp, vp, k_s_tok, k_s_head, v_s_tok, v_s_head);
+    else kv4_write_block_kernel<128, false><<<grid, THREADS, 0, s>>>(c, kp, vp, k_s_tok, k_s_head, v_s_tok, v_s_head);
+  } else if (blocks) {
+    if (f16) kv4_write_block_kernel<64, true><<<grid, THREADS, 0, s>>>(c, kp, vp, k_s_tok, k_s_head, v_s_tok, v_s_head);
+    else kv4_write_block_kernel<64, false><<<grid, THREADS, 0, s>>>(c, kp, vp, k_s_tok, k_s_head, v_s_tok, v_s_head);
+  } else if (dim == 128) {
     if (f16) kv4_write_kernel<128, true><<<grid, THREADS, 0, s>>>(c, kp, vp, k_s_tok, k_s_head, v_s_tok, v_s_head);
     else kv4_write_kernel<128, false><<<grid, THREADS, 0, s>>>(c, kp, vp, k_s_tok, k_s_head, v_s_tok, v_s_head);
   } else {
@@ -701,8 +831,12 @@ extern "C" int lbw_kv4_read(int64_t seqs, int64_t rows, int64_t heads, int64_t d
   if (((uintptr_t)k | (uintptr_t)v) % 16) return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const Pages c = {(uint8_t*)k4, (uint8_t*)ks, (uint8_t*)v4, (uint8_t*)vs, heads, pages, width, t_s_seq, seqs, rows, starts, lens, table};
-  const dim3 grid = grid_of((rows + 3) / 4);
-  if (dim == 128) kv4_read_kernel<128><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v);
+  const int64_t n = blocks_of(rows, seqs);
+  const bool blocks = starts && rows >= BLOCK_ROWS * seqs && n * heads <= 1 << 30;
+  const dim3 grid = grid_of(blocks ? n * heads : (rows + 3) / 4);
+  if (blocks && dim == 128) kv4_read_block_kernel<128><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v, n);
+  else if (blocks) kv4_read_block_kernel<64><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v, n);
+  else if (dim == 128) kv4_read_kernel<128><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v);
   else kv4_read_kernel<64><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v);
   return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
 }

@@ -24,6 +24,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 template <int N>
 using ic = std::integral_constant<int, N>;
 
+// Stands in a branch that a whole wave takes or not: the compiler would take both sides and select, for every tile what the
+// last ones need.
+__device__ __forceinline__ void branch_here() { asm volatile(""); }
+
 template <bool F16>
 __device__ __forceinline__ v16f mfma(const v4i a, const v4i b, const v16f c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(hf8, a), __builtin_bit_cast(hf8, b), c, 0, 0, 0);
@@ -49,12 +53,19 @@ __device__ __forceinline__ float sum_xor32(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Workgroups of `tiles` tiles of every head, numbered so that those of neighbouring heads (which read the same k and v)
-// run on one XCD (a workgroup's number mod 8) where the heads divide by 8: head and tile of a workgroup.
-__device__ __forceinline__ void head_tile(uint32_t id, uint32_t heads, uint32_t& head, uint32_t& tile) {
-  tile = id / heads;
-  head = id - tile * heads;
-  if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
+// The head and tile of a workgroup, numbered so that one XCD (a workgroup's number mod 8) has as few heads of k and v as it
+// can: with c the greatest common divisor of those heads and 8, XCD x takes the heads x mod c, + c, .. and every (8 / c)-th
+// tile of theirs, the heads of q that share one behind each other.
+inline uint32_t xcd_common(int64_t k_heads) { return k_heads % 8 == 0 ? 8 : k_heads % 4 == 0 ? 4 : k_heads % 2 == 0 ? 2 : 1; }
+inline int64_t xcd_groups(int64_t tiles, int64_t k_heads, int64_t group) {
+  const int64_t c = xcd_common(k_heads), each = 8 / c;
+  return (tiles + each - 1) / each * (k_heads / c) * group * 8;
+}
+__device__ __forceinline__ void head_tile(uint32_t id, uint32_t k_heads, uint32_t group, uint32_t common, uint32_t& head, uint32_t& tile) {
+  const uint32_t x = id & 7, r = id >> 3, per = k_heads / common, rest = r / group, g = r - rest * group;
+  const uint32_t t = rest / per, j = rest - t * per;
+  head = (x % common + common * j) * group + g;
+  tile = t * (8 / common) + x / common;
 }
 
 template <int DH>
@@ -66,16 +77,41 @@ __device__ __forceinline__ int swizzle(int r) {
   else return (r >> 1 & 1) << 2 | (r >> 2 & 3);   // (two rows share 256 bytes)
 }
 
-// 16 bytes a lane from the buffer `rs` at byte `off` to LDS at dst + 16 lane. Inline asm, for the builtin is taken to touch
-// any LDS, so that every LDS wait would wait for it too; it has no result register.
-__device__ __forceinline__ void dma16(const v4i rs, uint32_t off, uint8_t* lds) {
+// 16 bytes a lane from the buffer `rs` at byte off[i] to LDS at dst + 1024 i + 16 lane. Inline asm, for the builtin is taken to
+// touch any LDS, so that every LDS wait would wait for it too; it has no result register. One block for all of a wave's
+// loads: m0, which says where they go, is the compiler's before and after.
+template <int N>
+__device__ __forceinline__ void dma16(const v4i rs, const uint32_t (&off)[N], uint8_t* lds) {
+  static_assert(N == 2 || N == 4 || N == 8, "loads of a wave");
   uint32_t keep;
   const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)lds);
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
-               "s_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(off), "s"(rs), "s"(dst) : "memory");
+#define LBW_NEXT "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+#define LBW_LOAD(i) "buffer_load_dwordx4 %" #i ", %1, 0 offen lds\n\t"
+  if constexpr (N == 2) {
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t" LBW_LOAD(3) LBW_NEXT LBW_LOAD(4) "s_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(rs), "s"(dst), "v"(off[0]), "v"(off[1]) : "memory", "scc");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t" LBW_LOAD(3) LBW_NEXT LBW_LOAD(4) LBW_NEXT LBW_LOAD(5)
+                   LBW_NEXT LBW_LOAD(6) "s_mov_b32 m0, %0"
+                   : "=&s"(keep)
+                   : "s"(rs), "s"(dst + i * 1024), "v"(off[i]), "v"(off[i + 1]), "v"(off[i + 2]), "v"(off[i + 3])
+                   : "memory", "scc");
+  }
+#undef LBW_NEXT
+#undef LBW_LOAD
 }
 __device__ __forceinline__ void wait_dma() { __builtin_amdgcn_s_waitcnt(0x0F70); }   // vmcnt(0) alone
+// Until all but the last `ahead` (0 .. 2) tiles' loads are done, of PER loads each (memory reads return in order).
+template <int PER>
+__device__ __forceinline__ void wait_dma_but(int ahead) {
+  constexpr auto imm = [](int n) { return 0x0F70 | (n & 15) | (n >> 4) << 14; };
+  static_assert(2 * PER < 64, "vmcnt counts to 63");
+  if (ahead >= 2) __builtin_amdgcn_s_waitcnt(imm(2 * PER));
+  else if (ahead == 1) __builtin_amdgcn_s_waitcnt(imm(PER));
+  else __builtin_amdgcn_s_waitcnt(imm(0));
+}
 
 // Rows of a tensor's head from `base` on, a row every `stride` elements, `left` of them: the resource of one tile of R rows
 // ends with the last row that there is.
@@ -103,8 +139,7 @@ struct Loader {
     }
   }
   __device__ __forceinline__ void issue(const v4i rs, int w, uint8_t* lds) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) dma16(rs, off[i], lds + (w * N + i) * 1024);
+    dma16<N>(rs, off, lds + w * N * 1024);
   }
 };
 
@@ -158,6 +193,13 @@ __device__ __forceinline__ void load_rows(const uint16_t* base, int64_t stride, 
   for (int st = 0; st < DH / 16; ++st) f[st] = r < left ? *(const v4i*)(p + 16 * st) : v4i{0, 0, 0, 0};
 }
 
+// The values are there from here on: used in a loop that waits for its own loads by count, they must not be waited for again.
+template <int N>
+__device__ __forceinline__ void arrived(v4i (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 // The 32 columns that a wave holds of a result turned (lane l: column l & 31, values i of channel tile mt are channels
 // 32 mt + 8 (i >> 2) + 4 (l >> 5) + (i & 3)), times `scale`, as rows of the 16-bit type: through the wave's own part of LDS
 // (32 rows of 16 bytes more than a row) to whole rows in memory. Rows from `left` on are not written. REST: what the rounding
@@ -203,7 +245,7 @@ __device__ __forceinline__ void dma4(const float* p, int left, uint32_t off, uin
 
 struct Shape {
   int64_t seqs, q_rows, k_rows;
-  int q_heads, k_heads, group;
+  int q_heads, k_heads, group, common;   // common: xcd_common
   const int32_t *starts, *k_starts;
   int causal;
   float scale, sl2;   // sm_scale, and times log2(e)

@@ -73,6 +73,12 @@ struct Range {
   }
 };
 
+// log2 of a weight, as it is held (LIFT): s sl2 - lse.
+template <bool F16>
+__device__ __forceinline__ float weight_exponent(float s, float sl2, float lse) {
+  return F16 ? fmaf(s, sl2, LIFT<F16> - lse) : fmaf(s, sl2, -lse);
+}
+
 template <int MT>
 __device__ __forceinline__ void times(v16f (&o)[MT], float by) {
 #pragma unroll
@@ -89,19 +95,36 @@ __device__ __forceinline__ void pack16(const v16f& x, float scale, v4i (&f)[2]) 
     for (int e = 0; e < 4; ++e) f[u][e] = (int)pack<F16>(x[8 * u + 2 * e] * scale, x[8 * u + 2 * e + 1] * scale);
 }
 
+// c plus the two values of a word.
+template <bool F16>
+__device__ __forceinline__ float dot_ones(uint32_t w, float c) {
+  if constexpr (F16) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{(_Float16)1.f, (_Float16)1.f}, c, false);
+  } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.f, (__bf16)1.f}, c, false);
+  }
+}
+
 // ---------------------------------------------------------------- dK, dV
 
-constexpr int QR = 64;   // queries of a stage
-
-template <int DH, bool F16>
+// A workgroup takes 32 KW keys, 32 a wave, and its QW = 4 / KW waves of the same keys take every QW-th 32 queries, their sums
+// added at the end: with 128 keys a stage's queries serve four waves, with 32 there are four times as many workgroups, each a
+// quarter as long.
+template <int DH, bool F16, int KW>
 __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(BwdArgs a) {
-  constexpr int NS = DH / 16, MT = DH / 32, KT = 32 * WAVES, TILE = QR * row_bytes<DH>, STAGE = 2 * TILE + 2 * QR * 4;
-  constexpr int LDS = 2 * STAGE > WAVES * STAGING<DH> ? 2 * STAGE : WAVES * STAGING<DH>;
+  constexpr int QW = WAVES / KW, QR = QW == 4 ? 128 : 64, SUB = QR / 32 / QW;   // queries of a stage; 32s of a wave in it
+  constexpr int NS = DH / 16, MT = DH / 32, KT = 32 * KW, TILE = QR * row_bytes<DH>, STAGE = 2 * TILE + 2 * QR * 4;
+  // (the loads of a stage take longer than its products where memory is far: three stages ahead, where they fit)
+  constexpr int STAGES = STAGE > 40000 ? 2 : 4;
+  constexpr int SUMS = (WAVES - KW) * 2 * MT * 16 * 64 * 4;   // LDS bytes of the sums of all waves but the first of each 32 keys
+  constexpr int LDS = std::max(std::max(STAGES * STAGE, WAVES * STAGING<DH>), SUMS);
   __shared__ __align__(16) uint8_t lds[LDS];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = w % KW, qw = w / KW;
   uint32_t head, tile;
-  head_tile(group_id(), a.s.k_heads, head, tile);
+  head_tile(group_id(), a.s.k_heads, 1, a.s.common, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.k_heads * DH;
   zero_outside(a.s.k_starts, a.s.seqs, a.s.k_rows, a.dk + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
@@ -110,7 +133,7 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   if (at.seq < 0) return;
   const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
   const int n = qs.n, m = ks.n, shift = m - n;
-  const int k0 = at.tile * KT, key0 = k0 + 32 * w, key = key0 + (lane & 31);   // (the first keys have the most queries)
+  const int k0 = at.tile * KT, key0 = k0 + 32 * kw, key = key0 + (lane & 31);   // (the first keys have the most queries)
   // the first query that sees a key, and the stage it lies in
   const auto first = [&](int j) { return a.s.causal ? max(0, j - shift) : 0; };
   const int q_stage = first(k0) / QR, stages = max(0, (n + QR - 1) / QR - q_stage);
@@ -122,13 +145,33 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   Loader<DH, QR, WAVES> ql, dl;
   ql.init(w, lane, a.q_tok);
   dl.init(w, lane, a.do_tok);
+  arrived(kf);
+  arrived(vf);
   const int steps = stages * a.s.group;
-  const auto issue = [&](int g, int r, int stage) {
+  // What is loaded next: a head's queries from r on. Pointers that move on by a stage: made from the numbers each time, the
+  // scalar unit would take as long as the products.
+  const uint16_t *q_next, *d_next;
+  const float* stat_next;
+  int g_next = 0, r_next;
+  const auto head_from = [&](int g) {
     const int64_t h = (int64_t)head * a.s.group + g;
+    r_next = q_stage * QR;
+    q_next = a.q + (qs.first + r_next) * a.q_tok + h * a.q_head;
+    d_next = a.dout + (qs.first + r_next) * a.do_tok + h * a.do_head;
+    stat_next = (w < QR / 64 ? a.lse : a.delta) + h * a.s.q_rows + qs.first + r_next + w % (QR / 64) * 64;
+  };
+  head_from(0);
+  const auto issue = [&](int stage) {
     uint8_t* to = lds + stage * STAGE;
-    ql.issue(rows_buffer<DH>(a.q + (qs.first + r) * a.q_tok + h * a.q_head, a.q_tok, n - r, QR), w, to);
-    dl.issue(rows_buffer<DH>(a.dout + (qs.first + r) * a.do_tok + h * a.do_head, a.do_tok, n - r, QR), w, to + TILE);
-    if (w < 2) dma4((w ? a.delta : a.lse) + h * a.s.q_rows + qs.first + r, n - r, lane * 4, to + 2 * TILE + w * QR * 4);
+    ql.issue(rows_buffer<DH>(q_next, a.q_tok, n - r_next, QR), w, to);
+    dl.issue(rows_buffer<DH>(d_next, a.do_tok, n - r_next, QR), w, to + TILE);
+    // (64 values a wave: of the sums first, then of D)
+    if (w < 2 * QR / 64) dma4(stat_next, n - r_next - w % (QR / 64) * 64, lane * 4, to + 2 * TILE + w * 256);
+    r_next += QR;
+    q_next += QR * a.q_tok;
+    d_next += QR * a.do_tok;
+    stat_next += QR;
+    if (r_next >= n) head_from(++g_next);
   };
   RowReads<DH> rr;
   TurnedReads<DH> tr;
@@ -139,27 +182,47 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   for (int mt = 0; mt < MT; ++mt) dk[mt] = dv[mt] = zeros16();
   Range range;
 
-  if (steps > 0) issue(0, q_stage * QR, 0);
-  for (int step = 0, g = 0, r0 = q_stage * QR; step < steps; ++step) {
-    const int stage = step & 1, here = r0;
-    const uint8_t *qt = lds + stage * STAGE, *dt = qt + TILE;
-    wait_dma();
-    __syncthreads();
-    r0 += QR;
-    if (r0 >= n) {   // the next head's queries
-      r0 = q_stage * QR;
-      ++g;
+  // The sums stay in the accumulation registers: the compiler would move them to the others and back, 256 moves a step.
+  const auto stay = [&] {
+    if constexpr (DH == 128) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+a"(dk[mt]), "+a"(dv[mt]));
     }
-    if (step + 1 < steps) issue(g, r0, 1 - stage);
+  };
+  for (int i = 0; i < min(STAGES - 1, steps); ++i) issue(i);
+  for (int step = 0, here = q_stage * QR; step < steps; ++step, here = here + QR < n ? here + QR : q_stage * QR) {
+    const int stage = step % STAGES;
+    const uint8_t *qt = lds + stage * STAGE, *dt = qt + TILE;
+    stay();
+    const int ahead = min(STAGES - 2, steps - 1 - step);
+    if (w < 2 * QR / 64) wait_dma_but<2 * Loader<DH, QR, WAVES>::N + 1>(ahead);
+    else wait_dma_but<2 * Loader<DH, QR, WAVES>::N>(ahead);
+    __syncthreads();   // the stage is in LDS, and every wave is done with the one before it
+    if (step + STAGES - 1 < steps) issue((step + STAGES - 1) % STAGES);
 #pragma unroll 1
-    for (int x = 0; x < QR / 32; ++x) {
-      const int r = here + 32 * x;
+    for (int i32 = 0; i32 < SUB; ++i32) {
+      const int x = i32 * QW + qw, r = here + 32 * x;
       if (r >= n || r + 31 < w_first) continue;
+      // (reads in one go ahead of the products that use them: the compiler would wait for each by itself)
       v16f s = zeros16(), dp = zeros16();
+      v4i qa[NS], da[NS];
 #pragma unroll
-      for (int st = 0; st < NS; ++st) s = mfma<F16>(rr.get(qt, x, st), kf[st], s);
+      for (int st = 0; st < NS; ++st) {
+        qa[st] = rr.get(qt, x, st);
+        da[st] = rr.get(dt, x, st);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int st = 0; st < NS; ++st) dp = mfma<F16>(rr.get(dt, x, st), vf[st], dp);
+      for (int st = 0; st < NS; ++st) {
+        s = mfma<F16>(qa[st], kf[st], s);
+        dp = mfma<F16>(da[st], vf[st], dp);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      v4i td[2][MT], tq[2][MT];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) td[u][mt] = tr.get(dt, 2 * x + u, mt);
       const float* stats = (const float*)(qt + 2 * TILE) + 32 * x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -167,11 +230,16 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
         const float le[4] = {l.x, l.y, l.z, l.w}, de[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[4 * i + e], a.s.sl2, LIFT<F16> - le[e]));
-          if (r < w_all) p = r + 8 * i + 4 * hf + e >= own ? p : 0.f;
+          const float p = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[4 * i + e], a.s.sl2, le[e]));
           s[4 * i + e] = p;
-          dp[4 * i + e] = p == 0.f ? 0.f : p * (dp[4 * i + e] - de[e]);
+          dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
         }
+      }
+      if (r < w_all) {   // queries that do not see a key
+        branch_here();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (r + 8 * (i >> 2) + 4 * hf + (i & 3) < own) s[i] = dp[i] = 0.f;
       }
       v4i pf[2], df[2];
       pack16<F16>(s, 1.f, pf);
@@ -183,34 +251,75 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          dv[mt] = mfma<F16>(tr.get(dt, 2 * x + u, mt), pf[u], dv[mt]);
-          dk[mt] = mfma<F16>(tr.get(qt, 2 * x + u, mt), df[u], dk[mt]);
+        for (int mt = 0; mt < MT; ++mt) tq[u][mt] = tr.get(qt, 2 * x + u, mt);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) dv[mt] = mfma<F16>(td[u][mt], pf[u], dv[mt]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], df[u], dk[mt]);
+    }
+    stay();
+  }
+  __syncthreads();
+  const float lift = __builtin_amdgcn_exp2f(-LIFT<F16>);
+  float k_by = a.s.scale * lift / range.scale;
+  if constexpr (QW > 1) {   // the sums of the other waves of these keys, in their order
+    float* sums = (float*)lds + lane;
+    if (qw) {
+      float* mine = sums + (w - KW) * (2 * MT * 16 * 64);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          mine[(mt * 16 + i) * 64] = dk[mt][i] * k_by;
+          mine[((MT + mt) * 16 + i) * 64] = dv[mt][i];
+        }
+    }
+    __syncthreads();
+    if (qw) return;
+    times(dk, k_by);
+    k_by = 1.f;
+    for (int q = 1; q < QW; ++q) {
+      const float* other = sums + (q * KW + kw - KW) * (2 * MT * 16 * 64);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          dk[mt][i] += other[(mt * 16 + i) * 64];
+          dv[mt][i] += other[((MT + mt) * 16 + i) * 64];
         }
     }
   }
-  __syncthreads();
   if (key0 >= m) return;
-  const float lift = __builtin_amdgcn_exp2f(-LIFT<F16>);
-  uint8_t* mine = lds + w * STAGING<DH>;
-  store_turned<DH, F16>(dk, a.s.scale * lift / range.scale, mine, lane, a.dk + (ks.first + key0) * o_tok + head * DH, o_tok, m - key0);
+  // (staged where no other wave may still be reading: of the sums, those that it has read itself)
+  static_assert(STAGING<DH> <= 2 * MT * 16 * 64 * 4, "a wave's staging lies inside the sums it reads");
+  uint8_t* mine = lds + (QW > 1 ? kw * (2 * MT * 16 * 64 * 4) : w * STAGING<DH>);
+  store_turned<DH, F16>(dk, k_by, mine, lane, a.dk + (ks.first + key0) * o_tok + head * DH, o_tok, m - key0);
   __builtin_amdgcn_wave_barrier();
   store_turned<DH, F16>(dv, lift, mine, lane, a.dv + (ks.first + key0) * o_tok + head * DH, o_tok, m - key0);
 }
 
 // ---------------------------------------------------------------- dQ
 
-constexpr int KT = 64, QT = 32 * WAVES;
+constexpr int KT = 64;
 
-template <int DH, bool F16>
+// QW and the waves that share queries as in the forward.
+template <int DH, bool F16, int QW>
 __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
+  constexpr int KW = WAVES / QW, QT = 32 * QW;
+  static_assert(KW == 1 || KW == 2, "a tile has 64 keys");
   constexpr int NS = DH / 16, MT = DH / 32, TILE = KT * row_bytes<DH>, STAGE = 2 * TILE;
-  constexpr int LDS = 2 * STAGE > WAVES * STAGING<DH> ? 2 * STAGE : WAVES * STAGING<DH>;
+  constexpr int SUMS = KW > 1 ? QW * (MT * 16 + 1) * 256 : 0;
+  constexpr int LDS = std::max(2 * STAGE, std::max(WAVES * STAGING<DH>, SUMS));
   __shared__ __align__(16) uint8_t lds[LDS];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = w % QW, kw = w / QW;
   uint32_t head, tile;
-  head_tile(group_id(), a.s.q_heads, head, tile);
+  head_tile(group_id(), a.s.k_heads, a.s.group, a.s.common, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.q_heads * DH;
   zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.dq + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
@@ -219,7 +328,7 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
   const int n = qs.n, m = ks.n, shift = m - n;
   const int q0 = (at.tiles - 1 - at.tile) * QT;
-  const int row0 = q0 + 32 * w, row = row0 + (lane & 31);
+  const int row0 = q0 + 32 * qw, row = row0 + (lane & 31);
   const auto seen = [&](int r) { return a.s.causal ? max(0, min(m, min(r, n - 1) + shift + 1)) : m; };
   const int upto = seen(q0 + QT - 1), w_upto = row0 < n ? seen(row0 + 31) : 0, w_first = seen(row0), own = seen(row);
   const int tiles = (upto + KT - 1) / KT;
@@ -229,17 +338,23 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   Loader<DH, KT, WAVES> kl, vl;
   kl.init(w, lane, a.k_tok);
   vl.init(w, lane, a.v_tok);
-  const auto issue = [&](int t, int stage) {
-    const int64_t r = (int64_t)t * KT;
-    kl.issue(rows_buffer<DH>(kb + r * a.k_tok, a.k_tok, m - t * KT, KT), w, lds + stage * STAGE);
-    vl.issue(rows_buffer<DH>(vb + r * a.v_tok, a.v_tok, m - t * KT, KT), w, lds + stage * STAGE + TILE);
+  int left = m;
+  const auto issue = [&](int stage) {   // the next tile
+    kl.issue(rows_buffer<DH>(kb, a.k_tok, left, KT), w, lds + stage * STAGE);
+    vl.issue(rows_buffer<DH>(vb, a.v_tok, left, KT), w, lds + stage * STAGE + TILE);
+    kb += KT * a.k_tok;
+    vb += KT * a.v_tok;
+    left -= KT;
   };
-  if (tiles > 0) issue(0, 0);
+  if (tiles > 0) issue(0);
   v4i qf[NS], df[NS];
   load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, lane, qf);
   load_rows<DH>(a.dout + (qs.first + row0) * a.do_tok + head * a.do_head, a.do_tok, n - row0, lane, df);
   const int64_t stat = (int64_t)head * a.s.q_rows + qs.first + row;
-  const float lse = row < n ? a.lse[stat] : INFINITY, delta = row < n ? a.delta[stat] : 0.f;
+  float lse = row < n ? a.lse[stat] : INFINITY, delta = row < n ? a.delta[stat] : 0.f;
+  arrived(qf);
+  arrived(df);
+  asm volatile("" : "+v"(lse), "+v"(delta));
   RowReads<DH> rr;
   TurnedReads<DH> tr;
   rr.init(lane);
@@ -248,45 +363,104 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) dq[mt] = zeros16();
   Range range;
+  float eps = 0.f;   // sum of the lane's dS as rounded, times range.scale
 
   for (int t = 0; t < tiles; ++t) {
     const int stage = t & 1;
     const uint8_t *kt = lds + stage * STAGE, *vt = kt + TILE;
     wait_dma();
     __syncthreads();
-    if (t + 1 < tiles) issue(t + 1, 1 - stage);
+    if (t + 1 < tiles) issue(1 - stage);
 #pragma unroll 1
-    for (int x = 0; x < KT / 32; ++x) {
+    for (int x = kw; x < KT / 32; x += KW) {
       const int j0 = t * KT + 32 * x;
       if (j0 >= w_upto) continue;
       v16f s = zeros16(), dp = zeros16();
 #pragma unroll
-      for (int st = 0; st < NS; ++st) s = mfma<F16>(rr.get(kt, x, st), qf[st], s);
+      for (int st = 0; st < NS; ++st) {
+        s = mfma<F16>(rr.get(kt, x, st), qf[st], s);
+        dp = mfma<F16>(rr.get(vt, x, st), df[st], dp);
+      }
 #pragma unroll
-      for (int st = 0; st < NS; ++st) dp = mfma<F16>(rr.get(vt, x, st), df[st], dp);
-      const bool whole = j0 + 32 <= w_first;
+      for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[i], a.s.sl2, lse)) * (dp[i] - delta);
+      if (j0 + 32 > w_first) {   // keys that a query does not see
+        branch_here();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.s.sl2, LIFT<F16> - lse));
-        if (!whole) p = j0 + 8 * (i >> 2) + 4 * hf + (i & 3) < own ? p : 0.f;
-        dp[i] = p == 0.f ? 0.f : p * (dp[i] - delta);
+        for (int i = 0; i < 16; ++i)
+          if (j0 + 8 * (i >> 2) + 4 * hf + (i & 3) >= own) dp[i] = 0.f;
       }
       v4i pf[2];
       float by;
       if constexpr (F16) {
-        if (range.fit(dp, by)) times(dq, by);
+        if (range.fit(dp, by)) {
+          times(dq, by);
+          eps *= by;
+        }
       }
       pack16<F16>(dp, range.scale, pf);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) eps = dot_ones<F16>(pf[u][e], eps);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tr.get(kt, 2 * x + u, mt), pf[u], dq[mt]);
     }
   }
+  // dS adds up to zero over a query's keys; what the rounded values add up to is error, and where keys have a part in common
+  // (a mean that is not zero) all of it goes the same way. It is taken off over the keys of the last whole tile, evenly: dQ of
+  // keys with a mean of half their deviation 1.42 times the plain error of its own rounding, without this 1.53.
+  eps = sum_xor32(eps);
+  if constexpr (KW > 1) {   // the same of the wave of the other keys, at the smaller of their factors
+    __shared__ float other[QW * 64 * 2];
+    float* at = other + (qw * 64 + lane) * 2;
+    if (kw) at[0] = eps, at[1] = !F16 || range.set ? range.scale : INFINITY;
+    __syncthreads();
+    if (!kw) {
+      if constexpr (F16) {
+        const float both = fminf(range.set ? range.scale : INFINITY, at[1]), next = both < INFINITY ? both : 1.f;
+        times(dq, next / range.scale);
+        eps = eps * (next / range.scale) + (at[1] < INFINITY ? at[0] * (next / at[1]) : 0.f);
+        range.scale = next;
+      } else {
+        eps += at[0];
+      }
+    }
+  }
+  float by = a.s.scale * __builtin_amdgcn_exp2f(-LIFT<F16>) / range.scale;
+  const int last = tiles > 0 && m - (tiles - 1) * KT < KT / 2 ? tiles - 2 : tiles - 1, held = min(m - last * KT, KT);
+  if (kw == 0 && last >= 0 && held >= KT / 2) {
+    const float off = -eps / (float)held;
+    v4i f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = (int)pack<F16>(off, off);   // (keys that are not there are zeros)
+    const uint8_t* kt = lds + (last & 1) * STAGE;
+#pragma unroll
+    for (int u = 0; u < KT / 16; ++u)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tr.get(kt, u, mt), f, dq[mt]);
+  }
   __syncthreads();
+  if constexpr (KW > 1) {
+    float* other = (float*)lds + qw * (MT * 16) * 64 + lane;
+    if (kw) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) other[(mt * 16 + i) * 64] = dq[mt][i] * by;
+    }
+    __syncthreads();
+    if (kw) return;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dq[mt][i] = fmaf(dq[mt][i], by, other[(mt * 16 + i) * 64]);
+    by = 1.f;
+  }
   if (row0 >= n) return;
-  const float lift = __builtin_amdgcn_exp2f(-LIFT<F16>);
-  store_turned<DH, F16>(dq, a.s.scale * lift / range.scale, lds + w * STAGING<DH>, lane, a.dq + (qs.first + row0) * o_tok + head * DH,
+  static_assert(KW == 1 || STAGING<DH> <= MT * 16 * 256, "a wave's staging lies inside what it reads");
+  store_turned<DH, F16>(dq, by, lds + (KW > 1 ? qw * MT * 16 * 256 : w * STAGING<DH>), lane, a.dq + (qs.first + row0) * o_tok + head * DH,
                         o_tok, n - row0);
 }
 
@@ -295,12 +469,21 @@ void launch(BwdArgs a, hipStream_t stream) {
   const int64_t rows = a.s.q_rows * a.s.q_heads;
   packed_delta_kernel<DH, F16><<<grid_of((rows * (DH / 8) + THREADS - 1) / THREADS), THREADS, 0, stream>>>(a);
   if (a.dk) {
-    a.tiles = (uint32_t)places_of(a.s.k_rows, a.s.seqs, 32 * WAVES);
-    packed_dkv_kernel<DH, F16><<<grid_of((int64_t)a.tiles * a.s.k_heads), THREADS, 0, stream>>>(a);
+    // as many keys a workgroup as leave two for every CU
+    const auto groups = [&](int keys) { return xcd_groups(places_of(a.s.k_rows, a.s.seqs, keys), a.s.k_heads, 1); };
+    const int keys = groups(128) >= 512 ? 128 : groups(64) >= 512 ? 64 : 32;
+    a.tiles = (uint32_t)places_of(a.s.k_rows, a.s.seqs, keys);
+    const dim3 grid = grid_of(groups(keys));
+    if (keys == 128) packed_dkv_kernel<DH, F16, 4><<<grid, THREADS, 0, stream>>>(a);
+    else if (keys == 64) packed_dkv_kernel<DH, F16, 2><<<grid, THREADS, 0, stream>>>(a);
+    else packed_dkv_kernel<DH, F16, 1><<<grid, THREADS, 0, stream>>>(a);
   }
   if (a.dq) {
-    a.tiles = (uint32_t)places_of(a.s.q_rows, a.s.seqs, QT);
-    packed_dq_kernel<DH, F16><<<grid_of((int64_t)a.tiles * a.s.q_heads), THREADS, 0, stream>>>(a);
+    const auto groups = [&](int queries) { return xcd_groups(places_of(a.s.q_rows, a.s.seqs, queries), a.s.k_heads, a.s.group); };
+    const bool wide = groups(128) >= 512;   // (two a CU)
+    a.tiles = (uint32_t)places_of(a.s.q_rows, a.s.seqs, wide ? 128 : 64);
+    if (wide) packed_dq_kernel<DH, F16, 4><<<grid_of(groups(128)), THREADS, 0, stream>>>(a);
+    else packed_dq_kernel<DH, F16, 2><<<grid_of(groups(64)), THREADS, 0, stream>>>(a);
   }
 }
 
@@ -329,11 +512,11 @@ extern "C" int lbw_packed_attn_bwd(const void* d_out, const void* out, const voi
   for (const void* p : {out, rest, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)workspace})
     if ((uintptr_t)p % 16) return LBW_E_ALIGN;
   if ((uintptr_t)starts % 4 || (uintptr_t)k_starts % 4 || (uintptr_t)lse % 4) return LBW_E_ALIGN;
-  if (k_rows < 1 || places_of(q_rows, seqs, packed::QT) * q_heads > 1 << 30 || places_of(k_rows, seqs, 32 * packed::WAVES) * k_heads > 1 << 30 ||
+  if (k_rows < 1 || (places_of(q_rows, seqs, 64) + 8) * q_heads > 1 << 30 || (places_of(k_rows, seqs, 32) + 8) * k_heads > 1 << 30 ||
       q_rows * q_heads * dim / 8 / packed::THREADS > 1 << 30)
     return LBW_E_SHAPE;
   if (const int st = check_device()) return st;
-  packed::BwdArgs a = {{seqs, q_rows, k_rows, (int)q_heads, (int)k_heads, (int)(q_heads / k_heads), starts, k_starts, causal,
+  packed::BwdArgs a = {{seqs, q_rows, k_rows, (int)q_heads, (int)k_heads, (int)(q_heads / k_heads), (int)packed::xcd_common(k_heads), starts, k_starts, causal,
                         sm_scale, sm_scale * packed::LOG2E},
                        (const uint16_t*)d_out, (const uint16_t*)out, (const uint16_t*)rest, (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v,
                        do_s_tok, do_s_head, q_s_tok, q_s_head, k_s_tok, k_s_head, v_s_tok, v_s_head, lse, (float*)workspace,

@@ -574,3 +574,33 @@ def test_norm_rotary_weights_of_a_larger_buffer(dtype):
             (y, mag), grads = causal.norm_rotary(q, flat[part], torch.arange(5, 14, device=DEV), plan.freq, d=dy)
             _within(out[i].detach(), y, 36 * E * mag, f"at {at}")
             _within(got[part], grads["weight"][0], 256 * E * grads["weight"][1], f"dw at {at}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,lens", [([200], [200]), ([97], [161]), ([33, 0, 64, 31], [40, 7, 96, 95]), ([500, 3, 160], [10, 3, 161]),
+                                      ([64, 64], [64, 63]), ([32, 96], [0, 5000])])
+def test_cache_write_and_read_blocks(new, lens, d):
+    """Prompts: blocks of 32 tokens, whole and cut, tokens before the first and past the table, what lies beside them untouched."""
+    from lingbot_world_v2_realtime_amd import KV4Cache
+    g = _gen(sum(new) + d)
+    heads, pages = 3, 16
+    st, rows = _starts(new, 3), 3 + sum(new) + 5
+    table = _table(g, [min(4, -(-n // 64)) for n in lens], pages, 4)
+    table[0][1] = 77
+    k, v = (_rand(g, rows, heads, d, std=2.0, dtype=torch.bfloat16) for _ in range(2))
+    cache = _filled(g, pages, heads, d)
+    before = causal.unpack_pages(cache.k[0], cache.k_scale[0], cache.v[0], cache.v_scale[0])
+    args = (_dev(table), _dev(lens), _dev(st))
+    cache.write(0, k, v, *args)
+    at = causal.slots(st, lens, table, rows, pages)
+    after = causal.unpack_pages(cache.k[0], cache.k_scale[0], cache.v[0], cache.v_scale[0])
+    got = cache.read(0, *args, tokens=rows)
+    for x, old, now, r in zip((k, v), before, after, got):
+        value = causal.values(*causal.encode(x))
+        for i, slot in enumerate(at):
+            if slot is None:
+                assert not r[i].any(), i
+            else:
+                old[slot[0], :, slot[1]] = value[i]
+                assert torch.equal(r[i].double(), value[i]), i
+        assert torch.equal(old, now)
