@@ -95,6 +95,20 @@ __device__ __forceinline__ void pack16(const v16f& x, float scale, v4i (&f)[2]) 
     for (int e = 0; e < 4; ++e) f[u][e] = (int)pack<F16>(x[8 * u + 2 * e] * scale, x[8 * u + 2 * e + 1] * scale);
 }
 
+// What that rounding took off, rounded.
+template <bool F16>
+__device__ __forceinline__ void pack16_rest(const v16f& x, float scale, const v4i (&f)[2], v4i (&rest)[2]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      rest[u][e] = (int)pack<F16>(fmaf(x[8 * u + 2 * e], scale, -lo16<F16>((uint32_t)f[u][e])), fmaf(x[8 * u + 2 * e + 1], scale, -hi16<F16>((uint32_t)f[u][e])));
+}
+// Sequences so short that the roundings of dS do not average out (a gradient of few terms whose sum is smaller than they are:
+// up to twice the plain error): dS enters its products in two parts, each rounded, which costs a quarter more there and
+// nothing elsewhere.
+constexpr int SHORT = 128;
+
 // c plus the two values of a word.
 template <bool F16>
 __device__ __forceinline__ float dot_ones(uint32_t w, float c) {
@@ -138,6 +152,7 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   const auto first = [&](int j) { return a.s.causal ? max(0, j - shift) : 0; };
   const int q_stage = first(k0) / QR, stages = max(0, (n + QR - 1) / QR - q_stage);
   const int own = first(key), w_first = first(key0), w_all = first(key0 + 31);
+  const bool fine = min(n, m) <= SHORT;
 
   v4i kf[NS], vf[NS];
   load_rows<DH>(a.k + (ks.first + key0) * a.k_tok + head * a.k_head, a.k_tok, m - key0, lane, kf);
@@ -261,6 +276,15 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], df[u], dk[mt]);
+      if (fine) {
+        branch_here();
+        v4i rest[2];
+        pack16_rest<F16>(dp, range.scale, df, rest);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], rest[u], dk[mt]);
+      }
     }
     stay();
   }
@@ -362,6 +386,7 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   v16f dq[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) dq[mt] = zeros16();
+  const bool fine = min(n, m) <= SHORT;
   Range range;
   float eps = 0.f;   // sum of the lane's dS as rounded, times range.scale
 
@@ -406,10 +431,22 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tr.get(kt, 2 * x + u, mt), pf[u], dq[mt]);
+      if (fine) {
+        branch_here();
+        v4i rest[2];
+        pack16_rest<F16>(dp, range.scale, pf, rest);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) eps = dot_ones<F16>(rest[u][e], eps);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tr.get(kt, 2 * x + u, mt), rest[u], dq[mt]);
+        }
+      }
     }
   }
   // dS adds up to zero over a query's keys; what the rounded values add up to is error, and where keys have a part in common
-  // (a mean that is not zero) all of it goes the same way. It is taken off over the keys of the last whole tile, evenly: dQ of
+  // (a mean that is not zero) all of it goes the same way. It is taken off over the keys of the last tile (or the one before), evenly: dQ of
   // keys with a mean of half their deviation 1.42 times the plain error of its own rounding, without this 1.53.
   eps = sum_xor32(eps);
   if constexpr (KW > 1) {   // the same of the wave of the other keys, at the smaller of their factors
@@ -429,9 +466,10 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
     }
   }
   float by = a.s.scale * __builtin_amdgcn_exp2f(-LIFT<F16>) / range.scale;
-  const int last = tiles > 0 && m - (tiles - 1) * KT < KT / 2 ? tiles - 2 : tiles - 1, held = min(m - last * KT, KT);
-  if (kw == 0 && last >= 0 && held >= KT / 2) {
-    const float off = -eps / (float)held;
+  // Few keys say little of the mean: their part in it is taken less (by the 4 that half a deviation makes right).
+  const int last = tiles > 1 && m - (tiles - 1) * KT < KT / 2 ? tiles - 2 : tiles - 1, held = min(m - last * KT, KT);
+  if (kw == 0 && last >= 0) {
+    const float off = -eps / (float)(held + 4);
     v4i f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = (int)pack<F16>(off, off);   // (keys that are not there are zeros)
