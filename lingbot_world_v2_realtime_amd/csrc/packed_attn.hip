@@ -38,12 +38,11 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
   head_tile(group_id(), a.s.k_heads, a.s.group, a.s.common, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.q_heads * DH;
-  zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.out + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
-  const Place at = place(a.s.starts, a.s.seqs, a.s.q_rows, QT, tile);
+  const Where at = where(a.s.starts, a.s.k_starts, a.s.seqs, a.s.q_rows, a.s.k_rows, QT, tile);
+  zero_outside(at.begin, at.end, a.s.q_rows, a.out + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
   if (at.seq < 0) return;
-  const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
-  const int n = qs.n, m = ks.n, shift = m - n;
-  const int q0 = (at.tiles - 1 - at.tile) * QT;   // the tiles with the most keys first
+  const Span qs = at.own, ks = at.other;
+  const int n = qs.n, m = ks.n, shift = m - n, q0 = at.tile * QT;
   const int row0 = q0 + 32 * qw, row = row0 + (lane & 31);
   // keys that the tile's last query sees, and the wave's last and first
   const auto seen = [&](int r) { return a.s.causal ? max(0, min(m, min(r, n - 1) + shift + 1)) : m; };

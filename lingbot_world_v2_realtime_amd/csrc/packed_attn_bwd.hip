@@ -141,13 +141,13 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   head_tile(group_id(), a.s.k_heads, 1, a.s.common, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.k_heads * DH;
-  zero_outside(a.s.k_starts, a.s.seqs, a.s.k_rows, a.dk + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
-  zero_outside(a.s.k_starts, a.s.seqs, a.s.k_rows, a.dv + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
-  const Place at = place(a.s.k_starts, a.s.seqs, a.s.k_rows, KT, tile);
+  const Where at = where(a.s.k_starts, a.s.starts, a.s.seqs, a.s.k_rows, a.s.q_rows, KT, tile);
+  zero_outside(at.begin, at.end, a.s.k_rows, a.dk + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
+  zero_outside(at.begin, at.end, a.s.k_rows, a.dv + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
   if (at.seq < 0) return;
-  const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
+  const Span qs = at.other, ks = at.own;
   const int n = qs.n, m = ks.n, shift = m - n;
-  const int k0 = at.tile * KT, key0 = k0 + 32 * kw, key = key0 + (lane & 31);   // (the first keys have the most queries)
+  const int k0 = (at.tiles - 1 - at.tile) * KT, key0 = k0 + 32 * kw, key = key0 + (lane & 31);   // (the first keys have the most queries)
   // the first query that sees a key, and the stage it lies in
   const auto first = [&](int j) { return a.s.causal ? max(0, j - shift) : 0; };
   const int q_stage = first(k0) / QR, stages = max(0, (n + QR - 1) / QR - q_stage);
@@ -346,12 +346,11 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   head_tile(group_id(), a.s.k_heads, a.s.group, a.s.common, head, tile);
   if (tile >= a.tiles) return;
   const int64_t o_tok = (int64_t)a.s.q_heads * DH;
-  zero_outside(a.s.starts, a.s.seqs, a.s.q_rows, a.dq + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
-  const Place at = place(a.s.starts, a.s.seqs, a.s.q_rows, QT, tile);
+  const Where at = where(a.s.starts, a.s.k_starts, a.s.seqs, a.s.q_rows, a.s.k_rows, QT, tile);
+  zero_outside(at.begin, at.end, a.s.q_rows, a.dq + head * DH, o_tok, DH, tile, a.tiles, threadIdx.x, THREADS);
   if (at.seq < 0) return;
-  const Span qs = span(a.s.starts, at.seq, a.s.q_rows), ks = span(a.s.k_starts, at.seq, a.s.k_rows);
-  const int n = qs.n, m = ks.n, shift = m - n;
-  const int q0 = (at.tiles - 1 - at.tile) * QT;
+  const Span qs = at.own, ks = at.other;
+  const int n = qs.n, m = ks.n, shift = m - n, q0 = at.tile * QT;
   const int row0 = q0 + 32 * qw, row = row0 + (lane & 31);
   const auto seen = [&](int r) { return a.s.causal ? max(0, min(m, min(r, n - 1) + shift + 1)) : m; };
   const int upto = seen(q0 + QT - 1), w_upto = row0 < n ? seen(row0 + 31) : 0, w_first = seen(row0), own = seen(row);
