@@ -183,6 +183,51 @@ struct TurnedReads {
   }
 };
 
+// An infinity or NaN of a row that a column does not see must not reach it, but its weight of zero times either is NaN. So a
+// workgroup whose sums are not finite at its end (and whose columns do not all see the same) goes over its tiles once more,
+// and where a tile is partly seen takes such values out of the products (clean) and adds them, as they are, to the sums of
+// the columns that see them (add_odd). No other call pays for it, but for the look at the sums.
+__device__ __forceinline__ bool is_odd(float x) { return !(fabsf(x) < INFINITY); }
+template <int MT>
+__device__ __forceinline__ bool any_odd(const v16f (&o)[MT]) {
+  float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i & 3] = fmaf(o[mt][i], 0.f, z[i & 3]);
+  return __any(is_odd((z[0] + z[1]) + (z[2] + z[3])));
+}
+template <bool F16>
+__device__ __forceinline__ v4i clean(v4i f) {
+  constexpr uint32_t e = F16 ? 0x7C00 : 0x7F80;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = f[i];
+    f[i] = (w & e) == e ? w & 0xFFFF0000u : w;
+    f[i] = (w >> 16 & e) == e ? f[i] & 0xFFFF : f[i];
+  }
+  return f;
+}
+// Rows 32 x .. + 32 of a tile; sees(j): whether the lane's column sees row j of them.
+template <int DH, bool F16, class Sees>
+__device__ __forceinline__ void add_odd(v16f (&o)[DH / 32], const uint8_t* tile, int x, int hf, const Sees& sees) {
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) {
+    const uint8_t* row = tile + (32 * x + j) * row_bytes<DH>;
+    const bool s = sees(j);
+#pragma unroll
+    for (int mt = 0; mt < DH / 32; ++mt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint2 w = *(const uint2*)(row + (((4 * mt + c) ^ swizzle<DH>(j)) << 4) + 8 * hf);
+        const float v[4] = {lo16<F16>(w.x), hi16<F16>(w.x), lo16<F16>(w.y), hi16<F16>(w.y)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][4 * c + e] += s && is_odd(v[e]) ? v[e] : 0.f;
+        __builtin_amdgcn_sched_barrier(0);   // (few registers rather than speed)
+      }
+  }
+}
+
 // 32 rows of one wave straight into the lanes that a product's other operand wants them in: lane l, piece st holds the
 // channels 16 st + 8 (l >> 5) .. + 8 of row l & 31; rows that are not there are zero.
 template <int DH>

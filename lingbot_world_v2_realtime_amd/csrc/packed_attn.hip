@@ -25,13 +25,14 @@ struct FwdArgs {
 // QW waves side by side take 32 queries each; the 4 / QW that share queries take every (4 / QW)-th 32 keys, and join at the
 // end what each has: where 128 queries a workgroup would leave the card half empty, 64 make twice as many, half as long.
 template <int DH, bool F16, int QW>
-__global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_fwd_kernel(FwdArgs a) {
   constexpr int KW = WAVES / QW, QT = 32 * QW, XS = KT / 32 / KW;   // XS: 32 keys of a wave in a tile
   static_assert(KW == 1 || KW == 2, "a tile has 64 keys");
   constexpr int NS = DH / 16, MT = DH / 32, TILE = KT * row_bytes<DH>, STAGE = 2 * TILE;
   constexpr int SUMS = KW > 1 ? QW * (MT * 16 + 2) * 256 : 0;   // LDS bytes of what the second waves have
   constexpr int LDS = std::max(2 * STAGE, std::max(WAVES * STAGING<DH>, SUMS));
   __shared__ __align__(16) uint8_t lds[LDS];
+  __shared__ int odd[WAVES];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = w % QW, kw = w / QW;
   uint32_t head, tile;
@@ -49,12 +50,16 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
   const int upto = seen(q0 + QT - 1), w_upto = row0 < n ? seen(row0 + 31) : 0, w_first = seen(row0), own = seen(row);
   const int tiles = (upto + KT - 1) / KT;
 
-  const uint16_t* kb = a.k + ks.first * a.k_tok + (head / a.s.group) * a.k_head;
-  const uint16_t* vb = a.v + ks.first * a.v_tok + (head / a.s.group) * a.v_head;
+  const uint16_t *kb, *vb;
+  int left;
+  const auto from_start = [&] {
+    kb = a.k + ks.first * a.k_tok + (head / a.s.group) * a.k_head;
+    vb = a.v + ks.first * a.v_tok + (head / a.s.group) * a.v_head;
+    left = m;
+  };
   Loader<DH, KT, WAVES> kl, vl;
   kl.init(w, lane, a.k_tok);
   vl.init(w, lane, a.v_tok);
-  int left = m;
   const auto issue = [&](int stage) {   // the next tile
     kl.issue(rows_buffer<DH>(kb, a.k_tok, left, KT), w, lds + stage * STAGE);
     vl.issue(rows_buffer<DH>(vb, a.v_tok, left, KT), w, lds + stage * STAGE + TILE);
@@ -62,6 +67,7 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
     vb += KT * a.v_tok;
     left -= KT;
   };
+  from_start();
   if (tiles > 0) issue(0);
   v4i qf[NS];
   load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, lane, qf);
@@ -72,43 +78,46 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
   vr.init(lane);
 
   v16f o[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) o[mt] = zeros16();
-  float top = -INFINITY, total = 0.f;
+  float top, total;
 
-  const auto step = [&](int t, auto stage) {
-    const uint8_t* kt = lds + decltype(stage)::value * STAGE;
-    const uint8_t* vt = kt + TILE;
+  const auto arrive = [&](int t, int stage) __attribute__((always_inline)) {
     wait_dma();
     __syncthreads();   // the tile is in LDS, and every wave is done with the other stage
-    if (t + 1 < tiles) issue(1 - decltype(stage)::value);
-    const int j0 = t * KT + 32 * XS * kw;   // the wave's keys of the tile
+    if (t + 1 < tiles) issue(1 - stage);
+  };
+  // XN times 32 keys of a tile, from the x0-th on
+  const auto work = [&](int t, int stage, int x0, auto xn, auto again, const RowReads<DH>& kr, const TurnedReads<DH>& vr, int hf, int own, const v4i (&qf)[NS]) __attribute__((always_inline)) {
+    constexpr int XN = decltype(xn)::value;
+    const uint8_t* kt = lds + stage * STAGE;
+    const uint8_t* vt = kt + TILE;
+    const int j0 = t * KT + 32 * x0;
     if (j0 >= w_upto) return;
     // (reads in one go ahead of the products that use them: the compiler would wait for each by itself)
-    v16f s[XS];
-    v4i kf[XS][NS];
+    v16f s[XN];
+    v4i kf[XN][NS];
 #pragma unroll
     for (int st = 0; st < NS; ++st)
 #pragma unroll
-      for (int x = 0; x < XS; ++x) kf[x][st] = kr.get(kt, XS * kw + x, st);
+      for (int x = 0; x < XN; ++x) kf[x][st] = kr.get(kt, x0 + x, st);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int x = 0; x < XS; ++x) s[x] = zeros16();
+    for (int x = 0; x < XN; ++x) s[x] = zeros16();
 #pragma unroll
     for (int st = 0; st < NS; ++st)
 #pragma unroll
-      for (int x = 0; x < XS; ++x) s[x] = mfma<F16>(kf[x][st], qf[st], s[x]);
-    if (j0 + 32 * XS > w_first) {   // keys that a query does not see
+      for (int x = 0; x < XN; ++x) s[x] = mfma<F16>(kf[x][st], qf[st], s[x]);
+    const bool partly = j0 + 32 * XN > w_first;   // keys that a query does not see
+    if (partly) {
       branch_here();
 #pragma unroll
-      for (int x = 0; x < XS; ++x)
+      for (int x = 0; x < XN; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (j0 + 32 * x + 8 * (i >> 2) + 4 * hf + (i & 3) >= own) s[x][i] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < XS; ++x)
+    for (int x = 0; x < XN; ++x)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
     mx = max_xor32(mx) * a.s.sl2;
@@ -124,10 +133,10 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
       top = next;
     }
     const float off = (top == -INFINITY ? 0.f : -top) + LIFT<F16>;
-    v4i pf[2 * XS];
+    v4i pf[2 * XN];
     float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < 2 * XS; ++u) {
+    for (int u = 0; u < 2 * XN; ++u) {
       float p[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + j], a.s.sl2, off));
@@ -135,19 +144,67 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
       pf[u] = v4i{(int)pack<F16>(p[0], p[1]), (int)pack<F16>(p[2], p[3]), (int)pack<F16>(p[4], p[5]), (int)pack<F16>(p[6], p[7])};
     }
     total += sum;
+    if (decltype(again)::value && partly) {
 #pragma unroll
-    for (int u = 0; u < 2 * XS; ++u)
+      for (int u = 0; u < 2 * XN; ++u)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) o[mt] = mfma<F16>(vr.get(vt, 2 * XS * kw + u, mt), pf[u], o[mt]);
+        for (int mt = 0; mt < MT; ++mt) {
+          o[mt] = mfma<F16>(clean<F16>(vr.get(vt, 2 * x0 + u, mt)), pf[u], o[mt]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      add_odd<DH, F16>(o, vt, x0, hf, [&](int j) { return j0 + j < own; });   // (XN is 1)
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * XN; ++u)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt] = mfma<F16>(vr.get(vt, 2 * x0 + u, mt), pf[u], o[mt]);
   };
+  const auto clear = [&] {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) o[mt] = zeros16();
+    top = -INFINITY, total = 0.f;
+  };
+  clear();
   for (int t = 0; t < tiles; t += 2) {
-    step(t, ic<0>{});
-    if (t + 1 < tiles) step(t + 1, ic<1>{});
+    arrive(t, 0);
+    work(t, 0, XS * kw, ic<XS>{}, ic<0>{}, kr, vr, hf, own, qf);
+    if (t + 1 < tiles) {
+      arrive(t + 1, 1);
+      work(t + 1, 1, XS * kw, ic<XS>{}, ic<0>{}, kr, vr, hf, own, qf);
+    }
+  }
+  // (the lane's number again, unknown to the compiler: what it makes of it is not held in registers all through the loop)
+  int late = threadIdx.x;
+  asm volatile("" : "+v"(late));
+  late &= 63;
+  const bool bad = any_odd(o);
+  if (late == 0) odd[w] = bad;
+  __syncthreads();   // every wave is done with the stages
+  if (__builtin_expect(a.s.causal && __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]), 0)) {
+    kr.init(late);
+    vr.init(late);
+    kl.init(w, late, a.k_tok);
+    vl.init(w, late, a.v_tok);
+    from_start();
+    issue(0);   // (there is a tile: without one the sums are zeros)
+    clear();
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      arrive(t, t & 1);
+#pragma unroll 1
+      for (int x = XS * kw; x < XS * (kw + 1); ++x) {
+        int l = late;
+        asm volatile("" : "+v"(l));
+        load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, l, qf);   // (read again rather than kept)
+        work(t, t & 1, x, ic<1>{}, ic<1>{}, kr, vr, l >> 5, seen(row0 + (l & 31)), qf);
+      }
+    }
+    __syncthreads();
   }
   total = sum_xor32(total);
-  __syncthreads();   // every wave is done with the stages
   if constexpr (KW > 1) {
-    float* other = (float*)lds + qw * (MT * 16 + 2) * 64 + lane;
+    float* other = (float*)lds + qw * (MT * 16 + 2) * 64 + late;
     if (kw) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -172,13 +229,13 @@ __global__ __launch_bounds__(THREADS, 2) void packed_fwd_kernel(FwdArgs a) {
   static_assert(KW == 1 || STAGING<DH> <= (MT * 16 + 2) * 256, "a wave's staging lies inside what it reads");
   uint8_t* mine = lds + (KW > 1 ? qw * (MT * 16 + 2) * 256 : w * STAGING<DH>);
   const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-  store_turned<DH, F16>(o, inv, mine, lane, a.out + (qs.first + row0) * o_tok + head * DH, o_tok, n - row0);
+  store_turned<DH, F16>(o, inv, mine, late, a.out + (qs.first + row0) * o_tok + head * DH, o_tok, n - row0);
   if (a.rest) {
     __builtin_amdgcn_wave_barrier();
-    store_turned<DH, F16, true>(o, inv, mine, lane, a.rest + (qs.first + row0) * o_tok + head * DH, o_tok, n - row0);
+    store_turned<DH, F16, true>(o, inv, mine, late, a.rest + (qs.first + row0) * o_tok + head * DH, o_tok, n - row0);
   }
-  if (a.lse && row < n && lane < 32)
-    a.lse[(int64_t)head * a.s.q_rows + qs.first + row] = own > 0 ? top + __builtin_amdgcn_logf(total) - LIFT<F16> : INFINITY;
+  if (const int row = row0 + late; a.lse && row < n && late < 32)
+    a.lse[(int64_t)head * a.s.q_rows + qs.first + row] = seen(row) > 0 ? top + __builtin_amdgcn_logf(total) - LIFT<F16> : INFINITY;
 }
 
 template <int DH, bool F16>

@@ -109,18 +109,6 @@ __device__ __forceinline__ void pack16_rest(const v16f& x, float scale, const v4
 // nothing elsewhere.
 constexpr int SHORT = 128;
 
-// c plus the two values of a word.
-template <bool F16>
-__device__ __forceinline__ float dot_ones(uint32_t w, float c) {
-  if constexpr (F16) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{(_Float16)1.f, (_Float16)1.f}, c, false);
-  } else {
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.f, (__bf16)1.f}, c, false);
-  }
-}
-
 // ---------------------------------------------------------------- dK, dV
 
 // A workgroup takes 32 KW keys, 32 a wave, and its QW = 4 / KW waves of the same keys take every QW-th 32 queries, their sums
@@ -135,6 +123,7 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   constexpr int SUMS = (WAVES - KW) * 2 * MT * 16 * 64 * 4;   // LDS bytes of the sums of all waves but the first of each 32 keys
   constexpr int LDS = std::max(std::max(STAGES * STAGE, WAVES * STAGING<DH>), SUMS);
   __shared__ __align__(16) uint8_t lds[LDS];
+  __shared__ int odd[WAVES];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = w % KW, qw = w / KW;
   uint32_t head, tile;
@@ -193,8 +182,6 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   rr.init(lane);
   tr.init(lane);
   v16f dk[MT], dv[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) dk[mt] = dv[mt] = zeros16();
   Range range;
 
   // The sums stay in the accumulation registers: the compiler would move them to the others and back, 256 moves a step.
@@ -204,91 +191,117 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
       for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+a"(dk[mt]), "+a"(dv[mt]));
     }
   };
-  for (int i = 0; i < min(STAGES - 1, steps); ++i) issue(i);
-  for (int step = 0, here = q_stage * QR; step < steps; ++step, here = here + QR < n ? here + QR : q_stage * QR) {
-    const int stage = step % STAGES;
-    const uint8_t *qt = lds + stage * STAGE, *dt = qt + TILE;
-    stay();
-    const int ahead = min(STAGES - 2, steps - 1 - step);
-    if (w < 2 * QR / 64) wait_dma_but<2 * Loader<DH, QR, WAVES>::N + 1>(ahead);
-    else wait_dma_but<2 * Loader<DH, QR, WAVES>::N>(ahead);
-    __syncthreads();   // the stage is in LDS, and every wave is done with the one before it
-    if (step + STAGES - 1 < steps) issue((step + STAGES - 1) % STAGES);
+  const auto pass = [&](auto again) {
+    range = Range();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) dk[mt] = dv[mt] = zeros16();
+    for (int i = 0; i < min(STAGES - 1, steps); ++i) issue(i);
+    for (int step = 0, here = q_stage * QR; step < steps; ++step, here = here + QR < n ? here + QR : q_stage * QR) {
+      const int stage = step % STAGES;
+      const uint8_t *qt = lds + stage * STAGE, *dt = qt + TILE;
+      stay();
+      const int ahead = min(STAGES - 2, steps - 1 - step);
+      if (w < 2 * QR / 64) wait_dma_but<2 * Loader<DH, QR, WAVES>::N + 1>(ahead);
+      else wait_dma_but<2 * Loader<DH, QR, WAVES>::N>(ahead);
+      __syncthreads();   // the stage is in LDS, and every wave is done with the one before it
+      if (step + STAGES - 1 < steps) issue((step + STAGES - 1) % STAGES);
 #pragma unroll 1
-    for (int i32 = 0; i32 < SUB; ++i32) {
-      const int x = i32 * QW + qw, r = here + 32 * x;
-      if (r >= n || r + 31 < w_first) continue;
-      // (reads in one go ahead of the products that use them: the compiler would wait for each by itself)
-      v16f s = zeros16(), dp = zeros16();
-      v4i qa[NS], da[NS];
+      for (int i32 = 0; i32 < SUB; ++i32) {
+        const int x = i32 * QW + qw, r = here + 32 * x;
+        if (r >= n || r + 31 < w_first) continue;
+        // (reads in one go ahead of the products that use them: the compiler would wait for each by itself)
+        v16f s = zeros16(), dp = zeros16();
+        v4i qa[NS], da[NS];
 #pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        qa[st] = rr.get(qt, x, st);
-        da[st] = rr.get(dt, x, st);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        s = mfma<F16>(qa[st], kf[st], s);
-        dp = mfma<F16>(da[st], vf[st], dp);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      v4i td[2][MT], tq[2][MT];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) td[u][mt] = tr.get(dt, 2 * x + u, mt);
-      const float* stats = (const float*)(qt + 2 * TILE) + 32 * x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 l = *(const float4*)(stats + 8 * i + 4 * hf), d = *(const float4*)(stats + QR + 8 * i + 4 * hf);
-        const float le[4] = {l.x, l.y, l.z, l.w}, de[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[4 * i + e], a.s.sl2, le[e]));
-          s[4 * i + e] = p;
-          dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
+        for (int st = 0; st < NS; ++st) {
+          qa[st] = rr.get(qt, x, st);
+          da[st] = rr.get(dt, x, st);
         }
-      }
-      if (r < w_all) {   // queries that do not see a key
-        branch_here();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (r + 8 * (i >> 2) + 4 * hf + (i & 3) < own) s[i] = dp[i] = 0.f;
-      }
-      v4i pf[2], df[2];
-      pack16<F16>(s, 1.f, pf);
-      float by;
-      if constexpr (F16) {
-        if (range.fit(dp, by)) times(dk, by);
-      }
-      pack16<F16>(dp, range.scale, df);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) tq[u][mt] = tr.get(qt, 2 * x + u, mt);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) dv[mt] = mfma<F16>(td[u][mt], pf[u], dv[mt]);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], df[u], dk[mt]);
-      if (fine) {
-        branch_here();
-        v4i rest[2];
-        pack16_rest<F16>(dp, range.scale, df, rest);
+        for (int st = 0; st < NS; ++st) {
+          s = mfma<F16>(qa[st], kf[st], s);
+          dp = mfma<F16>(da[st], vf[st], dp);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        v4i td[2][MT], tq[2][MT];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], rest[u], dk[mt]);
+          for (int mt = 0; mt < MT; ++mt) td[u][mt] = tr.get(dt, 2 * x + u, mt);
+        const float* stats = (const float*)(qt + 2 * TILE) + 32 * x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 l = *(const float4*)(stats + 8 * i + 4 * hf), d = *(const float4*)(stats + QR + 8 * i + 4 * hf);
+          const float le[4] = {l.x, l.y, l.z, l.w}, de[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[4 * i + e], a.s.sl2, le[e]));
+            s[4 * i + e] = p;
+            dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
+          }
+        }
+        const bool partly = r < w_all;   // queries that do not see a key
+        if (partly) {
+          branch_here();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (r + 8 * (i >> 2) + 4 * hf + (i & 3) < own) s[i] = dp[i] = 0.f;
+        }
+        v4i pf[2], df[2];
+        pack16<F16>(s, 1.f, pf);
+        float by;
+        if constexpr (F16) {
+          if (range.fit(dp, by)) times(dk, by);
+        }
+        pack16<F16>(dp, range.scale, df);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) tq[u][mt] = tr.get(qt, 2 * x + u, mt);
+        if (decltype(again)::value && partly) {   // (a query that is not finite has weights that are not)
+          branch_here();
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              td[u][mt] = clean<F16>(td[u][mt]);
+              tq[u][mt] = clean<F16>(tq[u][mt]);
+            }
+          add_odd<DH, F16>(dv, dt, x, hf, [&](int j) { return r + j >= own; });
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) dv[mt] = mfma<F16>(td[u][mt], pf[u], dv[mt]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], df[u], dk[mt]);
+        if (fine) {
+          branch_here();
+          v4i rest[2];
+          pack16_rest<F16>(dp, range.scale, df, rest);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], rest[u], dk[mt]);
+        }
       }
+      stay();
     }
-    stay();
+  };
+  pass(ic<0>{});
+  const bool bad = any_odd(dk) | any_odd(dv);
+  if (lane == 0) odd[w] = bad;
+  __syncthreads();   // every wave is done with the stages
+  if (__builtin_expect(a.s.causal && __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]), 0)) {
+    g_next = 0;
+    head_from(0);
+    pass(ic<1>{});
+    __syncthreads();
   }
-  __syncthreads();
   const float lift = __builtin_amdgcn_exp2f(-LIFT<F16>);
   float k_by = a.s.scale * lift / range.scale;
   if constexpr (QW > 1) {   // the sums of the other waves of these keys, in their order
@@ -333,13 +346,14 @@ constexpr int KT = 64;
 
 // QW and the waves that share queries as in the forward.
 template <int DH, bool F16, int QW>
-__global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
+__global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_dq_kernel(BwdArgs a) {
   constexpr int KW = WAVES / QW, QT = 32 * QW;
   static_assert(KW == 1 || KW == 2, "a tile has 64 keys");
   constexpr int NS = DH / 16, MT = DH / 32, TILE = KT * row_bytes<DH>, STAGE = 2 * TILE;
-  constexpr int SUMS = KW > 1 ? QW * (MT * 16 + 1) * 256 : 0;
+  constexpr int SUMS = KW > 1 ? QW * MT * 16 * 256 : 0;
   constexpr int LDS = std::max(2 * STAGE, std::max(WAVES * STAGING<DH>, SUMS));
   __shared__ __align__(16) uint8_t lds[LDS];
+  __shared__ int odd[WAVES];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = w % QW, kw = w / QW;
   uint32_t head, tile;
@@ -353,15 +367,19 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   const int n = qs.n, m = ks.n, shift = m - n, q0 = at.tile * QT;
   const int row0 = q0 + 32 * qw, row = row0 + (lane & 31);
   const auto seen = [&](int r) { return a.s.causal ? max(0, min(m, min(r, n - 1) + shift + 1)) : m; };
-  const int upto = seen(q0 + QT - 1), w_upto = row0 < n ? seen(row0 + 31) : 0, w_first = seen(row0), own = seen(row);
+  const int upto = seen(q0 + QT - 1), w_upto = row0 < n ? seen(row0 + 31) : 0, w_first = seen(row0);
   const int tiles = (upto + KT - 1) / KT;
 
-  const uint16_t* kb = a.k + ks.first * a.k_tok + (head / a.s.group) * a.k_head;
-  const uint16_t* vb = a.v + ks.first * a.v_tok + (head / a.s.group) * a.v_head;
+  const uint16_t *kb, *vb;
+  int left;
+  const auto from_start = [&] {
+    kb = a.k + ks.first * a.k_tok + (head / a.s.group) * a.k_head;
+    vb = a.v + ks.first * a.v_tok + (head / a.s.group) * a.v_head;
+    left = m;
+  };
   Loader<DH, KT, WAVES> kl, vl;
   kl.init(w, lane, a.k_tok);
   vl.init(w, lane, a.v_tok);
-  int left = m;
   const auto issue = [&](int stage) {   // the next tile
     kl.issue(rows_buffer<DH>(kb, a.k_tok, left, KT), w, lds + stage * STAGE);
     vl.issue(rows_buffer<DH>(vb, a.v_tok, left, KT), w, lds + stage * STAGE + TILE);
@@ -369,6 +387,7 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
     vb += KT * a.v_tok;
     left -= KT;
   };
+  from_start();
   if (tiles > 0) issue(0);
   v4i qf[NS], df[NS];
   load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, lane, qf);
@@ -383,104 +402,91 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   rr.init(lane);
   tr.init(lane);
   v16f dq[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) dq[mt] = zeros16();
-  const bool fine = min(n, m) <= SHORT;
   Range range;
-  float eps = 0.f;   // sum of the lane's dS as rounded, times range.scale
-
-  for (int t = 0; t < tiles; ++t) {
-    const int stage = t & 1;
-    const uint8_t *kt = lds + stage * STAGE, *vt = kt + TILE;
-    wait_dma();
-    __syncthreads();
-    if (t + 1 < tiles) issue(1 - stage);
+  const auto pass = [&](auto again, int lane) __attribute__((always_inline)) {
+    range = Range();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) dq[mt] = zeros16();
+    for (int t = 0; t < tiles; ++t) {
+      const int stage = t & 1;
+      const uint8_t *kt = lds + stage * STAGE, *vt = kt + TILE;
+      wait_dma();
+      __syncthreads();
+      if (t + 1 < tiles) issue(1 - stage);
 #pragma unroll 1
-    for (int x = kw; x < KT / 32; x += KW) {
-      const int j0 = t * KT + 32 * x;
-      if (j0 >= w_upto) continue;
-      v16f s = zeros16(), dp = zeros16();
-#pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        s = mfma<F16>(rr.get(kt, x, st), qf[st], s);
-        dp = mfma<F16>(rr.get(vt, x, st), df[st], dp);
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[i], a.s.sl2, lse)) * (dp[i] - delta);
-      if (j0 + 32 > w_first) {   // keys that a query does not see
-        branch_here();
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (j0 + 8 * (i >> 2) + 4 * hf + (i & 3) >= own) dp[i] = 0.f;
-      }
-      v4i pf[2];
-      float by;
-      if constexpr (F16) {
-        if (range.fit(dp, by)) {
-          times(dq, by);
-          eps *= by;
+      for (int x = kw; x < KT / 32; x += KW) {
+        const int j0 = t * KT + 32 * x;
+        if (j0 >= w_upto) continue;
+        if constexpr (decltype(again)::value) {   // (read again rather than kept: the other pass has no registers to spare)
+          load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, lane, qf);
+          load_rows<DH>(a.dout + (qs.first + row0) * a.do_tok + head * a.do_head, a.do_tok, n - row0, lane, df);
         }
-      }
-      pack16<F16>(dp, range.scale, pf);
+        const int hf = lane >> 5, own = seen(row0 + (lane & 31));
+        v16f s = zeros16(), dp = zeros16();
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int st = 0; st < NS; ++st) {
+          s = mfma<F16>(rr.get(kt, x, st), qf[st], s);
+          dp = mfma<F16>(rr.get(vt, x, st), df[st], dp);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) eps = dot_ones<F16>(pf[u][e], eps);
+        for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[i], a.s.sl2, lse)) * (dp[i] - delta);
+        const bool partly = j0 + 32 > w_first;   // keys that a query does not see
+        if (partly) {
+          branch_here();
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tr.get(kt, 2 * x + u, mt), pf[u], dq[mt]);
-      if (fine) {
-        branch_here();
-        v4i rest[2];
+          for (int i = 0; i < 16; ++i)
+            if (j0 + 8 * (i >> 2) + 4 * hf + (i & 3) >= own) dp[i] = 0.f;
+        }
+        v4i pf[2], rest[2], tk[2][MT];
+        float by;
+        if constexpr (F16) {
+          if (range.fit(dp, by)) times(dq, by);
+        }
+        pack16<F16>(dp, range.scale, pf);
         pack16_rest<F16>(dp, range.scale, pf, rest);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) eps = dot_ones<F16>(rest[u][e], eps);
+          for (int mt = 0; mt < MT; ++mt) tk[u][mt] = tr.get(kt, 2 * x + u, mt);
+        if (decltype(again)::value && partly) {   // (a key that is not finite has weights that are not, where it is seen)
+          branch_here();
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tr.get(kt, 2 * x + u, mt), rest[u], dq[mt]);
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) tk[u][mt] = clean<F16>(tk[u][mt]);
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tk[u][mt], pf[u], dq[mt]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tk[u][mt], rest[u], dq[mt]);
       }
     }
-  }
-  // dS adds up to zero over a query's keys; what the rounded values add up to is error, and where keys have a part in common
-  // (a mean that is not zero) all of it goes the same way. It is taken off over the keys of the last tile (or the one before), evenly: dQ of
-  // keys with a mean of half their deviation 1.42 times the plain error of its own rounding, without this 1.53.
-  eps = sum_xor32(eps);
-  if constexpr (KW > 1) {   // the same of the wave of the other keys, at the smaller of their factors
-    __shared__ float other[QW * 64 * 2];
-    float* at = other + (qw * 64 + lane) * 2;
-    if (kw) at[0] = eps, at[1] = !F16 || range.set ? range.scale : INFINITY;
+  };
+  pass(ic<0>{}, lane);
+  // (the lane's number again, unknown to the compiler: what it makes of it is not held in registers all through the loop)
+  int late = threadIdx.x;
+  asm volatile("" : "+v"(late));
+  late &= 63;
+  const bool bad = any_odd(dq);
+  if (late == 0) odd[w] = bad;
+  __syncthreads();   // every wave is done with the stages
+  if (__builtin_expect(a.s.causal && __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]), 0)) {
+    rr.init(late);
+    tr.init(late);
+    kl.init(w, late, a.k_tok);
+    vl.init(w, late, a.v_tok);
+    from_start();
+    issue(0);   // (there is a tile: without one the sums are zeros)
+    pass(ic<1>{}, late);
     __syncthreads();
-    if (!kw) {
-      if constexpr (F16) {
-        const float both = fminf(range.set ? range.scale : INFINITY, at[1]), next = both < INFINITY ? both : 1.f;
-        times(dq, next / range.scale);
-        eps = eps * (next / range.scale) + (at[1] < INFINITY ? at[0] * (next / at[1]) : 0.f);
-        range.scale = next;
-      } else {
-        eps += at[0];
-      }
-    }
   }
   float by = a.s.scale * __builtin_amdgcn_exp2f(-LIFT<F16>) / range.scale;
-  // Few keys say little of the mean: their part in it is taken less (by the 4 that half a deviation makes right).
-  const int last = tiles > 1 && m - (tiles - 1) * KT < KT / 2 ? tiles - 2 : tiles - 1, held = min(m - last * KT, KT);
-  if (kw == 0 && last >= 0) {
-    const float off = -eps / (float)(held + 4);
-    v4i f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = (int)pack<F16>(off, off);   // (keys that are not there are zeros)
-    const uint8_t* kt = lds + (last & 1) * STAGE;
-#pragma unroll
-    for (int u = 0; u < KT / 16; ++u)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) dq[mt] = mfma<F16>(tr.get(kt, u, mt), f, dq[mt]);
-  }
-  __syncthreads();
-  if constexpr (KW > 1) {
-    float* other = (float*)lds + qw * (MT * 16) * 64 + lane;
+  if constexpr (KW > 1) {   // the same of the wave of the other keys
+    float* other = (float*)lds + qw * (MT * 16) * 64 + late;
     if (kw) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -497,7 +503,7 @@ __global__ __launch_bounds__(THREADS, 2) void packed_dq_kernel(BwdArgs a) {
   }
   if (row0 >= n) return;
   static_assert(KW == 1 || STAGING<DH> <= MT * 16 * 256, "a wave's staging lies inside what it reads");
-  store_turned<DH, F16>(dq, by, lds + (KW > 1 ? qw * MT * 16 * 256 : w * STAGING<DH>), lane, a.dq + (qs.first + row0) * o_tok + head * DH,
+  store_turned<DH, F16>(dq, by, lds + (KW > 1 ? qw * MT * 16 * 256 : w * STAGING<DH>), late, a.dq + (qs.first + row0) * o_tok + head * DH,
                         o_tok, n - row0);
 }
 
