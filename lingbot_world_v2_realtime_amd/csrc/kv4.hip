@@ -22,19 +22,6 @@ struct Pages {
   const int32_t *starts, *lens, *table;
 };
 
-// Where row r of a call's tokens belongs: its sequence and its place in it; seq < 0 for a row of none.
-struct Token {
-  int64_t seq, pos;
-};
-__device__ __forceinline__ Token token_of(const Pages& c, int64_t r) {
-  int64_t s = r, left = 1;   // (left: the sequence's rows from r on)
-  if (c.starts) {
-    s = last_of(c.seqs + 1, r, [&](int64_t i) { return (int64_t)c.starts[i]; });
-    if (s < 0 || s >= c.seqs) return {-1, 0};
-    left = min((int64_t)c.starts[s + 1], c.rows) - r;
-  }
-  return {s, (int64_t)c.lens[s] - left};
-}
 // The page of a sequence's token, or -1.
 __device__ __forceinline__ int64_t page_of(const Pages& c, int64_t seq, int64_t pos) {
   if (seq < 0 || pos < 0 || pos / PAGE >= c.width) return -1;
@@ -76,41 +63,46 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t& scale
   return w;
 }
 
-// A wave a token; 16 (8) lanes a head of K or V.
+// ---- one token a sequence: 16 (8) lanes a head of K or V, all heads at once, so that a call is one load and one store long
+
+struct Lane {
+  int64_t seq, tile;   // tile: of the token's page and the head; seq < 0: nothing to do, tile < 0: in no page
+  int64_t head;
+  int t;
+  bool is_k;
+};
+template <int LANES>
+__device__ __forceinline__ Lane lane_of(const Pages& c) {
+  const int64_t i = ((int64_t)group_id() * THREADS + threadIdx.x) / LANES, seq = i / (2 * c.heads), h2 = i - seq * 2 * c.heads;
+  if (seq >= c.seqs) return {-1, -1, 0, 0, false};
+  const int64_t pos = (int64_t)c.lens[seq] - 1, page = page_of(c, seq, pos), head = h2 < c.heads ? h2 : h2 - c.heads;
+  return {seq, page < 0 ? -1 : page * c.heads + head, head, (int)(pos & (PAGE - 1)), h2 < c.heads};
+}
+
 template <int DH, bool F16>
 __global__ __launch_bounds__(THREADS) void kv4_write_kernel(Pages c, const uint16_t* k, const uint16_t* v, int64_t k_tok, int64_t k_head,
                                                             int64_t v_tok, int64_t v_head) {
   constexpr int LANES = DH / 8;
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)group_id() * (THREADS / 64) + (threadIdx.x >> 6);
-  if (r >= c.rows) return;
-  const Token at = token_of(c, r);
-  const int64_t page = page_of(c, at.seq, at.pos);
-  if (page < 0) return;
-  const int t = (int)(at.pos % PAGE), c8 = lane % LANES, g = c8 >> 2, p = c8 & 3;
-  for (int64_t i0 = 0; i0 < 2 * c.heads; i0 += 64 / LANES) {
-    const int64_t i = i0 + lane / LANES;
-    const bool live = i < 2 * c.heads, is_k = i < c.heads;   // (groups of four lanes are live together)
-    const int64_t h = is_k ? i : i - c.heads, tile = page * c.heads + h;
-    float x[8] = {};
-    if (live) unpack8t<F16>(*(const v4i*)((is_k ? k + r * k_tok + h * k_head : v + r * v_tok + h * v_head) + 8 * c8), x);
-    uint32_t scale;
-    const uint32_t w = encode8(x, scale), other = dpp_u32<DPP_XOR2>(w);
-    if (!live) continue;
-    if (is_k) {
-      *(uint32_t*)(c.k4 + (tile * PAGE + t) * (DH / 2) + p * (DH / 8) + g * 4) = w;
-      if (p == 0) c.ks[(tile * PAGE + t) * (DH / 32) + g] = (uint8_t)scale;
-    } else {
-      // channels 8 (p & 1) + .. of the low (p < 2) or the high 16: the first four bytes by the one, the others by the other
-      uint8_t* to = c.v4 + tile * (PAGE * DH / 2);
-      const uint32_t lo = p < 2 ? w : other, hi = p < 2 ? other : w;
+  const Lane at = lane_of<LANES>(c);
+  if (at.tile < 0) return;   // (the lanes of a head together)
+  const int t = at.t, c8 = threadIdx.x % LANES, g = c8 >> 2, p = c8 & 3;
+  float x[8];
+  unpack8t<F16>(*(const v4i*)((at.is_k ? k + at.seq * k_tok + at.head * k_head : v + at.seq * v_tok + at.head * v_head) + 8 * c8), x);
+  uint32_t scale;
+  const uint32_t w = encode8(x, scale), other = dpp_u32<DPP_XOR2>(w);
+  if (at.is_k) {
+    *(uint32_t*)(c.k4 + (at.tile * PAGE + t) * (DH / 2) + p * (DH / 8) + g * 4) = w;
+    if (p == 0) c.ks[(at.tile * PAGE + t) * (DH / 32) + g] = (uint8_t)scale;
+  } else {
+    // channels 8 (p & 1) + .. of the low (p < 2) or the high 16: the first four bytes by the one, the others by the other
+    uint8_t* to = c.v4 + at.tile * (PAGE * DH / 2);
+    const uint32_t lo = p < 2 ? w : other, hi = p < 2 ? other : w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = (p < 2 ? 0 : 4) + e;
-        to[v_code_at<DH>(t, g, 8 * (p & 1) + n)] = (uint8_t)((lo >> 4 * n & 15) | (hi >> 4 * n & 15) << 4);
-      }
-      if (p == 0) c.vs[tile * (PAGE * DH / 32) + v_scale_at<DH>(t, g)] = (uint8_t)scale;
+    for (int e = 0; e < 4; ++e) {
+      const int n = (p < 2 ? 0 : 4) + e;
+      to[v_code_at<DH>(t, g, 8 * (p & 1) + n)] = (uint8_t)((lo >> 4 * n & 15) | (hi >> 4 * n & 15) << 4);
     }
+    if (p == 0) c.vs[at.tile * (PAGE * DH / 32) + v_scale_at<DH>(t, g)] = (uint8_t)scale;
   }
 }
 
@@ -127,30 +119,23 @@ __device__ __forceinline__ float scale_at(uint32_t w, int i) { return __uint_as_
 template <int DH>
 __global__ __launch_bounds__(THREADS) void kv4_read_kernel(Pages c, uint16_t* k, uint16_t* v) {
   constexpr int LANES = DH / 8;
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)group_id() * (THREADS / 64) + (threadIdx.x >> 6);
-  if (r >= c.rows) return;
-  const Token at = token_of(c, r);
-  const int64_t page = page_of(c, at.seq, at.pos);
-  const int t = (int)(at.pos % PAGE), c8 = lane % LANES, g = c8 >> 2, p = c8 & 3;
-  for (int64_t i = lane / LANES; i < 2 * c.heads; i += 64 / LANES) {
-    const bool is_k = i < c.heads;
-    const int64_t h = is_k ? i : i - c.heads, tile = page * c.heads + h;
-    v4i x = {0, 0, 0, 0};
-    if (page >= 0 && is_k) {
-      x = decode8(*(const uint32_t*)(c.k4 + (tile * PAGE + t) * (DH / 2) + p * (DH / 8) + g * 4), scale_at(c.ks[(tile * PAGE + t) * (DH / 32) + g], 0));
-    } else if (page >= 0) {
-      const uint8_t* from = c.v4 + tile * (PAGE * DH / 2);
-      uint32_t w = 0;
+  const Lane at = lane_of<LANES>(c);
+  if (at.seq < 0) return;
+  const int t = at.t, c8 = threadIdx.x % LANES, g = c8 >> 2, p = c8 & 3;
+  v4i x = {0, 0, 0, 0};
+  if (at.tile >= 0 && at.is_k) {
+    x = decode8(*(const uint32_t*)(c.k4 + (at.tile * PAGE + t) * (DH / 2) + p * (DH / 8) + g * 4), scale_at(c.ks[(at.tile * PAGE + t) * (DH / 32) + g], 0));
+  } else if (at.tile >= 0) {
+    const uint8_t* from = c.v4 + at.tile * (PAGE * DH / 2);
+    uint32_t w = 0;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) w |= (uint32_t)(from[v_code_at<DH>(t, g, 8 * (p & 1) + n)] >> (p < 2 ? 0 : 4) & 15) << 4 * n;
-      x = decode8(w, scale_at(c.vs[tile * (PAGE * DH / 32) + v_scale_at<DH>(t, g)], 0));
-    }
-    *(v4i*)((is_k ? k : v) + (r * c.heads + h) * DH + 8 * c8) = x;
+    for (int n = 0; n < 8; ++n) w |= (uint32_t)(from[v_code_at<DH>(t, g, 8 * (p & 1) + n)] >> (p < 2 ? 0 : 4) & 15) << 4 * n;
+    x = decode8(w, scale_at(c.vs[at.tile * (PAGE * DH / 32) + v_scale_at<DH>(t, g)], 0));
   }
+  *(v4i*)((at.is_k ? k : v) + (at.seq * c.heads + at.head) * DH + 8 * c8) = x;
 }
 
-// ---- prompts: a workgroup a head's 32 tokens between two multiples of 32, whose V codes are neighbours in memory
+// ---- several tokens: a workgroup a head's 32 tokens between two multiples of 32, whose V codes are neighbours in memory
 
 constexpr int BLOCK = 32;
 
@@ -269,9 +254,6 @@ __global__ __launch_bounds__(THREADS) void kv4_read_block_kernel(Pages c, uint16
     *(v4i*)(v + (b.row + t) * o_tok + head * DH + 8 * c8) = y;
   }
 }
-
-// Rows a sequence, about, from which on blocks are the better form (TODO).
-constexpr int64_t BLOCK_ROWS = 16;
 
 // ---------------------------------------------------------------- attention
 
@@ -785,6 +767,10 @@ int check_pages(int64_t seqs, int64_t rows, int64_t heads, int64_t dim, const in
     if ((uintptr_t)p % 4) return LBW_E_ALIGN;
   return LBW_OK;
 }
+// Workgroups of a write or read.
+int64_t groups_of(const int32_t* starts, int64_t rows, int64_t seqs, int64_t heads, int64_t dim) {
+  return starts ? blocks_of(rows, seqs) * heads : (seqs * 2 * heads * (dim / 8) + THREADS - 1) / THREADS;
+}
 bool aligned(const void* p, int64_t tok, int64_t head) { return (uintptr_t)p % 16 == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= 0 && head >= 0; }
 
 }  // namespace
@@ -802,8 +788,10 @@ extern "C" int lbw_kv4_write(const void* k, const void* v, int dtype, int64_t se
   if (!aligned(k, k_s_tok, k_s_head) || !aligned(v, v_s_tok, v_s_head)) return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const Pages c = {k4, ks, v4, vs, heads, pages, width, t_s_seq, seqs, rows, starts, lens, table};
-  const bool blocks = starts && rows >= BLOCK_ROWS * seqs && blocks_of(rows, seqs) * heads <= 1 << 30;
-  const dim3 grid = grid_of(blocks ? blocks_of(rows, seqs) * heads : (rows + 3) / 4);
+  const bool blocks = starts;
+  const int64_t groups = groups_of(starts, rows, seqs, heads, dim);
+  if (groups > 1 << 30) return LBW_E_SHAPE;
+  const dim3 grid = grid_of(groups);
   const uint16_t *kp = (const uint16_t*)k, *vp = (const uint16_t*)v;
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype == LBW_DTYPE_FP16;
@@ -831,9 +819,10 @@ extern "C" int lbw_kv4_read(int64_t seqs, int64_t rows, int64_t heads, int64_t d
   if (((uintptr_t)k | (uintptr_t)v) % 16) return LBW_E_ALIGN;
   if (const int st = check_device()) return st;
   const Pages c = {(uint8_t*)k4, (uint8_t*)ks, (uint8_t*)v4, (uint8_t*)vs, heads, pages, width, t_s_seq, seqs, rows, starts, lens, table};
-  const int64_t n = blocks_of(rows, seqs);
-  const bool blocks = starts && rows >= BLOCK_ROWS * seqs && n * heads <= 1 << 30;
-  const dim3 grid = grid_of(blocks ? n * heads : (rows + 3) / 4);
+  const int64_t n = blocks_of(rows, seqs), groups = groups_of(starts, rows, seqs, heads, dim);
+  if (groups > 1 << 30) return LBW_E_SHAPE;
+  const bool blocks = starts;
+  const dim3 grid = grid_of(groups);
   if (blocks && dim == 128) kv4_read_block_kernel<128><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v, n);
   else if (blocks) kv4_read_block_kernel<64><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v, n);
   else if (dim == 128) kv4_read_kernel<128><<<grid, THREADS, 0, (hipStream_t)stream>>>(c, (uint16_t*)k, (uint16_t*)v);

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_fwd_kernel(
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ int odd[WAVES];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = w % QW, kw = w / QW;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = w % QW, kw = KW > 1 ? w / QW : 0;
   uint32_t head, tile;
   head_tile(group_id(), a.s.k_heads, a.s.group, a.s.common, head, tile);
   if (tile >= a.tiles) return;
@@ -182,6 +182,8 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_fwd_kernel(
   if (late == 0) odd[w] = bad;
   __syncthreads();   // every wave is done with the stages
   if (__builtin_expect(a.s.causal && __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]), 0)) {
+    RowReads<DH> kr;
+    TurnedReads<DH> vr;
     kr.init(late);
     vr.init(late);
     kl.init(w, late, a.k_tok);
@@ -196,8 +198,9 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_fwd_kernel(
       for (int x = XS * kw; x < XS * (kw + 1); ++x) {
         int l = late;
         asm volatile("" : "+v"(l));
-        load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, l, qf);   // (read again rather than kept)
-        work(t, t & 1, x, ic<1>{}, ic<1>{}, kr, vr, l >> 5, seen(row0 + (l & 31)), qf);
+        v4i qx[NS];   // (read again rather than kept)
+        load_rows<DH>(a.q + (qs.first + row0) * a.q_tok + head * a.q_head, a.q_tok, n - row0, l, qx);
+        work(t, t & 1, x, ic<1>{}, ic<1>{}, kr, vr, l >> 5, seen(row0 + (l & 31)), qx);
       }
     }
     __syncthreads();
@@ -241,7 +244,9 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_fwd_kernel(
 template <int DH, bool F16>
 void launch(FwdArgs a, hipStream_t stream) {
   const auto groups = [&](int queries) { return xcd_groups(places_of(a.s.q_rows, a.s.seqs, queries), a.s.k_heads, a.s.group); };
-  const bool wide = groups(128) >= 512;   // (two a CU)
+  // Two a CU (us for 128 and 64 queries: 32 heads over 8, one sequence of 1024, 288 workgroups of 128: 31, 29; of 2048, 544: 61, 65;
+  // 4 of 1024: 59, 74).
+  const bool wide = groups(128) >= 512;
   a.tiles = (uint32_t)places_of(a.s.q_rows, a.s.seqs, wide ? 128 : 64);
   if (wide) packed_fwd_kernel<DH, F16, 4><<<grid_of(groups(128)), THREADS, 0, stream>>>(a);
   else packed_fwd_kernel<DH, F16, 2><<<grid_of(groups(64)), THREADS, 0, stream>>>(a);

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ int odd[WAVES];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = w % KW, qw = w / KW;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = w % KW, qw = QW > 1 ? w / KW : 0;
   uint32_t head, tile;
   head_tile(group_id(), a.s.k_heads, 1, a.s.common, head, tile);
   if (tile >= a.tiles) return;
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_dq_kernel(B
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ int odd[WAVES];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = w % QW, kw = w / QW;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = w % QW, kw = KW > 1 ? w / QW : 0;
   uint32_t head, tile;
   head_tile(group_id(), a.s.k_heads, a.s.group, a.s.common, head, tile);
   if (tile >= a.tiles) return;
@@ -512,9 +512,11 @@ void launch(BwdArgs a, hipStream_t stream) {
   const int64_t rows = a.s.q_rows * a.s.q_heads;
   packed_delta_kernel<DH, F16><<<grid_of((rows * (DH / 8) + THREADS - 1) / THREADS), THREADS, 0, stream>>>(a);
   if (a.dk) {
-    // as many keys a workgroup as leave two for every CU
+    // As many keys a workgroup as leave two for every CU, or, where each is short, more than one (measured, us, for 128, 64 and
+    // 32 keys: 32 heads over 8, 4 sequences of 1024: 172, 129, 183; one of 2048: 287, 180, 150; 16 over 16, one of 1024: 51, 40, 47).
     const auto groups = [&](int keys) { return xcd_groups(places_of(a.s.k_rows, a.s.seqs, keys), a.s.k_heads, 1); };
-    const int keys = groups(128) >= 512 ? 128 : groups(64) >= 512 ? 64 : 32;
+    const bool brief = a.s.q_rows / a.s.seqs * a.s.group <= 2048;
+    const int keys = groups(128) >= 512 ? 128 : groups(64) >= (brief ? 256 : 512) ? 64 : 32;
     a.tiles = (uint32_t)places_of(a.s.k_rows, a.s.seqs, keys);
     const dim3 grid = grid_of(groups(keys));
     if (keys == 128) packed_dkv_kernel<DH, F16, 4><<<grid, THREADS, 0, stream>>>(a);
@@ -523,7 +525,8 @@ void launch(BwdArgs a, hipStream_t stream) {
   }
   if (a.dq) {
     const auto groups = [&](int queries) { return xcd_groups(places_of(a.s.q_rows, a.s.seqs, queries), a.s.k_heads, a.s.group); };
-    const bool wide = groups(128) >= 512;   // (two a CU)
+    // (us for 128 and 64 queries: 32 heads, one sequence of 2048, 544 workgroups of 128: 105, 99; of 4096: 283, 283; 16 of 256: 68, 78)
+    const bool wide = groups(128) >= 1024;
     a.tiles = (uint32_t)places_of(a.s.q_rows, a.s.seqs, wide ? 128 : 64);
     if (wide) packed_dq_kernel<DH, F16, 4><<<grid_of(groups(128)), THREADS, 0, stream>>>(a);
     else packed_dq_kernel<DH, F16, 2><<<grid_of(groups(64)), THREADS, 0, stream>>>(a);
