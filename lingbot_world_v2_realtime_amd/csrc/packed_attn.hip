@@ -1,10 +1,17 @@
 // Attention over packed sequences, forward (include/lbw_causal.h): S = q k^T, softmax, times v, a tile of keys after
 // another with the running maximum and sum.
 //
-// A workgroup takes 128 queries of a head and sequence, 32 a wave, and walks the keys 64 at a time (two stages in LDS).
+// A workgroup takes 128 queries of a head and sequence, 32 a wave, or 64 by two waves each, and walks the keys 64 at a time (two
+// stages in LDS).
 // S^T = K Q^T on v_mfma_f32_32x32x16: a lane holds one query and 32 of the 64 keys, so the row's maximum and sum are
 // register work and one exchange between the wave's halves; P^T goes in the type of v from those registers into
 // O^T += V^T P^T, whose V^T comes from the rows of v by transposing LDS reads.
+//
+// Bound by the matrix units and the softmax's vector work beside them, of which either is busy about half of the time (two
+// waves a SIMD cover each other in part). 12 heads of 128, one sequence of 12064: 447 to 475 us, 0.94 to 1.0 PFLOP/s of the
+// products that are seen, 0.75 to 0.8 of what a library product of 8192^3 reaches here. 8 sequences of up to 1508, 32 heads over
+// 8: 96 us, 0.66 PFLOP/s (the diagonal tiles are half masked, the longest sequence's last tile is 24 steps). 61 captions of up
+// to 77, 16 heads of 64, fp16: 9.4 us, launch and one trip to memory and back.
 #include "lbw_packed.h"
 
 namespace lbw {
