@@ -333,6 +333,8 @@ struct Spot {
 };
 struct Line {
   const AttnArgs& a;
+  // (sums stop at MOST, which a call's work lies below: starts that fall can make more of it, and make none)
+  static constexpr uint32_t MOST = 1u << 30;
   uint32_t total, n, all_w, all_t, w, t, l;   // a lane's sequence of 64: units and tiles up to it, its tiles' units
   uint32_t own_w, own_t;
 
@@ -341,25 +343,26 @@ struct Line {
     l = own_t = 0;
     if (s < a.c.seqs) {
       const int count = a.c.starts ? span(a.c.starts, s, a.c.rows).n : 1;
-      own_t = (uint32_t)((count + a.tokens - 1) / a.tokens) * (uint32_t)a.row_tiles;
+      own_t = (uint32_t)min(((int64_t)count + a.tokens - 1) / a.tokens * a.row_tiles, (int64_t)MOST);
       l = (uint32_t)((min(max((int64_t)a.c.lens[s], (int64_t)0), a.c.width * PAGE) + UNIT - 1) / UNIT);
     }
-    w = own_w = own_t * l;
+    w = own_w = (uint32_t)min((uint64_t)own_t * l, (uint64_t)MOST);
     t = own_t;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const uint32_t x = __shfl_up(w, o), y = __shfl_up(t, o);
-      if ((threadIdx.x & 63) >= o) w += x, t += y;
+      if ((threadIdx.x & 63) >= o) w = min(w + x, MOST), t = min(t + y, MOST);
     }
     all_w = __shfl(w, 63), all_t = __shfl(t, 63);
   }
   __device__ __forceinline__ explicit Line(const AttnArgs& args) : a(args) {
+    uint32_t tiles = 0;
     total = 0;
     for (int64_t s0 = 0; s0 < a.c.seqs; s0 += 64) {
       look(s0);
-      total += all_w;
+      total = min(total + all_w, MOST), tiles = min(tiles + all_t, MOST);
     }
-    n = min(a.shares, total);
+    n = total < MOST && tiles <= (uint32_t)(a.segments - a.shares) ? min(a.shares, total) : 0;
   }
   // the sequence at which f(its units up to and with it, its number) becomes true
   template <typename F>
@@ -671,7 +674,7 @@ __global__ __launch_bounds__(THREADS) void kv4_join_kernel(AttnArgs a) {
     const Spot s = line.find([&](uint32_t, int64_t x) { return x == seq; });
     const int row_tile = a.row_tiles > 1 ? g / (16 * RT) : 0, heads_here = min(a.group - row_tile * 16 * RT, a.row_tiles > 1 ? 16 * RT : a.group);
     const uint32_t tile = (uint32_t)(token / a.tokens * a.row_tiles + row_tile);
-    if (s.units && tile < s.tiles) {
+    if (line.n && s.units && tile < s.tiles) {
       const uint32_t u = s.units_before + tile * s.units, first = line.owner(u);
       parts = (int)(line.owner(u + s.units - 1) - first) + 1;
       if (parts == 1) return;   // (the one segment wrote the row)

@@ -411,3 +411,22 @@ def test_smallest_calls():
     cache.write(0, q, q, _dev([[0]]), _dev([1]))
     assert torch.equal(cache.attend(0, q, _dev([[0]]), _dev([1])), x)
     assert not cache.attend(0, q, _dev([[0]]), _dev([0])).any()
+
+
+@pytest.mark.parametrize("seqs", [40, 200])
+def test_cache_with_falling_starts(seqs):
+    """Starts that fall have no particular answer; the calls end, stay inside their tensors, and leave what the table does not name."""
+    g = _gen(41)
+    rows, heads, d = 8, 2, 64
+    cache = _filled(g, 3 * seqs, heads, d)
+    before = [x.clone() for x in (cache.k, cache.k_scale, cache.v, cache.v_scale)]
+    q, k, v = (_rand(g, rows, h, d, dtype=torch.bfloat16) for h in (4, heads, heads))
+    table, lens = _dev([[i, -1, 2 * seqs + i] for i in range(seqs)]), _dev([150] * seqs)
+    for starts in ([0, rows] * (seqs // 2) + [0], [rows] * seqs + [0], [0] + [2 ** 31 - 1, -5] * (seqs // 2)):
+        args = (table, lens, _dev(starts))
+        cache.attend(0, q, *args)
+        cache.read(0, *args, tokens=rows)
+        cache.write(0, k, v, *args)
+    torch.cuda.synchronize()
+    for x, y in zip((cache.k, cache.k_scale, cache.v, cache.v_scale), before):
+        assert torch.equal(x[:, seqs:2 * seqs], y[:, seqs:2 * seqs])
