@@ -16,5 +16,7 @@ def packed_attention(q, k, v, starts, k_starts=None, sm_scale=None, causal=True)
     of no sequence, give 0. sm_scale: D^-1/2 by default. Returns [T, Hq, D] of q's type; differentiable in q, k and v.
 
     Products are of the inputs' type with fp32 sums, the softmax is fp32, its weights are rounded to the type before they
-    meet v (and, in the gradient, d_out and q or k), and every output once. Rows that are not 16-byte aligned are copied."""
+    meet v (and, in the gradient, d_out), and every output once; the gradient's other weights meet k in two parts of the type, and q
+    in one (two where a sequence has up to 128 queries or keys). An infinity or NaN reaches the rows that see it and no others.
+    Rows that are not 16-byte aligned are copied."""
     return kernels.block_binding().packed_attention(q, k, v, starts, k_starts, sm_scale, causal)
