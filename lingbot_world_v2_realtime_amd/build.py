@@ -3,6 +3,8 @@ only) into _block.so, in-tree next to this file."""
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -14,7 +16,7 @@ SOURCES = ["lbw_abi.hip", "kv_requant.hip", "quant_q.hip", "prologue.hip", "cros
 BINDING = ["block_binding.cpp", "causal_binding.cpp"]
 
 HIPCC_FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     # no packed-fp32 VALU ops anywhere
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wno-unused-command-line-argument",
@@ -27,16 +29,25 @@ def hipcc():
 
 
 def build_library(verbose=False):
-    """Compile every HIP source into liblbw_attn.so (always recompiles). Returns the library path."""
-    srcs = [os.path.join(HERE, "csrc", s) for s in SOURCES]
+    """Compile every HIP source, several side by side, and link them into liblbw_attn.so (always recompiles). Returns the library
+    path."""
     tmp = LIB + ".tmp"
-    cmd = [hipcc()] + HIPCC_FLAGS + ["-I", os.path.join(ROOT, "include")] + srcs + ["-o", tmp]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("hipcc failed building liblbw_attn.so")
+
+    def run(args):
+        cmd = [hipcc()] + HIPCC_FLAGS + args
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("hipcc failed building liblbw_attn.so")
+
+    jobs = min(int(os.environ.get("MAX_JOBS", 8)), os.cpu_count() or 1, len(SOURCES))
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(max(jobs, 1)) as pool:
+        outs = [os.path.join(objects, s + ".o") for s in SOURCES]
+        list(pool.map(run, [["-I", os.path.join(ROOT, "include"), "-c", os.path.join(HERE, "csrc", s), "-o", o]
+                            for s, o in zip(SOURCES, outs)]))
+        run(["-shared", *outs, "-o", tmp])
     os.replace(tmp, LIB)
     return LIB
 
