@@ -118,15 +118,17 @@ constexpr int SHORT = 128;
 
 // A workgroup takes 32 KW keys, 32 a wave, and its QW = 4 / KW waves of the same keys take every QW-th 32 queries, their sums
 // added at the end: with 128 keys a stage's queries serve four waves, with 32 there are four times as many workgroups, each a
-// quarter as long.
+// quarter as long. There no two waves share queries: each brings its own, two stages ahead of the barriers that the others
+// need, and has read the next queries from LDS before the products of these are done.
 template <int DH, bool F16, int KW>
 __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(BwdArgs a) {
-  constexpr int QW = WAVES / KW, QR = QW == 4 ? 128 : 64, SUB = QR / 32 / QW;   // queries of a stage; 32s of a wave in it
-  constexpr int NS = DH / 16, MT = DH / 32, KT = 32 * KW, TILE = QR * row_bytes<DH>, STAGE = 2 * TILE + 2 * QR * 4;
-  // (the loads of a stage take longer than its products where memory is far: three stages ahead, where they fit)
-  constexpr int STAGES = STAGE > 40000 ? 2 : 4;
+  constexpr bool ALONE = KW == 1;
+  constexpr int QW = WAVES / KW, QR = ALONE ? 32 : 64, SUB = ALONE ? 1 : QR / 32 / QW;   // queries of a stage; 32s of a wave in it
+  constexpr int NS = DH / 16, MT = DH / 32, KT = 32 * KW, TILE = QR * row_bytes<DH>, STAGE = 2 * TILE + 2 * 64 * 4;
+  // (the loads of a stage take longer than its products where memory is far)
+  constexpr int STAGES = ALONE ? 2 : 4, RINGS = ALONE ? WAVES : 1, LOADERS = ALONE ? 1 : WAVES;
   constexpr int SUMS = (WAVES - KW) * 2 * MT * 16 * 64 * 4;   // LDS bytes of the sums of all waves but the first of each 32 keys
-  constexpr int LDS = std::max(std::max(STAGES * STAGE, WAVES * STAGING<DH>), SUMS);
+  constexpr int LDS = std::max(std::max(RINGS * STAGES * STAGE, WAVES * STAGING<DH>), SUMS);
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ int odd[WAVES];
   const int lane = threadIdx.x & 63, hf = lane >> 5;
@@ -144,43 +146,58 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   const int k0 = (at.tiles - 1 - at.tile) * KT, key0 = k0 + 32 * kw, key = key0 + (lane & 31);   // (the first keys have the most queries)
   // the first query that sees a key, and the stage it lies in
   const auto first = [&](int j) { return a.s.causal ? max(0, j - shift) : 0; };
-  const int q_stage = first(k0) / QR, stages = max(0, (n + QR - 1) / QR - q_stage);
+  const int q_stage = first(k0) / QR, stages = max(0, (n + QR - 1) / QR - q_stage), each = ALONE ? WAVES : 1;
   const int own = first(key), w_first = first(key0), w_all = first(key0 + 31);
   const bool fine = min(n, m) <= SHORT;
 
   v4i kf[NS], vf[NS];
   load_rows<DH>(a.k + (ks.first + key0) * a.k_tok + head * a.k_head, a.k_tok, m - key0, lane, kf);
   load_rows<DH>(a.v + (ks.first + key0) * a.v_tok + head * a.v_head, a.v_tok, m - key0, lane, vf);
-  Loader<DH, QR, WAVES> ql, dl;
-  ql.init(w, lane, a.q_tok);
-  dl.init(w, lane, a.do_tok);
+  const int loader = ALONE ? 0 : w;
+  Loader<DH, QR, LOADERS> ql, dl;
+  ql.init(loader, lane, a.q_tok);
+  dl.init(loader, lane, a.do_tok);
   arrived(kf);
   arrived(vf);
-  const int steps = stages * a.s.group;
+  // of all heads' stages one behind the other: each, or (ALONE) every fourth from the wave's number on
+  const int steps = ALONE ? max(0, (stages * a.s.group - w + WAVES - 1) / WAVES) : stages * a.s.group;
   // What is loaded next: a head's queries from r on. Pointers that move on by a stage: made from the numbers each time, the
   // scalar unit would take as long as the products.
   const uint16_t *q_next, *d_next;
   const float* stat_next;
-  int g_next = 0, r_next;
-  const auto head_from = [&](int g) {
-    const int64_t h = (int64_t)head * a.s.group + g;
-    r_next = q_stage * QR;
+  int g_next, r_next;
+  const auto queries_from = [&](int r) {   // of head g_next, or of one behind it
+    while (r >= stages * QR) r -= stages * QR, ++g_next;
+    const int64_t h = (int64_t)head * a.s.group + g_next;
+    r_next = q_stage * QR + r;
     q_next = a.q + (qs.first + r_next) * a.q_tok + h * a.q_head;
     d_next = a.dout + (qs.first + r_next) * a.do_tok + h * a.do_head;
-    stat_next = (w < QR / 64 ? a.lse : a.delta) + h * a.s.q_rows + qs.first + r_next + w % (QR / 64) * 64;
+    stat_next = (w == 0 || ALONE ? a.lse : a.delta) + h * a.s.q_rows + qs.first + r_next;
   };
-  head_from(0);
-  const auto issue = [&](int stage) {
-    uint8_t* to = lds + stage * STAGE;
-    ql.issue(rows_buffer<DH>(q_next, a.q_tok, n - r_next, QR), w, to);
-    dl.issue(rows_buffer<DH>(d_next, a.do_tok, n - r_next, QR), w, to + TILE);
-    // (64 values a wave: of the sums first, then of D)
-    if (w < 2 * QR / 64) dma4(stat_next, n - r_next - w % (QR / 64) * 64, lane * 4, to + 2 * TILE + w * 256);
-    r_next += QR;
-    q_next += QR * a.q_tok;
-    d_next += QR * a.do_tok;
-    stat_next += QR;
-    if (r_next >= n) head_from(++g_next);
+  const auto restart = [&] {
+    g_next = 0;
+    if (steps > 0) queries_from(ALONE ? w * QR : 0);
+  };
+  restart();
+  const int64_t to_delta = a.delta - a.lse;
+  const int end = (q_stage + stages) * QR;
+  uint8_t* ring = lds + (ALONE ? w * STAGES * STAGE : 0);
+  const auto issue = [&](int stage) __attribute__((always_inline)) {
+    uint8_t* to = ring + stage * STAGE;
+    ql.issue(rows_buffer<DH>(q_next, a.q_tok, n - r_next, QR), loader, to);
+    dl.issue(rows_buffer<DH>(d_next, a.do_tok, n - r_next, QR), loader, to + TILE);
+    // (64 values a load: of the sums, then of D; one for each of the first two waves, where they share)
+    if (ALONE || w < 2) dma4(stat_next, n - r_next, lane * 4, to + 2 * TILE + (ALONE ? 0 : w * 256));
+    if (ALONE) dma4(stat_next + to_delta, n - r_next, lane * 4, to + 2 * TILE + 256);
+    r_next += each * QR;
+    q_next += each * QR * a.q_tok;
+    d_next += each * QR * a.do_tok;
+    stat_next += each * QR;
+    if (r_next >= end) {
+      const int over = r_next - end;
+      ++g_next;
+      queries_from(over);
+    }
   };
   RowReads<DH> rr;
   TurnedReads<DH> tr;
@@ -196,105 +213,154 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
       for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+a"(dk[mt]), "+a"(dv[mt]));
     }
   };
-  const auto pass = [&](auto again) {
+  v4i qa[NS], da[NS];
+  // (reads in one go ahead of the products that use them: the compiler would wait for each by itself)
+  const auto read = [&](const uint8_t* qt, int x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      qa[st] = rr.get(qt, x, st);
+      da[st] = rr.get(qt + TILE, x, st);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The 32 queries r .. + 32, x-th of the stage at qt, once read; meanwhile() runs when everything else of them is read.
+  const auto work = [&](const uint8_t* qt, int x, int r, auto again, const auto& meanwhile) __attribute__((always_inline)) {
+    const uint8_t* dt = qt + TILE;
+    v16f s = zeros16(), dp = zeros16();
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      s = mfma<F16>(qa[st], kf[st], s);
+      dp = mfma<F16>(da[st], vf[st], dp);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    v4i td[2][MT], tq[2][MT];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) td[u][mt] = tr.get(dt, 2 * x + u, mt);
+    const float* stats = (const float*)(qt + 2 * TILE) + 32 * x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 l = *(const float4*)(stats + 8 * i + 4 * hf), d = *(const float4*)(stats + 64 + 8 * i + 4 * hf);
+      const float le[4] = {l.x, l.y, l.z, l.w}, de[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[4 * i + e], a.s.sl2, le[e]));
+        s[4 * i + e] = p;
+        dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
+      }
+    }
+    const bool partly = r < w_all;   // queries that do not see a key
+    if (partly) {
+      branch_here();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (r + 8 * (i >> 2) + 4 * hf + (i & 3) < own) s[i] = dp[i] = 0.f;
+    }
+    v4i pf[2], df[2];
+    pack16<F16>(s, 1.f, pf);
+    float by;
+    if constexpr (F16) {
+      if (range.fit(dp, by)) times(dk, by);
+    }
+    pack16<F16>(dp, range.scale, df);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) tq[u][mt] = tr.get(qt, 2 * x + u, mt);
+    if (decltype(again)::value && partly) {   // (a query that is not finite has weights that are not)
+      branch_here();
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          td[u][mt] = clean<F16>(td[u][mt]);
+          tq[u][mt] = clean<F16>(tq[u][mt]);
+        }
+      add_odd<DH, F16>(dv, dt, x, hf, [&](int j) { return r + j >= own; });
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    meanwhile();
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) dv[mt] = mfma<F16>(td[u][mt], pf[u], dv[mt]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], df[u], dk[mt]);
+    if (fine) {
+      branch_here();
+      v4i rest[2];
+      pack16_rest<F16>(dp, range.scale, df, rest);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], rest[u], dk[mt]);
+    }
+  };
+  const auto pass = [&](auto again) __attribute__((always_inline)) {
     range = Range();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) dk[mt] = dv[mt] = zeros16();
-    for (int i = 0; i < min(STAGES - 1, steps); ++i) issue(i);
-    for (int step = 0, here = q_stage * QR; step < steps; ++step, here = here + QR < n ? here + QR : q_stage * QR) {
-      const int stage = step % STAGES;
-      const uint8_t *qt = lds + stage * STAGE, *dt = qt + TILE;
-      stay();
-      const int ahead = min(STAGES - 2, steps - 1 - step);
-      if (w < 2 * QR / 64) wait_dma_but<2 * Loader<DH, QR, WAVES>::N + 1>(ahead);
-      else wait_dma_but<2 * Loader<DH, QR, WAVES>::N>(ahead);
-      __syncthreads();   // the stage is in LDS, and every wave is done with the one before it
-      if (step + STAGES - 1 < steps) issue((step + STAGES - 1) % STAGES);
-#pragma unroll 1
-      for (int i32 = 0; i32 < SUB; ++i32) {
-        const int x = i32 * QW + qw, r = here + 32 * x;
-        if (r >= n || r + 31 < w_first) continue;
-        // (reads in one go ahead of the products that use them: the compiler would wait for each by itself)
-        v16f s = zeros16(), dp = zeros16();
-        v4i qa[NS], da[NS];
-#pragma unroll
-        for (int st = 0; st < NS; ++st) {
-          qa[st] = rr.get(qt, x, st);
-          da[st] = rr.get(dt, x, st);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int st = 0; st < NS; ++st) {
-          s = mfma<F16>(qa[st], kf[st], s);
-          dp = mfma<F16>(da[st], vf[st], dp);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        v4i td[2][MT], tq[2][MT];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) td[u][mt] = tr.get(dt, 2 * x + u, mt);
-        const float* stats = (const float*)(qt + 2 * TILE) + 32 * x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 l = *(const float4*)(stats + 8 * i + 4 * hf), d = *(const float4*)(stats + QR + 8 * i + 4 * hf);
-          const float le[4] = {l.x, l.y, l.z, l.w}, de[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(weight_exponent<F16>(s[4 * i + e], a.s.sl2, le[e]));
-            s[4 * i + e] = p;
-            dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
-          }
-        }
-        const bool partly = r < w_all;   // queries that do not see a key
-        if (partly) {
-          branch_here();
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (r + 8 * (i >> 2) + 4 * hf + (i & 3) < own) s[i] = dp[i] = 0.f;
-        }
-        v4i pf[2], df[2];
-        pack16<F16>(s, 1.f, pf);
-        float by;
-        if constexpr (F16) {
-          if (range.fit(dp, by)) times(dk, by);
-        }
-        pack16<F16>(dp, range.scale, df);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) tq[u][mt] = tr.get(qt, 2 * x + u, mt);
-        if (decltype(again)::value && partly) {   // (a query that is not finite has weights that are not)
-          branch_here();
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              td[u][mt] = clean<F16>(td[u][mt]);
-              tq[u][mt] = clean<F16>(tq[u][mt]);
-            }
-          add_odd<DH, F16>(dv, dt, x, hf, [&](int j) { return r + j >= own; });
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) dv[mt] = mfma<F16>(td[u][mt], pf[u], dv[mt]);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], df[u], dk[mt]);
-        if (fine) {
-          branch_here();
-          v4i rest[2];
-          pack16_rest<F16>(dp, range.scale, df, rest);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) dk[mt] = mfma<F16>(tq[u][mt], rest[u], dk[mt]);
-        }
+    if constexpr (ALONE) {
+      constexpr int LOADS = 2 * Loader<DH, QR, LOADERS>::N + 2;
+      int r = w * QR;   // from the first stage's start on
+      if (steps > 0) {
+        while (r >= stages * QR) r -= stages * QR;
+        issue(0);
+        if (steps > 1) issue(1);
+        wait_dma_but<LOADS>(steps > 1);
+        asm volatile("" ::: "memory");
+        if constexpr (!decltype(again)::value) read(ring, 0);
       }
-      stay();
+      for (int step = 0; step < steps; ++step) {
+        const uint8_t* here = ring + (step & 1) * STAGE;
+        const auto next = [&]() __attribute__((always_inline)) {
+          if (step + 1 < steps) {
+            // (lgkmcnt(0): the wave has these queries in registers, and the stage is free)
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+            asm volatile("" ::: "memory");
+            if (step + 2 < steps) issue(step & 1);
+            wait_dma_but<LOADS>(step + 2 < steps);
+            asm volatile("" ::: "memory");
+          }
+        };
+        stay();
+        if constexpr (decltype(again)::value) {   // (few registers rather than speed)
+          read(here, 0);
+          work(here, 0, q_stage * QR + r, again, [] {});
+          next();
+        } else {
+          work(here, 0, q_stage * QR + r, again, [&]() __attribute__((always_inline)) {
+            next();
+            if (step + 1 < steps) read(ring + (1 - (step & 1)) * STAGE, 0);
+          });
+        }
+        r += WAVES * QR;
+        while (r >= stages * QR) r -= stages * QR;
+        stay();
+      }
+    } else {
+      for (int i = 0; i < min(STAGES - 1, steps); ++i) issue(i);
+      for (int step = 0, here = q_stage * QR; step < steps; ++step, here = here + QR < n ? here + QR : q_stage * QR) {
+        const int stage = step % STAGES;
+        const uint8_t* qt = ring + stage * STAGE;
+        stay();
+        const int ahead = min(STAGES - 2, steps - 1 - step);
+        if (w < 2) wait_dma_but<2 * Loader<DH, QR, LOADERS>::N + 1>(ahead);
+        else wait_dma_but<2 * Loader<DH, QR, LOADERS>::N>(ahead);
+        __syncthreads();   // the stage is in LDS, and every wave is done with the one before it
+        if (step + STAGES - 1 < steps) issue((step + STAGES - 1) % STAGES);
+#pragma unroll 1
+        for (int i32 = 0; i32 < SUB; ++i32) {
+          const int x = i32 * QW + qw, r = here + 32 * x;
+          if (r >= n || r + 31 < w_first) continue;
+          read(qt, x);
+          work(qt, x, r, again, [] {});
+        }
+        stay();
+      }
     }
   };
   pass(ic<0>{});
@@ -302,8 +368,7 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
   if (lane == 0) odd[w] = bad;
   __syncthreads();   // every wave is done with the stages
   if (__builtin_expect(a.s.causal && __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]), 0)) {
-    g_next = 0;
-    head_from(0);
+    restart();
     pass(ic<1>{});
     __syncthreads();
   }
