@@ -6,9 +6,9 @@
 // workgroup for a tile of queries, which walks the keys. S and dO V^T are formed in both (7 products for 5), so that no
 // sum needs atomics: each has one order, whatever runs beside it.
 //
-// 5 sequences of up to 1508, 12 heads of 128 over 4: D 7.6 us, dK and dV 94, dQ 45, the forward 39. dK and dV take one wave a SIMD
-// (their sums are 128 registers a lane, K and V of the keys 64), whose reads, products and exponentials follow one another: the
-// longest workgroup's 36 steps of 128 queries are what the call waits for.
+// 5 sequences of up to 1508, 12 heads of 128 over 4: D 7.6 us, dK and dV 79, dQ 45, the forward 39. dK and dV take one wave a SIMD
+// (their sums are 128 registers a lane, K and V of the keys 64), whose products, exponentials and scalar work follow one
+// another: the longest workgroup's 36 steps of 128 queries are what the call waits for, 2.2 us each.
 #include "lbw_packed.h"
 
 namespace lbw {
@@ -583,9 +583,10 @@ void launch(BwdArgs a, hipStream_t stream) {
   packed_delta_kernel<DH, F16><<<grid_of((rows * (DH / 8) + THREADS - 1) / THREADS), THREADS, 0, stream>>>(a);
   if (a.dk) {
     // As many keys a workgroup as leave two for every CU, or, where each is short, more than one (measured, us, for 128, 64 and
-    // 32 keys: 32 heads over 8, 4 sequences of 1024: 172, 129, 183; one of 2048: 287, 180, 150; 16 over 16, one of 1024: 51, 40, 47).
+    // 32 keys: 32 heads over 8, 4 sequences of 1024: 175, 136, 162; one of 2048: 299, 185, 137; 12 over 12, one of 6000: 340, 353,
+    // 395; 16 over 16, one of 1024: 52, 40, 46).
     const auto groups = [&](int keys) { return xcd_groups(places_of(a.s.k_rows, a.s.seqs, keys), a.s.k_heads, 1); };
-    const bool brief = a.s.q_rows / a.s.seqs * a.s.group <= 2048;
+    const bool brief = a.s.q_rows / a.s.seqs * a.s.group <= 1024;
     const int keys = groups(128) >= 512 ? 128 : groups(64) >= (brief ? 256 : 512) ? 64 : 32;
     a.tiles = (uint32_t)places_of(a.s.k_rows, a.s.seqs, keys);
     const dim3 grid = grid_of(groups(keys));
