@@ -276,6 +276,7 @@ struct AttnArgs {
   float sl2;
   uint16_t* out;
   float *part, *stats;              // [heads][segments][tile_rows][DH], [..][2]: sums, and the maximum and sum of the weights
+  int2* parts;                      // [places][row_tiles]: a tile's first segment, and its last
 };
 
 __device__ __forceinline__ v4f mfma16(const v4i a, const v4i b, const v4f c) {
@@ -383,17 +384,16 @@ struct Line {
     return {-1, 0, 0, 0, 0};
   }
   __device__ __forceinline__ uint32_t share(uint32_t i) const { return (uint32_t)((uint64_t)i * total / n); }
-  // the workgroup that has unit u
-  __device__ __forceinline__ uint32_t owner(uint32_t u) const { return (uint32_t)((((uint64_t)u + 1) * n - 1) / total); }
 };
 
 // A segment: up to 16 RT rows (tokens x the heads that share a head of the cache) over a run of keys, 32 a step, by one wave. S^T = K Q^T on v_mfma_f32_16x16x32_bf16: a lane holds one row and 8 of the 32 keys; the row's maximum needs two
 // exchanges; P^T goes from those registers into O^T += V^T P^T. fp16 q and P enter as two bf16 values each, high and low.
-template <int DH, int RT>
-constexpr int ATTN_WAVES = RT == 1 ? (DH == 128 ? 3 : 4) : RT == 2 ? (DH == 128 ? 2 : 3) : (DH == 128 ? 1 : 2);   // a SIMD
+constexpr int RT = 1;   // 16-row tiles of a wave (with two, which leave room for fewer waves: 20 rows of 16 sequences 43 us for 39, 64 rows 64 for 67)
+template <int DH>
+constexpr int ATTN_WAVES = DH == 128 ? 3 : 4;   // a SIMD
 
-template <int DH, bool F16, int RT>
-__global__ __launch_bounds__(THREADS, (ATTN_WAVES<DH, RT>)) void kv4_attn_kernel(AttnArgs a) {
+template <int DH, bool F16>
+__global__ __launch_bounds__(THREADS, ATTN_WAVES<DH>) void kv4_attn_kernel(AttnArgs a) {
   constexpr int G = DH / 32, NT = DH / 16;
   const uint32_t id = __builtin_amdgcn_readfirstlane(group_id() * WAVES + (threadIdx.x >> 6)), heads = (uint32_t)a.c.heads;
   // where the wave is: a head, a sequence, a tile in it (tokens, part of the group), and the units of its keys
@@ -446,6 +446,13 @@ __global__ __launch_bounds__(THREADS, (ATTN_WAVES<DH, RT>)) void kv4_attn_kernel
   const uint32_t run = a.shares ? min(left, units - unit) : 0;
   const int k0 = (int)unit * UNIT, k1 = a.shares ? min(upto, k0 + (int)run * UNIT) : upto;
   const bool whole = !a.shares || run == units;
+  if (a.shares && head == 0) {   // where the tile's segments begin and end, for the join
+    const int64_t from = a.c.starts ? min(max((int64_t)a.c.starts[seq], (int64_t)0), a.c.rows) / a.tokens : 0;
+    int* at = (int*)(a.parts + (from + seq) * a.row_tiles + tile);
+    const int mine = (int)(id / heads + tiles_before + tile);
+    if (lane == 0 && unit == 0) at[0] = mine;
+    if (lane == 0 && unit + run == units) at[1] = mine;
+  }
 
   v4i qh[RT][G], ql[F16 ? RT : 1][G];
   int own[RT];   // keys that the lane's row sees
@@ -650,7 +657,7 @@ __global__ __launch_bounds__(THREADS, (ATTN_WAVES<DH, RT>)) void kv4_attn_kernel
 // The segments of a row's tile joined, where it has several, and zeros where it has none: a workgroup a row and head, DH / 4
 // lanes a segment, so that 8 (16) segments are read at once, four times over; each group of lanes keeps a running maximum and
 // sum, and the groups' are joined in LDS.
-template <int DH, bool F16, int RT>
+template <int DH, bool F16>
 __global__ __launch_bounds__(THREADS) void kv4_join_kernel(AttnArgs a) {
   constexpr int LANES = DH / 4, GROUPS = THREADS / LANES, AHEAD = 4, DT = F16 ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16;
   __shared__ __align__(16) v4f sums[GROUPS][LANES];
@@ -660,26 +667,26 @@ __global__ __launch_bounds__(THREADS) void kv4_join_kernel(AttnArgs a) {
   if (i >= a.c.rows * a.q_heads) return;
   const int64_t row = i / a.q_heads;
   const int hq = (int)(i - row * a.q_heads), head = hq / a.group, g = hq - head * a.group;
-  int64_t seq = row;
+  int64_t seq = row, place = row;
   int token = 0;
   if (a.c.starts) {
     seq = last_of(a.c.seqs + 1, row, [&](int64_t s) { return (int64_t)a.c.starts[s]; });
     if (seq >= a.c.seqs) seq = -1;
-    if (seq >= 0) token = (int)(row - span(a.c.starts, seq, a.c.rows).first);
+    if (seq >= 0) {
+      const int64_t from = span(a.c.starts, seq, a.c.rows).first;
+      token = (int)(row - from);
+      place = from / a.tokens + seq + token / a.tokens;
+    }
   }
   int parts = 0;
   int64_t at = 0;   // the first segment's row
-  if (seq >= 0) {
-    Line line(a);
-    const Spot s = line.find([&](uint32_t, int64_t x) { return x == seq; });
-    const int row_tile = a.row_tiles > 1 ? g / (16 * RT) : 0, heads_here = min(a.group - row_tile * 16 * RT, a.row_tiles > 1 ? 16 * RT : a.group);
-    const uint32_t tile = (uint32_t)(token / a.tokens * a.row_tiles + row_tile);
-    if (line.n && s.units && tile < s.tiles) {
-      const uint32_t u = s.units_before + tile * s.units, first = line.owner(u);
-      parts = (int)(line.owner(u + s.units - 1) - first) + 1;
-      if (parts == 1) return;   // (the one segment wrote the row)
-      at = (head * a.segments + first + s.tiles_before + tile) * a.tile_rows + token % a.tokens * heads_here + g - row_tile * 16 * RT;
-    }
+  if (seq >= 0 && a.c.lens[seq] > 0 && place < (int64_t)a.places) {
+    const int row_tile = g / (16 * RT), heads_here = min(a.group - row_tile * 16 * RT, a.row_tiles > 1 ? 16 * RT : a.group);
+    const int2 of = a.parts[place * a.row_tiles + row_tile];
+    // (starts that fall leave places that no wave has written)
+    parts = of.x >= 0 && of.y >= of.x && of.y < a.segments ? of.y - of.x + 1 : 0;
+    if (parts == 1) return;   // (the one segment wrote the row)
+    at = (head * a.segments + of.x) * a.tile_rows + token % a.tokens * heads_here + g - row_tile * 16 * RT;
   }
   float most = -INFINITY, total = 0.f;
   v4f x = {0.f, 0.f, 0.f, 0.f};
@@ -728,39 +735,36 @@ __global__ __launch_bounds__(THREADS) void kv4_join_kernel(AttnArgs a) {
   *(uint2*)(a.out + i * DH + lane * 4) = make_uint2(pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv));
 }
 
-// How a call's work is cut: 16-row tiles of a wave, tokens of its rows, waves for a group's heads; the waves that share a
-// head's work evenly (of all heads as many as run at once), or 0: each tile of rows has one of its own. That is so where its keys are one
-// unit at most (a second kernel would be there for nothing), and where the tiles are so many that they even out.
+// How a call's work is cut: tokens of a wave's rows, waves for a group's heads; the waves that share a head's work evenly (of
+// all heads as many as run at once), or 0: each tile of rows has one of its own. To share takes a second kernel and a look at
+// every sequence, about 2 us and 1 for 20 rows; not to share takes as long as the longest sequence's wave, 1.65 us a unit
+// (which the table's width bounds), unless there are several waves for every place, which even out by themselves. Measured,
+// us, shared and not (32 heads over 8, lengths of up to 100, 500 and 4000): 64 sequences 16, 12; 21, 23; 69, 127; 256: 31, 16;
+// 54, 39; 173, 206; 1024: 94, 42; 157, 110; 526, 536; 128 and 256 of 5 tokens each, up to 3000: 160, 169; 284, 234.
 struct Plan {
-  int rt, tokens, tile_rows, row_tiles, shares;
+  int tokens, tile_rows, row_tiles, shares;
   int64_t places, segments;
+  int64_t parts_at(int64_t heads, int64_t dim) const { return heads * segments * tile_rows * (dim + 2) * 4; }   // bytes
+  int64_t bytes(int64_t heads, int64_t dim) const { return shares ? parts_at(heads, dim) + places * row_tiles * 8 : 0; }
 };
 Plan plan(int64_t seqs, int64_t rows, int64_t group, int64_t heads, int64_t dim, bool single, int64_t width) {
   Plan p;
-  const int64_t each = single ? group : group * ((rows + seqs - 1) / seqs);   // rows of a sequence, about
-  p.rt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
-  p.tokens = (int)std::max<int64_t>(1, 16 * p.rt / group);
-  p.tile_rows = (int)std::min<int64_t>(16 * p.rt, p.tokens * group);
-  p.row_tiles = (int)((group + 16 * p.rt - 1) / (16 * p.rt));
+  p.tokens = (int)std::max<int64_t>(1, 16 * RT / group);
+  p.tile_rows = (int)std::min<int64_t>(16 * RT, p.tokens * group);
+  p.row_tiles = (int)((group + 16 * RT - 1) / (16 * RT));
   p.places = single ? seqs : places_of(rows, seqs, p.tokens);
-  const int waves = dim == 128 ? (p.rt == 1 ? 3 : p.rt == 2 ? 2 : 1) : (p.rt == 1 ? 4 : p.rt == 2 ? 3 : 2);   // ATTN_WAVES
+  const int waves = dim == 128 ? ATTN_WAVES<128> : ATTN_WAVES<64>;
   const int64_t tiles = p.places * p.row_tiles, most = (width * PAGE + UNIT - 1) / UNIT;
-  p.shares = most > 1 && tiles * heads < 16 * 1024 * waves && tiles * most < 1 << 30 ? (int)(1024 * waves / heads) : 0;
+  p.shares = 16 * most > rows + 40 && tiles * heads < 4 * 1024 * waves && tiles * most < 1 << 30 ? (int)(1024 * waves / heads) : 0;
   p.segments = p.shares ? p.shares + tiles : 0;
   return p;
 }
 
-template <int DH, bool F16, int RT>
+template <int DH, bool F16>
 void launch_attn(const AttnArgs& a, hipStream_t stream) {
   const int64_t grid = a.shares ? a.shares * a.c.heads : (int64_t)a.places * a.c.heads * a.row_tiles;
-  kv4_attn_kernel<DH, F16, RT><<<grid_of((grid + WAVES - 1) / WAVES), THREADS, 0, stream>>>(a);
-  if (a.shares) kv4_join_kernel<DH, F16, RT><<<grid_of(a.c.rows * a.q_heads), THREADS, 0, stream>>>(a);
-}
-template <int DH, bool F16>
-void launch_attn(const AttnArgs& a, int rt, hipStream_t stream) {
-  if (rt == 1) launch_attn<DH, F16, 1>(a, stream);
-  else if (rt == 2) launch_attn<DH, F16, 2>(a, stream);
-  else launch_attn<DH, F16, 4>(a, stream);
+  kv4_attn_kernel<DH, F16><<<grid_of((grid + WAVES - 1) / WAVES), THREADS, 0, stream>>>(a);
+  if (a.shares) kv4_join_kernel<DH, F16><<<grid_of(a.c.rows * a.q_heads), THREADS, 0, stream>>>(a);
 }
 
 int check_pages(int64_t seqs, int64_t rows, int64_t heads, int64_t dim, const int32_t* starts, const int32_t* lens,
@@ -843,7 +847,7 @@ extern "C" int64_t lbw_kv4_attn_workspace_bytes(int64_t seqs, int64_t rows, int6
                                                 int single) {
   if (seqs < 1 || rows < 1 || heads < 1 || q_heads < heads) return 0;
   const Plan p = plan(seqs, rows, q_heads / heads, heads, dim, single, width);
-  return heads * p.segments * p.tile_rows * (dim + 2) * 4;
+  return p.bytes(heads, dim);
 }
 
 extern "C" int lbw_kv4_attn(const void* q, int dtype, int64_t seqs, int64_t rows, int64_t q_heads, int64_t heads, int64_t dim,
@@ -864,9 +868,10 @@ extern "C" int lbw_kv4_attn(const void* q, int dtype, int64_t seqs, int64_t rows
   const AttnArgs a = {{(uint8_t*)k4, (uint8_t*)ks, (uint8_t*)v4, (uint8_t*)vs, heads, pages, width, t_s_seq, seqs, rows, starts, lens, table},
                       (const uint16_t*)q, q_s_tok, q_s_head, (int)q_heads, (int)(q_heads / heads), p.row_tiles, p.tokens, p.tile_rows,
                       (uint32_t)p.places, (uint32_t)p.shares, p.segments, sm_scale * LOG2E, (uint16_t*)out, part,
-                      part ? part + heads * p.segments * p.tile_rows * dim : nullptr};
+                      part ? part + heads * p.segments * p.tile_rows * dim : nullptr,
+                      part ? (int2*)((uint8_t*)part + p.parts_at(heads, dim)) : nullptr};
   const bool f16 = dtype == LBW_DTYPE_FP16;
-  if (dim == 128) f16 ? launch_attn<128, true>(a, p.rt, (hipStream_t)stream) : launch_attn<128, false>(a, p.rt, (hipStream_t)stream);
-  else f16 ? launch_attn<64, true>(a, p.rt, (hipStream_t)stream) : launch_attn<64, false>(a, p.rt, (hipStream_t)stream);
+  if (dim == 128) f16 ? launch_attn<128, true>(a, (hipStream_t)stream) : launch_attn<128, false>(a, (hipStream_t)stream);
+  else f16 ? launch_attn<64, true>(a, (hipStream_t)stream) : launch_attn<64, false>(a, (hipStream_t)stream);
   return hipGetLastError() == hipSuccess ? LBW_OK : LBW_E_LAUNCH;
 }

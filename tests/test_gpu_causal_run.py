@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import causal
-from test_gpu_causal import DEV, DT, E, _check_norm_rotary, _check_packed, _dev, _filled, _gen, _packed_bounds, _rand, _starts, _table, _within
+from test_gpu_causal import DEV, DT, E, _check_cache_attend, _check_norm_rotary, _check_packed, _dev, _filled, _gen, _packed_bounds, _rand, _starts, _table, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -413,15 +413,16 @@ def test_smallest_calls():
     assert not cache.attend(0, q, _dev([[0]]), _dev([0])).any()
 
 
+@pytest.mark.parametrize("width", [3, 60])
 @pytest.mark.parametrize("seqs", [40, 200])
-def test_cache_with_falling_starts(seqs):
+def test_cache_with_falling_starts(seqs, width):
     """Starts that fall have no particular answer; the calls end, stay inside their tensors, and leave what the table does not name."""
     g = _gen(41)
     rows, heads, d = 8, 2, 64
     cache = _filled(g, 3 * seqs, heads, d)
     before = [x.clone() for x in (cache.k, cache.k_scale, cache.v, cache.v_scale)]
     q, k, v = (_rand(g, rows, h, d, dtype=torch.bfloat16) for h in (4, heads, heads))
-    table, lens = _dev([[i, -1, 2 * seqs + i] for i in range(seqs)]), _dev([150] * seqs)
+    table, lens = _dev([[i, -1, 2 * seqs + i] + [-1] * (width - 3) for i in range(seqs)]), _dev([150] * seqs)
     for starts in ([0, rows] * (seqs // 2) + [0], [rows] * seqs + [0], [0] + [2 ** 31 - 1, -5] * (seqs // 2)):
         args = (table, lens, _dev(starts))
         cache.attend(0, q, *args)
@@ -430,3 +431,23 @@ def test_cache_with_falling_starts(seqs):
     torch.cuda.synchronize()
     for x, y in zip((cache.k, cache.k_scale, cache.v, cache.v_scale), before):
         assert torch.equal(x[:, seqs:2 * seqs], y[:, seqs:2 * seqs])
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "bf16"), (128, "fp16")])
+@pytest.mark.parametrize("seqs", [63, 64, 65, 130, 300])
+def test_cache_attend_shares_of_many_sequences(seqs, d, dtype):
+    """Keys shared evenly over waves, of more sequences than a wave has lanes (a wide table says that they may be long): single
+    tokens, and a few or none of each; lengths of 0, some that end a page."""
+    lens = [(67 * i) % 190 for i in range(seqs)]
+    lens[seqs // 2] = 1500
+    _check_cache_attend(seqs, [1] * seqs, lens, 4, 2, d, dtype, width=60, starts=False)
+    _check_cache_attend(seqs + 1, [(i * 7) % 4 for i in range(seqs)], lens, 6, 1, d, dtype, width=100)
+
+
+def test_cache_attend_whole_tiles():
+    """Each tile of rows by a wave of its own: many sequences under a narrow table, several tokens, many heads."""
+    lens = [(67 * i) % 250 for i in range(150)]
+    for dtype in DT:
+        if dtype != "fp32":
+            _check_cache_attend(50, [1] * 150, lens, 4, 2, 128, dtype, starts=False)
+            _check_cache_attend(51, [(i * 7) % 8 for i in range(150)], lens, 20, 1, 64, dtype, tail=3)
