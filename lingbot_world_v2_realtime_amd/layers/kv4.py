@@ -17,8 +17,8 @@ class KV4Cache:
     """Pages of 64 tokens for each of `layers` layers (include/lbw_causal.h has the layout): K and V as e2m1 codes with a
     power of two for each 32 channels of a token (OCP MXFP4). Which pages a sequence holds is the caller's to say: `table`
     int32 [S, pages of a sequence] and `lens` int32 [S] on the GPU, the tokens of each sequence with those of the call. A
-    call's tokens are the newest of each sequence: rows starts[s] .. starts[s + 1] (int32 [S + 1]) of k, v or q, the last
-    row the sequence's last token; starts None: one row for each sequence. What lies past a row of the table, or in a page that
+    call's tokens are the newest of each sequence: rows starts[s] .. starts[s + 1] (int32 [S + 1], not falling) of k, v or q,
+    the last row the sequence's last token; starts None: one row for each sequence. What lies past a row of the table, or in a page that
     the cache does not have, is not written, reads as 0 and is not attended. Nothing here waits for the GPU, so all of
     it can be captured in a HIP graph, and lengths and tables may change between replays; table's width bounds them."""
     k: torch.Tensor          # uint8 [layers, pages, heads, 64, D / 2]
