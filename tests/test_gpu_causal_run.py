@@ -451,3 +451,35 @@ def test_cache_attend_whole_tiles():
         if dtype != "fp32":
             _check_cache_attend(50, [1] * 150, lens, 4, 2, 128, dtype, starts=False)
             _check_cache_attend(51, [(i * 7) % 8 for i in range(150)], lens, 20, 1, 64, dtype, tail=3)
+
+
+@pytest.mark.parametrize("hq,hk", [(96, 12), (45, 45), (24, 24), (48, 24), (36, 36)])
+@pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16")])
+def test_packed_forms_of_several_sequences(hq, hk, d, dtype):
+    """Each size of a workgroup's tile over sequences of different lengths, heads that share XCDs in every way."""
+    _check_packed(hq + hk, [300, 0, 77, 129, 5, 640], [300, 12, 140, 100, 5, 640], hq, hk, d, dtype, tail=2)
+
+
+@pytest.mark.parametrize("seqs", [61, 62, 63])
+def test_packed_as_many_sequences_as_a_wave_looks_at(seqs):
+    lens = [(53 * i) % 170 for i in range(seqs)]
+    _check_packed(seqs, lens, [max(0, n + i % 5 - 2) for i, n in enumerate(lens)], 2, 1, 64, head=3, tail=5)
+
+
+def test_packed_is_the_same_every_time():
+    """No sum has an order of its own: a training step's bits, over and over, beside other work."""
+    from lingbot_world_v2_realtime_amd import packed_attention
+    g = _gen(60)
+    lens = [900, 33, 400, 128]
+    q, k, v = (_rand(g, sum(lens), h, 128, dtype=torch.bfloat16).requires_grad_() for h in (12, 4, 4))
+    do, st = _rand(g, sum(lens), 12, 128, dtype=torch.bfloat16), _dev(_starts(lens))
+    other, noise = torch.cuda.Stream(), torch.randn(2048, 2048, device=DEV)
+    want = None
+    for _ in range(6):
+        with torch.cuda.stream(other):
+            noise = noise @ noise * 1e-2
+        out = packed_attention(q, k, v, st)
+        got = (out.detach(), *torch.autograd.grad(out, (q, k, v), do))
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.cuda.synchronize()
