@@ -161,7 +161,7 @@ __device__ __forceinline__ Block block_of(const Pages& c, int64_t want) {
   const int64_t base = min(max((int64_t)c.starts[s], (int64_t)0), c.rows) / BLOCK + 2 * s;
   const int64_t pos = ((from >> 5) + want - base) * BLOCK;
   static_assert(BLOCK == 1 << 5, "the shift rounds down below zero too");
-  if (of.n == 0 || pos >= to) return {-1, 0, 0, 0, 0};
+  if (of.n == 0 || want < base || pos >= to) return {-1, 0, 0, 0, 0};   // (starts that fall: a sequence behind the number)
   return {s, of.first + pos - from, pos, (int)max(from - pos, (int64_t)0), (int)min(to - pos, (int64_t)BLOCK)};
 }
 
@@ -673,9 +673,10 @@ __global__ __launch_bounds__(THREADS) void kv4_join_kernel(AttnArgs a) {
     seq = last_of(a.c.seqs + 1, row, [&](int64_t s) { return (int64_t)a.c.starts[s]; });
     if (seq >= a.c.seqs) seq = -1;
     if (seq >= 0) {
-      const int64_t from = span(a.c.starts, seq, a.c.rows).first;
-      token = (int)(row - from);
-      place = from / a.tokens + seq + token / a.tokens;
+      const Span of = span(a.c.starts, seq, a.c.rows);
+      token = (int)(row - of.first);
+      place = of.first / a.tokens + seq + token / a.tokens;
+      if (token < 0 || token >= of.n) seq = -1;   // (starts that fall: a sequence that does not hold the row)
     }
   }
   int parts = 0;

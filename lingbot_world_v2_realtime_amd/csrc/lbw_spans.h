@@ -37,7 +37,8 @@ __device__ __forceinline__ int64_t last_of(int64_t n, int64_t want, F f) {
 
 // Tiles of T rows of every sequence, numbered with gaps: those of sequence s from starts[s] / T + s on, which leaves room for
 // every tile (a sequence from a to b has b / T - a / T + 1 at most) and needs no sum over the sequences before it. There are
-// places_of(rows) numbers; a number without a tile has seq < 0.
+// places_of(rows) numbers; a number without a tile has seq < 0 (one before its sequence's first, too: where starts fall, the
+// search may end at a sequence that begins behind it).
 struct Place {
   int seq, tile, tiles;   // (tiles: of the sequence)
 };
@@ -48,7 +49,7 @@ __device__ __forceinline__ Place place(const int32_t* starts, int64_t seqs, int6
   if (s < 0) return {-1, 0, 0};
   const int tiles = (span(starts, s, rows).n + T - 1) / T;
   const int64_t tile = want - base(s);
-  if (tile >= tiles) return {-1, 0, 0};
+  if (tile < 0 || tile >= tiles) return {-1, 0, 0};
   return {__builtin_amdgcn_readfirstlane((int)s), __builtin_amdgcn_readfirstlane((int)tile), __builtin_amdgcn_readfirstlane(tiles)};
 }
 

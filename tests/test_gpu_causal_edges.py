@@ -1,0 +1,97 @@
+"""Causal self-attention at the edges of what its calls allow: starts that have no meaning, which must leave every tensor's
+surroundings alone. Bounds as in test_gpu_causal.py.
+"""
+import pytest
+import torch
+
+from test_gpu_causal import DEV, _dev, _filled, _gen, _rand, _starts
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- starts that fall
+
+
+def _falling(seqs, rows):
+    """Starts of `seqs` sequences that rise and fall: searches among them end at sequences that begin behind what is searched."""
+    return {"up and down": ([0, rows] * (seqs + 1))[:seqs + 1], "saw": [97 * i % rows for i in range(seqs + 1)],
+            "one fall": [rows] * seqs + [0], "out of range": ([0] + [2 ** 31 - 1, -5] * seqs)[:seqs + 1]}
+
+
+class _Guarded:
+    """Tensors in the middle of larger ones, whose ends hold one value and have to go on doing so."""
+
+    def __init__(self, margin):
+        self.margin, self.all = margin, []
+
+    def make(self, x, value):
+        flat = torch.full((x.numel() + 2 * self.margin,), value, dtype=x.dtype, device=DEV)
+        inner = flat[self.margin:self.margin + x.numel()].view(x.shape)
+        inner.copy_(x)
+        self.all.append((flat, x.numel(), value))
+        return inner
+
+    def check(self):
+        for flat, n, value in self.all:
+            for end in (flat[:self.margin], flat[self.margin + n:]):
+                assert bool(end.isnan().all() if value != value else (end == value).all())
+
+
+@pytest.mark.parametrize("seqs", [63, 64, 65, 200])
+@pytest.mark.parametrize("heads", [1, 40])
+def test_packed_with_falling_starts(lib, seqs, heads):
+    """No particular answer, but nothing outside is read (NaN lies there, and the outputs are finite) or written."""
+    rows, d, g = 300, 64, _gen(seqs)
+    stream = torch.cuda.current_stream().cuda_stream
+    nan = float("nan")
+    for name, st in _falling(seqs, rows).items():
+        for starts, k_starts in ((st, st), (_starts([0] * (seqs - 1) + [rows]), st), (st, _starts([0] * (seqs - 1) + [rows]))):
+            box = _Guarded(8192 * heads)
+            q, k, v, do = (box.make(_rand(g, rows, heads, d, dtype=torch.bfloat16), nan) for _ in range(4))
+            zero = torch.zeros_like(q)
+            out, rest, dq, dk, dv = (box.make(zero, 7.0) for _ in range(5))
+            lse, ws = (box.make(torch.zeros(heads, rows, device=DEV), 7.0) for _ in range(2))
+            a, b = _dev(starts), _dev(k_starts)
+            strides = [heads * d, d]
+            assert lib.lbw_packed_attn_bwd_workspace_bytes(rows, rows, heads, heads) <= 4 * ws.numel()
+            assert lib.lbw_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, seqs, rows, rows, heads, heads, d, *strides * 3, a.data_ptr(),
+                                           b.data_ptr(), 1, 0.125, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), stream) == 0
+            assert lib.lbw_packed_attn_bwd(do.data_ptr(), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), 0,
+                                           seqs, rows, rows, heads, heads, d, *strides * 4, a.data_ptr(), b.data_ptr(), 1, 0.125, dq.data_ptr(),
+                                           dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), stream) == 0
+            torch.cuda.synchronize()
+            box.check()
+            assert all(bool(x.isfinite().all()) for x in (out, dq, dk, dv)), name
+
+
+@pytest.mark.parametrize("width", [2, 60])
+@pytest.mark.parametrize("rows", [8, 300])
+@pytest.mark.parametrize("seqs", [40, 64, 200])
+def test_cache_with_falling_starts_stays_inside(lib, seqs, rows, width):
+    """The cache's calls, by a wave a tile (narrow tables) and shared (wide ones): NaN around every input and in front of the
+    workspace, whose own words claim that a tile has two segments; nothing outside an output changes."""
+    heads, hq, d, g = 2, 4, 64, _gen(rows + seqs)
+    stream = torch.cuda.current_stream().cuda_stream
+    nan = float("nan")
+    table, lens = _dev([[i, seqs + i] + [-1] * (width - 2) for i in range(seqs)]), _dev([128] * seqs)
+    for name, st in _falling(seqs, rows).items():
+        box = _Guarded(1 << 16)
+        q, k, v = (box.make(_rand(g, rows, h, d, dtype=torch.bfloat16), nan) for h in (hq, heads, heads))
+        out, rk, rv = (box.make(torch.zeros(rows, h, d, dtype=torch.bfloat16, device=DEV), 7.0) for h in (hq, heads, heads))
+        cache, starts = _filled(g, 2 * seqs, heads, d), _dev(st)
+        parts = [box.make(x.view(-1), 7).view(x.shape) for x in (cache.k, cache.k_scale, cache.v, cache.v_scale)]
+        call = (starts.data_ptr(), lens.data_ptr(), table.data_ptr(), width, width, 2 * seqs, *(x.data_ptr() for x in parts))
+        bytes_ = lib.lbw_kv4_attn_workspace_bytes(seqs, rows, hq, heads, d, width, 0)
+        assert (bytes_ > 0) == (16 * width > rows + 40)
+        ws = torch.full((bytes_ // 4 + (2 << 16),), nan, device=DEV)
+        inner = ws[1 << 16:(1 << 16) + bytes_ // 4]
+        inner.fill_(1.0)
+        places = rows // 8 + seqs if bytes_ else 0   # (two words for each tile of 8 tokens lie at the end: its first segment and its last)
+        inner[inner.numel() - 2 * places:].view(torch.int32).copy_(torch.arange(2 * places, device=DEV) % 2)
+        assert lib.lbw_kv4_attn(q.data_ptr(), 0, seqs, rows, hq, heads, d, hq * d, d, *call, 0.125, out.data_ptr(), inner.data_ptr(), stream) == 0
+        assert lib.lbw_kv4_read(seqs, rows, heads, d, *call, rk.data_ptr(), rv.data_ptr(), stream) == 0
+        assert lib.lbw_kv4_write(k.data_ptr(), v.data_ptr(), 0, seqs, rows, heads, d, *[heads * d, d] * 2, *call, stream) == 0
+        torch.cuda.synchronize()
+        box.check()
+        assert bool(ws[:1 << 16].isnan().all() and ws[(1 << 16) + bytes_ // 4:].isnan().all())
+        assert all(bool(x.isfinite().all()) for x in (out, rk, rv)), name
