@@ -111,7 +111,8 @@ int lbw_kv4_read(int64_t seqs, int64_t rows, int64_t heads, int64_t dim, const i
                  const uint8_t* ks, const uint8_t* v4, const uint8_t* vs, void* k, void* v, void* stream);
 
 /*
- * Attention of q [rows][q_heads][dim] (bf16 or fp16) over the pages: row r of sequence s sees the tokens up to its own.
+ * Attention of q [rows][q_heads][dim] (bf16 or fp16) over the pages: row r of sequence s sees the tokens up to its own, those
+ * of them that are in the table where a length passes it.
  * Head h of q reads head h / (q_heads / heads). out packed, of q's type; a row that sees nothing, or of no sequence, is 0.
  * The values of the cache enter the products exactly, sums and softmax are fp32, its weights are rounded to bf16 for bf16
  * q and to twice that length for fp16. `workspace`: lbw_kv4_attn_workspace_bytes(...) bytes, 16-byte aligned; calls that

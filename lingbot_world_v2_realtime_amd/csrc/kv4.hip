@@ -437,11 +437,12 @@ __global__ __launch_bounds__(THREADS, ATTN_WAVES<DH>) void kv4_attn_kernel(AttnA
   const int count = __builtin_amdgcn_readfirstlane(of.n);
   const uint32_t row_tile = tile % a.row_tiles;
   const int token0 = (int)(tile / a.row_tiles) * a.tokens;
-  const int64_t len = min(max((int64_t)__builtin_amdgcn_readfirstlane(a.c.lens[seq]), (int64_t)0), a.c.width * PAGE);
+  // (the rows' places go by the length as it is, the keys end where the table does)
+  const int64_t held = __builtin_amdgcn_readfirstlane(a.c.lens[seq]), len = min(max(held, (int64_t)0), a.c.width * PAGE);
   // row i of the tile: token token0 + i / heads_here, head i % heads_here of the group (from row_tile on where they are many)
   const int group0 = row_tile * 16 * RT, heads_here = min(a.group - group0, a.row_tiles > 1 ? 16 * RT : a.group);
   const int rows = min(a.tokens, count - token0) * heads_here;
-  const int64_t seen = len - count + token0 + 1;   // keys that the first token sees
+  const int64_t seen = held - count + token0 + 1;   // keys that the first token sees, were all of them in the table
   const int upto = (int)max((int64_t)0, min(len, seen + min(a.tokens, count - token0) - 1));
   const uint32_t run = a.shares ? min(left, units - unit) : 0;
   const int k0 = (int)unit * UNIT, k1 = a.shares ? min(upto, k0 + (int)run * UNIT) : upto;

@@ -50,9 +50,9 @@ class KV4Cache:
 
     def attend(self, layer, q, table, lens, starts=None, sm_scale=None):
         """Attention of q [T, Hq, D] (bf16 or fp16, Hq a multiple of the cache's heads) over the pages, each row over the
-        tokens up to its own: a decoder's next token of every sequence, or a few drafted ones at once. Returns [T, Hq, D] of q's
-        type; rows that see nothing, and rows of no sequence, are 0. The cache's values enter the products exactly; softmax
-        and sums are fp32. Many tokens of a sequence at once are better served by packed_attention over read(). No
-        gradient."""
+        tokens up to its own (of those that the table holds): a decoder's next token of every sequence, or a few drafted ones
+        at once. Returns [T, Hq, D] of q's type; rows that see nothing, and rows of no sequence, are 0. The cache's values
+        enter the products exactly; softmax and sums are fp32. Many tokens of a sequence at once are better served by
+        packed_attention over read(). No gradient."""
         return kernels.block_binding().kv4_attend(self.k, self.k_scale, self.v, self.v_scale, layer, table, lens, starts, q,
                                                   sm_scale)

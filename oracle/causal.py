@@ -167,20 +167,22 @@ def slots(starts, lens, table, rows, pages):
 
 
 def cache_attend(q, k, v, starts, lens, table, scale=None):
-    """attend() of a call's rows over pages k, v [pages, heads, 64, D] of values."""
+    """attend() of a call's rows over pages k, v [pages, heads, 64, D] of values: a row sees the tokens up to its own, of those
+    that the table holds (its own may lie past it)."""
     heads, group = k.shape[1], q.shape[1] // k.shape[1]
     scale = q.shape[2] ** -0.5 if scale is None else scale
     like = {}
     for s, n in enumerate(lens):
         count = starts[s + 1] - starts[s]
-        n = min(max(n, 0), 64 * len(table[s]))
         if not count:
             continue
+        first = n - count   # the first row's place
+        n = min(max(n, 0), 64 * len(table[s]))
         at = [(table[s][t // 64], t % 64) for t in range(n)]
         held = torch.tensor([0 <= p < k.shape[0] for p, _ in at], dtype=torch.bool, device=q.device)
         page = torch.tensor([p if 0 <= p < k.shape[0] else 0 for p, _ in at], dtype=torch.long, device=q.device)
         place = torch.tensor([t for _, t in at], dtype=torch.long, device=q.device)
-        see = (torch.arange(n, device=q.device) < n - count + 1 + torch.arange(count, device=q.device)[:, None]) & held
+        see = (torch.arange(n, device=q.device) <= first + torch.arange(count, device=q.device)[:, None]) & held
         for h in range(q.shape[1]):
             r = attend(q[starts[s]:starts[s + 1], h], k[page, h // group, place], v[page, h // group, place], see, scale)
             for name, x in r.items():

@@ -122,3 +122,28 @@ def test_rotation_of_the_definitions_agrees():
     (y, _), _ = causal.norm_rotary(x, None, pos, freq, eps=0.0)
     r = x.square().mean(-1, keepdim=True).rsqrt()
     assert torch.allclose(y, block.rotary(x * r, pos, freq)[0])
+
+
+@pytest.mark.parametrize("counts,lens", [([5], [130]), ([10, 2], [70, 64]), ([70, 3, 1], [128, 200, 129]), ([4], [0]), ([4, 9], [-3, 2])])
+def test_cache_attend_sees_what_slots_hold(counts, lens):
+    """A row sees the held tokens up to its own place, as write and read place them, also where a length passes the table."""
+    g = _gen(sum(lens))
+    starts = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    table = [[2 * i, 2 * i + 1] for i in range(len(counts))]
+    table[0][0] = 90 if len(counts) > 1 else 0
+    pages, rows = 2 * len(counts), starts[-1]
+    k, v = (torch.randn(pages, 2, 64, 16, generator=g).double() for _ in range(2))
+    q = torch.randn(rows, 4, 16, generator=g)
+    out = causal.cache_attend(q, k, v, starts, lens, table)["out"]
+    for s, n in enumerate(lens):
+        held = causal.slots([0, max(n, 0)], [n], [table[s]], max(n, 0), pages)   # of each token of the sequence, where it lies
+        for r in range(starts[s], starts[s + 1]):
+            at = n - (starts[s + 1] - r)
+            seen = [slot for slot in held[:max(at + 1, 0)] if slot is not None]
+            for h in range(4):
+                if not seen:
+                    assert not out[r, h].any()
+                    continue
+                keys, vals = (torch.stack([x[p, h // 2, t] for p, t in seen]) for x in (k, v))
+                p = torch.softmax(keys @ q[r, h].double() / 4, 0)
+                assert torch.allclose(out[r, h], p @ vals)

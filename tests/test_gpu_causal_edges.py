@@ -1,10 +1,11 @@
 """Causal self-attention at the edges of what its calls allow: starts that have no meaning, which must leave every tensor's
-surroundings alone. Bounds as in test_gpu_causal.py.
+surroundings alone, and lengths past a table's width. Bounds as in test_gpu_causal.py.
 """
 import pytest
 import torch
 
-from test_gpu_causal import DEV, _dev, _filled, _gen, _rand, _starts
+from oracle import causal
+from test_gpu_causal import DEV, DT, _dev, _filled, _gen, _packed_bounds, _rand, _starts, _table, _together, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +96,42 @@ def test_cache_with_falling_starts_stays_inside(lib, seqs, rows, width):
         box.check()
         assert bool(ws[:1 << 16].isnan().all() and ws[(1 << 16) + bytes_ // 4:].isnan().all())
         assert all(bool(x.isfinite().all()) for x in (out, rk, rv)), name
+
+
+# ---------------------------------------------------------------- lengths past the table
+
+
+@pytest.mark.parametrize("counts,lens,width,hq,hk", [
+    ([5], [130], 2, 4, 2), ([10], [70], 1, 4, 1), ([3, 70, 5], [129, 150, 64], 2, 8, 2),   # a wave a tile
+    ([5, 9], [258, 300], 4, 4, 2), ([2, 1, 6], [700, 257, 255], 4, 40, 1), ([20], [3010], 47, 2, 2),   # shared
+    ([1, 30], [100, 2000], 1, 6, 3), ([7, 0, 3], [2 ** 31 - 1, 500, 66], 1, 2, 1)])
+@pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16")])
+def test_cache_attend_of_lengths_past_the_table(counts, lens, width, hq, hk, d, dtype):
+    """A row's place is that of write and read, whatever the table holds: rows inside it see the tokens up to their own, rows
+    past it all that there are."""
+    short = [min(n, 64 * width) for n in lens]
+    g = _gen(sum(counts))
+    st, t = _starts(counts, 2), DT[dtype]
+    pages = sum(-(-n // 64) for n in short) + 2
+    cache, table = _filled(g, pages, hk, d), _table(g, [-(-n // 64) for n in short], pages, width)
+    q = _rand(g, st[-1] + 3, hq, d, dtype=t)
+    out = cache.attend(0, q, _dev(table), _dev(lens), _dev(st))
+    assert torch.equal(out, cache.attend(0, q, _dev(table), _dev(lens), _dev(st)))
+    r = causal.cache_attend(q, *causal.unpack_pages(cache.k[0], cache.k_scale[0], cache.v[0], cache.v_scale[0]), st, lens, table)
+    h = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -16
+    _within(out, r["out"], (h + _packed_bounds(r, max(short), d, dtype)) * r["p_v"], f"{counts} of {lens}, {width} pages")
+    _together(out, r["out"], r["p2_v2"], f"{counts} of {lens}")
+
+
+def test_cache_rows_past_the_table_see_what_was_written():
+    """Written, read back and attended: a row whose own token lies inside the table answers as it does with a wider table."""
+    from lingbot_world_v2_realtime_amd import KV4Cache
+    g = _gen(71)
+    cache, st = KV4Cache.empty(1, 3, 2, 128, DEV), _dev([0, 60])
+    k, v = (_rand(g, 130, 2, 128, dtype=torch.bfloat16) for _ in range(2))
+    q, wide, narrow = _rand(g, 60, 4, 128, dtype=torch.bfloat16), _dev([[2, 0, 1]]), _dev([[2, 0]])
+    cache.write(0, k, v, wide, _dev([130]), _dev([0, 130]))
+    a, b = (cache.attend(0, q, t, _dev([130]), st) for t in (wide, narrow))
+    assert torch.equal(a[:58], b[:58]) and not torch.equal(a[58:], b[58:])
+    for row, n in ((0, 71), (57, 128), (59, 128)):
+        assert torch.equal(b[row], cache.attend(0, q[row:row + 1], narrow, _dev([n]))[0])
