@@ -238,7 +238,8 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_fwd_kernel(
   // (staged where no other wave may still be reading)
   static_assert(KW == 1 || STAGING<DH> <= (MT * 16 + 2) * 256, "a wave's staging lies inside what it reads");
   uint8_t* mine = lds + (KW > 1 ? qw * (MT * 16 + 2) * 256 : w * STAGING<DH>);
-  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  // A row that sees nothing is zero; one whose scores are all minus infinity has no softmax, and is NaN (0 / 0).
+  const float inv = total > 0.f || total != total ? 1.f / total : seen(row0 + (late & 31)) > 0 ? __builtin_nanf("") : 0.f;
   store_turned<DH, F16>(o, inv, mine, late, a.out + (qs.first + row0) * o_tok + head * DH, o_tok, n - row0);
   if (a.rest) {
     __builtin_amdgcn_wave_barrier();

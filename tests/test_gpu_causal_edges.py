@@ -1,11 +1,11 @@
 """Causal self-attention at the edges of what its calls allow: starts that have no meaning, which must leave every tensor's
-surroundings alone, and lengths past a table's width. Bounds as in test_gpu_causal.py.
+surroundings alone, lengths past a table's width, and infinities that leave a row no softmax. Bounds as in test_gpu_causal.py.
 """
 import pytest
 import torch
 
 from oracle import causal
-from test_gpu_causal import DEV, DT, _dev, _filled, _gen, _packed_bounds, _rand, _starts, _table, _together, _within
+from test_gpu_causal import DEV, DT, E, _dev, _filled, _gen, _packed_bounds, _rand, _starts, _table, _together, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +135,62 @@ def test_cache_rows_past_the_table_see_what_was_written():
     assert torch.equal(a[:58], b[:58]) and not torch.equal(a[58:], b[58:])
     for row, n in ((0, 71), (57, 128), (59, 128)):
         assert torch.equal(b[row], cache.attend(0, q[row:row + 1], narrow, _dev([n]))[0])
+
+
+# ---------------------------------------------------------------- scores that are all minus infinity
+
+
+def _held_together(x, value, bound, what):
+    """NaN where the definition has it, and within its bound elsewhere."""
+    assert torch.equal(x.isnan(), value.isnan()), what
+    keep = ~value.isnan()
+    _within(x[keep], value[keep], bound.expand_as(value)[keep], what)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads", [1, 80, 128])   # (the forms of a workgroup's tile)
+@pytest.mark.parametrize("causal_", [True, False])
+def test_packed_scores_of_minus_infinity(causal_, heads, d, dtype):
+    """A query whose infinity makes every score that it sees minus infinity has no softmax: its row is NaN, as the definition has
+    it, not the zeros of a row that sees nothing; so is its gradient, and those of the keys that it sees."""
+    from lingbot_world_v2_realtime_amd import packed_attention
+    g, t, lens, n = _gen(80), DT[dtype], [400, 33], 400
+    st = _starts(lens)
+    q, k, v, do = (_rand(g, sum(lens), heads, d, dtype=t) for _ in range(4))
+    k[..., 0] = k[..., 0].abs() + 0.125
+    rows = torch.arange(sum(lens), device=DEV)
+    for at in (0, 31, 130, 399):
+        bad, keep = q.clone(), (rows != at)[:, None, None]
+        bad[at, :, 0] = -float("inf")
+        leaves = [x.detach().requires_grad_() for x in (bad, k, v)]
+        out = packed_attention(*leaves, _dev(st), causal=causal_)
+        with torch.no_grad():
+            assert packed_attention(*leaves, _dev(st), causal=causal_)[at].isnan().all()
+        # (what the other rows have is what they have where this one's gradient is zero)
+        r = causal.packed(q[:, :1], k[:, :1], v[:, :1], st, st, causal=causal_, d_out=(do * keep)[:, :1])
+        h, rel = torch.finfo(t).eps / 2, _packed_bounds(r, n, d, dtype)
+        nan = torch.full((), float("nan"), dtype=torch.float64, device=DEV)
+        _held_together(out.detach()[:, :1], r["out"].where(keep, nan), (h + rel) * r["p_v"] + n * 2.0 ** -35, f"row {at}")
+        steps, top = E * (n / 16 + 16), rel.max()
+        unseen = ((rows > at) if causal_ else (rows >= n))[:, None, None]
+        for x, name in zip(torch.autograd.grad(out, leaves, do), ("dq", "dk", "dv")):
+            bound = (h + steps) * r[name + "_abs"] + (h + h * h) * r[name + "_wide16"] + (top + h * h + E * (d / 16 + 8)) * r[name + "_wide32"]
+            _held_together(x[:, :1], r[name].where(keep if name == "dq" else unseen, nan), bound, f"{name}, row {at}")
+
+
+def test_packed_key_of_minus_infinity():
+    """The same from a key's infinity: the row that sees it alone is NaN, those behind it give it no weight."""
+    from lingbot_world_v2_realtime_amd import packed_attention
+    for d, dtype in ((64, torch.float16), (128, torch.bfloat16)):
+        g = _gen(81)
+        q, k, v = (_rand(g, 70, 2, d, dtype=dtype) for _ in range(3))
+        q[..., 0] = q[..., 0].abs() + 0.125
+        k[0, :, 0] = -float("inf")
+        out = packed_attention(q, k, v, _dev([0, 70]))
+        r = causal.packed(q, k, v, [0, 70], [0, 70])
+        assert out[0].isnan().all() and out[1:].isfinite().all()
+        h = torch.finfo(dtype).eps / 2
+        k[0, :, 0] = 0
+        rel = _packed_bounds(causal.packed(q, k, v, [0, 70], [0, 70]), 70, d, dtype)
+        _held_together(out, r["out"], (h + rel) * v.double().abs().amax() + 70 * 2.0 ** -35, "out")
