@@ -264,6 +264,7 @@ __global__ __launch_bounds__(THREADS) void kv4_read_block_kernel(Pages c, uint16
 // ---------------------------------------------------------------- attention
 
 constexpr int KB = 32, WAVES = THREADS / 64;   // keys of a wave's step
+constexpr float LOWEST = -0x1.fffffep127f;
 
 struct AttnArgs {
   Pages c;
@@ -508,13 +509,14 @@ __global__ __launch_bounds__(THREADS, ATTN_WAVES<DH>) void kv4_attn_kernel(AttnA
     if (page >= 0) next.load(a.c, (int64_t)page * heads + head, key / KB & 1, lane);
     return page;
   };
-  int next_page = -1;
+  int next_page = -1, first_held = INT32_MAX;   // the first key in a page that there is
   if (k0 < k1) next_page = fetch(k0);
   for (int key = k0; key < k1; key += KB) {
     const int page = next_page;
     Step<DH> st = next;
     if (key + KB < k1) next_page = fetch(key + KB);
     if (page < 0) continue;
+    first_held = min(first_held, key);
     // Some row may not see all of these keys: those behind the last hold what they like, and a NaN must not reach the rows
     // that do not see it through a weight of zero. Their scales become 1 (127), and the NaN is put where it belongs below.
     const bool edge = key + KB > seen;
@@ -621,11 +623,14 @@ __global__ __launch_bounds__(THREADS, ATTN_WAVES<DH>) void kv4_attn_kernel(AttnA
   for (int rt = 0; rt < RT; ++rt) {
     const int i = rt * 16 + n;
     const float sum = sum_quarters(total[rt]);
+    // A sum of zero over keys that there are: all scores are minus infinity, and the row has no softmax (NaN), unless another
+    // segment has scores of it: to the join such a segment has a maximum, LOWEST, and a row that sees nothing has none.
+    const bool low = sum == 0.f && first_held < own[rt];
     if (i < rows) {
       if (whole) {
         const int tok = i / heads_here, h = i - tok * heads_here;
         uint16_t* to = a.out + ((first + token0 + tok) * a.q_heads + (int64_t)head * a.group + group0 + h) * DH + 4 * p;
-        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : low ? __builtin_nanf("") : 0.f;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
           constexpr int DT = F16 ? LBW_DTYPE_FP16 : LBW_DTYPE_BF16;
@@ -635,7 +640,7 @@ __global__ __launch_bounds__(THREADS, ATTN_WAVES<DH>) void kv4_attn_kernel(AttnA
         const int64_t at = ((int64_t)head * a.segments + id / heads + tiles_before + tile) * a.tile_rows + i;
 #pragma unroll
         for (int x = 0; x < NT; ++x) *(v4f*)(a.part + at * DH + 16 * x + 4 * p) = o[rt][x];
-        if (p == 0) *(float2*)(a.stats + at * 2) = make_float2(top[rt], sum);
+        if (p == 0) *(float2*)(a.stats + at * 2) = make_float2(low ? LOWEST : top[rt], sum);
       }
     }
   }
@@ -733,7 +738,7 @@ __global__ __launch_bounds__(THREADS) void kv4_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = fmaf(by, sums[k][lane][e], x[e]);
   }
-  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  const float inv = total > 0.f || total != total ? 1.f / total : top > -INFINITY ? __builtin_nanf("") : 0.f;
   *(uint2*)(a.out + i * DH + lane * 4) = make_uint2(pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv));
 }
 

@@ -194,3 +194,52 @@ def test_packed_key_of_minus_infinity():
         k[0, :, 0] = 0
         rel = _packed_bounds(causal.packed(q, k, v, [0, 70], [0, 70]), 70, d, dtype)
         _held_together(out, r["out"], (h + rel) * v.double().abs().amax() + 70 * 2.0 ** -35, "out")
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16")])
+@pytest.mark.parametrize("width,lens,counts", [(6, [130, 290, 40], [1, 1, 1]), (60, [130, 3000, 64], [1, 1, 1]), (60, [130, 3000, 40], [5, 2, 3]), (6, [130, 290, 40], [50, 20, 9])])
+def test_cache_scores_of_minus_infinity(width, lens, counts, d, dtype):
+    """The cache's attention likewise, by a wave and shared: a query's infinity against positive keys. Rows that see nothing, and rows
+    whose pages are all missing, stay zero."""
+    g, t = _gen(83), DT[dtype]
+    hq, hk, st = 6, 2, _starts(counts)
+    cache = _filled(g, 60, hk, d)
+    cache.k[..., 0] = cache.k[..., 0] & 0xF7 | 1   # channel 0 (a token's first code): 0.5 or more
+    table = _table(g, [-(-n // 64) for n in lens], 60, width)
+    table[2][0] = -1                               # the third sequence's only page
+    q = _rand(g, st[-1], hq, d, dtype=t)
+    one = counts == [1, 1, 1]
+    args = (_dev(table), _dev(lens), None if one else _dev(st))
+    want = cache.attend(0, q, *args)
+    kv = causal.unpack_pages(cache.k[0], cache.k_scale[0], cache.v[0], cache.v_scale[0])
+    assert bool((kv[0][..., 0] > 0).all())
+    for at in (0, st[1], st[2], st[3] - 1):
+        bad = q.clone()
+        bad[at, 1, 0] = -float("inf")
+        got = cache.attend(0, bad, *args)
+        keep = torch.ones(st[-1], hq, 1, dtype=torch.bool, device=DEV)
+        keep[at, 1] = at >= st[2]   # (the third's rows see no page that there is)
+        assert torch.equal(got.isnan(), ~keep.expand_as(got)), at
+        assert torch.equal(got.where(keep, torch.zeros_like(got)), want.where(keep, torch.zeros_like(got))), at
+        if at >= st[2]:
+            assert not got[at].any()
+
+
+def test_cache_scores_of_minus_infinity_in_a_part(lib):
+    """Scores that overflow to minus infinity over some of a row's pages and not over others: those weigh nothing."""
+    g = _gen(84)
+    cache = _filled(g, 60, 1, 64)
+    cache.k[..., 0] = cache.k[..., 0] & 0xF0 | 0xC     # channel 0: -2
+    cache.k_scale[..., 0] = 127
+    table = _dev([list(range(60))])
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=DEV)
+    q[0, 0, 0] = 2.0 ** 127
+    want = cache.attend(0, q, table, _dev([3840]), sm_scale=1.0)
+    assert want.isnan().all()                            # (every score is -2^128)
+    few = [7, 1000, 3839]
+    for t in few:
+        cache.k[0, t // 64, 0, t % 64, 0] &= 0xF0        # 0
+    got = cache.attend(0, q, table, _dev([3840]), sm_scale=1.0)
+    _, v = causal.unpack_pages(cache.k[0], cache.k_scale[0], cache.v[0], cache.v_scale[0])
+    mean = sum(v[t // 64, 0, t % 64] for t in few) / len(few)
+    _within(got[0, 0], mean, 2.0 ** -22 * mean.abs(), "three keys alike")
