@@ -250,12 +250,13 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 1 : 2) void packed_dkv_kernel(
         dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
       }
     }
-    const bool partly = r < w_all;   // queries that do not see a key
+    // queries that do not see a key; rows behind the last query are zeros, but a key that is not finite makes NaN of them
+    const bool partly = r < w_all || r + 32 > n;
     if (partly) {
       branch_here();
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (r + 8 * (i >> 2) + 4 * hf + (i & 3) < own) s[i] = dp[i] = 0.f;
+        if (const int row = r + 8 * (i >> 2) + 4 * hf + (i & 3); row < own || row >= n) s[i] = dp[i] = 0.f;
     }
     v4i pf[2], df[2];
     pack16<F16>(s, 1.f, pf);

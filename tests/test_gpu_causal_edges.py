@@ -243,3 +243,36 @@ def test_cache_scores_of_minus_infinity_in_a_part(lib):
     _, v = causal.unpack_pages(cache.k[0], cache.k_scale[0], cache.v[0], cache.v_scale[0])
     mean = sum(v[t // 64, 0, t % 64] for t in few) / len(few)
     _within(got[0, 0], mean, 2.0 ** -22 * mean.abs(), "three keys alike")
+
+
+def _grads_of_a_key_of_minus_infinity(heads, d, dtype, causal_, names):
+    """One key whose infinity makes its scores minus infinity, for every row that sees it: its weights are zero, and the other
+    rows' and keys' gradients those without it. Checks the first head's."""
+    from lingbot_world_v2_realtime_amd import packed_attention
+    g, t, n = _gen(82), DT[dtype], 400
+    q, k, v, do = (_rand(g, n, heads, d, dtype=t) for _ in range(4))
+    q[..., 0] = q[..., 0].abs() + 0.125
+    for at in (1, 31, 96, 130, 399):
+        bad, see, zero = k.clone(), causal.visible(n, n, causal_, DEV), k.clone()
+        bad[at, :, 0], zero[at, :, 0], see[:, at] = -float("inf"), 0, False
+        leaves = [x.detach().requires_grad_() for x in (q, bad, v)]
+        out = packed_attention(*leaves, _dev([0, n]), causal=causal_)
+        r = causal.attend(q[:, 0], zero[:, 0], v[:, 0], see, d ** -0.5, do[:, 0])
+        h, rel = torch.finfo(t).eps / 2, _packed_bounds(r, n, d, dtype)
+        _held_together(out.detach()[:, 0], r["out"], (h + rel) * r["p_v"] + n * 2.0 ** -35, f"out, key {at}")
+        # zero times its infinity is no number: in its channel, for every row that sees it
+        r["dq"][torch.arange(n, device=DEV) >= (at if causal_ else 0), 0] = float("nan")
+        steps, top = E * (n / 16 + 16), rel.max()
+        for x, name in zip(torch.autograd.grad(out, leaves, do), ("dq", "dk", "dv")):
+            if name in names:
+                bound = (h + steps) * r[name + "_abs"] + (h + h * h) * r[name + "_wide16"] + (top + h * h + E * (d / 16 + 8)) * r[name + "_wide32"]
+                _held_together(x[:, 0], r[name], bound, f"{name}, key {at}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads", [1, 80, 128])
+@pytest.mark.parametrize("causal_", [True, False])
+def test_packed_gradients_of_a_key_beside_rows_behind_the_last(causal_, heads, d, dtype):
+    """Rows behind the last query, which fill its tile, are no queries: such a key's dk and dv are zero, not NaN."""
+    _grads_of_a_key_of_minus_infinity(heads, d, dtype, causal_, ("dk", "dv"))
