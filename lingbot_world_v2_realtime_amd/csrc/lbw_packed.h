@@ -208,8 +208,9 @@ __device__ __forceinline__ v4i clean(v4i f) {
   }
   return f;
 }
-// Rows 32 x .. + 32 of a tile; sees(j): whether the lane's column sees row j of them.
-template <int DH, bool F16, class Sees>
+// Rows 32 x .. + 32 of a tile; sees(j): whether the lane's column sees row j of them. NAN_ALL: NaN for each such value, where
+// its weight can be zero, or NaN, but nothing else.
+template <int DH, bool F16, bool NAN_ALL = false, class Sees>
 __device__ __forceinline__ void add_odd(v16f (&o)[DH / 32], const uint8_t* tile, int x, int hf, const Sees& sees) {
 #pragma unroll 1
   for (int j = 0; j < 32; ++j) {
@@ -222,7 +223,7 @@ __device__ __forceinline__ void add_odd(v16f (&o)[DH / 32], const uint8_t* tile,
         const uint2 w = *(const uint2*)(row + (((4 * mt + c) ^ swizzle<DH>(j)) << 4) + 8 * hf);
         const float v[4] = {lo16<F16>(w.x), hi16<F16>(w.x), lo16<F16>(w.y), hi16<F16>(w.y)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][4 * c + e] += s && is_odd(v[e]) ? v[e] : 0.f;
+        for (int e = 0; e < 4; ++e) o[mt][4 * c + e] += s && is_odd(v[e]) ? (NAN_ALL ? __builtin_nanf("") : v[e]) : 0.f;
         __builtin_amdgcn_sched_barrier(0);   // (few registers rather than speed)
       }
   }

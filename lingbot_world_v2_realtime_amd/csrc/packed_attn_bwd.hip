@@ -519,8 +519,10 @@ __global__ __launch_bounds__(THREADS, DH == 128 ? 2 : 4) void packed_dq_kernel(B
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) tk[u][mt] = tr.get(kt, 2 * x + u, mt);
-        if (decltype(again)::value && partly) {   // (a key that is not finite has weights that are not, where it is seen)
+        if (decltype(again)::value && partly) {
           branch_here();
+          // a key that is not finite has weights that are not, where it is seen, or (its scores being minus infinity) zero
+          add_odd<DH, F16, true>(dq, kt, x, hf, [&](int j) { return j0 + j < own; });
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll

@@ -276,3 +276,12 @@ def _grads_of_a_key_of_minus_infinity(heads, d, dtype, causal_, names):
 def test_packed_gradients_of_a_key_beside_rows_behind_the_last(causal_, heads, d, dtype):
     """Rows behind the last query, which fill its tile, are no queries: such a key's dk and dv are zero, not NaN."""
     _grads_of_a_key_of_minus_infinity(heads, d, dtype, causal_, ("dk", "dv"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads", [1, 80, 128])
+@pytest.mark.parametrize("causal_", [True, False])
+def test_packed_gradient_of_rows_that_see_a_key_of_minus_infinity(causal_, heads, d, dtype):
+    """dq is NaN in the infinity's channel for the rows that see it, in a tile that is partly seen or wholly, and there alone."""
+    _grads_of_a_key_of_minus_infinity(heads, d, dtype, causal_, ("dq",))
