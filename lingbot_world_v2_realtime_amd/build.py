@@ -28,6 +28,12 @@ def hipcc():
     return os.path.join(rocm, "bin", "hipcc")
 
 
+def jobs():
+    """Compilers side by side: MAX_JOBS where it is a number, else 8; no more than processors or sources."""
+    want = os.environ.get("MAX_JOBS", "")
+    return max(1, min(int(want) if want.isdecimal() else 8, os.cpu_count() or 1, len(SOURCES)))
+
+
 def build_library(verbose=False):
     """Compile every HIP source, several side by side, and link them into liblbw_attn.so (always recompiles). Returns the library
     path."""
@@ -42,8 +48,7 @@ def build_library(verbose=False):
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("hipcc failed building liblbw_attn.so")
 
-    jobs = min(int(os.environ.get("MAX_JOBS", 8)), os.cpu_count() or 1, len(SOURCES))
-    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(max(jobs, 1)) as pool:
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(jobs()) as pool:
         outs = [os.path.join(objects, s + ".o") for s in SOURCES]
         list(pool.map(run, [["-I", os.path.join(ROOT, "include"), "-c", os.path.join(HERE, "csrc", s), "-o", o]
                             for s, o in zip(SOURCES, outs)]))

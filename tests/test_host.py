@@ -204,3 +204,13 @@ def test_same_device_guard():
     kernels._same_device("x", a, None, a)
     with pytest.raises(ValueError):
         kernels._same_device("x", a, b)
+
+
+@pytest.mark.parametrize("set_to", [None, "", "0", "1", "64", "many", "-2", "3.5"])
+def test_build_takes_any_number_of_jobs(monkeypatch, set_to):
+    from lingbot_world_v2_realtime_amd import build
+    monkeypatch.delenv("MAX_JOBS", raising=False)
+    if set_to is not None:
+        monkeypatch.setenv("MAX_JOBS", set_to)
+    assert 1 <= build.jobs() <= len(build.SOURCES)
+    assert set_to not in ("0", "1") or build.jobs() == 1
