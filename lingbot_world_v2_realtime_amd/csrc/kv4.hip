@@ -6,7 +6,7 @@
 // 32; its 16 bytes of V are 8 keys at 4 channels, in the order in which S^T leaves their weights in registers.
 //
 // All of it is bound by memory, or by a launch's latency where there is little. 6914 tokens of 8 heads of 128 written 9.5 us, read
-// back 9.5 (3.8 TB/s each); 64 sequences' single tokens 5.2 and 4.2. One query of 32 heads over 8 for each of 61 sequences of up to
+// back 9.5 (3.8 TB/s each); 64 sequences' single tokens 5.1 and 4.8, with starts (by blocks) 5.2 and 4.1. One query of 32 heads over 8 for each of 61 sequences of up to
 // 6032: 50 us and 5 to join the segments (204 MB: 3.7 TB/s in all); 5 tokens of 12 heads in fp16 over 7 sequences of up to
 // 24128: 44 and 5 (159 MB: 3.2); one sequence of 1508: 8 and 3.
 #include "lbw_spans.h"

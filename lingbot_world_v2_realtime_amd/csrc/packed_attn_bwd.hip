@@ -55,8 +55,8 @@ __global__ __launch_bounds__(THREADS) void packed_delta_kernel(BwdArgs a) {
 }
 
 // dS in fp16 may leave that type's range in either direction. Each lane (a query, or a key) holds its values times a power
-// of two of its own, so that the largest so far lies in [2^4, 2^14), and its sums with the same factor: `by` is what they have to be
-// multiplied by when it changes (seldom; 1 else).
+// of two of its own, so that the largest so far lies in [2^8, 2^14) (lower where that power would have to pass 2^126), and its
+// sums with the same factor: `by` is what they have to be multiplied by when it changes (seldom; 1 else).
 struct Range {
   float scale = 1.f;
   bool set = false;

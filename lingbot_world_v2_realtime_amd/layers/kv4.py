@@ -52,7 +52,8 @@ class KV4Cache:
         """Attention of q [T, Hq, D] (bf16 or fp16, Hq a multiple of the cache's heads) over the pages, each row over the
         tokens up to its own (of those that the table holds): a decoder's next token of every sequence, or a few drafted ones
         at once. Returns [T, Hq, D] of q's type; rows that see nothing, and rows of no sequence, are 0. The cache's values
-        enter the products exactly; softmax and sums are fp32. Many tokens of a sequence at once are better served by
-        packed_attention over read(). No gradient."""
+        enter the products exactly; softmax and sums are fp32, the softmax's weights are rounded to bf16 before they meet V
+        where q is bf16, and held in two bf16 values where it is fp16. Many tokens of a sequence at once are better served
+        by packed_attention over read(). No gradient."""
         return kernels.block_binding().kv4_attend(self.k, self.k_scale, self.v, self.v_scale, layer, table, lens, starts, q,
                                                   sm_scale)
