@@ -1,5 +1,6 @@
 """Causal self-attention at the edges of what its calls allow: starts that have no meaning, which must leave every tensor's
-surroundings alone, lengths past a table's width, and infinities that leave a row no softmax. Bounds as in test_gpu_causal.py.
+surroundings alone, lengths past a table's width, infinities that leave a row no softmax, rows and tables that lie anywhere, and as many
+sequences and heads as there may be. Bounds as in test_gpu_causal.py.
 """
 import pytest
 import torch
@@ -285,3 +286,89 @@ def test_packed_gradients_of_a_key_beside_rows_behind_the_last(causal_, heads, d
 def test_packed_gradient_of_rows_that_see_a_key_of_minus_infinity(causal_, heads, d, dtype):
     """dq is NaN in the infinity's channel for the rows that see it, in a tile that is partly seen or wholly, and there alone."""
     _grads_of_a_key_of_minus_infinity(heads, d, dtype, causal_, ("dq",))
+
+
+# ---------------------------------------------------------------- rows and tables that lie anywhere
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16")])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [70, 5, 33]])
+def test_cache_calls_of_views(counts, d, dtype):
+    """Parts of one projection, rows that the kernels do not load from (copied), one row for all heads, a table that is a part of a
+    wider one, and one row of it for every sequence: as their contiguous copies."""
+    from lingbot_world_v2_realtime_amd import KV4Cache
+    g, t, hq, hk, st = _gen(90), DT[dtype], 4, 2, _starts(counts)
+    rows, starts = st[-1], None if counts == [1, 1, 1] else _dev(st)
+
+    def fused(h):
+        return _rand(g, rows, h + 5, d, dtype=t)[:, 3:3 + h]
+
+    def odd(h):
+        return _rand(g, rows, h, d + 3, dtype=t)[..., 1:d + 1]
+
+    def turned(h):
+        return _rand(g, h, rows, d, dtype=t).transpose(0, 1)
+
+    def spread(h):
+        return _rand(g, rows, 1, d, dtype=t).expand(rows, h, d)
+
+    wide = _dev(_table(g, [3, 3, 3], 12, 9))
+    for make in (fused, odd, turned, spread):
+        for table, lens in ((wide[:, :3], _dev([130, 190, 64])), (wide[:1, :3].expand(3, 3), _dev([130] * 3))):
+            k, v, q = make(hk), make(hk), make(hq)
+            cache, other = (KV4Cache(*(x.clone() for x in (c.k, c.k_scale, c.v, c.v_scale))) for c in [_filled(_gen(91), 12, hk, d)] * 2)
+            args, plain = (table, lens, starts), (table.contiguous(), lens, starts)
+            if table.stride(0):   # (a page may be in the table once for the tokens of a write)
+                cache.write(0, k, v, *args)
+                other.write(0, k.contiguous(), v.contiguous(), *plain)
+                assert all(torch.equal(a, b) for a, b in zip((cache.k, cache.k_scale, cache.v, cache.v_scale), (other.k, other.k_scale, other.v, other.v_scale)))
+            assert torch.equal(cache.attend(0, q, *args), other.attend(0, q.contiguous(), *plain))
+            tokens = None if starts is None else rows
+            assert all(torch.equal(a, b) for a, b in zip(cache.read(0, *args, tokens=tokens), other.read(0, *plain, tokens=tokens)))
+
+
+def test_as_many_sequences_and_heads_as_there_may_be(lib):
+    """65535 sequences, most of them empty; 4096 heads."""
+    from lingbot_world_v2_realtime_amd import packed_attention
+    g, seqs = _gen(92), 65535
+    lens = torch.zeros(seqs, dtype=torch.int32, device=DEV)
+    for s, n in ((0, 3), (63, 70), (64, 1), (40000, 130), (65534, 65)):
+        lens[s] = n
+    st = torch.cat((torch.zeros(1, device=DEV), lens.cumsum(0))).int()
+    few = _dev([0, 3, 73, 74, 204, 269])
+    leaves = [_rand(g, 269, h, 64, dtype=torch.bfloat16).requires_grad_() for h in (2, 1, 1)]
+    do = _rand(g, 269, 2, 64, dtype=torch.bfloat16)
+    out, want = packed_attention(*leaves, st), packed_attention(*leaves, few)
+    r = causal.packed(*(x.detach() for x in leaves), few.tolist(), few.tolist(), d_out=do)
+    h = 2.0 ** -8
+    rel = _packed_bounds(r, 130, 64, "bf16")
+    for x in (out, want):
+        _within(x.detach(), r["out"], (h + rel) * r["p_v"] + 130 * 2.0 ** -35, "out")
+    for x, name in zip(torch.autograd.grad(out, leaves, do), ("dq", "dk", "dv")):
+        bound = (h + E * (130 / 8 + 16)) * r[name + "_abs"] + (h + h * h) * r[name + "_wide16"] + (rel.max() + h * h + 12 * E) * r[name + "_wide32"]
+        _within(x, r[name], bound, name)
+    cache = _filled(g, 8, 1, 64)
+    table = torch.full((seqs, 3), -1, dtype=torch.int32, device=DEV)
+    held = torch.zeros(seqs, dtype=torch.int32, device=DEV)
+    table[40000], table[65534, :2] = _dev([3, 5, 1]), _dev([0, 7])
+    held[40000], held[65534], held[5] = 150, 66, 9
+    q = _rand(g, 269, 2, 64, dtype=torch.bfloat16)
+    kv = causal.unpack_pages(cache.k[0], cache.k_scale[0], cache.v[0], cache.v_scale[0])
+    got = cache.attend(0, q, table, held, st)
+    r = causal.cache_attend(q, *kv, [74, 204, 269], [150, 66], [[3, 5, 1], [0, 7]])
+    _within(got, r["out"], (h + _packed_bounds(r, 150, 64, "bf16")) * r["p_v"], "attend")
+    rows = _rand(g, seqs, 2, 64, dtype=torch.bfloat16)
+    one = cache.attend(0, rows, table, held)
+    seen = torch.zeros(seqs, dtype=torch.bool, device=DEV)
+    seen[40000] = seen[65534] = True
+    assert not one[~seen].any() and bool(one[seen].any(-1).all())
+    r = causal.cache_attend(rows[seen], *kv, [0, 1, 2], [150, 66], [[3, 5, 1], [0, 7]])
+    _within(one[seen], r["out"], (h + _packed_bounds(r, 150, 64, "bf16")) * r["p_v"], "attend, one token each")
+    q, k, v = (_rand(g, 5, n, 64, dtype=torch.bfloat16) for n in (4096, 4096, 4096))
+    out = packed_attention(q, k, v, _dev([0, 5]))
+    one = packed_attention(q[:, -1:], k[:, -1:], v[:, -1:], _dev([0, 5]))
+    assert torch.equal(out[:, -1:], one)
+    cache = _filled(g, 2, 4096, 64)
+    a, b = (cache.attend(0, x, _dev([[1]]), _dev([5]), _dev([0, 5])) for x in (q, q))
+    small = type(cache)(*(x[:, :, -1:].contiguous() for x in (cache.k, cache.k_scale, cache.v, cache.v_scale)))
+    assert torch.equal(a, b) and torch.equal(a[:, -1:], small.attend(0, q[:, -1:], _dev([[1]]), _dev([5]), _dev([0, 5])))
